@@ -315,6 +315,105 @@ typedef struct {
 } p0_attn_dec_args;
 p0_status p0_attn_dec(p0_ctx *ctx, const p0_attn_dec_args *a);
 
+/* ---------------------------------------------------------------------------------------------- paged 4-bit cache */
+/* A KV cache for many sequences, held in 4 bits, in pages of P0_KV_PAGE tokens that sequences can share; no counterpart
+ * in the reference (its caches are contiguous fp16 arrays of one stream, engine/llm/gemma4.js:97-116).
+ * A page holds the same 64 tokens of every layer. Per layer and KV head: K, then V, each a [64][D] q4g32a.t64 tensor
+ * (D / 32 records of 1280 B; row = token % 64), so a layer's part of a page is nkv * 2 * D / 32 * 1280 bytes, heads in
+ * order. A code q stands for f16(q * s + mn), rounded once. page_stride is the distance from page to page in bytes, i.e.
+ * all layers' parts (0 = one layer's); a layer's view has its part's place in the page as pool_off.
+ * State on the device: table u32 [rows][table_ld], the page of each sequence's tokens 64 j .. 64 j + 63 (an entry >=
+ * pages, e.g. P0_KV_NONE, is no page: its tokens are not there), len u32 [rows] (a length beyond 64 * table_ld counts as
+ * that), and ref u32 [pages], how many table entries (and holders of the caller's own) refer to each page.
+ * Offsets of table and len in u32. rows <= 1024, D 64, 128, 256 or 512; pool_off, page_stride 16-byte aligned.
+ * Everything is read when the call's kernels run, so a call's arguments stay valid from step to step. The operators keep
+ * their scratch in the context's workspace: calls of one context run in stream order, also after p0_set_stream only if
+ * the caller orders the streams; the first call of a size may grow it (which waits for the stream), so it should not sit
+ * inside a stream capture. */
+#define P0_KV_PAGE 64u
+#define P0_KV_NONE 0xffffffffu
+enum { P0_F32 = 0, P0_F16 = 1 };
+typedef struct {
+  p0_buf pool; uint64_t pool_off, page_stride;
+  p0_buf table; uint32_t table_off, table_ld;
+  p0_buf len; uint32_t len_off;
+  uint32_t pages, rows, D, nkv;
+} p0_kv;
+/* rows of values: token i, head h at off + i * ld + h * ldh (elements; ld 0 = heads * D, ldh 0 = D), D contiguous */
+typedef struct { p0_buf buf; uint64_t off; uint32_t ld, ldh; } p0_rows;
+
+/* kv4Put: the n newest tokens' K and V rows (type P0_F32 or P0_F16) into their pages; kv4Get: the rows that the codes
+ * stand for (zeros where there is no page). Sequence b's new tokens are T of the n (T * rows = n), or, with cu (u32
+ * [rows + 1]), tokens cu[b] .. cu[b + 1] - 1; they are its last ones: token i of T has position len[b] - T + i (len
+ * counts them already). Per 32 dims: mn = f16(min), s = f16((max - mn) / 15) (0 -> 1), q = clamp(rint((x - mn) / s), 0,
+ * 15), each step in f32. Values are held at +-60000 and NaN counts as 0 first, so that what a code stands for is finite.
+ * Tokens without a page are dropped. */
+typedef struct {
+  p0_kv kv;
+  p0_rows k, v;
+  uint32_t type, n, T;
+  p0_buf cu; uint32_t cu_off;
+} p0_kv4_rows_args;
+p0_status p0_kv4_put(p0_ctx *ctx, const p0_kv4_rows_args *a);
+p0_status p0_kv4_get(p0_ctx *ctx, const p0_kv4_rows_args *a);
+
+/* kv4Attn: attention of the n newest tokens (laid out over the sequences as for kv4Put) with nh query heads, query head
+ * h reading KV head h / (nh / nkv): out = softmax over the visible keys of scale * (q . k), times v. The token at
+ * position p sees key j <= p if window is 0, j > p - window or j < sinks. A token that sees nothing gives zeros. What
+ * the memory of unseen keys holds does not matter. scale 0 = 1. type P0_F32: q, out f32, computed to about 2^-22;
+ * P0_F16: q, out f16, P rounded to f16. */
+typedef struct {
+  p0_kv kv;
+  p0_rows q, out;
+  uint32_t type, nh, n, T;
+  p0_buf cu; uint32_t cu_off;
+  uint32_t window, sinks;
+  float scale;
+} p0_kv4_attn_args;
+p0_status p0_kv4_attn(p0_ctx *ctx, const p0_kv4_attn_args *a);
+
+/* kvStep: one step of every sequence: fork, reorder or free (parent), give back what the window has passed, extend (add).
+ * New sequence i continues old sequence parent[i] (u32 [rows]; absent: i; >= rows: it is empty, its pages are given
+ * back) with length n = len[parent[i]]. It refers to the parent's pages, without those whose every token lies outside the
+ * window of position n and behind the first `sinks` (window 0: all are kept). If n is not a multiple of 64, the last page
+ * stays with the parent's first child; every further child gets a copy of it (all layers: page_stride bytes). Then
+ * add[i] (u32 [rows]; absent: addn) tokens are appended: new pages for those beyond the last page. Pages are taken from
+ * those with no reference left, lowest first, in the order of (sequence, page).
+ * All or nothing: stat[0] = 0 and stat[1] = the free pages left; or stat[0] = the pages that are missing (P0_KV_NONE if a
+ * sequence outgrows table_ld), stat[1] = the free pages of the old state, which the new one then equals. The new state
+ * (to_table with table_ld, to_len, to_ref, each from its buffer's start) must not overlap the old one. kv.D and kv.nkv are
+ * not used; page_stride must be given. */
+typedef struct {
+  p0_kv kv;
+  p0_buf ref, to_table, to_len, to_ref, parent, add;
+  uint32_t addn, window, sinks;
+  p0_buf stat;
+} p0_kv_step_args;
+p0_status p0_kv_step(p0_ctx *ctx, const p0_kv_step_args *a);
+
+/* kvCompact: the L pages with references move into pages 0 .. L - 1: the k-th such page >= L, in order, goes to the k-th
+ * free page < L. to_table: every entry of a moved page follows it; to_ref likewise; stat[0] = L, stat[1] = pages moved.
+ * Not in place, as kvStep. */
+typedef struct {
+  p0_kv kv;
+  p0_buf ref, to_table, to_ref, stat;
+} p0_kv_compact_args;
+p0_status p0_kv_compact(p0_ctx *ctx, const p0_kv_compact_args *a);
+
+/* beamSelect: for each group of `beams` (<= 16) rows of logits (f32, V of each row, ld 0 = V, off in floats), c[b, v] =
+ * score[b] + (x[b, v] - lse_b) in f32, lse_b = log(sum exp x[b, :]), and the `beams` largest c in order, ties to the lowest
+ * b * V + v. A beam with fin[b] != 0 (fin optional) has one candidate, (eos, score[b]). NaN and -inf are never chosen
+ * (a NaN or +inf logit makes its whole row NaN). Per slot: parent = the chosen row (of all groups * beams), token, score_out,
+ * fin_out (optional) = the token is eos or the parent has finished; a slot without a candidate: P0_KV_NONE, P0_KV_NONE,
+ * -inf, 0. score_out may be score, fin_out fin. parent is what kvStep takes. eos P0_KV_NONE: no such token (without fin). */
+typedef struct {
+  p0_buf logits; uint64_t off; uint32_t ld;
+  p0_buf score, fin;
+  uint32_t groups, beams, V, eos;
+  p0_buf parent, token, score_out, fin_out;
+} p0_beam_args;
+p0_status p0_beam_select(p0_ctx *ctx, const p0_beam_args *a);
+
 /* ---------------------------------------------------------------------------------------------- quantiser */
 /* packQ4 (engine/kcheck.js:22-38) on the device, bit for bit: W f32 [N][ldw] at w_off (bytes) -> q4g32a.t64 records
  * (N*K*5/8 bytes) at out_off. N % 64 == 0, K % 32 == 0. The dequantised value of code q is q*s + mn. */

@@ -8,5 +8,5 @@ the decode-path operators around the GEMV (embed, normadd, qkrope, attnDec, argm
 weight-pack store (p0pc0rn_b200.store, engine/core/store.js) that uploads pack shards into device buffers.
 """
 from .gpu import Buffer, Gpu, P0Error, createGpu, version  # noqa: F401
-from .ops import (argmax, argmaxM, attnDec, dequant_f16, dhead, embed, gemm, gemv, gemvM, gemvM_noalloc, normadd, pack_q4,  # noqa: F401
-                  pack_q8, qkrope)
+from .ops import (argmax, argmaxM, attnDec, beamSelect, bound, dequant_f16, dhead, embed, gemm, gemv, gemvM, gemvM_noalloc,  # noqa: F401
+                  kv4Attn, kv4Get, kv4Put, kvCompact, kvStep, normadd, pack_q4, pack_q8, qkrope)

@@ -19,13 +19,16 @@ GEPI = {"f16": 0, "f32": 1, "bias": 2, "resadd": 3, "swiglu": 4, "heads": 5, "on
 ACT = {"silu": 0, "gelu": 1}
 XPRO = {"f16": 0, "lnmod": 1, "rms": 2}
 P0_ROPE_INTER, P0_ROPE_HALF = 0, 1
+TYPE = {"f32": 0, "f16": 1}
+P0_KV_PAGE, P0_KV_NONE = 64, 0xffffffff
 
 # every symbol include/p0mm.h declares
 EXPORTS = ["p0_init", "p0_destroy", "p0_set_stream", "p0_set_overlap", "p0_last_error", "p0_stats", "p0_buffer", "p0_wrap", "p0_upload", "p0_read",
            "p0_free", "p0_done", "p0_device_ptr", "p0_gemv", "p0_gemvM", "p0_gemvM_noalloc", "p0_gemm", "p0_pack_q4", "p0_pack_q8",
            "p0_dequant_f16", "p0_version", "p0_argmaxM", "p0_embed", "p0_normadd", "p0_dhead",
            "p0_upload_file", "p0_qkrope", "p0_attn_dec", "p0_wait_selftest",
-           "p0_chain_begin", "p0_chain_end", "p0_chain_run", "p0_chain_info", "p0_chain_free", "p0_copy"]
+           "p0_chain_begin", "p0_chain_end", "p0_chain_run", "p0_chain_info", "p0_chain_free", "p0_copy",
+           "p0_kv4_put", "p0_kv4_get", "p0_kv4_attn", "p0_kv_step", "p0_kv_compact", "p0_beam_select"]
 P0_NOALLOC_SCRATCH_BYTES = 16 << 20   # include/p0mm.h
 P0_OVERLAP_WEIGHTS = 1
 P0_NOALLOC_COUNTER_BYTES = 64 << 10
@@ -95,6 +98,38 @@ class p0_attn_dec_args(ctypes.Structure):
                 ("nkv", _u32), ("kvLen", _u32), ("kStart", _u32), ("kEnd", _u32), ("ring", _u32)]
 
 
+class p0_kv(ctypes.Structure):
+    _fields_ = [("pool", p0_buf), ("pool_off", ctypes.c_uint64), ("page_stride", ctypes.c_uint64), ("table", p0_buf), ("table_off", _u32),
+                ("table_ld", _u32), ("len", p0_buf), ("len_off", _u32), ("pages", _u32), ("rows", _u32), ("D", _u32), ("nkv", _u32)]
+
+
+class p0_rows(ctypes.Structure):
+    _fields_ = [("buf", p0_buf), ("off", ctypes.c_uint64), ("ld", _u32), ("ldh", _u32)]
+
+
+class p0_kv4_rows_args(ctypes.Structure):
+    _fields_ = [("kv", p0_kv), ("k", p0_rows), ("v", p0_rows), ("type", _u32), ("n", _u32), ("T", _u32), ("cu", p0_buf), ("cu_off", _u32)]
+
+
+class p0_kv4_attn_args(ctypes.Structure):
+    _fields_ = [("kv", p0_kv), ("q", p0_rows), ("out", p0_rows), ("type", _u32), ("nh", _u32), ("n", _u32), ("T", _u32), ("cu", p0_buf),
+                ("cu_off", _u32), ("window", _u32), ("sinks", _u32), ("scale", ctypes.c_float)]
+
+
+class p0_kv_step_args(ctypes.Structure):
+    _fields_ = [("kv", p0_kv), ("ref", p0_buf), ("to_table", p0_buf), ("to_len", p0_buf), ("to_ref", p0_buf), ("parent", p0_buf), ("add", p0_buf),
+                ("addn", _u32), ("window", _u32), ("sinks", _u32), ("stat", p0_buf)]
+
+
+class p0_kv_compact_args(ctypes.Structure):
+    _fields_ = [("kv", p0_kv), ("ref", p0_buf), ("to_table", p0_buf), ("to_ref", p0_buf), ("stat", p0_buf)]
+
+
+class p0_beam_args(ctypes.Structure):
+    _fields_ = [("logits", p0_buf), ("off", ctypes.c_uint64), ("ld", _u32), ("score", p0_buf), ("fin", p0_buf), ("groups", _u32), ("beams", _u32),
+                ("V", _u32), ("eos", _u32), ("parent", p0_buf), ("token", p0_buf), ("score_out", p0_buf), ("fin_out", p0_buf)]
+
+
 _lib = None
 
 
@@ -141,6 +176,12 @@ def load():
     L.p0_chain_run.argtypes = [vp, vp]
     L.p0_chain_info.argtypes = [vp, vp] + [ctypes.POINTER(ctypes.c_uint32)] * 4
     L.p0_chain_free.argtypes = [vp, vp]
+    L.p0_kv4_put.argtypes = [vp, ctypes.POINTER(p0_kv4_rows_args)]
+    L.p0_kv4_get.argtypes = [vp, ctypes.POINTER(p0_kv4_rows_args)]
+    L.p0_kv4_attn.argtypes = [vp, ctypes.POINTER(p0_kv4_attn_args)]
+    L.p0_kv_step.argtypes = [vp, ctypes.POINTER(p0_kv_step_args)]
+    L.p0_kv_compact.argtypes = [vp, ctypes.POINTER(p0_kv_compact_args)]
+    L.p0_beam_select.argtypes = [vp, ctypes.POINTER(p0_beam_args)]
     L.p0_version.restype = ctypes.c_char_p
     for name in EXPORTS:
         if name != "p0_version":

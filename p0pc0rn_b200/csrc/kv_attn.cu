@@ -1,0 +1,571 @@
+// kv_attn.cu -- kv4Attn: attention of each sequence's newest tokens over its paged 4-bit cache (causal; whole context, or
+// a sliding window with the first `sinks` tokens kept visible). No counterpart in the reference, whose attnDec takes one
+// token over a contiguous fp16 cache (engine/llm/lops.js:236-321).
+//
+//   o_i = sum_j p_ij v_j,  p_i = softmax over the visible j of scale * (q_i . k_j),  k, v = f16(q * s + mn)
+//   visible: j <= pos_i and (window = 0 or j > pos_i - window or j < sinks);  nothing visible: o_i = 0
+//
+// Work. The query rows that share a KV head (new tokens x query heads of its group) form row blocks; a unit is one row
+// block of one sequence and KV head, its items are the pages that any of its rows sees. The units' items, in order, are
+// cut into equal runs, one per CTA, from the lengths on the device: long and short sequences, windows and empty slots
+// fill the GPU alike. A unit that lies in one run is finished there; otherwise each run leaves (m, l, acc) in the
+// workspace and the combine kernel joins them in run order, so results do not depend on timing.
+//
+// A page. One bulk copy brings a head's K and V records (D * 80 bytes); a ring of stages hides it. The codes become f16
+// pairs in registers (two codes per sub and fma on the half2 pipe) and go straight into mma.sync fragments: S = Q K^T
+// with a warp's share of the 64 keys, then O += P V with a warp's share of the dims, P going through shared memory. The
+// code words fit the fragments without moves: a K word holds 8 dims of one key (any dim order serves a dot product, q is
+// staged in that order), and two keys' V words give 4 or 8 (key, key + 1) pairs per byte permute.
+//
+// Precision. f32 queries and outputs: q and P are split into f16 high and low parts (about 22 bits) in rows r and r + 8
+// of the fragments; each page's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
+// f16 matrix operand), 16 rows per fragment.
+#include "kv.cuh"
+#include "launch.cuh"
+#include "tc.cuh"
+
+namespace {
+
+struct AttnJob {
+  KvView v;
+  KvRows q, out;
+  uint32_t hpg, window, sinks;
+  float scale;
+  uint32_t *err;
+  float *part;        // [grid][2][rows of a block][D + 2]
+  uint4 *desc;        // [grid]: (1 + last run, b, first row, KV head) of the unit that this run begins and others end
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t lds_u32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
+
+// what a unit's rows see: pages [0, sink_pages) and [from, last], or nothing (n = 0)
+struct Span {
+  uint32_t sink_pages, from, n;
+  uint32_t first_pos, end;   // first key inside the first row's window; one past the last row's position
+};
+__device__ __forceinline__ Span span_of(uint32_t len, uint32_t T, uint32_t t0, uint32_t t1, uint32_t window, uint32_t sinks) {
+  Span s;
+  // positions of rows t0 and t1 (0 <= t0 <= t1 < T): len - T + t, which may be negative
+  const int64_t p1 = (int64_t)len - T + t1, p0 = (int64_t)len - T + t0;
+  s.end = p1 < 0 ? 0u : (uint32_t)p1 + 1u;
+  s.first_pos = window && p0 - (int64_t)window + 1 > 0 ? (uint32_t)(p0 - (int64_t)window + 1) : 0u;
+  s.from = s.first_pos / kPage;
+  const uint32_t sp = (uint32_t)(((uint64_t)sinks + kPage - 1) / kPage);
+  s.sink_pages = sp < s.from ? sp : s.from;
+  s.n = s.end ? s.sink_pages + (s.end - 1) / kPage + 1 - s.from : 0u;
+  return s;
+}
+
+template <int D, bool F32, int NW, int RT>
+struct Cfg {
+  static constexpr int kThreads = NW * 32;
+  static constexpr int kRowsPer = F32 ? 8 : 16;          // query rows per fragment
+  static constexpr int kRows = kRowsPer * RT;            // of a block
+  static constexpr int kNpl = D / NW / 8;                // dims per lane and key in P V (output columns: 8 lanes x kNpl)
+  static constexpr int kNt = 8 / NW;                     // 8-key tiles per warp in Q K^T
+  static constexpr uint32_t kPart = D / 32 * 1280;
+  static constexpr int kStages = D >= 512 ? 2 : 3;
+  static constexpr uint32_t kQ = RT * D / 16 * 512;      // q fragments
+  static constexpr uint32_t kPRow = 64 * 2 + 16;         // a row of P, padded against bank conflicts
+  static constexpr uint32_t kP = RT * 16 * kPRow;
+  static constexpr uint32_t kSmem = kStages * 2 * kPart + kQ + kP;
+};
+
+template <int D, bool F32, int NW, int RT>
+__global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
+  dep_enter();
+  using C = Cfg<D, F32, NW, RT>;
+  constexpr int NPL = C::kNpl, NT = C::kNt, RR = C::kRowsPer, RB = C::kRows, NS = C::kStages;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t *ring = smem;
+  uint4 *qf = reinterpret_cast<uint4 *>(smem + NS * 2 * C::kPart);
+  uint8_t *ps = smem + NS * 2 * C::kPart + C::kQ;
+  uint32_t *pre = reinterpret_cast<uint32_t *>(smem + C::kSmem);   // [rows + 1] items before each sequence
+  __shared__ __align__(8) uint64_t full[NS];
+  __shared__ uint32_t abort_flag, page_ok[NS];
+  __shared__ float wmax[NW][RB], wsum[NW][RB];
+  __shared__ int32_t rpos[RB];
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g4 = lane >> 2, t4 = lane & 3u;
+  const uint32_t hpg = j.hpg, nkv = j.v.nkv, R = j.v.rows, W = j.window, S = j.sinks;
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) tc::mbar_init(&full[i], 1);
+    abort_flag = 0u;
+    tc::fence_mbar_init();
+  }
+  // items per sequence: over its row blocks, max(1, pages seen) per KV head (an empty unit is one item: it writes zeros)
+  for (uint32_t b = tid; b < R; b += C::kThreads) {
+    uint32_t lo, T = kv_tokens(j.v, b, lo), items = 0;
+    const uint32_t len = kv_len(j.v, b);
+    for (uint32_t r = 0; r < T * hpg; r += RB) {
+      const Span s = span_of(len, T, r / hpg, min(T * hpg - 1, r + RB - 1) / hpg, W, S);
+      items += max(1u, s.n);
+    }
+    pre[b + 1] = items * nkv;
+  }
+  if (tid == 0) pre[0] = 0u;
+  __syncthreads();
+  if (warp == 0) {   // inclusive sums
+    uint32_t carry = 0;
+    for (uint32_t b0 = 0; b0 < R; b0 += 32) {
+      uint32_t v = b0 + lane < R ? pre[b0 + lane + 1] : 0u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= (uint32_t)o) v += u;
+      }
+      if (b0 + lane < R) pre[b0 + lane + 1] = v + carry;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+  __syncthreads();
+  const uint32_t total = pre[R], G = min(gridDim.x, max(total, 1u));   // no run is empty
+  if (tid == 0) j.desc[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+  if (blockIdx.x >= G) return;
+  const uint32_t lo = (uint32_t)((uint64_t)total * blockIdx.x / G), hi = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / G);
+  uint32_t b = 0;
+  {
+    uint32_t a = 0, e = R;   // the last b with pre[b] <= lo and items of its own
+    while (e - a > 1) {
+      const uint32_t m = (a + e) >> 1;
+      if (pre[m] <= lo) a = m; else e = m;
+    }
+    b = a;
+  }
+  uint32_t at = lo, it = 0;   // item; pages through the ring so far
+  while (at < hi) {
+    while (pre[b + 1] <= at) b++;
+    uint32_t first, T = kv_tokens(j.v, b, first);
+    const uint32_t len = kv_len(j.v, b), rows = T * hpg;
+    // the unit of item `at`: row blocks in order, each with its KV heads in order
+    uint32_t base = pre[b], r0 = 0, n;
+    Span s;
+    for (;; r0 += RB) {
+      s = span_of(len, T, r0 / hpg, min(rows - 1, r0 + RB - 1) / hpg, W, S);
+      n = max(1u, s.n);
+      if (at < base + n * nkv) break;
+      base += n * nkv;
+    }
+    const uint32_t head = (at - base) / n, begin = base + head * n, from = at - begin, to = min(hi - begin, n);
+    const uint32_t nrow = min((uint32_t)RB, rows - r0);
+    const uint32_t steps = s.n ? to - from : 0u;
+    const uint8_t *heads = j.v.pool + (uint64_t)head * 2u * C::kPart;
+    const auto page_of = [&](uint32_t i) { return i < s.sink_pages ? i : s.from + (i - s.sink_pages); };
+    const auto issue = [&](uint32_t i) {   // item from + i of the unit into its ring slot
+      const uint32_t st = (it + i) % NS, p = j.v.table[(uint64_t)b * j.v.ld + page_of(from + i)];
+      page_ok[st] = p < j.v.pages;
+      if (p < j.v.pages) {
+        tc::mbar_expect_tx(&full[st], 2u * C::kPart);
+        bulk_load(ring + st * 2u * C::kPart, heads + p * j.v.stride, 2u * C::kPart, &full[st]);
+      } else {
+        tc::mbar_arrive(&full[st]);   // no such page: its keys are not there
+      }
+    };
+    if (tid == 0)
+      for (uint32_t i = 0; i < (uint32_t)NS && i < steps; i++) issue(i);
+    // the rows' positions and q fragments
+    if (tid < (uint32_t)RB) rpos[tid] = tid < nrow ? (int32_t)((int64_t)len - T + (r0 + tid) / hpg) : -1;
+    for (uint32_t e = tid; e < RT * (D / 16) * 32u; e += C::kThreads) {
+      const uint32_t ln = e & 31u, step = (e >> 5) % (D / 16), rt = (e >> 5) / (D / 16);
+      const uint32_t d0 = (step >> 1) * 32u + (ln & 3u) * 8u + (step & 1u) * 2u;   // the lane's word; codes d0, +4, +1, +5
+      float x[2][4];
+#pragma unroll
+      for (int half = 0; half < (F32 ? 1 : 2); half++) {
+        const uint32_t r = rt * RR + (ln >> 2) + 8u * half;
+        if (r < nrow) {
+          const uint64_t o = (uint64_t)(first + (r0 + r) / hpg) * j.q.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.q.ldh + d0;
+          if (F32) {
+            const float *q = reinterpret_cast<const float *>(j.q.base) + o;
+            x[half][0] = q[0]; x[half][1] = q[4]; x[half][2] = q[1]; x[half][3] = q[5];
+          } else {
+            const __half *q = reinterpret_cast<const __half *>(j.q.base) + o;
+            x[half][0] = __half2float(q[0]); x[half][1] = __half2float(q[4]); x[half][2] = __half2float(q[1]); x[half][3] = __half2float(q[5]);
+          }
+        } else {
+          x[half][0] = x[half][1] = x[half][2] = x[half][3] = 0.0f;
+        }
+      }
+      uint4 f;
+      f.x = pack2(x[0][0], x[0][1]);
+      f.z = pack2(x[0][2], x[0][3]);
+      if (F32) {   // rows + 8: what f16 leaves of the same rows
+        const float2 h0 = __half22float2(*reinterpret_cast<const __half2 *>(&f.x)), h1 = __half22float2(*reinterpret_cast<const __half2 *>(&f.z));
+        f.y = pack2(x[0][0] - h0.x, x[0][1] - h0.y);
+        f.w = pack2(x[0][2] - h1.x, x[0][3] - h1.y);
+      } else {
+        f.y = pack2(x[1][0], x[1][1]);
+        f.w = pack2(x[1][2], x[1][3]);
+      }
+      qf[e] = f;
+    }
+    __syncthreads();
+    constexpr int RH = F32 ? 1 : 2;   // rows of a lane per fragment: g4 (and g4 + 8)
+    float o[RT][NPL][4], m[RT][RH], l[RT][RH];
+    int32_t pos[RT][RH];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+      for (int i = 0; i < NPL; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[rt][i][e] = 0.0f;
+#pragma unroll
+      for (int h = 0; h < RH; h++) {
+        m[rt][h] = -INFINITY;
+        l[rt][h] = 0.0f;
+        pos[rt][h] = rpos[rt * RR + g4 + 8 * h];
+      }
+    }
+    bool lost = false;
+    for (uint32_t i = 0; i < steps; i++) {
+      const uint32_t st = (it + i) % NS, page = page_of(from + i), key0 = page * kPage;
+      if (!tc::mbar_wait(&full[st], ((it + i) / NS) & 1u, &abort_flag, j.err, 0x4a1u, P0_SPIN_LIMIT)) lost = true;
+      const uint8_t *kp = ring + st * 2u * C::kPart, *vp = kp + C::kPart;
+      // ---- S = Q K^T: this warp's 8-key tiles
+      float sc[RT][NT][4];
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) sc[rt][nt][e] = 0.0f;
+#pragma unroll 4
+      for (int g = 0; g < D / 32; g++) {
+        uint32_t kb[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const uint32_t key = (warp * NT + nt) * 8u + g4;
+          const uint32_t w = lds_u32(kp + g * 1280 + key * 16u + t4 * 4u), sm = lds_u32(kp + g * 1280 + 1024 + key * 4u);
+          const uint32_t s2 = __byte_perm(sm, 0, 0x1010), mn2 = __byte_perm(sm, 0, 0x3232);
+#pragma unroll
+          for (int e = 0; e < 4; e++) kb[nt][e] = kv_deq2((w >> (4 * e)) & 0x000F000Fu, s2, mn2);   // dims (e, e + 4)
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            const uint4 f = qf[(rt * (D / 16) + 2 * g + half) * 32 + lane];
+            const uint32_t a[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) mma_f16(sc[rt][nt], a, kb[nt][2 * half], kb[nt][2 * half + 1]);
+          }
+      }
+      // ---- mask, the page's row maxima
+      const bool ok = page_ok[st] != 0u;
+      float x[RT][NT][RH][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int h = 0; h < RH; h++) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int32_t key = (int32_t)(key0 + (warp * NT + nt) * 8u + 2u * t4 + e);
+              const bool see = ok && key <= pos[rt][h] && (!W || (int64_t)key > (int64_t)pos[rt][h] - W || (uint32_t)key < S);
+              const float v = F32 ? sc[rt][nt][e] + sc[rt][nt][e + 2] : sc[rt][nt][2 * h + e];
+              x[rt][nt][h][e] = see ? v * j.scale : -INFINITY;
+              mx = fmaxf(mx, x[rt][nt][h][e]);
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (t4 == 0) wmax[warp][rt * RR + g4 + 8 * h] = mx;
+        }
+      __syncthreads();   // the previous page's P V is done: its ring slot is free
+      if (tid == 0 && i > 0 && i - 1 + NS < steps) issue(i - 1 + NS);
+      // ---- P = exp(x - m), into shared memory as f16 (f32: high and low parts)
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int h = 0; h < RH; h++) {
+          const uint32_t r = rt * RR + g4 + 8 * h;
+          float mn = m[rt][h];
+#pragma unroll
+          for (int w = 0; w < NW; w++) mn = fmaxf(mn, wmax[w][r]);
+          const float ref = mn == -INFINITY ? 0.0f : mn;
+          const float keep = expf(m[rt][h] - ref);   // 0 while nothing has been seen
+          m[rt][h] = mn;
+          l[rt][h] *= keep;
+#pragma unroll
+          for (int nt = 0; nt < NPL; nt++) {
+            if (F32) {
+#pragma unroll
+              for (int e = 0; e < 4; e++) o[rt][nt][e] *= keep;
+            } else {
+              o[rt][nt][2 * h] *= keep;
+              o[rt][nt][2 * h + 1] *= keep;
+            }
+          }
+          uint8_t *row = ps + (rt * 16 + g4 + 8 * h) * C::kPRow;
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            const float p0 = expf(x[rt][nt][h][0] - ref), p1 = expf(x[rt][nt][h][1] - ref);
+            l[rt][h] += p0 + p1;
+            const uint32_t hi2 = pack2(p0, p1), col = ((warp * NT + nt) * 8u + 2u * t4) * 2u;
+            *reinterpret_cast<uint32_t *>(row + col) = hi2;
+            if (F32) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi2));
+              *reinterpret_cast<uint32_t *>(row + 8 * C::kPRow + col) = pack2(p0 - f.x, p1 - f.y);
+            }
+          }
+        }
+      __syncthreads();
+      // ---- O += P V: this warp's dims. Slots that no row of the unit sees hold zeros, whatever the memory holds
+      const bool edge = !ok || key0 + kPage > s.end || (key0 < s.first_pos && key0 + kPage > S);
+      float c[RT][NPL][4];
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int nt = 0; nt < NPL; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) c[rt][nt][e] = 0.0f;
+      const uint32_t d0 = warp * (D / NW) + g4 * NPL;                 // the lane's first dim
+      const uint32_t swap = NPL == 8 ? (g4 >> 2) & 1u : 0u;          // the second group of 32 dims starts with the odd key: other banks
+      const uint8_t *vg = vp + d0 / 32u * 1280u, *vw = vg + (d0 % 32u) / 8u * 4u;
+#pragma unroll
+      for (int ks = 0; ks < 4; ks++) {
+        uint32_t vb[NPL][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t key = ks * 16 + h * 8 + 2 * t4;
+          const uint32_t w0 = lds_u32(vw + (key + swap) * 16u), w1 = lds_u32(vw + (key + 1u - swap) * 16u);
+          uint2 sm = *reinterpret_cast<const uint2 *>(vg + 1024u + key * 4u);
+          if (edge) {
+            const uint32_t k0 = key0 + key, k1 = k0 + 1u;
+            if (!ok || k0 >= s.end || (k0 < s.first_pos && k0 >= S)) sm.x = 0u;
+            if (!ok || k1 >= s.end || (k1 < s.first_pos && k1 >= S)) sm.y = 0u;
+          }
+          const uint32_t s2 = __byte_perm(sm.x, sm.y, 0x5410), mn2 = __byte_perm(sm.x, sm.y, 0x7632);   // (key, key + 1)
+          if constexpr (NPL == 8) {
+            const uint32_t u = __byte_perm(w0, w1, swap ? 0x1054u : 0x5410u), v = __byte_perm(w0, w1, swap ? 0x3276u : 0x7632u);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              vb[e][h] = kv_deq2((u >> (4 * e)) & 0x000F000Fu, s2, mn2);
+              vb[e + 4][h] = kv_deq2((v >> (4 * e)) & 0x000F000Fu, s2, mn2);
+            }
+          } else if constexpr (NPL == 4) {
+            const uint32_t u = __byte_perm(w0, w1, (d0 & 4u) ? 0x7632u : 0x5410u);
+#pragma unroll
+            for (int e = 0; e < NPL; e++) vb[e][h] = kv_deq2((u >> (4 * e)) & 0x000F000Fu, s2, mn2);
+          } else {
+            const uint32_t by = (d0 & 7u) / 2u;
+            const uint32_t u = __byte_perm(w0, w1, by | (by << 4) | ((4u + by) << 8) | ((4u + by) << 12));
+#pragma unroll
+            for (int e = 0; e < NPL; e++) vb[e][h] = kv_deq2((u >> (4 * e)) & 0x000F000Fu, s2, mn2);
+          }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+          const uint8_t *row = ps + (rt * 16 + g4) * C::kPRow + (ks * 16 + 2 * t4) * 2;
+          const uint32_t a[4] = {lds_u32(row), lds_u32(row + 8 * C::kPRow), lds_u32(row + 16), lds_u32(row + 8 * C::kPRow + 16)};
+#pragma unroll
+          for (int nt = 0; nt < NPL; nt++) mma_f16(c[rt][nt], a, vb[nt][0], vb[nt][1]);
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int nt = 0; nt < NPL; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[rt][nt][e] += c[rt][nt][e];
+      if (__syncthreads_or(lost)) { lost = true; break; }
+    }
+    if (lost) {   // a copy did not arrive in time: j.err says so. Let the copies in flight land before the CTA leaves
+      for (uint32_t i = 0; i < steps; i++)
+        for (uint32_t k = 0; k < (1u << 16) && !tc::mbar_try(&full[(it + i) % NS], ((it + i) / NS) & 1u); k++) {}
+      return;
+    }
+    it += steps;
+    // ---- the rows' sums over the warps, then out or into the workspace
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+      for (int h = 0; h < RH; h++) {
+        float t = l[rt][h];
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        if (t4 == 0) wsum[warp][rt * RR + g4 + 8 * h] = t;
+      }
+    __syncthreads();
+    const bool whole = from == 0 && to == n;
+    // a run has at most one part of a unit that began earlier (slot 0) and one of a unit that goes on after it (slot 1)
+    float *part = j.part + ((uint64_t)blockIdx.x * 2u + (from ? 0u : 1u)) * RB * (D + 2);
+    if (!whole && from == 0 && tid == 0) {
+      // runs end where total * (c + 1) / G does: the last one of this unit holds item begin + n - 1
+      const uint32_t c = (uint32_t)((((uint64_t)begin + n) * G - 1) / total);
+      j.desc[blockIdx.x] = make_uint4(1u + c, b, r0, head);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+      for (int h = 0; h < RH; h++) {
+        const uint32_t r = rt * RR + g4 + 8 * h;
+        if (r >= nrow) continue;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) sum += wsum[w][r];
+        const float inv = whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+        float y[2][NPL];   // dims 2 t4 * NPL .. and (2 t4 + 1) * NPL ..: contiguous
+#pragma unroll
+        for (int nt = 0; nt < NPL; nt++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) y[e][nt] = (F32 ? o[rt][nt][e] + o[rt][nt][e + 2] : o[rt][nt][2 * h + e]) * inv;
+        const uint32_t d = warp * (D / NW) + 2 * t4 * NPL;
+        if (whole) {
+          const uint64_t q = (uint64_t)(first + (r0 + r) / hpg) * j.out.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.out.ldh + d;
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int nt = 0; nt < NPL; nt++) {
+              if (F32) reinterpret_cast<float *>(j.out.base)[q + e * NPL + nt] = y[e][nt];
+              else reinterpret_cast<__half *>(j.out.base)[q + e * NPL + nt] = __float2half_rn(y[e][nt]);
+            }
+        } else {
+          float *p = part + (uint64_t)r * (D + 2);
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int nt = 0; nt < NPL; nt++) p[d + e * NPL + nt] = y[e][nt];
+          if (warp == 0 && t4 == 0) {
+            p[D] = m[rt][h];
+            p[D + 1] = sum;
+          }
+        }
+      }
+    at = begin + to;
+    __syncthreads();   // q fragments, wsum and rpos are free
+  }
+}
+
+// joins the parts of the units that several runs share: CTA (c, r) takes row r of the unit that run c begins.
+// M = max m, o = sum exp(m - M) acc / sum exp(m - M) l, in run order
+template <int D, bool F32, int RB>
+__global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnJob j) {
+  dep_enter();
+  constexpr int L = D / 4, K = 256 / L > 0 ? 256 / L : 1;   // lanes per row (4 dims each), parts at a time
+  __shared__ float4 acc[K][L];
+  __shared__ float ms[256], sums[K];
+  const uint4 u = j.desc[blockIdx.x];
+  const uint32_t r = blockIdx.y;
+  if (!u.x) return;
+  const uint32_t b = u.y, r0 = u.z, head = u.w, hpg = j.hpg;
+  uint32_t first;
+  const uint32_t T = kv_tokens(j.v, b, first);
+  if (r0 + r >= T * hpg) return;
+  const uint32_t n = u.x - blockIdx.x;   // parts: this run's slot 1, then slot 0 of the following runs
+  const auto part = [&](uint32_t i) {
+    return j.part + ((uint64_t)(blockIdx.x + i) * 2u + (i ? 0u : 1u)) * RB * (D + 2) + (uint64_t)r * (D + 2);
+  };
+  float M = -INFINITY;
+  for (uint32_t i = threadIdx.x; i < n; i += 256) M = fmaxf(M, part(i)[D]);
+  ms[threadIdx.x] = M;
+  __syncthreads();
+  for (int s = 128; s > 0; s >>= 1) {
+    if ((int)threadIdx.x < s) ms[threadIdx.x] = fmaxf(ms[threadIdx.x], ms[threadIdx.x + s]);
+    __syncthreads();
+  }
+  M = ms[0];
+  const float ref = M == -INFINITY ? 0.0f : M;
+  const uint32_t k = threadIdx.x / L, e = threadIdx.x % L;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float sum = 0.0f;
+  for (uint32_t i = k; i < n; i += K) {
+    const float *p = part(i);
+    const float w = expf(p[D] - ref);
+    const float2 a = *reinterpret_cast<const float2 *>(p + 4 * e), c = *reinterpret_cast<const float2 *>(p + 4 * e + 2);
+    o.x = fmaf(w, a.x, o.x);
+    o.y = fmaf(w, a.y, o.y);
+    o.z = fmaf(w, c.x, o.z);
+    o.w = fmaf(w, c.y, o.w);
+    sum = fmaf(w, p[D + 1], sum);
+  }
+  acc[k][e] = o;
+  if (e == 0) sums[k] = sum;
+  __syncthreads();
+  if (k) return;
+  for (int i = 1; i < K; i++) {
+    const float4 a = acc[i][e];
+    o.x += a.x;
+    o.y += a.y;
+    o.z += a.z;
+    o.w += a.w;
+    sum += sums[i];
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  const uint64_t q = (uint64_t)(first + (r0 + r) / hpg) * j.out.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.out.ldh + 4 * e;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (F32) reinterpret_cast<float *>(j.out.base)[q + i] = y[i];
+    else reinterpret_cast<__half *>(j.out.base)[q + i] = __float2half_rn(y[i]);
+  }
+}
+
+template <int D, bool F32, int NW, int RT>
+p0_status attn_launch(p0_ctx *c, AttnJob &j) {
+  using C = Cfg<D, F32, NW, RT>;
+  const size_t smem = C::kSmem + ((size_t)j.v.rows + 1) * 4;
+  const auto kern = kv4_attn_kernel<D, F32, NW, RT>;
+  int per = 0;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, C::kThreads, smem);
+  if (e != cudaSuccess || per < 1) { cudaGetLastError(); return p0_fail(c, P0_EDEVICE, "kv4Attn: the kernel does not fit this device"); }
+  const uint32_t G = (uint32_t)(per * c->sm_count);
+  uint32_t *cnt;
+  void *ws;
+  const size_t parts = (size_t)G * 2 * C::kRows * (D + 2) * 4;
+  p0_status st = p0_workspace(c, 0, (size_t)G * sizeof(uint4) + parts, &cnt, &ws);
+  if (st) return st;
+  j.desc = (uint4 *)ws;
+  j.part = (float *)(j.desc + G);
+  launch_dep(kern, dim3(G), dim3(C::kThreads), smem, c->stream, j);
+  if ((st = p0_launched(c, "kv4Attn"))) return st;
+  launch_dep(kv4_attn_join_kernel<D, F32, C::kRows>, dim3(G, C::kRows), dim3(256), 0, c->stream, j);
+  return p0_launched(c, "kv4Attn join");
+}
+
+}  // namespace
+
+extern "C" p0_status p0_kv4_attn(p0_ctx *c, const p0_kv4_attn_args *a) {
+  if (!c || !a) return P0_EINVAL;
+  const char *op = "kv4Attn";
+  if (a->type > P0_F16) return p0_fail(c, P0_EINVAL, "%s: type %u", op, a->type);
+  if (!a->n) return P0_OK;
+  AttnJob j = {};
+  p0_status st;
+  if ((st = kv_view(c, a->kv, true, op, &j.v))) return st;
+  if (!a->nh || a->nh % a->kv.nkv) return p0_fail(c, P0_EINVAL, "%s: %u query heads over %u KV heads", op, a->nh, a->kv.nkv);
+  if ((st = kv_new_tokens(c, a->n, a->T, a->cu, a->cu_off, op, &j.v))) return st;
+  if ((st = kv_rows(c, a->q, a->n, a->nh, a->kv.D, a->type, op, "q", &j.q))) return st;
+  if ((st = kv_rows(c, a->out, a->n, a->nh, a->kv.D, a->type, op, "out", &j.out))) return st;
+  j.hpg = a->nh / a->kv.nkv;
+  j.window = a->window;
+  j.sinks = a->sinks;
+  j.scale = a->scale != 0.0f ? a->scale : 1.0f;
+  j.err = c->d_err;
+  // the kernels count query rows and items (pages of row blocks) in 32 bits
+  const uint64_t rows = (uint64_t)a->n * j.hpg;
+  if (rows > 0x7fffffffu || (rows / 8 + a->kv.rows + 1) * a->kv.nkv * a->kv.table_ld > 0xffffffffull)
+    return p0_fail(c, P0_EINVAL, "%s: %u tokens x %u heads over %u pages pass 32 bits", op, a->n, a->nh, a->kv.table_ld);
+  cudaSetDevice(c->device);
+  const bool f32 = a->type == P0_F32;
+  switch (a->kv.D) {
+    case 64: return f32 ? attn_launch<64, true, 4, 1>(c, j) : attn_launch<64, false, 4, 1>(c, j);
+    case 128: return f32 ? attn_launch<128, true, 4, 1>(c, j) : attn_launch<128, false, 4, 1>(c, j);
+    case 256: return f32 ? attn_launch<256, true, 4, 1>(c, j) : attn_launch<256, false, 4, 1>(c, j);
+    default: return f32 ? attn_launch<512, true, 8, 1>(c, j) : attn_launch<512, false, 8, 1>(c, j);
+  }
+}

@@ -7,18 +7,11 @@
 #include <cuda_fp16.h>
 
 #include "internal.h"
+#include "launch.cuh"
 
 namespace {
 
 constexpr int kT = 256;   // threads per CTA
-
-// Programmatic dependent launch: every operator kernel is launched so that it may start while the kernel ahead of it is
-// still running; it waits for that kernel (griddepcontrol.wait: all prerequisite grids complete, their writes visible)
-// before it reads anything, then lets the kernel after it launch at once. Without such a launch both are no-ops.
-__device__ __forceinline__ void dep_enter() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
 
 __device__ __forceinline__ float h2f(uint32_t h16) { return __half2float(__ushort_as_half((unsigned short)(h16 & 0xffffu))); }
 
@@ -421,21 +414,6 @@ __global__ void __launch_bounds__(kT) attn_combine_kernel(const float *__restric
 }
 
 
-// a kernel launch that lets the kernel start before the one ahead of it on the stream finishes (see dep_enter)
-template <typename Kern, typename... Args>
-cudaError_t launch_dep(Kern k, dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, args...);
-}
 }  // namespace
 
 extern "C" {

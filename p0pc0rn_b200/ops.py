@@ -1,4 +1,4 @@
-"""The three matmul operators with the reference's own argument objects, over the C ABI.
+"""The operators with the reference's own argument objects, over the C ABI.
 
   gemv(g, a)   -> nsplit   engine/llm/lops.js:108-141       (a = {w, x: {buf, rowB}, N, K, kPer, pro, epi, y: {buf},
                                                             ldy, stat: {buf, off}, norm: {buf, off}, ev: {buf, off},
@@ -210,3 +210,116 @@ def attnDec(g, a):
                               handle(a["out"]["buf"]), int(a["D"]), int(a["nh"]), int(a.get("nkv") or 1), int(a.get("kvLen") or 0),
                               int(a["kStart"]), int(a["kEnd"]), int(a.get("ring") or 0))
     g._check(g._lib.p0_attn_dec(g.ctx, ctypes.byref(args)))
+
+
+# ---------------------------------------------------------------- paged 4-bit cache and beam search
+# Each operator's arguments become a C struct once per call; a loop that repeats a call keeps it with bound().
+def _kv(kv):
+    pool, table, ln = kv["pool"], kv["table"], kv["len"]
+    return L.p0_kv(handle(pool["buf"]), int(pool.get("off") or 0), int(pool.get("stride") or 0), handle(table["buf"]), int(table.get("off") or 0),
+                   int(table["ld"]), handle(ln["buf"]), int(ln.get("off") or 0), int(kv["pages"]), int(kv["rows"]), int(kv.get("D") or 0),
+                   int(kv.get("nkv") or 0))
+
+
+def _rows(r):
+    return L.p0_rows(handle(r["buf"]), int(r.get("off") or 0), int(r.get("ld") or 0), int(r.get("ldh") or 0))
+
+
+def _type(a, op):
+    t = a.get("type") or "f32"
+    if t not in L.TYPE:
+        raise P0Error(L.P0_EINVAL, "%s: type %s" % (op, t))
+    return L.TYPE[t]
+
+
+def _kv4_rows_args(a, op):
+    cu = a.get("cu")
+    return L.p0_kv4_rows_args(_kv(a["kv"]), _rows(a["k"]), _rows(a["v"]), _type(a, op), int(a["n"]), int(a.get("T") or 0), _b(cu),
+                              int((cu or {}).get("off") or 0))
+
+
+def _kv4_attn_args(a):
+    cu = a.get("cu")
+    return L.p0_kv4_attn_args(_kv(a["kv"]), _rows(a["q"]), _rows(a["out"]), _type(a, "kv4Attn"), int(a["nh"]), int(a["n"]), int(a.get("T") or 0),
+                              _b(cu), int((cu or {}).get("off") or 0), int(a.get("window") or 0), int(a.get("sinks") or 0),
+                              float(a.get("scale") or 0.0))
+
+
+def _kv_step_args(a):
+    to, add = a["to"], a.get("add")
+    num = not isinstance(add, dict)
+    return L.p0_kv_step_args(_kv(a["kv"]), handle(a["ref"]["buf"]), handle(to["table"]["buf"]), handle(to["len"]["buf"]), handle(to["ref"]["buf"]),
+                             _b(a.get("parent")), _b(None if num else add), int(add or 0) if num else 0, int(a.get("window") or 0),
+                             int(a.get("sinks") or 0), handle(a["stat"]["buf"]))
+
+
+def _kv_compact_args(a):
+    to = a["to"]
+    return L.p0_kv_compact_args(_kv(a["kv"]), handle(a["ref"]["buf"]), handle(to["table"]["buf"]), handle(to["ref"]["buf"]), handle(a["stat"]["buf"]))
+
+
+def _beam_args(a):
+    lg, eos = a["logits"], a.get("eos")
+    return L.p0_beam_args(handle(lg["buf"]), int(lg.get("off") or 0), int(lg.get("ld") or 0), handle(a["score"]["buf"]), _b(a.get("fin")),
+                          int(a["groups"]), int(a["beams"]), int(a["V"]), L.P0_KV_NONE if eos is None else int(eos), handle(a["parent"]["buf"]),
+                          handle(a["token"]["buf"]), handle(a["scoreOut"]["buf"]), _b(a.get("finOut")))
+
+
+def kv4Put(g, a):
+    """a = {kv, k, v: {buf, off, ld, ldh}, type ('f32' | 'f16'), n, T or cu: {buf, off}}: the n newest tokens' K and V rows
+    quantised into their pages. kv = {pool: {buf, off, stride}, pages, table: {buf, off, ld}, len: {buf, off}, rows, D,
+    nkv} is one layer's view of the cache (p0_kv in include/p0mm.h)."""
+    bound(kv4Put, g, a)()
+
+
+def kv4Get(g, a):
+    """a as kv4Put's, with k and v the rows to write: the values the newest tokens' codes stand for"""
+    bound(kv4Get, g, a)()
+
+
+def kv4Attn(g, a):
+    """a = {kv, q, out: {buf, off, ld, ldh}, type, nh, n, T or cu, window, sinks, scale}: attention of each sequence's
+    newest tokens over its pages (causal; window 0 = the whole context, else the last `window` keys and the first
+    `sinks`)"""
+    bound(kv4Attn, g, a)()
+
+
+def kvStep(g, a):
+    """a = {kv, ref, to: {table, len, ref}, parent (optional), add ({buf} or a number), window, sinks, stat}: forks,
+    reorders, frees, trims and extends the sequences' pages; the new state goes to `to`, stat = {pages missing, free}"""
+    bound(kvStep, g, a)()
+
+
+def kvCompact(g, a):
+    """a = {kv, ref, to: {table, ref}, stat}: the pages in use moved into the lowest ones; stat = {in use, moved}"""
+    bound(kvCompact, g, a)()
+
+
+def beamSelect(g, a):
+    """a = {logits: {buf, off, ld}, score, fin (optional), groups, beams, V, eos, parent, token, scoreOut, finOut
+    (optional)}: the best `beams` continuations of each group's beams; parent is what kvStep takes"""
+    bound(beamSelect, g, a)()
+
+
+_BOUND = {
+    kv4Put: ("p0_kv4_put", lambda a: _kv4_rows_args(a, "kv4Put")),
+    kv4Get: ("p0_kv4_get", lambda a: _kv4_rows_args(a, "kv4Get")),
+    kv4Attn: ("p0_kv4_attn", _kv4_attn_args),
+    kvStep: ("p0_kv_step", _kv_step_args),
+    kvCompact: ("p0_kv_compact", _kv_compact_args),
+    beamSelect: ("p0_beam_select", _beam_args),
+}
+
+
+def bound(op, g, a):
+    """the call op(g, a) with its arguments converted once: a function without arguments that makes it (and checks it)
+    again each time. For loops whose buffers stay and whose lengths live on the device; a's later changes are not seen."""
+    name, make = _BOUND[op]
+    entry, args = getattr(g._lib, name), make(a)
+    ref = ctypes.byref(args)
+
+    def call():
+        st = entry(g.ctx, ref)
+        if st:
+            g._check(st)
+    return call

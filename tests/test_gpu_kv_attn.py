@@ -1,0 +1,194 @@
+"""kv4Attn on the GPU against softmax attention in 64 bits over the same codes (tests/kv_ref.py): every element within the
+bound that kv_ref.attention_bound derives from the roundings of the kernel's arithmetic."""
+import numpy as np
+import pytest
+
+import p0pc0rn_b200 as p0
+
+from . import kv_ref as R
+from .test_gpu_kv import kv_args
+
+pytestmark = pytest.mark.gpu
+
+
+def run(g, c, q, counts, nh, type_, window=0, sinks=0, scale=0.0, lay=(0, 0, 0), out_lay=(0, 0, 0), bufs=None):
+    """out [n][nh][D] as the call wrote it; every other element of the output buffer must keep its fill"""
+    dt = np.float32 if type_ == "f32" else np.float16
+    n = sum(counts)
+    bufs, kv = kv_args(g, c, bufs)
+
+    def rows(x, lay):
+        ld, ldh, off = lay[0] or nh * c.D, lay[1] or c.D, lay[2]
+        at = off + np.arange(n)[:, None, None] * ld + np.arange(nh)[None, :, None] * ldh + np.arange(c.D)
+        buf = np.full(at.max() + 1, -77, dt)
+        if x is not None:
+            buf[at] = x
+        return buf, at, {"off": off, "ld": ld, "ldh": ldh}
+
+    (qb, _, qa), (ob, oi, oa) = rows(q, lay), rows(None, out_lay)
+    cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    new = {"n": n, "T": counts[0]} if len(set(counts)) == 1 else {"n": n, "cu": {"buf": g.upload(np.concatenate([[9], cu]).astype(np.uint32)), "off": 1}}
+    o = g.upload(ob)
+    p0.kv4Attn(g, {"kv": kv, "q": {"buf": g.upload(qb), **qa}, "out": {"buf": o, **oa}, "type": type_, "nh": nh, "window": window, "sinks": sinks,
+                   "scale": scale, **new})
+    g.done()
+    got = g.read(o, 0, ob.nbytes, dt)
+    keep = np.ones(ob.size, bool)
+    keep[oi] = False
+    assert np.all(got[keep] == -77)
+    return got[oi]
+
+
+def check(got, c, q, counts, nh, type_, window=0, sinks=0, scale=1.0):
+    want, spread, size = R.attention(c, q, counts, nh, window, sinks, scale)
+    tol = R.attention_bound(spread, size, want, c.D, int(c.table.shape[1]), type_ == "f16")
+    err = np.abs(got.astype(np.float64) - want)
+    assert np.all(err <= tol), (float((err / tol).max()), np.unravel_index((err / tol).argmax(), err.shape))
+    seen = spread.any(-1)
+    assert not got[~seen].any()                                      # rows that see nothing are zeros
+    return want
+
+
+CASES = [
+    # lens, new tokens, nh, nkv, D, window, sinks
+    ([1], [1], 8, 1, 256, 0, 0),
+    ([63, 64, 65, 0, 1000], [1] * 5, 8, 2, 128, 0, 0),               # page borders; an empty sequence
+    ([700, 3, 129], [1] * 3, 6, 2, 64, 100, 4),                      # window and sinks, three heads a group
+    ([900], [1], 4, 4, 512, 64, 70),                                 # sinks over two pages; no shared heads
+    ([600, 128], [1] * 2, 3, 1, 256, 1, 0),                          # a window of one key
+    ([500, 40], [5, 5], 8, 2, 256, 0, 0),
+    ([300, 8, 5], [8, 8, 8], 8, 1, 128, 40, 2),                      # the last sequence is shorter than its tokens: rows that see nothing
+    ([200, 90, 64], [33, 7, 64], 4, 2, 64, 0, 0),                    # ragged
+    ([130, 260], [130, 1], 2, 1, 512, 50, 3),
+    ([64 * 5], [3], 16, 1, 256, 0, 0),
+    ([2000] + [1] * 20, [1] * 21, 2, 2, 64, 0, 0),                   # one long, many short
+]
+
+
+@pytest.mark.parametrize("type_", ["f32", "f16"])
+@pytest.mark.parametrize("lens,counts,nh,nkv,D,window,sinks", CASES)
+def test_attn(g, lens, counts, nh, nkv, D, window, sinks, type_):
+    rng = np.random.default_rng(D + len(lens))
+    c = R.Cache(rng, lens, nkv, D)
+    c.fill_fast(rng)
+    q = (rng.standard_normal((sum(counts), nh, D)) * (3.0 / D ** 0.5)).astype(np.float32 if type_ == "f32" else np.float16)
+    got = run(g, c, q, counts, nh, type_, window, sinks)
+    check(got, c, q, counts, nh, type_, window, sinks)
+
+
+@pytest.mark.parametrize("type_,lay,out_lay", [("f32", (0, 0, 3), (901, 129, 1)), ("f16", (1153, 131, 7), (0, 0, 0)), ("f16", (128, 128 * 21, 0), (128, 128 * 21, 8))])
+def test_attn_strides_layers_scale(g, type_, lay, out_lay):
+    # odd offsets and strides, head-major rows, the last layer of a page, a scale; the other layers hold NaN
+    rng = np.random.default_rng(8)
+    lens, counts, nh, nkv, D = [150, 400, 77], [7, 7, 7], 4, 2, 128
+    part = nkv * 2 * D // 32 * 1280
+    c = R.Cache(rng, lens, nkv, D, stride=3 * part, off=2 * part)
+    c.pool[:] = 0xFF
+    c.fill_fast(rng)
+    q = rng.standard_normal((21, nh, D)).astype(np.float32 if type_ == "f32" else np.float16)
+    got = run(g, c, q, counts, nh, type_, scale=0.11, lay=lay, out_lay=out_lay)
+    check(got, c, q, counts, nh, type_, scale=float(np.float32(0.11)))
+
+
+@pytest.mark.parametrize("type_", ["f32", "f16"])
+@pytest.mark.parametrize("T,window,sinks", [(1, 0, 0), (1, 70, 5), (6, 70, 5), (90, 70, 66)])
+def test_attn_ignores_what_nobody_sees(g, type_, T, window, sinks):
+    # NaN scales and infinite minima in every slot outside what some row of the call sees, and pages that are not there
+    rng = np.random.default_rng(9)
+    lens, nh, nkv, D = [333, 200], 4, 1, 128
+    c = R.Cache(rng, lens, nkv, D)
+    c.fill_fast(rng)
+    for b, n in enumerate(lens):
+        seen = set()
+        for i in range(T):
+            seen |= set(np.nonzero(R.visible(n - T + i, n, window, sinks))[0].tolist())
+        c.poison_unseen(b, seen)
+    c.table[0, -1] = c.pages + 9
+    q = (rng.standard_normal((2 * T, nh, D)) * 0.3).astype(np.float32 if type_ == "f32" else np.float16)
+    check(run(g, c, q, [T, T], nh, type_, window, sinks), c, q, [T, T], nh, type_, window, sinks)
+
+
+@pytest.mark.parametrize("type_,T", [("f32", 1), ("f16", 3), ("f16", 100)])
+def test_attn_missing_pages(g, type_, T):
+    # a page that was given back, one beyond the pool, and a sequence without any: their keys are not there
+    rng = np.random.default_rng(10)
+    lens, nh, nkv, D = [400, 300, 130], 2, 1, 64
+    c = R.Cache(rng, lens, nkv, D)
+    c.fill_fast(rng)
+    c.table[0, 2], c.table[1, 0], c.table[2, :] = R.NONE, c.pages, R.NONE
+    q = rng.standard_normal((3 * T, nh, D)).astype(np.float32 if type_ == "f32" else np.float16) * np.float16(0.4)
+    check(run(g, c, q, [T] * 3, nh, type_), c, q, [T] * 3, nh, type_)
+
+
+def test_attn_long_table_offsets(g):
+    # a length beyond the table counts as the table's; pool offsets past 32 bits: pages 400 MB apart
+    rng = np.random.default_rng(11)
+    c = R.Cache(rng, [64 * 15], 1, 64, spare=0, ld=15)
+    c.fill_fast(rng)
+    q = rng.standard_normal((1, 2, 64)).astype(np.float32)
+    stride = 400 << 20
+    pool = g.buffer((c.pages - 1) * stride + c.stride, "pool")
+    for p in range(c.pages):
+        g.write(pool, c.pool[p], p * stride)
+    lens = np.array([1 << 31], np.uint32)
+    bufs = {"pool": pool, "table": g.upload(c.table), "len": g.upload(lens)}
+    _, kv = kv_args(g, c, bufs)
+    kv["pool"]["stride"] = stride
+    o = g.buffer(2 * 64 * 4)
+    p0.kv4Attn(g, {"kv": kv, "q": {"buf": g.upload(q)}, "out": {"buf": o}, "type": "f32", "nh": 2, "n": 1, "T": 1})
+    got = g.read(o, 0, 512, np.float32).reshape(1, 2, 64)
+    check(got, c, q, [1], 2, "f32")
+    g.free(pool)
+
+
+def test_attn_same_bits_and_other_stream(g):
+    # the same call gives the same bits, and so does it on another stream of the caller's
+    import torch
+    rng = np.random.default_rng(12)
+    lens, nh, D = [3000, 10, 700], 8, 256
+    c = R.Cache(rng, lens, 1, D)
+    c.fill_fast(rng)
+    q = (rng.standard_normal((3, nh, D)) * 0.2).astype(np.float32)
+    first = run(g, c, q, [1] * 3, nh, "f32")
+    for _ in range(3):
+        assert np.array_equal(run(g, c, q, [1] * 3, nh, "f32").view(np.uint32), first.view(np.uint32))
+    s = torch.cuda.Stream()
+    g.done()
+    g.set_stream(s.cuda_stream)
+    try:
+        assert np.array_equal(run(g, c, q, [1] * 3, nh, "f32").view(np.uint32), first.view(np.uint32))
+    finally:
+        g.done()
+        g.set_stream(0)
+
+
+def test_attn_cu_out_of_order(g):
+    # a cu that decreases or passes n gives no tokens out of range: rows of no sequence keep what they held
+    rng = np.random.default_rng(13)
+    c = R.Cache(rng, [100, 50, 70], 1, 64)
+    c.fill_fast(rng)
+    q = rng.standard_normal((10, 2, 64)).astype(np.float32) * 0.4
+    bufs, kv = kv_args(g, c)
+    o = g.upload(np.full(10 * 128, -77, np.float32))
+    p0.kv4Attn(g, {"kv": kv, "q": {"buf": g.upload(q)}, "out": {"buf": o}, "type": "f32", "nh": 2, "n": 10,
+                   "cu": {"buf": g.upload(np.array([4, 2, 4000000000, 4000000000], np.uint32))}})
+    got = g.read(o, 0, 10 * 512, np.float32).reshape(10, 2, 64)
+    assert np.all(got[:2] == -77)
+    c2 = R.Cache(rng, [50], 1, 64)
+    c2.table, c2.pool, c2.pages, c2.ld = c.table[1:2], c.pool, c.pages, c.ld
+    check(got[2:], c2, q[2:], [8], 2, "f32")                         # sequence 1 has tokens 2 .. 9, the others none
+
+
+def test_attn_refusals(g):
+    rng = np.random.default_rng(14)
+    c = R.Cache(rng, [100, 70], 2, 64)
+    _, kv = kv_args(g, c)
+    x = g.buffer(2 * 4 * 64 * 4)
+    a = {"kv": kv, "q": {"buf": x}, "out": {"buf": x}, "type": "f32", "nh": 4, "n": 2, "T": 1}
+    for msg, change in (("3 query heads over 2 KV heads", {"nh": 3}), ("0 query heads", {"nh": 0}), ("D 32 must be", {"kv": {**kv, "D": 32}}),
+                        ("q range", {"q": {"buf": x, "off": 1}}), ("out range", {"out": {"buf": x, "ld": 257}}), ("type bf16", {"type": "bf16"}),
+                        ("cu range", {"cu": {"buf": g.buffer(4), "off": 2}}), ("n 4 is not", {"n": 4}), ("1025 sequences", {"kv": {**kv, "rows": 1025}})):
+        with pytest.raises(p0.P0Error, match=msg):
+            p0.kv4Attn(g, {**a, **change})
+    p0.kv4Attn(g, {**a, "n": 0})                                     # no tokens: nothing to do
+    g.done()
