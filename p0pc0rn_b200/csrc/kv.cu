@@ -10,7 +10,7 @@
 p0_status kv_view(p0_ctx *c, const p0_kv &kv, bool layer, const char *op, KvView *v) {
   if (!kv.rows || kv.rows > kKvMaxRows) return p0_fail(c, P0_EINVAL, "%s: %u sequences (1 to %u)", op, kv.rows, kKvMaxRows);
   if (!kv.pages || kv.pages > 0x7fffffffu) return p0_fail(c, P0_EINVAL, "%s: %u pages", op, kv.pages);
-  if (!kv.table_ld || kv.table_ld > (1u << 25)) return p0_fail(c, P0_EINVAL, "%s: table rows of %u pages (1 to 2^25)", op, kv.table_ld);
+  if (!kv.table_ld || kv.table_ld > (1u << 23)) return p0_fail(c, P0_EINVAL, "%s: table rows of %u pages (1 to 2^23)", op, kv.table_ld);
   uint64_t part = 0, need = kv.page_stride;
   if (layer) {
     if (kv.D != 64 && kv.D != 128 && kv.D != 256 && kv.D != 512) return p0_fail(c, P0_EINVAL, "%s: D %u must be 64, 128, 256 or 512", op, kv.D);
@@ -34,6 +34,7 @@ p0_status kv_view(p0_ctx *c, const p0_kv &kv, bool layer, const char *op, KvView
 }
 
 p0_status kv_new_tokens(p0_ctx *c, uint32_t n, uint32_t T, p0_buf cu, uint32_t cu_off, const char *op, KvView *v) {
+  if (n > (1u << 28)) return p0_fail(c, P0_EINVAL, "%s: %u tokens in one call (at most 2^28)", op, n);   // positions stay well inside 32 bits
   v->n = n;
   v->T = T;
   if (cu.id) {

@@ -5,11 +5,10 @@
 //   o_i = sum_j p_ij v_j,  p_i = softmax over the visible j of scale * (q_i . k_j),  k, v = f16(q * s + mn)
 //   visible: j <= pos_i and (window = 0 or j > pos_i - window or j < sinks);  nothing visible: o_i = 0
 //
-// Work. The query rows that share a KV head (new tokens x query heads of its group) form row blocks; a unit is one row
-// block of one sequence and KV head, its items are the pages that any of its rows sees. The units' items, in order, are
-// cut into equal runs, one per CTA, from the lengths on the device: long and short sequences, windows and empty slots
-// fill the GPU alike. A unit that lies in one run is finished there; otherwise each run leaves (m, l, acc) in the
-// workspace and the combine kernel joins them in run order, so results do not depend on timing.
+// Work is cut as kv_attn.cuh says: the pages that row blocks see, in order, in equal runs, one per CTA, from the lengths on
+// the device: long and short sequences, windows and empty slots fill the GPU alike. A unit that lies in one run is
+// finished there; otherwise each run leaves (m, l, acc) in the workspace and the join kernel adds them in run order, so
+// results do not depend on timing.
 //
 // A page. One bulk copy brings a head's K and V records (D * 80 bytes); a ring of stages hides it. The codes become f16
 // pairs in registers (two codes per sub and fma on the half2 pipe) and go straight into mma.sync fragments: S = Q K^T
@@ -20,21 +19,9 @@
 // Precision. f32 queries and outputs: q and P are split into f16 high and low parts (about 22 bits) in rows r and r + 8
 // of the fragments; each page's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
 // f16 matrix operand), 16 rows per fragment.
-#include "kv.cuh"
-#include "launch.cuh"
-#include "tc.cuh"
+#include "kv_attn.cuh"
 
 namespace {
-
-struct AttnJob {
-  KvView v;
-  KvRows q, out;
-  uint32_t hpg, window, sinks;
-  float scale;
-  uint32_t *err;
-  float *part;        // [grid][2][rows of a block][D + 2]
-  uint4 *desc;        // [grid]: (1 + last run, b, first row, KV head) of the unit that this run begins and others end
-};
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -51,24 +38,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 __device__ __forceinline__ uint32_t lds_u32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
-
-// what a unit's rows see: pages [0, sink_pages) and [from, last], or nothing (n = 0)
-struct Span {
-  uint32_t sink_pages, from, n;
-  uint32_t first_pos, end;   // first key inside the first row's window; one past the last row's position
-};
-__device__ __forceinline__ Span span_of(uint32_t len, uint32_t T, uint32_t t0, uint32_t t1, uint32_t window, uint32_t sinks) {
-  Span s;
-  // positions of rows t0 and t1 (0 <= t0 <= t1 < T): len - T + t, which may be negative
-  const int64_t p1 = (int64_t)len - T + t1, p0 = (int64_t)len - T + t0;
-  s.end = p1 < 0 ? 0u : (uint32_t)p1 + 1u;
-  s.first_pos = window && p0 - (int64_t)window + 1 > 0 ? (uint32_t)(p0 - (int64_t)window + 1) : 0u;
-  s.from = s.first_pos / kPage;
-  const uint32_t sp = (uint32_t)(((uint64_t)sinks + kPage - 1) / kPage);
-  s.sink_pages = sp < s.from ? sp : s.from;
-  s.n = s.end ? s.sink_pages + (s.end - 1) / kPage + 1 - s.from : 0u;
-  return s;
-}
 
 template <int D, bool F32, int NW, int RT>
 struct Cfg {
@@ -100,72 +69,30 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
   __shared__ float wmax[NW][RB], wsum[NW][RB];
   __shared__ int32_t rpos[RB];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g4 = lane >> 2, t4 = lane & 3u;
-  const uint32_t hpg = j.hpg, nkv = j.v.nkv, R = j.v.rows, W = j.window, S = j.sinks;
+  const uint32_t hpg = j.hpg, R = j.v.rows, W = j.window, S = j.sinks;
   if (tid == 0) {
     for (int i = 0; i < NS; i++) tc::mbar_init(&full[i], 1);
     abort_flag = 0u;
     tc::fence_mbar_init();
   }
-  // items per sequence: over its row blocks, max(1, pages seen) per KV head (an empty unit is one item: it writes zeros)
-  for (uint32_t b = tid; b < R; b += C::kThreads) {
-    uint32_t lo, T = kv_tokens(j.v, b, lo), items = 0;
-    const uint32_t len = kv_len(j.v, b);
-    for (uint32_t r = 0; r < T * hpg; r += RB) {
-      const Span s = span_of(len, T, r / hpg, min(T * hpg - 1, r + RB - 1) / hpg, W, S);
-      items += max(1u, s.n);
-    }
-    pre[b + 1] = items * nkv;
-  }
-  if (tid == 0) pre[0] = 0u;
-  __syncthreads();
-  if (warp == 0) {   // inclusive sums
-    uint32_t carry = 0;
-    for (uint32_t b0 = 0; b0 < R; b0 += 32) {
-      uint32_t v = b0 + lane < R ? pre[b0 + lane + 1] : 0u;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= (uint32_t)o) v += u;
-      }
-      if (b0 + lane < R) pre[b0 + lane + 1] = v + carry;
-      carry += __shfl_sync(0xffffffffu, v, 31);
-    }
-  }
-  __syncthreads();
+  plan_items<RB, 1, 0>(j, pre);
   const uint32_t total = pre[R], G = min(gridDim.x, max(total, 1u));   // no run is empty
   if (tid == 0) j.desc[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
   if (blockIdx.x >= G) return;
   const uint32_t lo = (uint32_t)((uint64_t)total * blockIdx.x / G), hi = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / G);
-  uint32_t b = 0;
-  {
-    uint32_t a = 0, e = R;   // the last b with pre[b] <= lo and items of its own
-    while (e - a > 1) {
-      const uint32_t m = (a + e) >> 1;
-      if (pre[m] <= lo) a = m; else e = m;
-    }
-    b = a;
-  }
+  uint32_t b = find_sequence(pre, R, lo);
   uint32_t at = lo, it = 0;   // item; pages through the ring so far
   while (at < hi) {
     while (pre[b + 1] <= at) b++;
-    uint32_t first, T = kv_tokens(j.v, b, first);
-    const uint32_t len = kv_len(j.v, b), rows = T * hpg;
-    // the unit of item `at`: row blocks in order, each with its KV heads in order
-    uint32_t base = pre[b], r0 = 0, n;
-    Span s;
-    for (;; r0 += RB) {
-      s = span_of(len, T, r0 / hpg, min(rows - 1, r0 + RB - 1) / hpg, W, S);
-      n = max(1u, s.n);
-      if (at < base + n * nkv) break;
-      base += n * nkv;
-    }
-    const uint32_t head = (at - base) / n, begin = base + head * n, from = at - begin, to = min(hi - begin, n);
+    const Unit u = find_unit<RB, 1, 0>(j, pre, b, at);
+    const Span &s = u.s;
+    const uint32_t first = u.first, T = u.T, len = u.len, rows = u.rows, r0 = u.r0, head = u.head, begin = u.begin, n = u.n;
+    const uint32_t from = at - begin, to = min(hi - begin, n);
     const uint32_t nrow = min((uint32_t)RB, rows - r0);
     const uint32_t steps = s.n ? to - from : 0u;
     const uint8_t *heads = j.v.pool + (uint64_t)head * 2u * C::kPart;
-    const auto page_of = [&](uint32_t i) { return i < s.sink_pages ? i : s.from + (i - s.sink_pages); };
     const auto issue = [&](uint32_t i) {   // item from + i of the unit into its ring slot
-      const uint32_t st = (it + i) % NS, p = j.v.table[(uint64_t)b * j.v.ld + page_of(from + i)];
+      const uint32_t st = (it + i) % NS, p = j.v.table[(uint64_t)b * j.v.ld + page_at(s, from + i)];
       page_ok[st] = p < j.v.pages;
       if (p < j.v.pages) {
         tc::mbar_expect_tx(&full[st], 2u * C::kPart);
@@ -177,7 +104,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
     if (tid == 0)
       for (uint32_t i = 0; i < (uint32_t)NS && i < steps; i++) issue(i);
     // the rows' positions and q fragments
-    if (tid < (uint32_t)RB) rpos[tid] = tid < nrow ? (int32_t)((int64_t)len - T + (r0 + tid) / hpg) : -1;
+    if (tid < (uint32_t)RB) rpos[tid] = tid < nrow ? (int32_t)(len - T + (r0 + tid) / hpg) : -1;
     for (uint32_t e = tid; e < RT * (D / 16) * 32u; e += C::kThreads) {
       const uint32_t ln = e & 31u, step = (e >> 5) % (D / 16), rt = (e >> 5) / (D / 16);
       const uint32_t d0 = (step >> 1) * 32u + (ln & 3u) * 8u + (step & 1u) * 2u;   // the lane's word; codes d0, +4, +1, +5
@@ -230,7 +157,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
     }
     bool lost = false;
     for (uint32_t i = 0; i < steps; i++) {
-      const uint32_t st = (it + i) % NS, page = page_of(from + i), key0 = page * kPage;
+      const uint32_t st = (it + i) % NS, page = page_at(s, from + i), key0 = page * kPage;
       if (!tc::mbar_wait(&full[st], ((it + i) / NS) & 1u, &abort_flag, j.err, 0x4a1u, P0_SPIN_LIMIT)) lost = true;
       const uint8_t *kp = ring + st * 2u * C::kPart, *vp = kp + C::kPart;
       // ---- S = Q K^T: this warp's 8-key tiles
@@ -275,7 +202,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               const int32_t key = (int32_t)(key0 + (warp * NT + nt) * 8u + 2u * t4 + e);
-              const bool see = ok && key <= pos[rt][h] && (!W || (int64_t)key > (int64_t)pos[rt][h] - W || (uint32_t)key < S);
+              const bool see = ok && key <= pos[rt][h] && (!W || key > pos[rt][h] - (int32_t)W || (uint32_t)key < S);
               const float v = F32 ? sc[rt][nt][e] + sc[rt][nt][e + 2] : sc[rt][nt][2 * h + e];
               x[rt][nt][h][e] = see ? v * j.scale : -INFINITY;
               mx = fmaxf(mx, x[rt][nt][h][e]);
@@ -404,9 +331,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
     // a run has at most one part of a unit that began earlier (slot 0) and one of a unit that goes on after it (slot 1)
     float *part = j.part + ((uint64_t)blockIdx.x * 2u + (from ? 0u : 1u)) * RB * (D + 2);
     if (!whole && from == 0 && tid == 0) {
-      // runs end where total * (c + 1) / G does: the last one of this unit holds item begin + n - 1
-      const uint32_t c = (uint32_t)((((uint64_t)begin + n) * G - 1) / total);
-      j.desc[blockIdx.x] = make_uint4(1u + c, b, r0, head);
+      j.desc[blockIdx.x] = make_uint4(1u + run_of(begin + n - 1u, total, G), b, r0, head);
     }
 #pragma unroll
     for (int rt = 0; rt < RT; rt++)
@@ -552,8 +477,9 @@ extern "C" p0_status p0_kv4_attn(p0_ctx *c, const p0_kv4_attn_args *a) {
   if ((st = kv_rows(c, a->q, a->n, a->nh, a->kv.D, a->type, op, "q", &j.q))) return st;
   if ((st = kv_rows(c, a->out, a->n, a->nh, a->kv.D, a->type, op, "out", &j.out))) return st;
   j.hpg = a->nh / a->kv.nkv;
-  j.window = a->window;
-  j.sinks = a->sinks;
+  const uint32_t most = a->kv.table_ld * kPage;          // no position is that large, so positions and bounds fit 31 bits
+  j.window = a->window < most ? a->window : 0u;          // a longer window hides nothing
+  j.sinks = a->sinks < most ? a->sinks : most;
   j.scale = a->scale != 0.0f ? a->scale : 1.0f;
   j.err = c->d_err;
   // the kernels count query rows and items (pages of row blocks) in 32 bits
@@ -562,6 +488,10 @@ extern "C" p0_status p0_kv4_attn(p0_ctx *c, const p0_kv4_attn_args *a) {
     return p0_fail(c, P0_EINVAL, "%s: %u tokens x %u heads over %u pages pass 32 bits", op, a->n, a->nh, a->kv.table_ld);
   cudaSetDevice(c->device);
   const bool f32 = a->type == P0_F32;
+  if (!f32) {
+    bool taken = false;
+    if ((st = kv4_attn_prompt(c, j, &taken)) || taken) return st;
+  }
   switch (a->kv.D) {
     case 64: return f32 ? attn_launch<64, true, 4, 1>(c, j) : attn_launch<64, false, 4, 1>(c, j);
     case 128: return f32 ? attn_launch<128, true, 4, 1>(c, j) : attn_launch<128, false, 4, 1>(c, j);

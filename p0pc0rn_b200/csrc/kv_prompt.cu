@@ -1,0 +1,617 @@
+// kv_prompt.cu -- kv4Attn for prompts: f16 queries with many rows per KV head, on the tensor cores.
+//
+// Two kernels. The first turns the pages that the call sees into f16 once (each serves every row block of its sequence),
+// as the tiles that the matrix instructions read: K as [64 keys][64 dims] blocks, V transposed as [D dims][64 keys], both
+// rows of 128 bytes in the 128-byte swizzle, so that plain bulk copies bring them to shared memory. Slots that no row of
+// the call sees become zeros.
+// The second is attention over tiles of 128 keys (two pages) for 256 query rows (of one KV head: tokens x its query heads)
+// by a pair of CTAs, each with 128 of the rows. The pair's MMAs (cta_group::2) read half of K and V from either CTA's
+// shared memory: a CTA loads one of the two pages of K and half of V's dims, half the bytes out of L2 that a CTA on its
+// own would need for the same rows, and the ring holds two tiles of D = 256. In each CTA one warp issues the bulk copies,
+// one the pair's MMAs (the odd CTA's tells the even one's what has landed), eight hold half a row (64 keys) per thread:
+//   S_j = Q K_j^T     tcgen05.mma, 256 x 128 x D, f32 in tensor memory: S_j+1 runs while softmax_j computes, as soon as it has
+//                     read S_j (D = 256: one buffer) or S_j-1 (two)
+//   P_j = 2^(S_j c - m)   the row's maximum by its two threads through shared memory; f16 in tensor memory, two buffers
+//   O  += P_j V_j     tcgen05.mma with P from tensor memory
+// Nothing in tensor memory is written while an MMA that was not waited for may read it (MMAs of different shapes or
+// accumulators have no order among themselves).
+// m is the row's maximum as of the last time O was rescaled: P may grow to 2^8 (harmless in f16 and f32) before O, in
+// tensor memory, is read and written again, which then happens in few tiles.
+// Work is cut into equal runs of key tiles as in kv_attn.cuh, one per pair; a unit's parts meet in the join kernel.
+#include "kv_attn.cuh"
+
+namespace {
+
+constexpr uint32_t kRB = 256, kCR = 128, kPP = 2;   // query rows of a block and of a CTA, pages of a key tile
+constexpr uint32_t kE = 4;                   // a unit's beginning and end cost about as much as four key tiles
+constexpr int kSoft = 256, kThreads = kSoft + 64;   // warps 0-7: softmax (0-3 the tile's first page, 4-7 its second); 8: copies; 9: MMAs
+
+template <int D>
+struct Cfg {
+  static constexpr uint32_t kKB = D / 64;                      // 64-dim blocks of K
+  static constexpr uint32_t kStage = D * 128;                  // of the ring: a page of K, or half of V's dims of two pages
+  static constexpr uint32_t kQ = kKB * 16384;
+  static constexpr int kStages = D == 256 ? 4 : 8;
+  static constexpr uint32_t kSlot = D * 256;                   // a page of one head in f16: K blocks, then V
+  static constexpr uint32_t kOut = 32 * 80;                    // a warp's 32 x 32 f16 of the output, rows padded to 80 bytes
+  // tensor memory: O at 0, then P and S, 64 and 128 columns a buffer
+  static constexpr uint32_t kSB = D == 256 ? 1 : 2, kColS = 256, kColP = D == 256 ? 384 : 128;
+  static constexpr uint32_t kSmem = 1024 + kQ + kStages * kStage + 8 * kOut;
+};
+
+// The pages of sequence b that the call sees, in order: those of the span over all its tokens. exo[b] = pages before it.
+__device__ __forceinline__ Span whole_span(const AttnJob &j, uint32_t b) {
+  uint32_t lo;
+  const uint32_t T = kv_tokens(j.v, b, lo);
+  return T ? span_of(kv_len(j.v, b), T, 0, T - 1, j.window, j.sinks) : span_of(0, 1, 0, 0, 0, 0);
+}
+__device__ __forceinline__ void plan_pages(const AttnJob &j, uint32_t *exo) {
+  for (uint32_t b = threadIdx.x; b < j.v.rows; b += blockDim.x) exo[b + 1] = whole_span(j, b).n;
+  if (threadIdx.x == 0) exo[0] = 0u;
+  __syncthreads();
+  if (threadIdx.x < 32) warp_sums(exo + 1, j.v.rows);
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------- pages to f16 tiles
+constexpr int kET = 256;
+template <int D>
+__global__ void __launch_bounds__(kET) kv4_widen_kernel(AttnJob j) {
+  dep_enter();
+  extern __shared__ uint32_t exo[];
+  plan_pages(j, exo);
+  const uint32_t total = exo[j.v.rows], nkv = j.v.nkv;
+  constexpr uint32_t part = D / 32 * 1280;
+  uint32_t b = 0;
+  for (uint64_t w2 = blockIdx.x; w2 < (uint64_t)total * nkv * 2u; w2 += gridDim.x) {   // K, or V, of a page and head
+    const uint64_t w = w2 >> 1;
+    const uint32_t i = (uint32_t)(w / nkv), head = (uint32_t)(w % nkv);
+    while (exo[b + 1] <= i) b++;
+    const Span s = whole_span(j, b);
+    const uint32_t jp = page_at(s, i - exo[b]), page = j.v.table[(uint64_t)b * j.v.ld + jp], key0 = jp * kPage;
+    const bool ok = page < j.v.pages;
+    const uint8_t *rec = j.v.pool + (ok ? page : 0u) * j.v.stride + (uint64_t)head * 2u * part + (w2 & 1u) * part;
+    uint8_t *to = j.wide + w * Cfg<D>::kSlot + (w2 & 1u) * (D * 128);
+    const auto there = [&](uint32_t k) { return ok && key0 + k < s.end && (key0 + k >= s.first_pos || key0 + k < j.sinks); };
+    if (!(w2 & 1u)) {
+      // K: a thread turns one word (8 dims of a key) into 16 bytes; 8 lanes make a key's 128-byte row of a block
+      constexpr uint32_t U = 64u * (D / 8) / kET;
+      uint32_t x[U], sm[U];
+#pragma unroll
+      for (uint32_t n = 0; n < U; n++) {
+        const uint32_t e = n * kET + threadIdx.x, c = e & 7u, key = (e >> 3) & 63u, g = (e >> 9) * 2u + (c >> 2);
+        x[n] = *reinterpret_cast<const uint32_t *>(rec + g * 1280u + key * 16u + (c & 3u) * 4u);
+        sm[n] = *reinterpret_cast<const uint32_t *>(rec + g * 1280u + 1024u + key * 4u);
+      }
+#pragma unroll
+      for (uint32_t n = 0; n < U; n++) {
+        const uint32_t e = n * kET + threadIdx.x, c = e & 7u, key = (e >> 3) & 63u, blk = e >> 9;
+        uint4 o = make_uint4(0u, 0u, 0u, 0u);
+        if (there(key)) {
+          const uint32_t s2 = __byte_perm(sm[n], 0, 0x1010), mn2 = __byte_perm(sm[n], 0, 0x3232), y = x[n] >> 4;
+          o.x = kv_deq2(__byte_perm(x[n], y, 0x4400) & 0x000F000Fu, s2, mn2);   // byte i: dims 2i, 2i + 1
+          o.y = kv_deq2(__byte_perm(x[n], y, 0x5511) & 0x000F000Fu, s2, mn2);
+          o.z = kv_deq2(__byte_perm(x[n], y, 0x6622) & 0x000F000Fu, s2, mn2);
+          o.w = kv_deq2(__byte_perm(x[n], y, 0x7733) & 0x000F000Fu, s2, mn2);
+        }
+        *reinterpret_cast<uint4 *>(to + blk * 8192u + key * 128u + ((c ^ (key & 7u)) * 16u)) = o;
+      }
+    } else {
+      // V: a thread turns the words of 8 keys (the same 8 dims) into 8 dims' 16-byte runs of 8 keys
+      for (uint32_t e = threadIdx.x; e < 8u * (D / 8); e += kET) {
+        const uint32_t kc = e & 7u, dw = e >> 3;
+        const uint8_t *g = rec + (dw >> 2) * 1280u;
+        uint32_t x[8], o[8][4];
+        uint2 sm[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) x[k] = *reinterpret_cast<const uint32_t *>(g + (kc * 8u + k) * 16u + (dw & 3u) * 4u);
+#pragma unroll
+        for (uint32_t p = 0; p < 4; p++) sm[p] = *reinterpret_cast<const uint2 *>(g + 1024u + (kc * 8u + 2u * p) * 4u);
+#pragma unroll
+        for (uint32_t p = 0; p < 4; p++) {
+          const uint32_t key = kc * 8u + 2u * p;
+          if (!there(key)) sm[p].x = 0u;
+          if (!there(key + 1)) sm[p].y = 0u;
+          const uint32_t s2 = __byte_perm(sm[p].x, sm[p].y, 0x5410), mn2 = __byte_perm(sm[p].x, sm[p].y, 0x7632);
+          const uint32_t lo = __byte_perm(x[2 * p], x[2 * p + 1], 0x5410), hi = __byte_perm(x[2 * p], x[2 * p + 1], 0x7632);
+#pragma unroll
+          for (uint32_t d = 0; d < 4; d++) {
+            o[d][p] = kv_deq2((lo >> (4 * d)) & 0x000F000Fu, s2, mn2);
+            o[d + 4][p] = kv_deq2((hi >> (4 * d)) & 0x000F000Fu, s2, mn2);
+          }
+        }
+#pragma unroll
+        for (uint32_t d = 0; d < 8; d++)
+          *reinterpret_cast<uint4 *>(to + (dw * 8u + d) * 128u + ((kc ^ d) * 16u)) = make_uint4(o[d][0], o[d][1], o[d][2], o[d][3]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- attention
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    uint32_t t[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) t[i] = r[16 * h + i];
+    tc::tmem_st16(taddr + 16u * h, t);
+  }
+}
+
+template <int D>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnJob j) {
+  dep_enter();
+  using C = Cfg<D>;
+  constexpr int NS = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *qs = smem, *ring = smem + C::kQ, *stg = ring + NS * C::kStage;
+  uint32_t *pre = reinterpret_cast<uint32_t *>(smem_raw + C::kSmem), *exo = pre + j.v.rows + 1;
+  // full / empty: the ring; other: the odd CTA's stage has landed; sfull: S of a tile is there, sread: both CTAs have read it;
+  // pfull: both CTAs' P is there; odone: P V of a tile is done (each by buffer)
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], other[NS], sfull[2], sread[2], pfull[2], odone[2], mdone;
+  __shared__ uint32_t tmem_slot, abort_word;
+  __shared__ float mx2[2][2][kCR], l2[2][kCR];   // [tile parity][half of the tile][row]
+  __shared__ uint64_t qrow[kCR], orow[kCR];      // the rows' places in q and out
+  volatile uint32_t *abort_flag = &abort_word;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = tc::cluster_rank(), run = blockIdx.x >> 1;
+  const uint32_t hpg = j.hpg, nkv = j.v.nkv, R = j.v.rows, W = j.window, S = j.sinks;
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+      tc::mbar_init(&other[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      tc::mbar_init(&sfull[i], 1);
+      tc::mbar_init(&sread[i], 2 * kSoft / 32);
+      tc::mbar_init(&pfull[i], 2 * kSoft / 32);
+      tc::mbar_init(&odone[i], 1);
+    }
+    tc::mbar_init(&mdone, 1);
+    abort_word = 0u;
+    tc::fence_mbar_init();
+  }
+  if (warp == 8) {
+    tc::tmem_alloc_pair(&tmem_slot, 512);
+    tc::tmem_relinquish_pair();
+  }
+  plan_pages(j, exo);
+  plan_items<kRB, kPP, kE>(j, pre);
+  tc::fence_before();
+  tc::cluster_sync();
+  tc::fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t total = pre[R], runs = gridDim.x >> 1, G = min(runs, max(total, 1u));
+  if (tid == 0 && rank == 0) j.desc[run] = make_uint4(0u, 0u, 0u, 0u);
+  const uint32_t lo = run < G ? (uint32_t)((uint64_t)total * run / G) : 0u, hi = run < G ? (uint32_t)((uint64_t)total * (run + 1) / G) : 0u;
+  uint32_t b = lo < hi ? find_sequence(pre, R, lo) : 0u;
+  uint32_t st = 0, tile = 0;   // ring stages and key tiles so far (each role counts its own uses alike)
+  const float c = fabsf(j.scale) * 1.44269504088896340736f;
+  const uint32_t flip = j.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale turns q around, so that maxima stay maxima
+  // A wait that gives up sets the CTA's abort word, after which all its waits give up at once; every warp still walks the
+  // same units and barriers to the end
+  for (uint32_t at = lo; at < hi;) {
+    while (pre[b + 1] <= at) b++;
+    const Unit u = find_unit<kRB, kPP, kE>(j, pre, b, at);
+    const Span &s = u.s;
+    const uint32_t from = max(at - u.begin, kE) - kE, nt = u.n - kE, end = min(hi - u.begin, u.n), to = max(end, kE) - kE;
+    at = u.begin + end;
+    if (from == to) continue;   // this run holds none of the unit's tiles
+    const uint32_t tiles = s.n ? to - from : 0u;
+    const uint32_t rc = u.r0 + rank * kCR, nrow = rc < u.rows ? min(kCR, u.rows - rc) : 0u;   // this CTA's rows
+    if (warp == 8) {
+      // ------------------------------------------------------------ copies
+      const Span all = whole_span(j, b);
+      const uint8_t *base = j.wide + ((uint64_t)exo[b] * nkv + u.head) * C::kSlot;
+      const auto slot = [&](uint32_t i) {   // page i of the unit's span (an odd last tile repeats its first page)
+        const uint32_t jp = page_at(s, min(i, s.n - 1u)), k = jp < all.sink_pages ? jp : all.sink_pages + (jp - all.from);
+        return base + (uint64_t)k * nkv * C::kSlot;
+      };
+      const auto stage = [&]() -> uint8_t * {
+        if (!tc::mbar_wait(&empty[st % NS], ((st / NS) & 1u) ^ 1u, abort_flag, j.err, 0x4b1u, P0_SPIN_LIMIT)) return nullptr;
+        tc::mbar_expect_tx(&full[st % NS], C::kStage);
+        return ring + (st % NS) * C::kStage;
+      };
+      const auto load_k = [&](uint32_t i) {
+        uint8_t *d = stage();
+        if (!d) return false;
+        bulk_load(d, slot(2u * i + rank), C::kStage, &full[st % NS]);
+        st++;
+        return true;
+      };
+      const auto load_v = [&](uint32_t i) {
+        uint8_t *d = stage();
+        if (!d) return false;
+        for (uint32_t h = 0; h < 2; h++)
+          bulk_load(d + h * (C::kStage / 2), slot(2u * i + h) + D * 128 + rank * (C::kStage / 2), C::kStage / 2, &full[st % NS]);
+        st++;
+        return true;
+      };
+      bool ok = true;
+      if (lane == 0 && tiles) ok = load_k(from);   // ahead of the barrier: under the previous unit's end
+      __syncwarp();
+      tc::cluster_sync();
+      if (lane == 0 && ok)
+        for (uint32_t i = 0; i < tiles; i++) {
+          if (i + 1 < tiles && !load_k(from + i + 1)) break;
+          if (!load_v(from + i)) break;
+        }
+      __syncwarp();
+    } else if (warp == 9) {
+      // ------------------------------------------------------------ the pair's MMAs (even CTA), word of what landed (odd CTA)
+      const auto tell = [&]() {
+        const bool ok = tc::mbar_wait(&full[st % NS], (st / NS) & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
+        if (ok) tc::mbar_arrive_rank(&other[st % NS], 0);
+        st++;
+        return ok;
+      };
+      bool told = tiles && rank == 1;
+      if (lane == 0 && told) told = tell();   // the first K, as it was issued, ahead of the barrier
+      __syncwarp();
+      tc::cluster_sync();
+      tc::fence_after();
+      if (lane == 0 && rank == 1) {
+        for (uint32_t i = 1; i < 2u * tiles && told; i++) told = tell();
+      } else if (lane == 0 && tiles) {
+        constexpr uint32_t is = tc::idesc_f16_f32(256, 128), iv = tc::idesc_f16_f32(256, D);
+        const auto arrived = [&]() {
+          const bool ok = tc::mbar_wait(&full[st % NS], (st / NS) & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT) &&
+                          tc::mbar_wait(&other[st % NS], (st / NS) & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
+          tc::fence_after();
+          return ok;
+        };
+        const auto scores = [&](uint32_t t) {
+          if (!arrived()) return false;
+          const uint32_t sb = t % C::kSB, dst = tmem + C::kColS + sb * 128u, ks = tc::smem_u32(ring + (st % NS) * C::kStage), q0 = tc::smem_u32(qs);
+#pragma unroll
+          for (uint32_t x = 0; x < C::kKB * 4u; x++)
+            tc::mma_ss_f16_pair(dst, tc::desc_sw128(q0 + (x >> 2) * 16384u + (x & 3u) * 32u), tc::desc_sw128(ks + (x >> 2) * 8192u + (x & 3u) * 32u), is, x != 0u);
+          tc::mma_commit_pair(&empty[st % NS]);
+          st++;
+          tc::mma_commit_pair(&sfull[sb]);
+          return true;
+        };
+        bool ok = scores(tile);
+        for (uint32_t i = 0; i < tiles && ok; i++) {
+          const uint32_t t = tile + i;
+          if (i + 1 < tiles) {   // over S of tile t + 1 - kSB (i + 1 >= kSB: of this unit, or read before its end)
+            const uint32_t o = t + 1u - C::kSB;
+            if (i + 1 >= C::kSB && !(ok = tc::mbar_wait(&sread[o % C::kSB], (o / C::kSB) & 1u, abort_flag, j.err, 0x4b9u, P0_SPIN_LIMIT))) break;
+            tc::fence_after();
+            if (!(ok = scores(t + 1))) break;
+          }
+          if (!(ok = tc::mbar_wait(&pfull[t & 1u], (t >> 1) & 1u, abort_flag, j.err, 0x4b4u, P0_SPIN_LIMIT))) break;
+          tc::fence_after();
+          if (!(ok = arrived())) break;
+          const uint32_t pa = tmem + C::kColP + (t & 1u) * 64u, vs = tc::smem_u32(ring + (st % NS) * C::kStage);
+#pragma unroll
+          for (uint32_t x = 0; x < 8u; x++)
+            tc::mma_ts_f16_pair(tmem, pa + x * 8u, tc::desc_sw128(vs + (x >> 2) * (C::kStage / 2) + (x & 3u) * 32u), iv, (i | x) != 0u);
+          tc::mma_commit_pair(&empty[st % NS]);
+          st++;
+          tc::mma_commit_pair(&odone[t & 1u]);
+        }
+      }
+      __syncwarp();
+    } else {
+      // ------------------------------------------------------------ q rows, swizzled (a warp reads a row at a time); zeros beyond
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");   // the previous unit's rows are written
+      if (tid < kCR) {
+        const uint32_t row = rc + tid, tok = row / hpg;
+        qrow[tid] = (uint64_t)(u.first + tok) * j.q.ld + (uint64_t)(u.head * hpg + row - tok * hpg) * j.q.ldh;
+        orow[tid] = (uint64_t)(u.first + tok) * j.out.ld + (uint64_t)(u.head * hpg + row - tok * hpg) * j.out.ldh;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+      {
+        constexpr uint32_t CH = D / 8, RW = CH < 32 ? 32 / CH : 1, PASS = kCR / (8 * RW);   // 16-byte chunks of a row, rows of a warp's pass
+        const uint32_t d8 = lane % CH, rr = lane / CH;
+        const __half *qb = reinterpret_cast<const __half *>(j.q.base) + d8 * 8u;
+        uint4 x[PASS];
+#pragma unroll
+        for (uint32_t p = 0; p < PASS; p++) {
+          const uint32_t r = (p * 8u + warp) * RW + rr;
+          x[p] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < nrow) {
+            const __half *q = qb + qrow[r];
+            if (j.q.wide) {
+              x[p] = *reinterpret_cast<const uint4 *>(q);
+            } else {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) w[i] = (uint32_t)__half_as_ushort(q[2 * i]) | ((uint32_t)__half_as_ushort(q[2 * i + 1]) << 16);
+              x[p] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+#pragma unroll
+        for (uint32_t p = 0; p < PASS; p++) {
+          const uint32_t r = (p * 8u + warp) * RW + rr;
+          *reinterpret_cast<uint4 *>(qs + (d8 >> 3) * 16384u + r * 128u + (((d8 & 7u) ^ (r & 7u)) * 16u)) =
+              make_uint4(x[p].x ^ flip, x[p].y ^ flip, x[p].z ^ flip, x[p].w ^ flip);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the generic writes before the MMAs' reads
+      tc::fence_before();
+      tc::cluster_sync();
+      tc::fence_after();
+      // ------------------------------------------------------------ softmax: half h of row r
+      const uint32_t r = tid & 127u, h = tid >> 7, lanes = ((warp & 3u) * 32u) << 16;
+      const int32_t pos = r < nrow ? (int32_t)(u.len - u.T + (rc + r) / hpg) : -1;
+      const int32_t pos0 = (int32_t)(u.len - u.T + u.r0 / hpg), pos1 = (int32_t)s.end - 1;   // of the block
+      float m = -INFINITY, l = 0.0f;
+      const uint32_t *trow = j.v.table + (uint64_t)b * j.v.ld;
+      const auto entry = [&](uint32_t i) { return 2u * i + h < s.n ? trow[page_at(s, 2u * i + h)] : P0_KV_NONE; };
+      bool ok = true;
+      uint32_t next = tiles ? entry(from) : P0_KV_NONE;
+      for (uint32_t i = 0; i < tiles; i++) {   // a warp that gave up keeps meeting the others at the barrier
+        const uint32_t t = tile + i, jp = page_at(s, min(2u * (from + i) + h, s.n - 1u));
+        const bool here = next < j.v.pages;
+        if (i + 1 < tiles) next = entry(from + i + 1);
+        ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(&sfull[t % C::kSB], (t / C::kSB) & 1u, abort_flag, j.err, 0x4b6u, P0_SPIN_LIMIT));
+        const uint32_t sc = tmem + lanes + C::kColS + (t % C::kSB) * 128u, pc = tmem + lanes + C::kColP + (t & 1u) * 64u;
+        uint32_t x[2][32];
+        float mx = -INFINITY;
+        if (ok) {
+          tc::fence_after();
+          tc::tmem_ld32(sc + 64u * h, x[0]);
+          tc::tmem_ld32(sc + 64u * h + 32u, x[1]);
+          tc::tmem_wait_ld();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_peer(&sread[t % C::kSB], 0);   // the even CTA's MMAs wait for both
+          // keys that this row does not see; a page that the whole block sees needs no look
+          const int32_t k0 = (int32_t)(jp * kPage);
+          if (!(here && k0 + 63 <= pos0 && (!W || k0 > pos1 - (int32_t)W || (uint32_t)k0 + 63u < S))) {
+            // keys up to `gone` are behind the window, those below `sink` are kept all the same
+            const int32_t last = here ? pos - k0 : -1, gone = W ? pos - (int32_t)W - k0 : -1;
+            const int32_t sink = S > (uint32_t)k0 ? (int32_t)min(S - (uint32_t)k0, kPage) : 0;
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+#pragma unroll
+              for (int e = 0; e < 32; e++) {
+                const int32_t k = q * 32 + e;
+                if (!(k <= last && (k > gone || k < sink))) x[q][e] = 0xff800000u;
+              }
+          }
+          float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int e = 0; e < 32; e++) y[e & 3] = fmaxf(y[e & 3], __uint_as_float(x[q][e]));
+          mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * c;
+          if (mx != mx) mx = -INFINITY;   // -inf times a scale of 0
+        }
+        mx2[t & 1u][h][r] = mx;
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+        if (!ok) continue;
+        mx = fmaxf(mx, mx2[t & 1u][h ^ 1u][r]);
+        // O follows a maximum that has grown by more than 2^8 (or that is a row's first)
+        const bool grow = mx > m + 8.0f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? exp2_fast(m - mx) : 1.0f;
+          if (grow) m = mx;
+          l *= f;
+          if (i) {
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(&odone[(t - 1u) & 1u], ((t - 1u) >> 1) & 1u, abort_flag, j.err, 0x4b7u, P0_SPIN_LIMIT));
+            tc::fence_after();
+#pragma unroll 1
+            for (uint32_t d = h * (D / 2); ok && d < (h + 1u) * (D / 2); d += 32u) {
+              uint32_t o[32];
+              tc::tmem_ld32(tmem + lanes + d, o);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(tmem + lanes + d, o);
+            }
+          }
+        }
+        if (i > 1) {   // P of tile t - 2 has been used (before that it lies in a unit whose end was waited for)
+          ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(&odone[t & 1u], ((t >> 1) - 1u) & 1u, abort_flag, j.err, 0x4bbu, P0_SPIN_LIMIT));
+          if (!ok) continue;
+          tc::fence_after();
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const float a = exp2_fast(fmaf(__uint_as_float(x[q][2 * e]), c, -ref)), d = exp2_fast(fmaf(__uint_as_float(x[q][2 * e + 1]), c, -ref));
+            sum[2 * (e & 1)] += a;
+            sum[2 * (e & 1) + 1] += d;
+            p[e] = pack2(a, d);
+          }
+          tc::tmem_st16(pc + 32u * h + 16u * q, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc::tmem_wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_peer(&pfull[t & 1u], 0);
+      }
+      l2[h][r] = l;
+      asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+      l += l2[h ^ 1u][r];
+      if (ok && tiles) {
+        const uint32_t t = tile + tiles - 1u;
+        if (tiles > 1) ok = tc::mbar_wait(&odone[(t - 1u) & 1u], ((t - 1u) >> 1) & 1u, abort_flag, j.err, 0x4bau, P0_SPIN_LIMIT);
+        ok = ok && tc::mbar_wait(&odone[t & 1u], (t >> 1) & 1u, abort_flag, j.err, 0x4b8u, P0_SPIN_LIMIT);
+        tc::fence_after();
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      const bool whole = from == 0 && to == nt;
+      float *part = j.part + (((uint64_t)run * 2u + (from ? 0u : 1u)) * 2u + rank) * kCR * (D + 2);   // [D][rows], then m and l
+      if (!whole && from == 0 && tid == 0 && rank == 0) j.desc[run] = make_uint4(1u + run_of(u.begin + u.n - 1u, total, G), b, u.r0, u.head);
+      if (ok) {
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        uint8_t *so = stg + warp * C::kOut;
+#pragma unroll 1
+        for (uint32_t d = h * (D / 2); d < (h + 1u) * (D / 2); d += 32u) {
+          uint32_t o[32];
+          __syncwarp();
+          if (tiles) {
+            tc::tmem_ld32(tmem + lanes + d, o);
+            tc::tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = 0u;
+          }
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) part[(d + e) * kCR + r] = __uint_as_float(o[e]);
+          } else {   // through shared memory: 8 rows' 64 bytes a store
+            uint4 y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) w[i] = pack2(__uint_as_float(o[8 * e + 2 * i]) * inv, __uint_as_float(o[8 * e + 2 * i + 1]) * inv);
+              *reinterpret_cast<uint4 *>(so + lane * 80u + e * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) y[k] = *reinterpret_cast<const uint4 *>(so + (8u * k + (lane >> 2)) * 80u + (lane & 3u) * 16u);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) {
+              const uint32_t row = (warp & 3u) * 32u + 8u * k + (lane >> 2);
+              if (row >= nrow) continue;
+              __half *out = reinterpret_cast<__half *>(j.out.base) + orow[row] + d + 8u * (lane & 3u);
+              if (j.out.wide) {
+                *reinterpret_cast<uint4 *>(out) = y[k];
+              } else {
+                const uint32_t w[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
+#pragma unroll
+                for (int i = 0; i < 8; i++) out[i] = __ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i & 1))));
+              }
+            }
+          }
+        }
+        if (!whole && h == 0) {
+          part[D * kCR + r] = m;
+          part[(D + 1) * kCR + r] = l;
+        }
+      }
+      tc::fence_before();   // O is read before the next unit's MMAs write it
+    }
+    st = __shfl_sync(0xffffffffu, st, 0);   // the issuing lane's count
+    tile += tiles;
+  }
+  __syncthreads();
+  if (abort_word && lane == 0) {   // a wait gave up (j.err says which): nothing may be in flight when the CTA leaves. Bounded
+    volatile uint32_t never = 0;
+    if (warp == 8)
+      for (uint32_t i = st > (uint32_t)NS ? st - NS : 0; i < st; i++) tc::mbar_wait(&full[i % NS], (i / NS) & 1u, &never, j.err, 0x4b2u, P0_SPIN_LIMIT);
+    if (warp == 9 && rank == 0) {
+      tc::mma_commit_pair(&mdone);
+      tc::mbar_wait(&mdone, 0, &never, j.err, 0x4b5u, P0_SPIN_LIMIT);
+    }
+  }
+  __syncwarp();
+  tc::fence_before();
+  tc::cluster_sync();   // neither CTA frees its tensor memory or exits while the other may still use it
+  if (warp == 8) {
+    tc::fence_after();
+    tc::tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// joins the parts of a unit that several runs share: CTA (run, 32 dims, 128 of the rows), a thread per row. M = max m, o = sum
+// 2^(m - M) acc / sum 2^(m - M) l, in run order
+template <int D>
+__global__ void __launch_bounds__(kCR) kv4_prompt_join_kernel(AttnJob j) {
+  dep_enter();
+  const uint4 w = j.desc[blockIdx.x];
+  if (!w.x) return;
+  const uint32_t r = threadIdx.x, d0 = blockIdx.y * 32u, rank = blockIdx.z, b = w.y, r0 = w.z + rank * kCR, head = w.w, hpg = j.hpg;
+  uint32_t first;
+  const uint32_t T = kv_tokens(j.v, b, first), n = w.x - blockIdx.x;
+  if (r0 + r >= T * hpg) return;
+  const auto part = [&](uint32_t i) { return j.part + (((uint64_t)(blockIdx.x + i) * 2u + (i ? 0u : 1u)) * 2u + rank) * kCR * (D + 2) + r; };
+  float M = -INFINITY;
+#pragma unroll 4
+  for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part(i)[D * kCR]);
+  const float ref = M == -INFINITY ? 0.0f : M;
+  float acc[32], sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 32; e++) acc[e] = 0.0f;
+#pragma unroll 2
+  for (uint32_t i = 0; i < n; i++) {
+    const float *p = part(i);
+    float x[32];
+#pragma unroll
+    for (int e = 0; e < 32; e++) x[e] = p[(d0 + e) * kCR];
+    const float f = exp2f(p[D * kCR] - ref);
+    sum = fmaf(f, p[(D + 1) * kCR], sum);
+#pragma unroll
+    for (int e = 0; e < 32; e++) acc[e] = fmaf(f, x[e], acc[e]);
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  __half *out = reinterpret_cast<__half *>(j.out.base) + (uint64_t)(first + (r0 + r) / hpg) * j.out.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.out.ldh + d0;
+  uint32_t y[16];
+#pragma unroll
+  for (int e = 0; e < 16; e++) y[e] = pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  if (j.out.wide) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) reinterpret_cast<uint4 *>(out)[e] = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; e++) out[e] = __ushort_as_half((unsigned short)(y[e / 2] >> (16 * (e & 1))));
+  }
+}
+
+template <int D>
+p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
+  using C = Cfg<D>;
+  const uint32_t R = j.v.rows, G = (uint32_t)c->sm_count / 2;
+  const size_t smem = C::kSmem + ((size_t)R + 1) * 8;
+  uint32_t *cnt;
+  void *ws;
+  const size_t desc = ((size_t)G * sizeof(uint4) + 255) / 256 * 256, parts = ((size_t)G * 2 * kRB * (D + 2) * 4 + 255) / 256 * 256;
+  p0_status st = p0_workspace(c, 0, desc + parts + wide_bytes, &cnt, &ws);
+  if (st) return st;
+  j.desc = (uint4 *)ws;
+  j.part = (float *)((uint8_t *)ws + desc);
+  j.wide = (uint8_t *)ws + desc + parts;
+  const auto kern = kv4_prompt_kernel<D>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) { cudaGetLastError(); return p0_fail(c, P0_EDEVICE, "kv4Attn: the prompt kernel does not fit this device"); }
+  launch_dep(kv4_widen_kernel<D>, dim3((unsigned)c->sm_count * 4u), dim3(kET), ((size_t)R + 1) * 4, c->stream, j);
+  if ((st = p0_launched(c, "kv4Attn pages"))) return st;
+  launch_dep(kern, dim3(2 * G), dim3(kThreads), smem, c->stream, j);
+  if ((st = p0_launched(c, "kv4Attn prompt"))) return st;
+  launch_dep(kv4_prompt_join_kernel<D>, dim3(G, D / 32, 2), dim3(kCR), 0, c->stream, j);
+  return p0_launched(c, "kv4Attn join");
+}
+
+}  // namespace
+
+p0_status kv4_attn_prompt(p0_ctx *c, AttnJob &j, bool *taken) {
+  *taken = false;
+  const uint64_t rows = (uint64_t)j.v.n * j.hpg, D = j.v.D;
+  if (rows / j.v.rows < 64) return P0_OK;
+  const uint64_t wide = (uint64_t)j.v.rows * j.v.ld * j.v.nkv * D * 256;
+  if (wide > (4ull << 30) || j.v.rows > 256 || D == 512) return P0_OK;
+  *taken = true;
+  switch (D) {
+    case 64: return prompt_launch<64>(c, j, wide);
+    case 128: return prompt_launch<128>(c, j, wide);
+    default: return prompt_launch<256>(c, j, wide);
+  }
+}

@@ -136,6 +136,29 @@ def attention(c, q, counts, nh, window=0, sinks=0, scale=1.0):
     return out, spread, size
 
 
+def attention_prompt(c, q, counts, nh, window=0, sinks=0, scale=1.0):
+    """attention(), a head's rows at a time"""
+    n, D = q.shape[0], c.D
+    out, spread, size = np.zeros((n, nh, D)), np.zeros((n, nh, D)), np.zeros((n, nh))
+    at = 0
+    for b, T in enumerate(counts):
+        ln = min(int(c.lens[b]), c.ld * PAGE)
+        see = np.stack([visible(ln - T + i, ln, window, sinks) for i in range(T)])
+        for h in range(c.nkv):
+            (k, there), (v, _) = c.values(b, 0, h, ln), c.values(b, 1, h, ln)
+            mask = see & there
+            any_ = mask.any(-1)
+            for hq in range(h * nh // c.nkv, (h + 1) * nh // c.nkv):
+                x = q[at:at + T, hq].astype(np.float64)
+                s = np.where(mask, scale * (x @ k.T), -np.inf)
+                p = np.exp(s - np.where(any_, s.max(-1, initial=-np.inf), 0.0)[:, None])
+                p /= np.maximum(p.sum(-1, keepdims=True), 1e-300)
+                out[at:at + T, hq], spread[at:at + T, hq] = p @ v, p @ np.abs(v)
+                size[at:at + T, hq] = abs(scale) * np.where(mask, np.abs(x) @ np.abs(k).T, 0.0).max(-1, initial=0.0)
+        at += T
+    return out, spread, size
+
+
 def attention_bound(spread, size, out, D, pages, f16):
     """How far a right kernel's output may be from 64 bits, element by element. f32: q split into two f16 parts leaves
     2^-22 |q|, at most D / 16 + D / 32 sums of f32 in a score, P split leaves 2^-22 p, exp within 2^-21, one f32 sum a

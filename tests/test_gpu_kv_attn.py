@@ -39,8 +39,8 @@ def run(g, c, q, counts, nh, type_, window=0, sinks=0, scale=0.0, lay=(0, 0, 0),
     return got[oi]
 
 
-def check(got, c, q, counts, nh, type_, window=0, sinks=0, scale=1.0):
-    want, spread, size = R.attention(c, q, counts, nh, window, sinks, scale)
+def check(got, c, q, counts, nh, type_, window=0, sinks=0, scale=1.0, ref=R.attention):
+    want, spread, size = ref(c, q, counts, nh, window, sinks, scale)
     tol = R.attention_bound(spread, size, want, c.D, int(c.table.shape[1]), type_ == "f16")
     err = np.abs(got.astype(np.float64) - want)
     assert np.all(err <= tol), (float((err / tol).max()), np.unravel_index((err / tol).argmax(), err.shape))
@@ -74,6 +74,45 @@ def test_attn(g, lens, counts, nh, nkv, D, window, sinks, type_):
     q = (rng.standard_normal((sum(counts), nh, D)) * (3.0 / D ** 0.5)).astype(np.float32 if type_ == "f32" else np.float16)
     got = run(g, c, q, counts, nh, type_, window, sinks)
     check(got, c, q, counts, nh, type_, window, sinks)
+
+
+PROMPTS = [
+    # lens, new tokens, nh, nkv, D, window, sinks, scale
+    ([1900], [700], 8, 1, 256, 0, 0, 0.0),                           # several key tiles a run, parts of units joined
+    ([900, 64, 1300], [900, 64, 40], 8, 1, 256, 0, 0, 0.0),          # from the first token on; units of one tile; an odd page
+    ([1500, 700], [500, 300], 4, 1, 256, 200, 70, -0.7),             # window, sinks over two pages, a negative scale
+    ([1300, 500, 260], [640, 100, 260], 8, 2, 128, 0, 0, 0.3),
+    ([2000, 300], [600, 300], 6, 2, 128, 300, 4, 0.0),
+    ([1100, 900], [700, 64], 16, 4, 64, 0, 0, 0.0),
+    ([100, 20, 640], [130, 30, 100], 8, 1, 64, 90, 1, 2.0),          # sequences shorter than their tokens: rows that see nothing
+]
+
+
+@pytest.mark.parametrize("lens,counts,nh,nkv,D,window,sinks,scale", PROMPTS)
+def test_prompt(g, lens, counts, nh, nkv, D, window, sinks, scale):
+    rng = np.random.default_rng(D + counts[0])
+    c = R.Cache(rng, lens, nkv, D)
+    c.fill_fast(rng)
+    q = (rng.standard_normal((sum(counts), nh, D)) * (3.0 / D ** 0.5)).astype(np.float16)
+    got = run(g, c, q, counts, nh, "f16", window, sinks, scale)
+    check(got, c, q, counts, nh, "f16", window, sinks, float(np.float32(scale or 1.0)), ref=R.attention_prompt)
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("T", [1, 400])
+def test_attn_growing_scores(g, D, T):
+    # every later page holds larger scores, by more than 2^8 in P: what was summed before has to follow the maximum
+    rng = np.random.default_rng(15)
+    c = R.Cache(rng, [900], 1, D)
+    c.fill_fast(rng)
+    for j in range(c.ld):
+        if c.table[0, j] < c.pages:
+            rec = c.pool[c.table[0, j], :c.part].reshape(-1, 1280)
+            rec[:, 1024:] = np.tile(np.array([0.0, 0.02 * j], np.float16).view(np.uint8), 64)   # k = 0.02 j in every dim
+    q = (np.ones((T, 2, D)) * (600.0 / D) + rng.standard_normal((T, 2, D)) * 0.01).astype(np.float16)
+    check(run(g, c, q, [T], 2, "f16"), c, q, [T], 2, "f16", ref=R.attention_prompt)
+    if T == 1:
+        check(run(g, c, q.astype(np.float32), [T], 2, "f32"), c, q, [T], 2, "f32", ref=R.attention_prompt)
 
 
 @pytest.mark.parametrize("type_,lay,out_lay", [("f32", (0, 0, 3), (901, 129, 1)), ("f16", (1153, 131, 7), (0, 0, 0)), ("f16", (128, 128 * 21, 0), (128, 128 * 21, 8))])
