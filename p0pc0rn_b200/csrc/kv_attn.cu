@@ -28,6 +28,15 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same from zero
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
 __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src),
                "r"(bytes), "r"(tc::smem_u32(bar))
@@ -39,33 +48,33 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 __device__ __forceinline__ uint32_t lds_u32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
 
-template <int D, bool F32, int NW, int RT>
+template <int D, bool F32, int NW, int RT, int KP>
 struct Cfg {
   static constexpr int kThreads = NW * 32;
   static constexpr int kRowsPer = F32 ? 8 : 16;          // query rows per fragment
   static constexpr int kRows = kRowsPer * RT;            // of a block
   static constexpr int kNpl = D / NW / 8;                // dims per lane and key in P V (output columns: 8 lanes x kNpl)
-  static constexpr int kNt = 8 / NW;                     // 8-key tiles per warp in Q K^T
-  static constexpr uint32_t kPart = D / 32 * 1280;
-  static constexpr int kStages = D >= 512 ? 2 : 3;
+  static constexpr int kNt = 8 * KP / NW;                // 8-key tiles per warp in Q K^T
+  static constexpr uint32_t kPart = D / 32 * 1280, kStage = KP * 2 * kPart;
+  static constexpr int kStages = D >= 256 ? 2 : 3;
   static constexpr uint32_t kQ = RT * D / 16 * 512;      // q fragments
-  static constexpr uint32_t kPRow = 64 * 2 + 16;         // a row of P, padded against bank conflicts
+  static constexpr uint32_t kPRow = 64 * KP * 2 + 16;    // a row of P, padded against bank conflicts
   static constexpr uint32_t kP = RT * 16 * kPRow;
-  static constexpr uint32_t kSmem = kStages * 2 * kPart + kQ + kP;
+  static constexpr uint32_t kSmem = kStages * kStage + kQ + kP;
 };
 
-template <int D, bool F32, int NW, int RT>
+template <int D, bool F32, int NW, int RT, int KP>
 __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
   dep_enter();
-  using C = Cfg<D, F32, NW, RT>;
+  using C = Cfg<D, F32, NW, RT, KP>;
   constexpr int NPL = C::kNpl, NT = C::kNt, RR = C::kRowsPer, RB = C::kRows, NS = C::kStages;
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t *ring = smem;
-  uint4 *qf = reinterpret_cast<uint4 *>(smem + NS * 2 * C::kPart);
-  uint8_t *ps = smem + NS * 2 * C::kPart + C::kQ;
+  uint4 *qf = reinterpret_cast<uint4 *>(smem + NS * C::kStage);
+  uint8_t *ps = smem + NS * C::kStage + C::kQ;
   uint32_t *pre = reinterpret_cast<uint32_t *>(smem + C::kSmem);   // [rows + 1] items before each sequence
   __shared__ __align__(8) uint64_t full[NS];
-  __shared__ uint32_t abort_flag, page_ok[NS];
+  __shared__ uint32_t abort_flag, page_ok[NS][KP];
   __shared__ float wmax[NW][RB], wsum[NW][RB];
   __shared__ int32_t rpos[RB];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g4 = lane >> 2, t4 = lane & 3u;
@@ -75,16 +84,18 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
     abort_flag = 0u;
     tc::fence_mbar_init();
   }
-  plan_items<RB, 1, 0>(j, pre);
+  plan_items<RB, KP, 0>(j, pre);
   const uint32_t total = pre[R], G = min(gridDim.x, max(total, 1u));   // no run is empty
   if (tid == 0) j.desc[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
   if (blockIdx.x >= G) return;
   const uint32_t lo = (uint32_t)((uint64_t)total * blockIdx.x / G), hi = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / G);
   uint32_t b = find_sequence(pre, R, lo);
-  uint32_t at = lo, it = 0;   // item; pages through the ring so far
+  const float scale = F32 ? j.scale : j.scale * 1.44269504088896340736f;   // f16: scores and maxima in powers of two
+  const auto ex = [](float x) { return F32 ? expf(x) : exp2f(x); };
+  uint32_t at = lo, it = 0;   // item; items through the ring so far
   while (at < hi) {
     while (pre[b + 1] <= at) b++;
-    const Unit u = find_unit<RB, 1, 0>(j, pre, b, at);
+    const Unit u = find_unit<RB, KP, 0>(j, pre, b, at);
     const Span &s = u.s;
     const uint32_t first = u.first, T = u.T, len = u.len, rows = u.rows, r0 = u.r0, head = u.head, begin = u.begin, n = u.n;
     const uint32_t from = at - begin, to = min(hi - begin, n);
@@ -92,13 +103,25 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
     const uint32_t steps = s.n ? to - from : 0u;
     const uint8_t *heads = j.v.pool + (uint64_t)head * 2u * C::kPart;
     const auto issue = [&](uint32_t i) {   // item from + i of the unit into its ring slot
-      const uint32_t st = (it + i) % NS, p = j.v.table[(uint64_t)b * j.v.ld + page_at(s, from + i)];
-      page_ok[st] = p < j.v.pages;
-      if (p < j.v.pages) {
-        tc::mbar_expect_tx(&full[st], 2u * C::kPart);
-        bulk_load(ring + st * 2u * C::kPart, heads + p * j.v.stride, 2u * C::kPart, &full[st]);
+      const uint32_t st = (it + i) % NS;
+      uint32_t p[KP], bytes = 0;
+#pragma unroll
+      for (int k = 0; k < KP; k++) {
+        const uint32_t pi = (from + i) * KP + k;
+        p[k] = pi < s.n ? j.v.table[(uint64_t)b * j.v.ld + page_at(s, pi)] : P0_KV_NONE;
+      }
+#pragma unroll
+      for (int k = 0; k < KP; k++) {
+        page_ok[st][k] = p[k] < j.v.pages;
+        bytes += p[k] < j.v.pages ? 2u * C::kPart : 0u;
+      }
+      if (bytes) {
+        tc::mbar_expect_tx(&full[st], bytes);
+#pragma unroll
+        for (int k = 0; k < KP; k++)
+          if (p[k] < j.v.pages) bulk_load(ring + st * C::kStage + k * 2u * C::kPart, heads + p[k] * j.v.stride, 2u * C::kPart, &full[st]);
       } else {
-        tc::mbar_arrive(&full[st]);   // no such page: its keys are not there
+        tc::mbar_arrive(&full[st]);   // no such pages: their keys are not there
       }
     };
     if (tid == 0)
@@ -155,12 +178,22 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
         pos[rt][h] = rpos[rt * RR + g4 + 8 * h];
       }
     }
+    const int32_t pos0 = (int32_t)(len - T + r0 / hpg), pos1 = (int32_t)s.end - 1;   // of the block's rows
     bool lost = false;
     for (uint32_t i = 0; i < steps; i++) {
-      const uint32_t st = (it + i) % NS, page = page_at(s, from + i), key0 = page * kPage;
+      const uint32_t st = (it + i) % NS, pi = (from + i) * KP;
       if (!tc::mbar_wait(&full[st], ((it + i) / NS) & 1u, &abort_flag, j.err, 0x4a1u, P0_SPIN_LIMIT)) lost = true;
-      const uint8_t *kp = ring + st * 2u * C::kPart, *vp = kp + C::kPart;
-      // ---- S = Q K^T: this warp's 8-key tiles
+      const uint8_t *stage = ring + st * C::kStage;
+      uint32_t key0[KP], ok[KP];
+#pragma unroll
+      for (int k = 0; k < KP; k++) {
+        key0[k] = page_at(s, pi + k) * kPage;
+        ok[k] = page_ok[st][k];
+      }
+      // ---- S = Q K^T: this warp's 8-key tiles, all of one page
+      const int kpw = KP == 1 ? 0 : (int)(warp / (NW / KP));
+      const uint32_t wk = (warp % (NW / KP)) * NT;                     // its first tile in the page
+      const uint8_t *kp = stage + kpw * 2u * C::kPart;
       float sc[RT][NT][4];
 #pragma unroll
       for (int rt = 0; rt < RT; rt++)
@@ -173,11 +206,9 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
         uint32_t kb[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          const uint32_t key = (warp * NT + nt) * 8u + g4;
+          const uint32_t key = (wk + nt) * 8u + g4;
           const uint32_t w = lds_u32(kp + g * 1280 + key * 16u + t4 * 4u), sm = lds_u32(kp + g * 1280 + 1024 + key * 4u);
-          const uint32_t s2 = __byte_perm(sm, 0, 0x1010), mn2 = __byte_perm(sm, 0, 0x3232);
-#pragma unroll
-          for (int e = 0; e < 4; e++) kb[nt][e] = kv_deq2((w >> (4 * e)) & 0x000F000Fu, s2, mn2);   // dims (e, e + 4)
+          kv_deq8(w, __byte_perm(sm, 0, 0x1010), __byte_perm(sm, 0, 0x3232), kb[nt]);   // dims (e, e + 4)
         }
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
@@ -189,8 +220,10 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
             for (int nt = 0; nt < NT; nt++) mma_f16(sc[rt][nt], a, kb[nt][2 * half], kb[nt][2 * half + 1]);
           }
       }
-      // ---- mask, the page's row maxima
-      const bool ok = page_ok[st] != 0u;
+      // ---- mask (a page that the whole block sees needs none), the row maxima
+      const int32_t k0 = (int32_t)(KP == 1 ? key0[0] : key0[kpw]);
+      const bool here = (KP == 1 ? ok[0] : ok[kpw]) != 0u;
+      const bool plain = here && k0 + 63 <= pos0 && (!W || k0 > pos1 - (int32_t)W || (uint32_t)k0 + 63u < S);
       float x[RT][NT][RH][2];
 #pragma unroll
       for (int rt = 0; rt < RT; rt++)
@@ -200,22 +233,28 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
 #pragma unroll
           for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-              const int32_t key = (int32_t)(key0 + (warp * NT + nt) * 8u + 2u * t4 + e);
-              const bool see = ok && key <= pos[rt][h] && (!W || key > pos[rt][h] - (int32_t)W || (uint32_t)key < S);
-              const float v = F32 ? sc[rt][nt][e] + sc[rt][nt][e + 2] : sc[rt][nt][2 * h + e];
-              x[rt][nt][h][e] = see ? v * j.scale : -INFINITY;
-              mx = fmaxf(mx, x[rt][nt][h][e]);
-            }
+            for (int e = 0; e < 2; e++) x[rt][nt][h][e] = (F32 ? sc[rt][nt][e] + sc[rt][nt][e + 2] : sc[rt][nt][2 * h + e]) * scale;
+          if (!plain) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const int32_t key = k0 + (int32_t)((wk + nt) * 8u + 2u * t4) + e;
+                if (!(here && key <= pos[rt][h] && (!W || key > pos[rt][h] - (int32_t)W || (uint32_t)key < S))) x[rt][nt][h][e] = -INFINITY;
+              }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) mx = fmaxf(mx, fmaxf(x[rt][nt][h][0], x[rt][nt][h][1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           if (t4 == 0) wmax[warp][rt * RR + g4 + 8 * h] = mx;
         }
-      __syncthreads();   // the previous page's P V is done: its ring slot is free
+      __syncthreads();   // the previous item's P V is done: its ring slot is free
       if (tid == 0 && i > 0 && i - 1 + NS < steps) issue(i - 1 + NS);
       // ---- P = exp(x - m), into shared memory as f16 (f32: high and low parts)
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++)
+      for (int rt = 0; rt < RT; rt++) {
+        float keep[RH];
 #pragma unroll
         for (int h = 0; h < RH; h++) {
           const uint32_t r = rt * RR + g4 + 8 * h;
@@ -223,23 +262,13 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
 #pragma unroll
           for (int w = 0; w < NW; w++) mn = fmaxf(mn, wmax[w][r]);
           const float ref = mn == -INFINITY ? 0.0f : mn;
-          const float keep = expf(m[rt][h] - ref);   // 0 while nothing has been seen
+          keep[h] = mn == m[rt][h] ? 1.0f : ex(m[rt][h] - ref);   // 0 while nothing has been seen
           m[rt][h] = mn;
-          l[rt][h] *= keep;
-#pragma unroll
-          for (int nt = 0; nt < NPL; nt++) {
-            if (F32) {
-#pragma unroll
-              for (int e = 0; e < 4; e++) o[rt][nt][e] *= keep;
-            } else {
-              o[rt][nt][2 * h] *= keep;
-              o[rt][nt][2 * h + 1] *= keep;
-            }
-          }
+          l[rt][h] *= keep[h];
           uint8_t *row = ps + (rt * 16 + g4 + 8 * h) * C::kPRow;
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
-            const float p0 = expf(x[rt][nt][h][0] - ref), p1 = expf(x[rt][nt][h][1] - ref);
+            const float p0 = ex(x[rt][nt][h][0] - ref), p1 = ex(x[rt][nt][h][1] - ref);
             l[rt][h] += p0 + p1;
             const uint32_t hi2 = pack2(p0, p1), col = ((warp * NT + nt) * 8u + 2u * t4) * 2u;
             *reinterpret_cast<uint32_t *>(row + col) = hi2;
@@ -249,68 +278,75 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
             }
           }
         }
-      __syncthreads();
-      // ---- O += P V: this warp's dims. Slots that no row of the unit sees hold zeros, whatever the memory holds
-      const bool edge = !ok || key0 + kPage > s.end || (key0 < s.first_pos && key0 + kPage > S);
-      float c[RT][NPL][4];
+        if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[RH - 1] != 1.0f)) {
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++)
+          for (int nt = 0; nt < NPL; nt++)
 #pragma unroll
-        for (int nt = 0; nt < NPL; nt++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) c[rt][nt][e] = 0.0f;
-      const uint32_t d0 = warp * (D / NW) + g4 * NPL;                 // the lane's first dim
-      const uint32_t swap = NPL == 8 ? (g4 >> 2) & 1u : 0u;          // the second group of 32 dims starts with the odd key: other banks
-      const uint8_t *vg = vp + d0 / 32u * 1280u, *vw = vg + (d0 % 32u) / 8u * 4u;
-#pragma unroll
-      for (int ks = 0; ks < 4; ks++) {
-        uint32_t vb[NPL][2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t key = ks * 16 + h * 8 + 2 * t4;
-          const uint32_t w0 = lds_u32(vw + (key + swap) * 16u), w1 = lds_u32(vw + (key + 1u - swap) * 16u);
-          uint2 sm = *reinterpret_cast<const uint2 *>(vg + 1024u + key * 4u);
-          if (edge) {
-            const uint32_t k0 = key0 + key, k1 = k0 + 1u;
-            if (!ok || k0 >= s.end || (k0 < s.first_pos && k0 >= S)) sm.x = 0u;
-            if (!ok || k1 >= s.end || (k1 < s.first_pos && k1 >= S)) sm.y = 0u;
-          }
-          const uint32_t s2 = __byte_perm(sm.x, sm.y, 0x5410), mn2 = __byte_perm(sm.x, sm.y, 0x7632);   // (key, key + 1)
-          if constexpr (NPL == 8) {
-            const uint32_t u = __byte_perm(w0, w1, swap ? 0x1054u : 0x5410u), v = __byte_perm(w0, w1, swap ? 0x3276u : 0x7632u);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              vb[e][h] = kv_deq2((u >> (4 * e)) & 0x000F000Fu, s2, mn2);
-              vb[e + 4][h] = kv_deq2((v >> (4 * e)) & 0x000F000Fu, s2, mn2);
-            }
-          } else if constexpr (NPL == 4) {
-            const uint32_t u = __byte_perm(w0, w1, (d0 & 4u) ? 0x7632u : 0x5410u);
-#pragma unroll
-            for (int e = 0; e < NPL; e++) vb[e][h] = kv_deq2((u >> (4 * e)) & 0x000F000Fu, s2, mn2);
-          } else {
-            const uint32_t by = (d0 & 7u) / 2u;
-            const uint32_t u = __byte_perm(w0, w1, by | (by << 4) | ((4u + by) << 8) | ((4u + by) << 12));
-#pragma unroll
-            for (int e = 0; e < NPL; e++) vb[e][h] = kv_deq2((u >> (4 * e)) & 0x000F000Fu, s2, mn2);
-          }
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-          const uint8_t *row = ps + (rt * 16 + g4) * C::kPRow + (ks * 16 + 2 * t4) * 2;
-          const uint32_t a[4] = {lds_u32(row), lds_u32(row + 8 * C::kPRow), lds_u32(row + 16), lds_u32(row + 8 * C::kPRow + 16)};
-#pragma unroll
-          for (int nt = 0; nt < NPL; nt++) mma_f16(c[rt][nt], a, vb[nt][0], vb[nt][1]);
+            for (int e = 0; e < 4; e++) o[rt][nt][e] *= keep[F32 ? 0 : e >> 1];
         }
       }
+      __syncthreads();
+      // ---- O += P V: this warp's dims. Slots that no row of the unit sees hold zeros, whatever the memory holds
+      const uint32_t d0 = warp * (D / NW) + g4 * NPL;                 // the lane's first dim
+      const uint32_t swap = NPL == 8 ? (g4 >> 2) & 1u : 0u;          // the second group of 32 dims starts with the odd key: other banks
+      float c[RT][NPL][4];
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++)
+      for (int k = 0; k < KP; k++) {
+        const bool edge = !ok[k] || key0[k] + kPage > s.end || (key0[k] < s.first_pos && key0[k] + kPage > S);
+        const uint8_t *vg = stage + k * 2u * C::kPart + C::kPart + d0 / 32u * 1280u, *vw = vg + (d0 % 32u) / 8u * 4u;
 #pragma unroll
-        for (int nt = 0; nt < NPL; nt++)
+        for (int ks = 0; ks < 4; ks++) {
+          uint32_t vb[2][NPL == 8 ? 8 : 4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) o[rt][nt][e] += c[rt][nt][e];
-      if (__syncthreads_or(lost)) { lost = true; break; }
+          for (int h = 0; h < 2; h++) {
+            const uint32_t key = ks * 16 + h * 8 + 2 * t4;
+            const uint32_t w0 = lds_u32(vw + (key + swap) * 16u), w1 = lds_u32(vw + (key + 1u - swap) * 16u);
+            uint2 sm = *reinterpret_cast<const uint2 *>(vg + 1024u + key * 4u);
+            if (edge) {
+              const uint32_t ka = key0[k] + key, kb = ka + 1u;
+              if (!ok[k] || ka >= s.end || (ka < s.first_pos && ka >= S)) sm.x = 0u;
+              if (!ok[k] || kb >= s.end || (kb < s.first_pos && kb >= S)) sm.y = 0u;
+            }
+            const uint32_t s2 = __byte_perm(sm.x, sm.y, 0x5410), mn2 = __byte_perm(sm.x, sm.y, 0x7632);   // (key, key + 1)
+            uint32_t q[4];
+            if constexpr (NPL == 8) {
+              kv_deq8(__byte_perm(w0, w1, swap ? 0x1054u : 0x5410u), s2, mn2, q);
+#pragma unroll
+              for (int e = 0; e < 4; e++) vb[h][e] = q[e];
+              kv_deq8(__byte_perm(w0, w1, swap ? 0x3276u : 0x7632u), s2, mn2, q);
+#pragma unroll
+              for (int e = 0; e < 4; e++) vb[h][e + 4] = q[e];
+            } else if constexpr (NPL == 4) {
+              kv_deq8(__byte_perm(w0, w1, (d0 & 4u) ? 0x7632u : 0x5410u), s2, mn2, vb[h]);
+            } else {
+              const uint32_t by = (d0 & 7u) / 2u, w = __byte_perm(w0, w1, by | (by << 4) | ((4u + by) << 8) | ((4u + by) << 12));
+              vb[h][0] = kv_deq2(w & 0x000F000Fu, s2, mn2);
+              vb[h][1] = kv_deq2((w >> 4) & 0x000F000Fu, s2, mn2);
+            }
+          }
+#pragma unroll
+          for (int rt = 0; rt < RT; rt++) {
+            uint32_t a[4];
+            ldsm_x4(tc::smem_u32(ps + (rt * 16 + (lane & 15u)) * C::kPRow + k * 128 + ks * 32 + (lane >> 4) * 16u), a);
+#pragma unroll
+            for (int nt = 0; nt < NPL; nt++) {
+              if (!F32) mma_f16(o[rt][nt], a, vb[0][nt], vb[1][nt]);
+              else if (k == 0 && ks == 0) mma_f16_zero(c[rt][nt], a, vb[0][nt], vb[1][nt]);
+              else mma_f16(c[rt][nt], a, vb[0][nt], vb[1][nt]);
+            }
+          }
+        }
+      }
+      if (F32) {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+          for (int nt = 0; nt < NPL; nt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[rt][nt][e] += c[rt][nt][e];
+      }
     }
-    if (lost) {   // a copy did not arrive in time: j.err says so. Let the copies in flight land before the CTA leaves
+    if (__syncthreads_or(lost)) {   // a copy did not arrive in time: j.err says so. Let the copies in flight land before the CTA leaves
       for (uint32_t i = 0; i < steps; i++)
         for (uint32_t k = 0; k < (1u << 16) && !tc::mbar_try(&full[(it + i) % NS], ((it + i) / NS) & 1u); k++) {}
       return;
@@ -363,7 +399,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
 #pragma unroll
           for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int nt = 0; nt < NPL; nt++) p[d + e * NPL + nt] = y[e][nt];
+            for (int nt = 0; nt < NPL; nt += 2) *reinterpret_cast<float2 *>(p + d + e * NPL + nt) = make_float2(y[e][nt], y[e][nt + 1]);
           if (warp == 0 && t4 == 0) {
             p[D] = m[rt][h];
             p[D + 1] = sum;
@@ -409,7 +445,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnJob j) {
   float sum = 0.0f;
   for (uint32_t i = k; i < n; i += K) {
     const float *p = part(i);
-    const float w = expf(p[D] - ref);
+    const float w = F32 ? expf(p[D] - ref) : exp2f(p[D] - ref);
     const float2 a = *reinterpret_cast<const float2 *>(p + 4 * e), c = *reinterpret_cast<const float2 *>(p + 4 * e + 2);
     o.x = fmaf(w, a.x, o.x);
     o.y = fmaf(w, a.y, o.y);
@@ -439,11 +475,11 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnJob j) {
   }
 }
 
-template <int D, bool F32, int NW, int RT>
+template <int D, bool F32, int NW, int RT, int KP>
 p0_status attn_launch(p0_ctx *c, AttnJob &j) {
-  using C = Cfg<D, F32, NW, RT>;
+  using C = Cfg<D, F32, NW, RT, KP>;
   const size_t smem = C::kSmem + ((size_t)j.v.rows + 1) * 4;
-  const auto kern = kv4_attn_kernel<D, F32, NW, RT>;
+  const auto kern = kv4_attn_kernel<D, F32, NW, RT, KP>;
   int per = 0;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, C::kThreads, smem);
@@ -460,6 +496,13 @@ p0_status attn_launch(p0_ctx *c, AttnJob &j) {
   if ((st = p0_launched(c, "kv4Attn"))) return st;
   launch_dep(kv4_attn_join_kernel<D, F32, C::kRows>, dim3(G, C::kRows), dim3(256), 0, c->stream, j);
   return p0_launched(c, "kv4Attn join");
+}
+
+template <int D, bool F32, int NW, int MAXRT, int KP>
+p0_status pick(p0_ctx *c, AttnJob &j, uint32_t frags) {
+  if (frags <= 1) return attn_launch<D, F32, NW, 1, KP>(c, j);
+  if (frags == 2 || MAXRT == 2) return attn_launch<D, F32, NW, 2, KP>(c, j);
+  return attn_launch<D, F32, NW, MAXRT, KP>(c, j);
 }
 
 }  // namespace
@@ -492,10 +535,13 @@ extern "C" p0_status p0_kv4_attn(p0_ctx *c, const p0_kv4_attn_args *a) {
     bool taken = false;
     if ((st = kv4_attn_prompt(c, j, &taken)) || taken) return st;
   }
+  // fragments per block: one, or two, or four (two for D = 512, whose sums fill the registers), so that a page is dequantised
+  // for as many rows at once as there are
+  const uint32_t per = a->T && !a->cu.id ? a->T * j.hpg : (uint32_t)((rows + a->kv.rows - 1) / a->kv.rows), frags = (per + (f32 ? 7u : 15u)) / (f32 ? 8u : 16u);
   switch (a->kv.D) {
-    case 64: return f32 ? attn_launch<64, true, 4, 1>(c, j) : attn_launch<64, false, 4, 1>(c, j);
-    case 128: return f32 ? attn_launch<128, true, 4, 1>(c, j) : attn_launch<128, false, 4, 1>(c, j);
-    case 256: return f32 ? attn_launch<256, true, 4, 1>(c, j) : attn_launch<256, false, 4, 1>(c, j);
-    default: return f32 ? attn_launch<512, true, 8, 1>(c, j) : attn_launch<512, false, 8, 1>(c, j);
+    case 64: return f32 ? pick<64, true, 4, 4, 2>(c, j, frags) : pick<64, false, 4, 4, 2>(c, j, frags);
+    case 128: return f32 ? pick<128, true, 8, 4, 2>(c, j, frags) : pick<128, false, 8, 4, 2>(c, j, frags);
+    case 256: return f32 ? pick<256, true, 8, 4, 2>(c, j, frags) : pick<256, false, 8, 4, 2>(c, j, frags);
+    default: return f32 ? pick<512, true, 8, 2, 1>(c, j, frags) : pick<512, false, 8, 2, 1>(c, j, frags);
   }
 }
