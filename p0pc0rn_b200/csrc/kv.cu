@@ -193,8 +193,8 @@ __global__ void __launch_bounds__(kT) kv4_get_kernel(RowsJob j) {
     const uint32_t s2 = __byte_perm(sm, 0, 0x1010), mn2 = __byte_perm(sm, 0, 0x3232);
 #pragma unroll
     for (int i = 0; i < 4; i++) {   // codes 2i, 2i + 1
-      const uint32_t pair = ((word >> (8 * i)) & 15u) | (((word >> (8 * i + 4)) & 15u) << 16);
-      v[i] = kv_deq2(pair, s2, mn2);
+      const uint32_t low = (word >> (8 * i)) & 0xffu;
+      v[i] = kv_deq2(low | low << 12, s2, mn2);
     }
   }
   const KvRows &r = p.vsel ? j.vv : j.k;

@@ -55,25 +55,34 @@ __device__ __forceinline__ bool kv_place(const KvView &v, uint32_t i, uint32_t &
   return true;
 }
 
-// a pair of codes in the low nibbles of a word's halves -> f16(q * s + mn) of both, each rounded once
+// kv_deq2: the codes in the low nibbles of a word's halves -> f16(q * s + mn) of both, each rounded once
 __device__ __forceinline__ uint32_t kv_fma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-__device__ __forceinline__ uint32_t kv_deq2(uint32_t pair, uint32_t s2, uint32_t mn2) {
-  uint32_t q;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(q) : "r"(pair | 0x64006400u), "r"(0x64006400u));   // (1024 + q) - 1024, exact
-  return kv_fma2(q, s2, mn2);
+// (w & mask) | 0x64006400: 1024 + the masked code of both halves (one lop3; written as two operators it takes two)
+__device__ __forceinline__ uint32_t kv_code2(uint32_t w, uint32_t mask) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(0x64006400u));
+  return d;
+}
+__device__ __forceinline__ uint32_t kv_sub1024(uint32_t x) {
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x64006400u));   // (1024 + q) - 1024, exact
+  return d;
+}
+__device__ __forceinline__ uint32_t kv_deq2(uint32_t w, uint32_t s2, uint32_t mn2) {
+  return kv_fma2(kv_sub1024(kv_code2(w, 0x000F000Fu)), s2, mn2);
 }
 // the four pairs of a word, nibbles 0..3 of its halves. A nibble one place up makes 1024 + 16 q, which one fma turns into q
 // as exactly as the subtraction does: one shift a word instead of three
-__device__ __forceinline__ void kv_deq8(uint32_t w, uint32_t s2, uint32_t mn2, uint32_t (&v)[4]) {
+__device__ __forceinline__ void kv_deq8(uint32_t w, uint32_t s2, uint32_t mn2, uint32_t *v) {
   const uint32_t w8 = w >> 8;
-  v[0] = kv_deq2(w & 0x000F000Fu, s2, mn2);
-  v[1] = kv_fma2(kv_fma2((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD400D400u), s2, mn2);   // x / 16 - 64
-  v[2] = kv_deq2(w8 & 0x000F000Fu, s2, mn2);
-  v[3] = kv_fma2(kv_fma2((w8 & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD400D400u), s2, mn2);
+  v[0] = kv_deq2(w, s2, mn2);
+  v[1] = kv_fma2(kv_fma2(kv_code2(w, 0x00F000F0u), 0x2C002C00u, 0xD400D400u), s2, mn2);   // x / 16 - 64
+  v[2] = kv_deq2(w8, s2, mn2);
+  v[3] = kv_fma2(kv_fma2(kv_code2(w8, 0x00F000F0u), 0x2C002C00u, 0xD400D400u), s2, mn2);
 }
 
 // the host side: resolves and checks a view (layer: its D and nkv too), the new tokens' layout, and rows of values

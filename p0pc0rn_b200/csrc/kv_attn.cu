@@ -10,14 +10,18 @@
 // finished there; otherwise each run leaves (m, l, acc) in the workspace and the join kernel adds them in run order, so
 // results do not depend on timing.
 //
-// A page. One bulk copy brings a head's K and V records (D * 80 bytes); a ring of stages hides it. The codes become f16
-// pairs in registers (two codes per sub and fma on the half2 pipe) and go straight into mma.sync fragments: S = Q K^T
-// with a warp's share of the 64 keys, then O += P V with a warp's share of the dims, P going through shared memory. The
-// code words fit the fragments without moves: a K word holds 8 dims of one key (any dim order serves a dot product, q is
-// staged in that order), and two keys' V words give 4 or 8 (key, key + 1) pairs per byte permute.
+// An item, one or two pages: bulk copies bring a head's K and V records to shared memory, a ring of stages hides them. K records
+// lie 1312 bytes apart there, so that a quarter warp's 16-byte reads of four records fall in different banks. The codes
+// become f16 pairs in registers (kv_deq8) and go straight into mma.sync fragments without moves: any order of the dims
+// serves a dot product, so a lane takes 32 dims of one group of a key (q is staged in that order): one 16-byte read and
+// one (s, mn) for 32 codes; two keys' V words give 8 (key, key + 1) pairs by two byte permutes.
+//   S = Q K^T   a warp takes 8 or 16 of the item's keys
+//   P = exp(S - m) through shared memory, m over all warps
+//   O += P V    a warp takes 64 (or 32) dims and a share of the keys; the shares meet when the unit ends
+// The instructions per code, about 2 for each of K and V, bound a batch of long contexts: 4 warp instructions a cycle.
 //
 // Precision. f32 queries and outputs: q and P are split into f16 high and low parts (about 22 bits) in rows r and r + 8
-// of the fragments; each page's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
+// of the fragments; each item's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
 // f16 matrix operand), 16 rows per fragment.
 #include "kv_attn.cuh"
 
@@ -46,28 +50,40 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t lds_u32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
 
-template <int D, bool F32, int NW, int RT, int KP>
+constexpr uint32_t kRec = 1312;   // a K record's place in shared memory
+
+template <int D, bool F32, int NPL, int RT, int KP>
 struct Cfg {
-  static constexpr int kThreads = NW * 32;
+  static constexpr int kNW = 8, kThreads = kNW * 32;
   static constexpr int kRowsPer = F32 ? 8 : 16;          // query rows per fragment
   static constexpr int kRows = kRowsPer * RT;            // of a block
-  static constexpr int kNpl = D / NW / 8;                // dims per lane and key in P V (output columns: 8 lanes x kNpl)
-  static constexpr int kNt = 8 * KP / NW;                // 8-key tiles per warp in Q K^T
-  static constexpr uint32_t kPart = D / 32 * 1280, kStage = KP * 2 * kPart;
+  static constexpr int kNt = 8 * KP / kNW;               // 8-key tiles per warp in Q K^T
+  static constexpr int kDs = D / (8 * NPL);              // warps over the dims in P V (NPL dims a lane and key),
+  static constexpr int kKs = kNW / kDs;                  // and over the keys
+  static constexpr int kSteps = KP * 4 / kKs;            // 16-key steps per warp
+  static constexpr uint32_t kRecs = D / 32, kPart = kRecs * 1280, kK = kRecs * kRec, kPage2 = kK + kPart;   // K and V of a page
+  static constexpr uint32_t kStage = KP * kPage2;
   static constexpr int kStages = D >= 256 ? 2 : 3;
   static constexpr uint32_t kQ = RT * D / 16 * 512;      // q fragments
   static constexpr uint32_t kPRow = 64 * KP * 2 + 16;    // a row of P, padded against bank conflicts
   static constexpr uint32_t kP = RT * 16 * kPRow;
   static constexpr uint32_t kSmem = kStages * kStage + kQ + kP;
+  static_assert(kKs == 1 || (uint32_t)(RT * D * 64) <= kStages * kStage, "the key shares meet in the ring");
 };
 
-template <int D, bool F32, int NW, int RT, int KP>
-__global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
+template <int D, bool F32, int NPL, int RT, int KP>
+__global__ void __launch_bounds__(256) kv4_attn_kernel(AttnJob j) {
   dep_enter();
-  using C = Cfg<D, F32, NW, RT, KP>;
-  constexpr int NPL = C::kNpl, NT = C::kNt, RR = C::kRowsPer, RB = C::kRows, NS = C::kStages;
+  using C = Cfg<D, F32, NPL, RT, KP>;
+  constexpr int NT = C::kNt, RR = C::kRowsPer, RB = C::kRows, NS = C::kStages, NW = C::kNW;
+  constexpr int KW = D >= 128 ? 4 : 2;   // a lane's K words at a time: of one group (D = 64: half of one)
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t *ring = smem;
   uint4 *qf = reinterpret_cast<uint4 *>(smem + NS * C::kStage);
@@ -75,7 +91,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
   uint32_t *pre = reinterpret_cast<uint32_t *>(smem + C::kSmem);   // [rows + 1] items before each sequence
   __shared__ __align__(8) uint64_t full[NS];
   __shared__ uint32_t abort_flag, page_ok[NS][KP];
-  __shared__ float wmax[NW][RB], wsum[NW][RB];
+  __shared__ __align__(16) float wmax[RB][NW], wsum[RB][NW];
   __shared__ int32_t rpos[RB];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g4 = lane >> 2, t4 = lane & 3u;
   const uint32_t hpg = j.hpg, R = j.v.rows, W = j.window, S = j.sinks;
@@ -91,7 +107,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
   const uint32_t lo = (uint32_t)((uint64_t)total * blockIdx.x / G), hi = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / G);
   uint32_t b = find_sequence(pre, R, lo);
   const float scale = F32 ? j.scale : j.scale * 1.44269504088896340736f;   // f16: scores and maxima in powers of two
-  const auto ex = [](float x) { return F32 ? expf(x) : exp2f(x); };
+  const auto ex = [](float x) { return exp2_fast(F32 ? x * 1.44269504088896340736f : x); };
   uint32_t at = lo, it = 0;   // item; items through the ring so far
   while (at < hi) {
     while (pre[b + 1] <= at) b++;
@@ -102,35 +118,40 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
     const uint32_t nrow = min((uint32_t)RB, rows - r0);
     const uint32_t steps = s.n ? to - from : 0u;
     const uint8_t *heads = j.v.pool + (uint64_t)head * 2u * C::kPart;
-    const auto issue = [&](uint32_t i) {   // item from + i of the unit into its ring slot
-      const uint32_t st = (it + i) % NS;
-      uint32_t p[KP], bytes = 0;
-#pragma unroll
-      for (int k = 0; k < KP; k++) {
-        const uint32_t pi = (from + i) * KP + k;
-        p[k] = pi < s.n ? j.v.table[(uint64_t)b * j.v.ld + page_at(s, pi)] : P0_KV_NONE;
-      }
-#pragma unroll
-      for (int k = 0; k < KP; k++) {
-        page_ok[st][k] = p[k] < j.v.pages;
-        bytes += p[k] < j.v.pages ? 2u * C::kPart : 0u;
-      }
-      if (bytes) {
-        tc::mbar_expect_tx(&full[st], bytes);
-#pragma unroll
-        for (int k = 0; k < KP; k++)
-          if (p[k] < j.v.pages) bulk_load(ring + st * C::kStage + k * 2u * C::kPart, heads + p[k] * j.v.stride, 2u * C::kPart, &full[st]);
-      } else {
-        tc::mbar_arrive(&full[st]);   // no such pages: their keys are not there
-      }
+    // warp 0 brings an item's records, a K record or a page's V a lane; it looks an item's pages up one item ahead
+    constexpr uint32_t PR = C::kRecs + 1;
+    static_assert(KP * PR <= 32, "a lane per copy");
+    const uint32_t ck = lane / PR, cr = lane % PR;
+    const auto look_up = [&](uint32_t i) {   // the page that this lane copies from for item from + i of the unit
+      const uint32_t pi = (from + i) * KP + ck;
+      return ck < (uint32_t)KP && i < steps && pi < s.n ? j.v.table[(uint64_t)b * j.v.ld + page_at(s, pi)] : P0_KV_NONE;
     };
-    if (tid == 0)
+    uint32_t ahead = P0_KV_NONE;
+    const auto issue = [&](uint32_t i) {
+      const uint32_t st = (it + i) % NS, p = ahead;
+      const bool have = p < j.v.pages;
+      const uint32_t n_k = __popc(__ballot_sync(0xffffffffu, have && cr < C::kRecs)), n_v = __popc(__ballot_sync(0xffffffffu, have && cr == C::kRecs));
+      if (cr == 0 && ck < (uint32_t)KP) page_ok[st][ck] = have;
+      __syncwarp();
+      if (lane == 0) {
+        if (n_k) tc::mbar_expect_tx(&full[st], n_k * 1280u + n_v * C::kPart);
+        else tc::mbar_arrive(&full[st]);   // no such pages: their keys are not there
+      }
+      __syncwarp();
+      if (have)
+        bulk_load(ring + st * C::kStage + ck * C::kPage2 + cr * kRec, heads + p * j.v.stride + cr * 1280u, cr < C::kRecs ? 1280u : C::kPart, &full[st]);
+      ahead = look_up(i + 1);
+    };
+    if (warp == 0) {
+      ahead = look_up(0);
       for (uint32_t i = 0; i < (uint32_t)NS && i < steps; i++) issue(i);
+    }
     // the rows' positions and q fragments
     if (tid < (uint32_t)RB) rpos[tid] = tid < nrow ? (int32_t)(len - T + (r0 + tid) / hpg) : -1;
     for (uint32_t e = tid; e < RT * (D / 16) * 32u; e += C::kThreads) {
       const uint32_t ln = e & 31u, step = (e >> 5) % (D / 16), rt = (e >> 5) / (D / 16);
-      const uint32_t d0 = (step >> 1) * 32u + (ln & 3u) * 8u + (step & 1u) * 2u;   // the lane's word; codes d0, +4, +1, +5
+      const uint32_t wi = step >> 1, l4 = ln & 3u;   // the lane's K word wi; its codes d0, +4, +1, +5
+      const uint32_t d0 = (D >= 128 ? ((wi >> 2) * 4u + l4) * 32u + (wi & 3u) * 8u : l4 * 16u + wi * 8u) + (step & 1u) * 2u;
       float x[2][4];
 #pragma unroll
       for (int half = 0; half < (F32 ? 1 : 2); half++) {
@@ -162,6 +183,12 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
       qf[e] = f;
     }
     __syncthreads();
+    // this warp's dims and keys in P V
+    const uint32_t ds = warp % C::kDs, kshare = warp / C::kDs;
+    const uint32_t d0 = ds * (8 * NPL) + g4 * NPL;                 // the lane's first dim
+    const uint32_t swap = NPL == 8 ? (g4 >> 2) & 1u : 0u;          // the second group of 32 dims starts with the odd key: other banks
+    const uint32_t step0 = kshare * C::kSteps;                     // the warp's first 16-key step of an item (kSteps divides 4, or is the item)
+    const uint32_t voff = (step0 / 4u) * C::kPage2 + C::kK + d0 / 32u * 1280u, word = (d0 % 32u) / 8u * 4u;
     constexpr int RH = F32 ? 1 : 2;   // rows of a lane per fragment: g4 (and g4 + 8)
     float o[RT][NPL][4], m[RT][RH], l[RT][RH];
     int32_t pos[RT][RH];
@@ -193,7 +220,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
       // ---- S = Q K^T: this warp's 8-key tiles, all of one page
       const int kpw = KP == 1 ? 0 : (int)(warp / (NW / KP));
       const uint32_t wk = (warp % (NW / KP)) * NT;                     // its first tile in the page
-      const uint8_t *kp = stage + kpw * 2u * C::kPart;
+      const uint8_t *kp = stage + kpw * C::kPage2 + (D >= 128 ? t4 * kRec : (t4 >> 1) * kRec);
       float sc[RT][NT][4];
 #pragma unroll
       for (int rt = 0; rt < RT; rt++)
@@ -201,24 +228,39 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int e = 0; e < 4; e++) sc[rt][nt][e] = 0.0f;
-#pragma unroll 4
-      for (int g = 0; g < D / 32; g++) {
-        uint32_t kb[NT][4];
+#pragma unroll
+      for (int g = 0; g < (D >= 128 ? D / 128 : 1); g++) {
+        uint32_t w[NT][KW], s2[NT], mn2[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
           const uint32_t key = (wk + nt) * 8u + g4;
-          const uint32_t w = lds_u32(kp + g * 1280 + key * 16u + t4 * 4u), sm = lds_u32(kp + g * 1280 + 1024 + key * 4u);
-          kv_deq8(w, __byte_perm(sm, 0, 0x1010), __byte_perm(sm, 0, 0x3232), kb[nt]);   // dims (e, e + 4)
+          const uint8_t *rec = kp + g * 4 * kRec;
+          if constexpr (KW == 4) {
+            const uint4 u4 = *reinterpret_cast<const uint4 *>(rec + key * 16u);
+            w[nt][0] = u4.x; w[nt][1] = u4.y; w[nt][2] = u4.z; w[nt][3] = u4.w;
+          } else {
+            const uint2 u2 = *reinterpret_cast<const uint2 *>(rec + key * 16u + (t4 & 1u) * 8u);
+            w[nt][0] = u2.x; w[nt][1] = u2.y;
+          }
+          const uint32_t sm = lds_u32(rec + 1024 + key * 4u);
+          s2[nt] = __byte_perm(sm, 0, 0x1010);
+          mn2[nt] = __byte_perm(sm, 0, 0x3232);
         }
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
+        for (int wi = 0; wi < KW; wi++) {
+          uint32_t kb[NT][4];
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            const uint4 f = qf[(rt * (D / 16) + 2 * g + half) * 32 + lane];
-            const uint32_t a[4] = {f.x, f.y, f.z, f.w};
+          for (int nt = 0; nt < NT; nt++) kv_deq8(w[nt][wi], s2[nt], mn2[nt], kb[nt]);   // dims (e, e + 4)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) mma_f16(sc[rt][nt], a, kb[nt][2 * half], kb[nt][2 * half + 1]);
-          }
+          for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              const uint4 f = qf[(rt * (D / 16) + 2 * (g * KW + wi) + half) * 32 + lane];
+              const uint32_t a[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++) mma_f16(sc[rt][nt], a, kb[nt][2 * half], kb[nt][2 * half + 1]);
+            }
+        }
       }
       // ---- mask (a page that the whole block sees needs none), the row maxima
       const int32_t k0 = (int32_t)(KP == 1 ? key0[0] : key0[kpw]);
@@ -247,10 +289,23 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
           for (int nt = 0; nt < NT; nt++) mx = fmaxf(mx, fmaxf(x[rt][nt][h][0], x[rt][nt][h][1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          if (t4 == 0) wmax[warp][rt * RR + g4 + 8 * h] = mx;
+          if (t4 == 0) wmax[rt * RR + g4 + 8 * h][warp] = mx;
         }
       __syncthreads();   // the previous item's P V is done: its ring slot is free
-      if (tid == 0 && i > 0 && i - 1 + NS < steps) issue(i - 1 + NS);
+      if (warp == 0 && i > 0 && i - 1 + NS < steps) issue(i - 1 + NS);
+      // slots that no row of the unit sees hold zeros, whatever the memory holds: their (s, mn) of V
+#pragma unroll
+      for (int k = 0; k < KP; k++) {
+        const uint32_t ky = key0[k];
+        if (!ok[k] || ky + kPage > s.end || (ky < s.first_pos && ky + kPage > S)) {
+          uint8_t *vs = ring + st * C::kStage + k * C::kPage2 + C::kK + 1024u;
+          for (uint32_t e = tid; e < 64u * C::kRecs; e += C::kThreads) {
+            const uint32_t key = ky + (e & 63u);
+            if (!ok[k] || key >= s.end || (key < s.first_pos && key >= S)) *reinterpret_cast<uint32_t *>(vs + (e >> 6) * 1280u + (e & 63u) * 4u) = 0u;
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy into this slot
+        }
+      }
       // ---- P = exp(x - m), into shared memory as f16 (f32: high and low parts)
 #pragma unroll
       for (int rt = 0; rt < RT; rt++) {
@@ -259,8 +314,8 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
         for (int h = 0; h < RH; h++) {
           const uint32_t r = rt * RR + g4 + 8 * h;
           float mn = m[rt][h];
-#pragma unroll
-          for (int w = 0; w < NW; w++) mn = fmaxf(mn, wmax[w][r]);
+          const float4 wa = *reinterpret_cast<const float4 *>(&wmax[r][0]), wb = *reinterpret_cast<const float4 *>(&wmax[r][4]);
+          mn = fmaxf(mn, fmaxf(fmaxf(fmaxf(wa.x, wa.y), fmaxf(wa.z, wa.w)), fmaxf(fmaxf(wb.x, wb.y), fmaxf(wb.z, wb.w))));
           const float ref = mn == -INFINITY ? 0.0f : mn;
           keep[h] = mn == m[rt][h] ? 1.0f : ex(m[rt][h] - ref);   // 0 while nothing has been seen
           m[rt][h] = mn;
@@ -286,54 +341,40 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
         }
       }
       __syncthreads();
-      // ---- O += P V: this warp's dims. Slots that no row of the unit sees hold zeros, whatever the memory holds
-      const uint32_t d0 = warp * (D / NW) + g4 * NPL;                 // the lane's first dim
-      const uint32_t swap = NPL == 8 ? (g4 >> 2) & 1u : 0u;          // the second group of 32 dims starts with the odd key: other banks
+      // ---- O += P V: this warp's dims and keys
       float c[RT][NPL][4];
 #pragma unroll
-      for (int k = 0; k < KP; k++) {
-        const bool edge = !ok[k] || key0[k] + kPage > s.end || (key0[k] < s.first_pos && key0[k] + kPage > S);
-        const uint8_t *vg = stage + k * 2u * C::kPart + C::kPart + d0 / 32u * 1280u, *vw = vg + (d0 % 32u) / 8u * 4u;
+      for (int ks = 0; ks < C::kSteps; ks++) {
+        const uint8_t *vg = stage + voff + (C::kSteps > 4 ? (ks / 4) * C::kPage2 : 0u), *vw = vg + word;
+        const uint32_t row16 = (C::kSteps >= 4 ? ks % 4 : step0 % 4u + ks) * 16u;   // in the page
+        uint32_t vb[2][NPL];
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-          uint32_t vb[2][NPL == 8 ? 8 : 4];
+        for (int h = 0; h < 2; h++) {
+          const uint32_t key = row16 + h * 8 + 2 * t4;
+          const uint32_t w0 = lds_u32(vw + (key + swap) * 16u), w1 = lds_u32(vw + (key + 1u - swap) * 16u);
+          const uint2 sm = *reinterpret_cast<const uint2 *>(vg + 1024u + key * 4u);
+          const uint32_t s2 = __byte_perm(sm.x, sm.y, 0x5410), mn2 = __byte_perm(sm.x, sm.y, 0x7632);   // (key, key + 1)
+          uint32_t q[4];
+          if constexpr (NPL == 8) {
+            kv_deq8(__byte_perm(w0, w1, swap ? 0x1054u : 0x5410u), s2, mn2, q);
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const uint32_t key = ks * 16 + h * 8 + 2 * t4;
-            const uint32_t w0 = lds_u32(vw + (key + swap) * 16u), w1 = lds_u32(vw + (key + 1u - swap) * 16u);
-            uint2 sm = *reinterpret_cast<const uint2 *>(vg + 1024u + key * 4u);
-            if (edge) {
-              const uint32_t ka = key0[k] + key, kb = ka + 1u;
-              if (!ok[k] || ka >= s.end || (ka < s.first_pos && ka >= S)) sm.x = 0u;
-              if (!ok[k] || kb >= s.end || (kb < s.first_pos && kb >= S)) sm.y = 0u;
-            }
-            const uint32_t s2 = __byte_perm(sm.x, sm.y, 0x5410), mn2 = __byte_perm(sm.x, sm.y, 0x7632);   // (key, key + 1)
-            uint32_t q[4];
-            if constexpr (NPL == 8) {
-              kv_deq8(__byte_perm(w0, w1, swap ? 0x1054u : 0x5410u), s2, mn2, q);
+            for (int e = 0; e < 4; e++) vb[h][e] = q[e];
+            kv_deq8(__byte_perm(w0, w1, swap ? 0x3276u : 0x7632u), s2, mn2, q);
 #pragma unroll
-              for (int e = 0; e < 4; e++) vb[h][e] = q[e];
-              kv_deq8(__byte_perm(w0, w1, swap ? 0x3276u : 0x7632u), s2, mn2, q);
-#pragma unroll
-              for (int e = 0; e < 4; e++) vb[h][e + 4] = q[e];
-            } else if constexpr (NPL == 4) {
-              kv_deq8(__byte_perm(w0, w1, (d0 & 4u) ? 0x7632u : 0x5410u), s2, mn2, vb[h]);
-            } else {
-              const uint32_t by = (d0 & 7u) / 2u, w = __byte_perm(w0, w1, by | (by << 4) | ((4u + by) << 8) | ((4u + by) << 12));
-              vb[h][0] = kv_deq2(w & 0x000F000Fu, s2, mn2);
-              vb[h][1] = kv_deq2((w >> 4) & 0x000F000Fu, s2, mn2);
-            }
+            for (int e = 0; e < 4; e++) vb[h][e + 4] = q[e];
+          } else {
+            kv_deq8(__byte_perm(w0, w1, (d0 & 4u) ? 0x7632u : 0x5410u), s2, mn2, vb[h]);
           }
+        }
 #pragma unroll
-          for (int rt = 0; rt < RT; rt++) {
-            uint32_t a[4];
-            ldsm_x4(tc::smem_u32(ps + (rt * 16 + (lane & 15u)) * C::kPRow + k * 128 + ks * 32 + (lane >> 4) * 16u), a);
+        for (int rt = 0; rt < RT; rt++) {
+          uint32_t a[4];
+          ldsm_x4(tc::smem_u32(ps + (rt * 16 + (lane & 15u)) * C::kPRow + (step0 + ks) * 32u + (lane >> 4) * 16u), a);
 #pragma unroll
-            for (int nt = 0; nt < NPL; nt++) {
-              if (!F32) mma_f16(o[rt][nt], a, vb[0][nt], vb[1][nt]);
-              else if (k == 0 && ks == 0) mma_f16_zero(c[rt][nt], a, vb[0][nt], vb[1][nt]);
-              else mma_f16(c[rt][nt], a, vb[0][nt], vb[1][nt]);
-            }
+          for (int nt = 0; nt < NPL; nt++) {
+            if (!F32) mma_f16(o[rt][nt], a, vb[0][nt], vb[1][nt]);
+            else if (ks == 0) mma_f16_zero(c[rt][nt], a, vb[0][nt], vb[1][nt]);
+            else mma_f16(c[rt][nt], a, vb[0][nt], vb[1][nt]);
           }
         }
       }
@@ -360,9 +401,32 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
         float t = l[rt][h];
         t += __shfl_xor_sync(0xffffffffu, t, 1);
         t += __shfl_xor_sync(0xffffffffu, t, 2);
-        if (t4 == 0) wsum[warp][rt * RR + g4 + 8 * h] = t;
+        if (t4 == 0) wsum[rt * RR + g4 + 8 * h][warp] = t;
       }
     __syncthreads();
+    // ---- the key shares of O meet in the first one, through the ring (no copy is in flight)
+#pragma unroll 1
+    for (int k = 1; k < C::kKs; k++) {
+      float *x = reinterpret_cast<float *>(ring) + (size_t)ds * (RT * NPL * 4 * 32) + lane;
+      if (kshare == (uint32_t)k) {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+          for (int nt = 0; nt < NPL; nt++)
+#pragma unroll
+            for (int e = 0; e < (F32 ? 2 : 4); e++) x[((rt * NPL + nt) * 4 + e) * 32] = F32 ? o[rt][nt][e] + o[rt][nt][e + 2] : o[rt][nt][e];
+      }
+      __syncthreads();
+      if (kshare == 0) {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+          for (int nt = 0; nt < NPL; nt++)
+#pragma unroll
+            for (int e = 0; e < (F32 ? 2 : 4); e++) o[rt][nt][e] += x[((rt * NPL + nt) * 4 + e) * 32];
+      }
+      __syncthreads();
+    }
     const bool whole = from == 0 && to == n;
     // a run has at most one part of a unit that began earlier (slot 0) and one of a unit that goes on after it (slot 1)
     float *part = j.part + ((uint64_t)blockIdx.x * 2u + (from ? 0u : 1u)) * RB * (D + 2);
@@ -374,17 +438,17 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
 #pragma unroll
       for (int h = 0; h < RH; h++) {
         const uint32_t r = rt * RR + g4 + 8 * h;
-        if (r >= nrow) continue;
+        if (r >= nrow || kshare) continue;
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; w++) sum += wsum[w][r];
+        for (int w = 0; w < NW; w++) sum += wsum[r][w];
         const float inv = whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
         float y[2][NPL];   // dims 2 t4 * NPL .. and (2 t4 + 1) * NPL ..: contiguous
 #pragma unroll
         for (int nt = 0; nt < NPL; nt++)
 #pragma unroll
           for (int e = 0; e < 2; e++) y[e][nt] = (F32 ? o[rt][nt][e] + o[rt][nt][e + 2] : o[rt][nt][2 * h + e]) * inv;
-        const uint32_t d = warp * (D / NW) + 2 * t4 * NPL;
+        const uint32_t d = ds * (8 * NPL) + 2 * t4 * NPL;
         if (whole) {
           const uint64_t q = (uint64_t)(first + (r0 + r) / hpg) * j.out.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.out.ldh + d;
 #pragma unroll
@@ -407,6 +471,7 @@ __global__ void __launch_bounds__(NW * 32) kv4_attn_kernel(AttnJob j) {
         }
       }
     at = begin + to;
+    if (C::kKs > 1) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring was written: before the next unit's copies
     __syncthreads();   // q fragments, wsum and rpos are free
   }
 }
@@ -475,11 +540,11 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnJob j) {
   }
 }
 
-template <int D, bool F32, int NW, int RT, int KP>
+template <int D, bool F32, int NPL, int RT, int KP>
 p0_status attn_launch(p0_ctx *c, AttnJob &j) {
-  using C = Cfg<D, F32, NW, RT, KP>;
+  using C = Cfg<D, F32, NPL, RT, KP>;
   const size_t smem = C::kSmem + ((size_t)j.v.rows + 1) * 4;
-  const auto kern = kv4_attn_kernel<D, F32, NW, RT, KP>;
+  const auto kern = kv4_attn_kernel<D, F32, NPL, RT, KP>;
   int per = 0;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, C::kThreads, smem);
@@ -498,11 +563,14 @@ p0_status attn_launch(p0_ctx *c, AttnJob &j) {
   return p0_launched(c, "kv4Attn join");
 }
 
-template <int D, bool F32, int NW, int MAXRT, int KP>
+// fragments per block: one, two or four, so that a page is dequantised for as many rows at once as there are (at D = 512 two:
+// the sums fill the registers; four of f32 take 32 dims a warp instead of 64)
+template <int D, bool F32, int KP>
 p0_status pick(p0_ctx *c, AttnJob &j, uint32_t frags) {
-  if (frags <= 1) return attn_launch<D, F32, NW, 1, KP>(c, j);
-  if (frags == 2 || MAXRT == 2) return attn_launch<D, F32, NW, 2, KP>(c, j);
-  return attn_launch<D, F32, NW, MAXRT, KP>(c, j);
+  if (frags <= 1) return attn_launch<D, F32, 8, 1, KP>(c, j);
+  if (frags == 2 || D == 512) return attn_launch<D, F32, 8, 2, KP>(c, j);
+  if constexpr (D < 512) return attn_launch<D, F32, F32 ? 4 : 8, 4, KP>(c, j);
+  return P0_OK;
 }
 
 }  // namespace
@@ -535,13 +603,11 @@ extern "C" p0_status p0_kv4_attn(p0_ctx *c, const p0_kv4_attn_args *a) {
     bool taken = false;
     if ((st = kv4_attn_prompt(c, j, &taken)) || taken) return st;
   }
-  // fragments per block: one, or two, or four (two for D = 512, whose sums fill the registers), so that a page is dequantised
-  // for as many rows at once as there are
   const uint32_t per = a->T && !a->cu.id ? a->T * j.hpg : (uint32_t)((rows + a->kv.rows - 1) / a->kv.rows), frags = (per + (f32 ? 7u : 15u)) / (f32 ? 8u : 16u);
   switch (a->kv.D) {
-    case 64: return f32 ? pick<64, true, 4, 4, 2>(c, j, frags) : pick<64, false, 4, 4, 2>(c, j, frags);
-    case 128: return f32 ? pick<128, true, 8, 4, 2>(c, j, frags) : pick<128, false, 8, 4, 2>(c, j, frags);
-    case 256: return f32 ? pick<256, true, 8, 4, 2>(c, j, frags) : pick<256, false, 8, 4, 2>(c, j, frags);
-    default: return f32 ? pick<512, true, 8, 2, 1>(c, j, frags) : pick<512, false, 8, 2, 1>(c, j, frags);
+    case 64: return f32 ? pick<64, true, 2>(c, j, frags) : pick<64, false, 2>(c, j, frags);
+    case 128: return f32 ? pick<128, true, 2>(c, j, frags) : pick<128, false, 2>(c, j, frags);
+    case 256: return f32 ? pick<256, true, 2>(c, j, frags) : pick<256, false, 2>(c, j, frags);
+    default: return f32 ? pick<512, true, 1>(c, j, frags) : pick<512, false, 1>(c, j, frags);
   }
 }

@@ -89,10 +89,10 @@ __global__ void __launch_bounds__(kET) kv4_widen_kernel(AttnJob j) {
         uint4 o = make_uint4(0u, 0u, 0u, 0u);
         if (there(key)) {
           const uint32_t s2 = __byte_perm(sm[n], 0, 0x1010), mn2 = __byte_perm(sm[n], 0, 0x3232), y = x[n] >> 4;
-          o.x = kv_deq2(__byte_perm(x[n], y, 0x4400) & 0x000F000Fu, s2, mn2);   // byte i: dims 2i, 2i + 1
-          o.y = kv_deq2(__byte_perm(x[n], y, 0x5511) & 0x000F000Fu, s2, mn2);
-          o.z = kv_deq2(__byte_perm(x[n], y, 0x6622) & 0x000F000Fu, s2, mn2);
-          o.w = kv_deq2(__byte_perm(x[n], y, 0x7733) & 0x000F000Fu, s2, mn2);
+          o.x = kv_deq2(__byte_perm(x[n], y, 0x4400), s2, mn2);   // byte i: dims 2i, 2i + 1
+          o.y = kv_deq2(__byte_perm(x[n], y, 0x5511), s2, mn2);
+          o.z = kv_deq2(__byte_perm(x[n], y, 0x6622), s2, mn2);
+          o.w = kv_deq2(__byte_perm(x[n], y, 0x7733), s2, mn2);
         }
         *reinterpret_cast<uint4 *>(to + blk * 8192u + key * 128u + ((c ^ (key & 7u)) * 16u)) = o;
       }
@@ -116,8 +116,8 @@ __global__ void __launch_bounds__(kET) kv4_widen_kernel(AttnJob j) {
           const uint32_t lo = __byte_perm(x[2 * p], x[2 * p + 1], 0x5410), hi = __byte_perm(x[2 * p], x[2 * p + 1], 0x7632);
 #pragma unroll
           for (uint32_t d = 0; d < 4; d++) {
-            o[d][p] = kv_deq2((lo >> (4 * d)) & 0x000F000Fu, s2, mn2);
-            o[d + 4][p] = kv_deq2((hi >> (4 * d)) & 0x000F000Fu, s2, mn2);
+            o[d][p] = kv_deq2((lo >> (4 * d)), s2, mn2);
+            o[d + 4][p] = kv_deq2((hi >> (4 * d)), s2, mn2);
           }
         }
 #pragma unroll
