@@ -400,7 +400,7 @@ typedef struct {
 } p0_kv_compact_args;
 p0_status p0_kv_compact(p0_ctx *ctx, const p0_kv_compact_args *a);
 
-/* beamSelect: for each group of `beams` (<= 16) rows of logits (f32, V of each row, ld 0 = V, off in floats), c[b, v] =
+/* beamSelect: for each group of `beams` (<= 16) rows of logits (f32, V <= 2^24 of each row, ld 0 = V, off in floats), c[b, v] =
  * score[b] + (x[b, v] - lse_b) in f32, lse_b = log(sum exp x[b, :]), and the `beams` largest c in order, ties to the lowest
  * b * V + v. A beam with fin[b] != 0 (fin optional) has one candidate, (eos, score[b]). NaN and -inf are never chosen
  * (a NaN or +inf logit makes its whole row NaN). Per slot: parent = the chosen row (of all groups * beams), token, score_out,

@@ -69,23 +69,28 @@ namespace {
 constexpr int kT = 256;
 
 // ---------------------------------------------------------------- kv4Put / kv4Get
-// A warp takes 8 consecutive tokens of one group of 32 dims (a lane: one token's code word, 8 dims), so that it reads
-// or writes 8 whole runs of 32 values and, where the tokens are neighbours in a page, 128 contiguous bytes of codes.
+// A warp takes 8 consecutive tokens of one head's K or V and a run of its groups of 32 dims (a lane: one token's code word, 8
+// dims), so that it finds the tokens' places once, reads or writes whole runs of 32 values and, where the tokens are
+// neighbours in a page, 128 contiguous bytes of codes.
 constexpr float kHold = 60000.0f;   // 15 * f16(range / 15) + f16(-60000) stays finite in f16
+constexpr uint32_t kGroups = 4;     // groups whose values a lane holds at a time
 
 struct RowsJob {
   KvView v;
   uint8_t *rec;         // the pool again, writable for kv4Put
   KvRows k, vv;
+  uint32_t runs;        // of groups: warps per 8 tokens, head and K or V
   uint64_t warps;       // of the whole call
 };
 
-struct Place { uint32_t group, vsel, head, tok, word; bool in; };
+struct Place { uint32_t g0, g1, vsel, head, tok, word; bool in; };
 __device__ __forceinline__ Place place_of(const RowsJob &j, uint64_t w) {
   const uint32_t lane = threadIdx.x & 31u, G = j.v.D / 32u;
   Place p;
-  p.group = (uint32_t)(w % G);
-  w /= G;
+  const uint32_t run = (uint32_t)(w % j.runs);
+  p.g0 = G * run / j.runs;
+  p.g1 = G * (run + 1) / j.runs;
+  w /= j.runs;
   p.vsel = (uint32_t)(w & 1u);
   w >>= 1;
   p.head = (uint32_t)(w % j.v.nkv);
@@ -95,15 +100,14 @@ __device__ __forceinline__ Place place_of(const RowsJob &j, uint64_t w) {
   p.in = p.tok < j.v.n;
   return p;
 }
-// the record of a place's token row, or null where the token has no page
+// the first record of a place's token row, or null where the token has no page
 __device__ __forceinline__ uint8_t *record_of(const RowsJob &j, const Place &p, uint32_t &slot) {
   uint32_t b, pos;
   if (!p.in || !kv_place(j.v, p.tok, b, pos)) return nullptr;
   const uint32_t page = j.v.table[(uint64_t)b * j.v.ld + pos / kPage];
   if (page >= j.v.pages) return nullptr;
   slot = pos % kPage;
-  const uint32_t part = j.v.D / 32u * 1280u;
-  return j.rec + page * j.v.stride + (uint64_t)(p.head * 2u + p.vsel) * part + p.group * 1280u;
+  return j.rec + page * j.v.stride + (uint64_t)(p.head * 2u + p.vsel) * (j.v.D / 32u * 1280u);
 }
 
 template <bool F16, bool WIDE>
@@ -136,6 +140,27 @@ __device__ __forceinline__ void load8(const uint8_t *base, uint64_t at, float (&
   }
 }
 
+// The codes clamp(rint(fl(d / s)), 0, 15) of 8 values d = fl(x - mn) as a word, with r = fl(1 / s). d * r is within two units in
+// the last place of the quotient, so it rounds to the same whole number unless it lies next to a half, and then the divisions
+// decide. y + 1.5 * 2^23 rounds y to a whole number, half to even, and holds it in its low bits.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float mn, float s, float r) {
+  constexpr float kRound = 12582912.0f;
+  uint32_t word = 0;
+  float off = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(x[e], mn), r), 0.0f), 15.0f), t = __fadd_rn(y, kRound);
+    off = fmaxf(off, fabsf(__fsub_rn(y, __fsub_rn(t, kRound))));
+    word |= (__float_as_uint(t) & 15u) << (4 * e);
+  }
+  if (off > 0.4999f) {
+    word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], mn), s)), 0.0f), 15.0f) << (4 * e);
+  }
+  return word;
+}
+
 // per 32 dims: mn = f16(min), s = f16((max - mn) / 15) (0 -> 1), q = clamp(rhe((x - mn) / s), 0, 15), every step rounded
 // in f32 as written (pack_q4 takes f64 for the division: a value on the border of two codes may land on the other)
 template <bool F16, bool WIDE>
@@ -144,38 +169,57 @@ __global__ void __launch_bounds__(kT) kv4_put_kernel(RowsJob j) {
   const uint64_t w = ((uint64_t)blockIdx.x * kT + threadIdx.x) / 32u;
   if (w >= j.warps) return;
   const Place p = place_of(j, w);
-  uint32_t slot = 0;
-  uint8_t *rec = record_of(j, p, slot);
-  float x[8] = {};
   const KvRows &r = p.vsel ? j.vv : j.k;
-  if (rec) load8<F16, WIDE>(r.base, p.tok * r.ld + p.head * r.ldh + p.group * 32u + p.word * 8u, x);
-  float lo = kHold, hi = -kHold;
+  const uint64_t at = p.tok * r.ld + p.head * r.ldh + p.word * 8u;
+  uint32_t slot = 0;
+  uint8_t *rec = nullptr;
+  for (uint32_t g0 = p.g0; g0 < p.g1; g0 += kGroups) {
+    float x[kGroups][8] = {};
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    x[i] = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -kHold), kHold);
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-  }
+    for (uint32_t i = 0; i < kGroups; i++)   // on their way while the place is looked up
+      if (p.in && g0 + i < p.g1) load8<F16, WIDE>(r.base, at + (g0 + i) * 32u, x[i]);
+    if (g0 == p.g0) rec = record_of(j, p, slot);
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {   // the four lanes of a token
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (!rec) return;
-  const __half mnh = __float2half_rn(lo + 0.0f);   // a minimum of -0 is stored as +0, whichever zero the reduction kept
-  const float mn = __half2float(mnh);
-  __half sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, mn), 15.0f));
-  if (__half2float(sh) == 0.0f) sh = __float2half_rn(1.0f);
-  const float s = __half2float(sh);
-  uint32_t word = 0;
+    for (uint32_t i = 0; i < kGroups; i++) {
+      if (g0 + i >= p.g1) break;
+      float lo = kHold, hi = -kHold;
+      bool fine = true;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float q = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], mn), s)), 0.0f), 15.0f);
-    word |= (uint32_t)q << (4 * i);
+      for (int e = 0; e < 8; e++) {
+        fine = fine && fabsf(x[i][e]) <= kHold;
+        lo = fminf(lo, x[i][e]);
+        hi = fmaxf(hi, x[i][e]);
+      }
+      if (!fine) {   // held at +-60000, NaN as 0
+        lo = kHold;
+        hi = -kHold;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x[i][e] = x[i][e] != x[i][e] ? 0.0f : fminf(fmaxf(x[i][e], -kHold), kHold);
+          lo = fminf(lo, x[i][e]);
+          hi = fmaxf(hi, x[i][e]);
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {   // the four lanes of a token
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      const __half mnh = __float2half_rn(lo + 0.0f);   // a minimum of -0 is stored as +0, whichever zero the reduction kept
+      const float mn = __half2float(mnh);
+      __half sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, mn), 15.0f));
+      if (__half2float(sh) == 0.0f) sh = __float2half_rn(1.0f);
+      const float s = __half2float(sh), inv = __fdiv_rn(1.0f, s);
+      const uint32_t word = codes_of(x[i], mn, s, inv);
+      if (rec) {
+        uint8_t *to = rec + (g0 + i) * 1280u;
+        *reinterpret_cast<uint32_t *>(to + slot * 16u + p.word * 4u) = word;
+        if (p.word == 0)
+          *reinterpret_cast<uint32_t *>(to + 1024u + slot * 4u) = (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mnh) << 16);
+      }
+    }
   }
-  *reinterpret_cast<uint32_t *>(rec + slot * 16u + p.word * 4u) = word;
-  if (p.word == 0)
-    *reinterpret_cast<uint32_t *>(rec + 1024u + slot * 4u) = (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mnh) << 16);
 }
 
 // the values of the same rows; a row without a page reads as zeros
@@ -186,36 +230,43 @@ __global__ void __launch_bounds__(kT) kv4_get_kernel(RowsJob j) {
   if (w >= j.warps) return;
   const Place p = place_of(j, w);
   if (!p.in) return;
-  uint32_t slot = 0, v[4] = {0u, 0u, 0u, 0u};
-  if (const uint8_t *rec = record_of(j, p, slot)) {
-    const uint32_t word = *reinterpret_cast<const uint32_t *>(rec + slot * 16u + p.word * 4u);
-    const uint32_t sm = *reinterpret_cast<const uint32_t *>(rec + 1024u + slot * 4u);
-    const uint32_t s2 = __byte_perm(sm, 0, 0x1010), mn2 = __byte_perm(sm, 0, 0x3232);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {   // codes 2i, 2i + 1
-      const uint32_t low = (word >> (8 * i)) & 0xffu;
-      v[i] = kv_deq2(low | low << 12, s2, mn2);
-    }
-  }
   const KvRows &r = p.vsel ? j.vv : j.k;
-  const uint64_t at = p.tok * r.ld + p.head * r.ldh + p.group * 32u + p.word * 8u;
-  if (F16) {
-    __half *h = reinterpret_cast<__half *>(r.base) + at;
-    if (WIDE) *reinterpret_cast<uint4 *>(h) = make_uint4(v[0], v[1], v[2], v[3]);
-    else
+  uint32_t slot = 0;
+  const uint8_t *rec = record_of(j, p, slot);
+  for (uint32_t g0 = p.g0; g0 < p.g1; g0 += kGroups) {
+    uint32_t word[kGroups] = {}, sm[kGroups] = {};
 #pragma unroll
-      for (int i = 0; i < 8; i++) h[i] = __ushort_as_half((unsigned short)(v[i / 2] >> (16 * (i & 1))));
-  } else {
-    float *f = reinterpret_cast<float *>(r.base) + at;
-    float x[8];
+    for (uint32_t i = 0; i < kGroups; i++) {
+      if (!rec || g0 + i >= p.g1) break;
+      word[i] = *reinterpret_cast<const uint32_t *>(rec + (g0 + i) * 1280u + slot * 16u + p.word * 4u);
+      sm[i] = *reinterpret_cast<const uint32_t *>(rec + (g0 + i) * 1280u + 1024u + slot * 4u);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = __half2float(__ushort_as_half((unsigned short)(v[i / 2] >> (16 * (i & 1)))));
-    if (WIDE) {
-      *reinterpret_cast<float4 *>(f) = make_float4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<float4 *>(f + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    } else
+    for (uint32_t i = 0; i < kGroups; i++) {
+      if (g0 + i >= p.g1) break;
+      const uint32_t s2 = __byte_perm(sm[i], 0, 0x1010), mn2 = __byte_perm(sm[i], 0, 0x3232), y = word[i] >> 4;
+      const uint32_t v[4] = {kv_deq2(__byte_perm(word[i], y, 0x4400), s2, mn2), kv_deq2(__byte_perm(word[i], y, 0x5511), s2, mn2),   // byte i: 2i, 2i + 1
+                             kv_deq2(__byte_perm(word[i], y, 0x6622), s2, mn2), kv_deq2(__byte_perm(word[i], y, 0x7733), s2, mn2)};
+      const uint64_t at = p.tok * r.ld + p.head * r.ldh + (g0 + i) * 32u + p.word * 8u;
+      if (F16) {
+        __half *h = reinterpret_cast<__half *>(r.base) + at;
+        if (WIDE) *reinterpret_cast<uint4 *>(h) = make_uint4(v[0], v[1], v[2], v[3]);
+        else
 #pragma unroll
-      for (int i = 0; i < 8; i++) f[i] = x[i];
+          for (int e = 0; e < 8; e++) h[e] = __ushort_as_half((unsigned short)(v[e / 2] >> (16 * (e & 1))));
+      } else {
+        float *f = reinterpret_cast<float *>(r.base) + at;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __half2float(__ushort_as_half((unsigned short)(v[e / 2] >> (16 * (e & 1)))));
+        if (WIDE) {
+          *reinterpret_cast<float4 *>(f) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4 *>(f + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else
+#pragma unroll
+          for (int e = 0; e < 8; e++) f[e] = x[e];
+      }
+    }
   }
 }
 
@@ -394,66 +445,51 @@ struct CompactJob {
   KvView v;
   const uint32_t *ref;
   uint32_t *to_table, *to_ref, *stat;
-  uint32_t *cnt;        // [2][kPC]: live pages, then movers | holes of each share
-  uint32_t *mover, *hole, *rank;   // [pages] each
+  uint32_t *cnt;        // [kPC] live pages of each CTA's share, then the live pages below L
+  uint32_t *live, *hole, *rank;   // [pages] each: the k-th live page, the k-th free page below L; of a page, the live pages before it
 };
 
-// L live pages: the k-th live page at L or beyond moves to the k-th free page below L
+// L live pages: the k-th live page at L or beyond moves to the k-th free page below L. With f(p) = the live pages before p,
+// a free page p < L is the (p - f(p))-th hole, and a live page p >= L the (f(p) - f(L))-th to move: one scan gives both.
+// A CTA takes a run of the pages, a thread a run of those
 __global__ void __cluster_dims__(kPC, 1, 1) __launch_bounds__(kPT) kv_compact_plan(CompactJob j) {
   dep_enter();
   __shared__ uint32_t red[32];
   const uint32_t P = j.v.pages, tid = plan_tid(), all = kPC * kPT;
-  const uint32_t per = (P + kPC - 1) / kPC, lo = min(P, blockIdx.x * per), hi = min(P, lo + per);
+  const uint32_t per = (P + all - 1) / all, lo = min((uint64_t)P, (uint64_t)tid * per), hi = min(P, lo + per);
   uint32_t n = 0, sum;
-  for (uint32_t p = lo + threadIdx.x; p < hi; p += kPT) n += j.ref[p] != 0u;
-  cta_scan(n, red, sum);
+  for (uint32_t p = lo; p < hi; p++) n += j.ref[p] != 0u;
+  uint32_t f = cta_scan(n, red, sum) - n;
   if (threadIdx.x == 0) j.cnt[blockIdx.x] = sum;
   tc::cluster_sync();
   uint32_t L = 0;
-  for (uint32_t k = 0; k < kPC; k++) L += __ldcg(&j.cnt[k]);
-  n = 0;
-  for (uint32_t p = lo + threadIdx.x; p < hi; p += kPT) n += (j.ref[p] != 0u) == (p >= L);   // movers, or holes
-  // a share that straddles L counts both kinds: split it into two sums
-  uint32_t nm = 0;
-  for (uint32_t p = lo + threadIdx.x; p < hi; p += kPT) nm += j.ref[p] != 0u && p >= L;
-  uint32_t both, movers;
-  cta_scan(n, red, both);
-  cta_scan(nm, red, movers);
-  if (threadIdx.x == 0) {
-    j.cnt[kPC + blockIdx.x] = movers;
-    j.cnt[2 * kPC + blockIdx.x] = both - movers;
-  }
-  tc::cluster_sync();
-  uint32_t m0 = 0, h0 = 0, M = 0;
   for (uint32_t k = 0; k < kPC; k++) {
-    const uint32_t m = __ldcg(&j.cnt[kPC + k]), h = __ldcg(&j.cnt[2 * kPC + k]);
-    if (k < blockIdx.x) { m0 += m; h0 += h; }
-    M += m;
+    const uint32_t c = __ldcg(&j.cnt[k]);
+    if (k < blockIdx.x) f += c;
+    L += c;
   }
-  for (uint32_t p0 = lo; p0 < hi; p0 += kPT) {
-    const uint32_t p = p0 + threadIdx.x;
-    const bool live = p < hi && j.ref[p] != 0u, mv = live && p >= L, ho = p < hi && !live && p < L;
-    uint32_t tm, th;
-    const uint32_t km = m0 + cta_scan(mv ? 1u : 0u, red, tm) - 1u, kh = h0 + cta_scan(ho ? 1u : 0u, red, th) - 1u;
-    if (mv) { j.mover[km] = p; j.rank[p] = km; }
-    if (ho) { j.hole[kh] = p; j.rank[p] = kh; }
-    m0 += tm;
-    h0 += th;
+  for (uint32_t p = lo; p < hi; p++) {
+    if (p == L) j.cnt[kPC] = f;
+    j.rank[p] = f;
+    if (j.ref[p]) j.live[f++] = p;
+    else if (p < L) j.hole[p - f] = p;
   }
+  if (tid == 0 && L == P) j.cnt[kPC] = L;
   tc::cluster_sync();
+  const uint32_t fL = __ldcg(&j.cnt[kPC]);
   for (uint64_t e = tid; e < (uint64_t)j.v.rows * j.v.ld; e += all) {
     uint32_t p = j.v.table[e];
-    if (p < P && p >= L && j.ref[p] != 0u) p = __ldcg(&j.hole[__ldcg(&j.rank[p])]);
+    if (p < P && p >= L && j.ref[p]) p = __ldcg(&j.hole[__ldcg(&j.rank[p]) - fL]);
     j.to_table[e] = p;
   }
   for (uint32_t p = tid; p < P; p += all) {
     uint32_t r = 0;
-    if (p < L) r = j.ref[p] ? j.ref[p] : j.ref[__ldcg(&j.mover[__ldcg(&j.rank[p])])];
+    if (p < L) r = j.ref[p] ? j.ref[p] : j.ref[__ldcg(&j.live[fL + p - __ldcg(&j.rank[p])])];
     j.to_ref[p] = r;
   }
   if (tid == 0) {
     j.stat[0] = L;
-    j.stat[1] = M;
+    j.stat[1] = L - fL;
   }
 }
 
@@ -477,10 +513,13 @@ __global__ void __launch_bounds__(kCopyT) kv_copy_tails(uint8_t *pool, uint64_t 
   copy_run(reinterpret_cast<const uint4 *>(pool + m.x * stride) + at, reinterpret_cast<uint4 *>(pool + m.y * stride) + at, n - at);
 }
 // kvCompact: the moves' runs of 16 KB dealt to a grid of fixed size (the host does not know the number of moves)
-__global__ void __launch_bounds__(kCopyT) kv_copy_moves(uint8_t *pool, uint64_t stride, const uint32_t *__restrict__ stat,
-                                                        const uint32_t *__restrict__ mover, const uint32_t *__restrict__ hole) {
+__global__ void __launch_bounds__(kCopyT) kv_copy_moves(uint8_t *pool, uint64_t stride, const uint32_t *__restrict__ cnt,
+                                                        const uint32_t *__restrict__ live, const uint32_t *__restrict__ hole) {
   dep_enter();
-  const uint64_t n = stride / 16, runs = (n + kCopyT * kCopyU - 1) / (kCopyT * kCopyU), all = runs * stat[1];
+  uint32_t L = 0;
+  for (uint32_t k = 0; k < kPC; k++) L += cnt[k];
+  const uint32_t *mover = live + cnt[kPC];
+  const uint64_t n = stride / 16, runs = (n + kCopyT * kCopyU - 1) / (kCopyT * kCopyU), all = runs * (L - cnt[kPC]);
   for (uint64_t r = blockIdx.x; r < all; r += gridDim.x) {
     const uint64_t k = r / runs, at = r % runs * (kCopyT * kCopyU);
     copy_run(reinterpret_cast<const uint4 *>(pool + mover[k] * stride) + at, reinterpret_cast<uint4 *>(pool + hole[k] * stride) + at, n - at);
@@ -499,7 +538,10 @@ p0_status rows_call(p0_ctx *c, const p0_kv4_rows_args *a, bool put) {
   if ((st = kv_rows(c, a->k, a->n, a->kv.nkv, a->kv.D, a->type, op, "k", &j.k))) return st;
   if ((st = kv_rows(c, a->v, a->n, a->kv.nkv, a->kv.D, a->type, op, "v", &j.vv))) return st;
   j.rec = const_cast<uint8_t *>(j.v.pool);
-  j.warps = (uint64_t)((a->n + 7) / 8) * a->kv.nkv * 2 * (a->kv.D / 32);
+  // a warp takes four groups; where there are few tokens, one
+  const uint64_t eights = (uint64_t)((a->n + 7) / 8) * a->kv.nkv * 2, G = a->kv.D / 32;
+  j.runs = (uint32_t)(eights < 8u * (uint32_t)c->sm_count ? G : (G + kGroups - 1) / kGroups);
+  j.warps = eights * j.runs;
   const uint64_t grid = (j.warps + kT / 32 - 1) / (kT / 32);
   if (grid > 0x7fffffffu) return p0_fail(c, P0_EINVAL, "%s: %u tokens in one call", op, a->n);
   const bool f16 = a->type == P0_F16, wide = j.k.wide && j.vv.wide;
@@ -593,13 +635,13 @@ p0_status p0_kv_compact(p0_ctx *c, const p0_kv_compact_args *a) {
   cudaSetDevice(c->device);
   if ((st = p0_workspace(c, 0, 256 + P * 12, &cnt, &ws))) return st;
   j.cnt = (uint32_t *)ws;
-  j.mover = (uint32_t *)((uint8_t *)ws + 256);
-  j.hole = j.mover + P;
+  j.live = (uint32_t *)((uint8_t *)ws + 256);
+  j.hole = j.live + P;
   j.rank = j.hole + P;
   launch_dep(kv_compact_plan, dim3(kPC), dim3(kPT), 0, c->stream, j);
   if ((st = p0_launched(c, op))) return st;
   launch_dep(kv_copy_moves, dim3((unsigned)c->sm_count * 8u), dim3(kCopyT), 0, c->stream, const_cast<uint8_t *>(j.v.pool), j.v.stride,
-             (const uint32_t *)j.stat, (const uint32_t *)j.mover, (const uint32_t *)j.hole);
+             (const uint32_t *)j.cnt, (const uint32_t *)j.live, (const uint32_t *)j.hole);
   return p0_launched(c, "kvCompact copy");
 }
 

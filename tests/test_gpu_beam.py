@@ -146,13 +146,28 @@ def test_strides_in_place(g):
     check((g.read(pt[0], 0, 24, np.uint32), g.read(pt[1], 0, 24, np.uint32), g.read(s, 0, 24, np.float32), g.read(f, 0, 24, np.uint32)), want)
 
 
+@pytest.mark.parametrize("order", ["rising", "falling", "steps"])
+def test_ordered_rows(g, order):
+    # rows in rising order: everything reaches the bound that the first logits gave
+    V = 70001
+    x = np.arange(V, dtype=np.float32)[None] * np.float32(1e-3) + np.zeros((4, 1), np.float32)
+    if order == "falling":
+        x = x[:, ::-1].copy()
+    if order == "steps":
+        x = np.floor(x * 10) / 10
+    x = x.astype(np.float32)
+    score = np.array([0.0, -0.25, -0.5, -7.0], np.float32)
+    for groups, k in ((1, 4), (2, 2), (4, 1)):
+        check(run(g, x, score, groups, k), R.beam(x, score, groups, k, None))
+
+
 def test_refusals(g):
     b = g.buffer(4000)
     a = {"logits": {"buf": b}, "score": {"buf": b}, "groups": 1, "beams": 4, "V": 100, "eos": 1, "parent": {"buf": b}, "token": {"buf": b},
          "scoreOut": {"buf": b}}
     for msg, change in (("17 beams", {"beams": 17}), ("0 beams", {"beams": 0}), ("pass 32 bits", {"V": 0xffffffff // 4 + 1}), ("row stride 99", {"logits": {"buf": b, "ld": 99}}),
                         ("logits range", {"V": 251}), ("eos 100 outside", {"eos": 100, "fin": {"buf": b}}), ("missing binding score", {"score": {"buf": None}}),
-                        ("65536 rows", {"groups": 16384}), ("at most 4096 chunks", {"V": 4 << 20 | 1})):
+                        ("65536 rows", {"groups": 16384}), ("a vocabulary of 16777217", {"V": 16777217})):
         with pytest.raises(p0.P0Error, match=msg):
             p0.beamSelect(g, {**a, **change})
     g.done()

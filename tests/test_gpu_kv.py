@@ -95,6 +95,27 @@ def test_put_page_equals_packed_weights_layout(g):
     assert np.array_equal(g.read(out, 0, 64 * 256 * 2, np.float16).reshape(64, 256).astype(np.float64), want)
 
 
+def test_put_halves_and_scales(g):
+    # quotients on, and next to, halves: groups whose scale is exactly 2^k, values at (n + 1/2) * 2^k and their neighbours
+    rng = np.random.default_rng(6)
+    c = R.Cache(rng, [640], 1, 64)
+    x = np.zeros((640, 2, 32), np.float32)
+    for t in range(640):
+        k = np.float32(2.0 ** rng.integers(-12, 8))
+        v = (rng.integers(0, 16, (2, 32)) + rng.choice([0.0, 0.5, 0.25], (2, 32))).astype(np.float32) * k
+        v = np.nextafter(v, np.where(rng.random((2, 32)) < 0.5, np.float32(-np.inf), np.float32(np.inf)), dtype=np.float32) if t % 2 else v
+        v[:, 0], v[:, 1] = 0, 15 * k
+        x[t] = np.clip(v, 0, 15 * k) + (rng.integers(-8, 8) * k if t % 3 == 0 else 0)
+    x = x.reshape(640, 64)
+    bufs, kv = kv_args(g, c)
+    xb = g.upload(x)
+    p0.kv4Put(g, {"kv": kv, "k": {"buf": xb}, "v": {"buf": xb}, "type": "f32", "n": 640, "T": 640})
+    for t in range(640):
+        c.write(0, t, 0, 0, x[t])
+        c.write(0, t, 1, 0, x[t])
+    assert np.array_equal(g.read(bufs["pool"], 0, c.pool.nbytes).reshape(c.pool.shape), c.pool)
+
+
 def test_put_drops_tokens_without_a_page(g):
     rng = np.random.default_rng(4)
     c = R.Cache(rng, [100, 70], 1, 64)
