@@ -76,6 +76,36 @@ def test_attn(g, lens, counts, nh, nkv, D, window, sinks, type_):
     check(got, c, q, counts, nh, type_, window, sinks)
 
 
+# contexts (and tables) long enough that whole pages go to warps
+LONG = [
+    # lens, nh, nkv, D, window, sinks
+    ([9000, 700, 0, 4097, 64, 1], 8, 1, 256, 0, 0),
+    ([5000, 12000], 8, 2, 256, 6000, 70),
+    ([70, 8000, 3333, 10], 4, 4, 128, 0, 0),
+    ([6000, 2500, 7777], 16, 2, 64, 4000, 4),
+]
+
+
+@pytest.mark.parametrize("type_", ["f32", "f16"])
+@pytest.mark.parametrize("lens,nh,nkv,D,window,sinks", LONG)
+def test_attn_long(g, lens, nh, nkv, D, window, sinks, type_):
+    rng = np.random.default_rng(D + len(lens))
+    c = R.Cache(rng, lens, nkv, D, ld=2500)
+    c.fill_fast(rng)
+    c.table[0, 3], c.table[-1, 0] = c.pages + 1, R.NONE if lens[-1] > 100 else c.table[-1, 0]
+    for b, n in enumerate(lens):
+        seen = set(np.nonzero(R.visible(n - 1, n, window, sinks))[0].tolist())
+        c.poison_unseen(b, seen)
+    q = (rng.standard_normal((len(lens), nh, D)) * (3.0 / D ** 0.5)).astype(np.float32 if type_ == "f32" else np.float16)
+    got = run(g, c, q, [1] * len(lens), nh, type_, window, sinks)
+    want, spread, size = R.attention(c, q, [1] * len(lens), nh, window, sinks)
+    tol = R.attention_bound(spread, size, want, D, 200, type_ == "f16")
+    err = np.abs(got.astype(np.float64) - want)
+    assert np.all(err <= tol), float((err / tol).max())
+    assert not got[~spread.any(-1)].any()
+    assert np.array_equal(run(g, c, q, [1] * len(lens), nh, type_, window, sinks).view(np.uint8), got.view(np.uint8))
+
+
 PROMPTS = [
     # lens, new tokens, nh, nkv, D, window, sinks, scale
     ([1900], [700], 8, 1, 256, 0, 0, 0.0),                           # several key tiles a run, parts of units joined
