@@ -59,14 +59,14 @@ __device__ __forceinline__ uint32_t lds_u32(const uint8_t *p) { return *reinterp
 
 constexpr uint32_t kRec = 1312;   // a K record's place in shared memory
 
-template <int D, bool F32, int NPL, int RT, int KP>
+template <int D, bool F32, int NPL, int RT, int KP, int NW>
 struct Cfg {
-  static constexpr int kNW = 8, kThreads = kNW * 32;
+  static constexpr int kThreads = NW * 32;
   static constexpr int kRowsPer = F32 ? 8 : 16;          // query rows per fragment
   static constexpr int kRows = kRowsPer * RT;            // of a block
-  static constexpr int kNt = 8 * KP / kNW;               // 8-key tiles per warp in Q K^T
+  static constexpr int kNt = 8 * KP / NW;               // 8-key tiles per warp in Q K^T
   static constexpr int kDs = D / (8 * NPL);              // warps over the dims in P V (NPL dims a lane and key),
-  static constexpr int kKs = kNW / kDs;                  // and over the keys
+  static constexpr int kKs = NW / kDs;                  // and over the keys
   static constexpr int kSteps = KP * 4 / kKs;            // 16-key steps per warp
   static constexpr uint32_t kRecs = D / 32, kPart = kRecs * 1280, kK = kRecs * kRec, kPage2 = kK + kPart;   // K and V of a page
   static constexpr uint32_t kStage = KP * kPage2;
@@ -78,11 +78,11 @@ struct Cfg {
   static_assert(kKs == 1 || (uint32_t)(RT * D * 64) <= kStages * kStage, "the key shares meet in the ring");
 };
 
-template <int D, bool F32, int NPL, int RT, int KP>
-__global__ void __launch_bounds__(256) kv4_attn_kernel(AttnJob j) {
+template <int D, bool F32, int NPL, int RT, int KP, int NW>
+__global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel(AttnJob j) {
   dep_enter();
-  using C = Cfg<D, F32, NPL, RT, KP>;
-  constexpr int NT = C::kNt, RR = C::kRowsPer, RB = C::kRows, NS = C::kStages, NW = C::kNW;
+  using C = Cfg<D, F32, NPL, RT, KP, NW>;
+  constexpr int NT = C::kNt, RR = C::kRowsPer, RB = C::kRows, NS = C::kStages;
   constexpr int KW = D >= 128 ? 4 : 2;   // a lane's K words at a time: of one group (D = 64: half of one)
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t *ring = smem;
@@ -314,8 +314,11 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(AttnJob j) {
         for (int h = 0; h < RH; h++) {
           const uint32_t r = rt * RR + g4 + 8 * h;
           float mn = m[rt][h];
-          const float4 wa = *reinterpret_cast<const float4 *>(&wmax[r][0]), wb = *reinterpret_cast<const float4 *>(&wmax[r][4]);
-          mn = fmaxf(mn, fmaxf(fmaxf(fmaxf(wa.x, wa.y), fmaxf(wa.z, wa.w)), fmaxf(fmaxf(wb.x, wb.y), fmaxf(wb.z, wb.w))));
+#pragma unroll
+          for (int w = 0; w < NW; w += 4) {
+            const float4 x4 = *reinterpret_cast<const float4 *>(&wmax[r][w]);
+            mn = fmaxf(mn, fmaxf(fmaxf(x4.x, x4.y), fmaxf(x4.z, x4.w)));
+          }
           const float ref = mn == -INFINITY ? 0.0f : mn;
           keep[h] = mn == m[rt][h] ? 1.0f : ex(m[rt][h] - ref);   // 0 while nothing has been seen
           m[rt][h] = mn;
@@ -540,397 +543,11 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnJob j) {
   }
 }
 
-// ---------------------------------------------------------------- one fragment of rows: a page a warp
-// The same arithmetic for batches of long contexts with at most one fragment of rows per KV head (D <= 256): a warp takes
-// whole pages on its own, with its own m, l and O over all dims, so there is no barrier and no P in shared memory between
-// its pages (the score fragments of two key tiles are the P fragment of P V); the warps' results meet when the unit ends.
-// About 2700 warp instructions a page of D = 256, against 4000 where eight warps share it. A warp's K slot is filled again
-// as soon as the scores are made, its V slot after P V: either copy has half a page's work to arrive.
-template <int D, bool F32>
-struct WCfg {
-  static constexpr int kNW = D >= 128 ? 8 : 12, kThreads = kNW * 32;
-  static constexpr int kRows = F32 ? 8 : 16;
-  static constexpr uint32_t kRecs = D / 32, kPart = kRecs * 1280, kK = kRecs * kRec, kSlot = kK + kPart;
-  static constexpr uint32_t kQ = D / 16 * 512;
-  static constexpr uint32_t kSmem = kNW * kSlot + kQ;
-  static constexpr uint32_t kE = 6;   // pages of a run that a unit's beginning and end cost
-  static_assert(kRows * D * 4 <= (int)kSlot, "a warp's O goes into its own slot");
-};
-
-template <int D, bool F32>
-__global__ void __launch_bounds__(WCfg<D, F32>::kThreads, 1) kv4_attn_pages_kernel(AttnJob j) {
-  dep_enter();
-  using C = WCfg<D, F32>;
-  constexpr int NW = C::kNW, RB = C::kRows, RH = F32 ? 1 : 2, SEG = D / 64;
-  constexpr int KW = D >= 128 ? 4 : 2, KG = D >= 128 ? D / 128 : 1;
-  extern __shared__ __align__(16) uint8_t smem[];
-  uint4 *qf = reinterpret_cast<uint4 *>(smem + NW * C::kSlot);
-  uint32_t *pre = reinterpret_cast<uint32_t *>(smem + C::kSmem);   // [rows + 1] items before each sequence
-  __shared__ __align__(8) uint64_t kbar[NW], vbar[NW];
-  __shared__ uint32_t abort_flag;
-  __shared__ float wm[RB][NW], wl[RB][NW];
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g4 = lane >> 2, t4 = lane & 3u;
-  const uint32_t hpg = j.hpg, R = j.v.rows, W = j.window, S = j.sinks;
-  uint8_t *ks = smem + warp * C::kSlot, *vs = ks + C::kK;
-  if (tid == 0) {
-    for (int i = 0; i < NW; i++) {
-      tc::mbar_init(&kbar[i], 1);
-      tc::mbar_init(&vbar[i], 1);
-    }
-    abort_flag = 0u;
-    tc::fence_mbar_init();
-  }
-  plan_items<RB, 1, C::kE>(j, pre);
-  const uint32_t total = pre[R], G = min(gridDim.x, max(total, 1u));   // no run is empty
-  if (tid == 0) j.desc[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
-  if (blockIdx.x >= G) return;
-  const uint32_t lo = (uint32_t)((uint64_t)total * blockIdx.x / G), hi = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / G);
-  uint32_t b = find_sequence(pre, R, lo);
-  const float scale = F32 ? j.scale : j.scale * 1.44269504088896340736f;   // f16: scores and maxima in powers of two
-  const auto ex = [](float x) { return exp2_fast(F32 ? x * 1.44269504088896340736f : x); };
-  uint32_t kuse = 0, vuse = 0;   // of this warp's barriers
-  bool lost = false;
-  for (uint32_t at = lo; at < hi;) {   // a warp that gave up a wait still walks the units and their barriers
-    while (pre[b + 1] <= at) b++;
-    const Unit u = find_unit<RB, 1, C::kE>(j, pre, b, at);
-    const Span &s = u.s;
-    const uint32_t from = max(at - u.begin, C::kE) - C::kE, nt = u.n - C::kE, end = min(hi - u.begin, u.n), to = max(end, C::kE) - C::kE;
-    at = u.begin + end;
-    if (from == to) continue;   // this run holds none of the unit's pages
-    const uint32_t steps = s.n ? to - from : 0u, nrow = min((uint32_t)RB, u.rows - u.r0);
-    const uint8_t *heads = j.v.pool + (uint64_t)u.head * 2u * C::kPart;
-    const uint32_t *trow = j.v.table + (uint64_t)b * j.v.ld;
-    const auto look_up = [&](uint32_t i) { return i < steps ? trow[page_at(s, from + i)] : P0_KV_NONE; };
-    const auto copy_k = [&](uint32_t p) {   // a record a lane
-      if (p >= j.v.pages) return;
-      if (lane == 0) tc::mbar_expect_tx(&kbar[warp], C::kPart);
-      __syncwarp();
-      if (lane < C::kRecs) bulk_load(ks + lane * kRec, heads + p * j.v.stride + lane * 1280u, 1280u, &kbar[warp]);
-    };
-    const auto copy_v = [&](uint32_t p) {
-      if (p >= j.v.pages || lane) return;
-      tc::mbar_expect_tx(&vbar[warp], C::kPart);
-      bulk_load(vs, heads + p * j.v.stride + C::kPart, C::kPart, &vbar[warp]);
-    };
-    // this warp's pages: from + warp, + NW, ..; one is in the slots, the next one's number is known, the one after looked up
-    uint32_t p_now = look_up(warp), p_next = look_up(warp + NW);
-    if (!lost) {
-      copy_k(p_now);
-      copy_v(p_now);
-    }
-    // q fragments, as for kv4_attn_kernel
-    for (uint32_t e = tid; e < (D / 16) * 32u; e += C::kThreads) {
-      const uint32_t ln = e & 31u, step = e >> 5, wi = step >> 1, l4 = ln & 3u;
-      const uint32_t d0 = (D >= 128 ? ((wi >> 2) * 4u + l4) * 32u + (wi & 3u) * 8u : l4 * 16u + wi * 8u) + (step & 1u) * 2u;
-      float x[2][4] = {};
-#pragma unroll
-      for (int half = 0; half < RH; half++) {
-        const uint32_t r = (ln >> 2) + 8u * half;
-        if (r < nrow) {
-          const uint64_t o = (uint64_t)(u.first + (u.r0 + r) / hpg) * j.q.ld + (uint64_t)(u.head * hpg + (u.r0 + r) % hpg) * j.q.ldh + d0;
-          if (F32) {
-            const float *q = reinterpret_cast<const float *>(j.q.base) + o;
-            x[half][0] = q[0]; x[half][1] = q[4]; x[half][2] = q[1]; x[half][3] = q[5];
-          } else {
-            const __half *q = reinterpret_cast<const __half *>(j.q.base) + o;
-            x[half][0] = __half2float(q[0]); x[half][1] = __half2float(q[4]); x[half][2] = __half2float(q[1]); x[half][3] = __half2float(q[5]);
-          }
-        }
-      }
-      uint4 f;
-      f.x = pack2(x[0][0], x[0][1]);
-      f.z = pack2(x[0][2], x[0][3]);
-      if (F32) {
-        const float2 h0 = __half22float2(*reinterpret_cast<const __half2 *>(&f.x)), h1 = __half22float2(*reinterpret_cast<const __half2 *>(&f.z));
-        f.y = pack2(x[0][0] - h0.x, x[0][1] - h0.y);
-        f.w = pack2(x[0][2] - h1.x, x[0][3] - h1.y);
-      } else {
-        f.y = pack2(x[1][0], x[1][1]);
-        f.w = pack2(x[1][2], x[1][3]);
-      }
-      qf[e] = f;
-    }
-    float o[SEG][8][4], m[RH], l[RH];
-    int32_t pos[RH];
-#pragma unroll
-    for (int g = 0; g < SEG; g++)
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[g][i][e] = 0.0f;
-#pragma unroll
-    for (int h = 0; h < RH; h++) {
-      const uint32_t r = g4 + 8 * h;
-      m[h] = -INFINITY;
-      l[h] = 0.0f;
-      pos[h] = r < nrow ? (int32_t)(u.len - u.T + (u.r0 + r) / hpg) : -1;
-    }
-    const int32_t pos0 = (int32_t)(u.len - u.T + u.r0 / hpg), pos1 = (int32_t)s.end - 1;   // of the block's rows
-    __syncthreads();
-    for (uint32_t i = warp; i < steps && !lost; i += NW) {
-      const int32_t k0 = (int32_t)(page_at(s, from + i) * kPage);
-      const bool here = p_now < j.v.pages;
-      const uint32_t p_after = look_up(i + 2 * NW);
-      if (here) {
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(&kbar[warp], kuse & 1u, &abort_flag, j.err, 0x4d1u, P0_SPIN_LIMIT))) { lost = true; break; }
-        kuse++;
-        // ---- S = Q K^T, four of the page's 8-key tiles at a time
-        float sc[8][4];
-#pragma unroll
-        for (int n = 0; n < 8; n++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) sc[n][e] = 0.0f;
-#pragma unroll
-        for (int n0 = 0; n0 < 8; n0 += 4)
-#pragma unroll
-          for (int g = 0; g < KG; g++) {
-            const uint8_t *rec = ks + (D >= 128 ? g * 4 * kRec + t4 * kRec : (t4 >> 1) * kRec);
-            uint32_t w[4][KW], s2[4], mn2[4];
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-              const uint32_t key = (n0 + n) * 8u + g4;
-              if constexpr (KW == 4) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(rec + key * 16u);
-                w[n][0] = x.x; w[n][1] = x.y; w[n][2] = x.z; w[n][3] = x.w;
-              } else {
-                const uint2 x = *reinterpret_cast<const uint2 *>(rec + key * 16u + (t4 & 1u) * 8u);
-                w[n][0] = x.x; w[n][1] = x.y;
-              }
-              const uint32_t sm = lds_u32(rec + 1024 + key * 4u);
-              s2[n] = __byte_perm(sm, 0, 0x1010);
-              mn2[n] = __byte_perm(sm, 0, 0x3232);
-            }
-#pragma unroll
-            for (int wi = 0; wi < KW; wi++) {
-              const uint4 f0 = qf[2 * (g * KW + wi) * 32 + lane], f1 = qf[(2 * (g * KW + wi) + 1) * 32 + lane];
-              const uint32_t a0[4] = {f0.x, f0.y, f0.z, f0.w}, a1[4] = {f1.x, f1.y, f1.z, f1.w};
-#pragma unroll
-              for (int n = 0; n < 4; n++) {
-                uint32_t kb[4];
-                kv_deq8(w[n][wi], s2[n], mn2[n], kb);   // dims (e, e + 4)
-                mma_f16(sc[n0 + n], a0, kb[0], kb[1]);
-                mma_f16(sc[n0 + n], a1, kb[2], kb[3]);
-              }
-            }
-          }
-        __syncwarp();
-        copy_k(p_next);
-        // ---- mask (a page that the whole block sees needs none), the row maxima
-        float mx[RH];
-#pragma unroll
-        for (int h = 0; h < RH; h++) mx[h] = -INFINITY;
-        const bool plain = k0 + 63 <= pos0 && (!W || k0 > pos1 - (int32_t)W || (uint32_t)k0 + 63u < S);
-#pragma unroll
-        for (int n = 0; n < 8; n++)
-#pragma unroll
-          for (int h = 0; h < RH; h++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              float &x = sc[n][2 * h + e];
-              x = (F32 ? sc[n][e] + sc[n][e + 2] : x) * scale;
-            }
-        if (!plain) {
-#pragma unroll
-          for (int n = 0; n < 8; n++)
-#pragma unroll
-            for (int h = 0; h < RH; h++)
-#pragma unroll
-              for (int e = 0; e < 2; e++) {
-                const int32_t key = k0 + (int32_t)(n * 8u + 2u * t4) + e;
-                if (!(key <= pos[h] && (!W || key > pos[h] - (int32_t)W || (uint32_t)key < S))) sc[n][2 * h + e] = -INFINITY;
-              }
-        }
-#pragma unroll
-        for (int h = 0; h < RH; h++) {
-#pragma unroll
-          for (int n = 0; n < 8; n++) mx[h] = fmaxf(mx[h], fmaxf(sc[n][2 * h], sc[n][2 * h + 1]));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        }
-        // ---- P = exp(x - m): the P fragment of 16 keys is the scores' of two tiles (f32: low parts in rows + 8)
-        uint32_t pa[4][4];
-        float keep[RH];
-#pragma unroll
-        for (int h = 0; h < RH; h++) {
-          const float mn = fmaxf(m[h], mx[h]), ref = mn == -INFINITY ? 0.0f : mn;
-          keep[h] = mn == m[h] ? 1.0f : ex(m[h] - ref);   // 0 while nothing has been seen
-          m[h] = mn;
-          l[h] *= keep[h];
-#pragma unroll
-          for (int n = 0; n < 8; n++) {
-            const float p0 = ex(sc[n][2 * h] - ref), p1 = ex(sc[n][2 * h + 1] - ref);
-            l[h] += p0 + p1;
-            const uint32_t hi2 = pack2(p0, p1);
-            pa[n / 2][2 * (n & 1) + h] = hi2;
-            if (F32) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi2));
-              pa[n / 2][2 * (n & 1) + 1] = pack2(p0 - f.x, p1 - f.y);
-            }
-          }
-        }
-        if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[RH - 1] != 1.0f)) {
-#pragma unroll
-          for (int g = 0; g < SEG; g++)
-#pragma unroll
-            for (int n = 0; n < 8; n++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) o[g][n][e] *= keep[F32 ? 0 : e >> 1];
-        }
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(&vbar[warp], vuse & 1u, &abort_flag, j.err, 0x4d2u, P0_SPIN_LIMIT))) { lost = true; break; }
-        vuse++;
-        // slots that no row of the unit sees hold zeros, whatever the memory holds: their (s, mn)
-        if ((uint32_t)k0 + kPage > s.end || ((uint32_t)k0 < s.first_pos && (uint32_t)k0 + kPage > S)) {
-          for (uint32_t e = lane; e < 64u * C::kRecs; e += 32u) {
-            const uint32_t key = (uint32_t)k0 + (e & 63u);
-            if (key >= s.end || (key < s.first_pos && key >= S)) *reinterpret_cast<uint32_t *>(vs + (e >> 6) * 1280u + 1024u + (e & 63u) * 4u) = 0u;
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy into the slot
-          __syncwarp();
-        }
-        // ---- O += P V, 64 dims at a time
-        const uint32_t swap = (g4 >> 2) & 1u;   // the second group of 32 dims starts with the odd key: other banks
-#pragma unroll
-        for (int g = 0; g < SEG; g++) {
-          float c[8][4];
-          const uint8_t *vg = vs + (2 * g + (g4 >> 2)) * 1280u, *vw = vg + (g4 & 3u) * 4u;
-#pragma unroll
-          for (int k4 = 0; k4 < 4; k4++) {
-            uint32_t vb[2][8];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const uint32_t key = k4 * 16 + h * 8 + 2 * t4;
-              const uint32_t w0 = lds_u32(vw + (key + swap) * 16u), w1 = lds_u32(vw + (key + 1u - swap) * 16u);
-              const uint2 sm = *reinterpret_cast<const uint2 *>(vg + 1024u + key * 4u);
-              const uint32_t s2 = __byte_perm(sm.x, sm.y, 0x5410), mn2 = __byte_perm(sm.x, sm.y, 0x7632);   // (key, key + 1)
-              kv_deq8(__byte_perm(w0, w1, swap ? 0x1054u : 0x5410u), s2, mn2, vb[h]);
-              kv_deq8(__byte_perm(w0, w1, swap ? 0x3276u : 0x7632u), s2, mn2, vb[h] + 4);
-            }
-#pragma unroll
-            for (int n = 0; n < 8; n++) {
-              if (!F32) mma_f16(o[g][n], pa[k4], vb[0][n], vb[1][n]);
-              else if (k4 == 0) mma_f16_zero(c[n], pa[k4], vb[0][n], vb[1][n]);
-              else mma_f16(c[n], pa[k4], vb[0][n], vb[1][n]);
-            }
-          }
-          if (F32) {
-#pragma unroll
-            for (int n = 0; n < 8; n++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) o[g][n][e] += c[n][e];
-          }
-        }
-        __syncwarp();
-        copy_v(p_next);
-      } else {   // no such page: its keys are not there
-        copy_k(p_next);
-        copy_v(p_next);
-      }
-      p_now = p_next;
-      p_next = p_after;
-    }
-    // ---- the warps' results meet: O in their own slots (no copy is in flight)
-#pragma unroll
-    for (int h = 0; h < RH; h++) {
-      float t = l[h];
-      t += __shfl_xor_sync(0xffffffffu, t, 1);
-      t += __shfl_xor_sync(0xffffffffu, t, 2);
-      if (t4 == 0) {
-        wm[g4 + 8 * h][warp] = m[h];
-        wl[g4 + 8 * h][warp] = t;
-      }
-    }
-    if (!lost) {
-      float *ow = reinterpret_cast<float *>(ks);
-#pragma unroll
-      for (int h = 0; h < RH; h++)
-#pragma unroll
-        for (int g = 0; g < SEG; g++)
-#pragma unroll
-          for (int e = 0; e < 2; e++)
-#pragma unroll
-            for (int n = 0; n < 8; n += 4) {
-              float y[4];
-#pragma unroll
-              for (int i = 0; i < 4; i++) y[i] = F32 ? o[g][n + i][e] + o[g][n + i][e + 2] : o[g][n + i][2 * h + e];
-              *reinterpret_cast<float4 *>(ow + (g4 + 8 * h) * D + g * 64 + (2 * t4 + e) * 8 + n) = make_float4(y[0], y[1], y[2], y[3]);
-            }
-    }
-    if (__syncthreads_or(lost)) {   // a copy did not arrive in time: j.err says so. Those in flight land before the CTA leaves (bounded)
-      for (uint32_t k = 0; k < (1u << 16) && !tc::mbar_try(&kbar[warp], kuse & 1u); k++) {}
-      for (uint32_t k = 0; k < (1u << 16) && !tc::mbar_try(&vbar[warp], vuse & 1u); k++) {}
-      return;
-    }
-    const bool whole = from == 0 && to == nt;
-    // a run has at most one part of a unit that began earlier (slot 0) and one of a unit that goes on after it (slot 1)
-    float *part = j.part + ((uint64_t)blockIdx.x * 2u + (from ? 0u : 1u)) * RB * (D + 2);
-    if (!whole && from == 0 && tid == 0) j.desc[blockIdx.x] = make_uint4(1u + run_of(u.begin + u.n - 1u, total, G), b, u.r0, u.head);
-    for (uint32_t e = tid; e < nrow * (D / 4); e += C::kThreads) {
-      const uint32_t r = e / (D / 4), d = e % (D / 4) * 4u;
-      float M = -INFINITY, sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < NW; w++) M = fmaxf(M, wm[r][w]);
-      const float ref = M == -INFINITY ? 0.0f : M;
-      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int w = 0; w < NW; w++) {
-        const float f = ex(wm[r][w] - ref);
-        if (f == 0.0f) continue;
-        const float4 x = *reinterpret_cast<const float4 *>(smem + w * C::kSlot + (r * D + d) * 4u);
-        sum = fmaf(f, wl[r][w], sum);
-        y.x = fmaf(f, x.x, y.x);
-        y.y = fmaf(f, x.y, y.y);
-        y.z = fmaf(f, x.z, y.z);
-        y.w = fmaf(f, x.w, y.w);
-      }
-      if (whole) {
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-        const float z[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
-        const uint64_t q = (uint64_t)(u.first + (u.r0 + r) / hpg) * j.out.ld + (uint64_t)(u.head * hpg + (u.r0 + r) % hpg) * j.out.ldh + d;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          if (F32) reinterpret_cast<float *>(j.out.base)[q + i] = z[i];
-          else reinterpret_cast<__half *>(j.out.base)[q + i] = __float2half_rn(z[i]);
-        }
-      } else {
-        float *p = part + (uint64_t)r * (D + 2);
-        *reinterpret_cast<float2 *>(p + d) = make_float2(y.x, y.y);
-        *reinterpret_cast<float2 *>(p + d + 2) = make_float2(y.z, y.w);
-        if (d == 0) {
-          p[D] = M;
-          p[D + 1] = sum;
-        }
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the slots were written: before the next unit's copies
-    __syncthreads();
-  }
-}
-
-template <int D, bool F32>
-p0_status pages_launch(p0_ctx *c, AttnJob &j) {
-  using C = WCfg<D, F32>;
-  const size_t smem = C::kSmem + ((size_t)j.v.rows + 1) * 4;
-  const auto kern = kv4_attn_pages_kernel<D, F32>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) { cudaGetLastError(); return p0_fail(c, P0_EDEVICE, "kv4Attn: the kernel does not fit this device"); }
-  const uint32_t G = (uint32_t)c->sm_count;
-  uint32_t *cnt;
-  void *ws;
-  p0_status st = p0_workspace(c, 0, (size_t)G * sizeof(uint4) + (size_t)G * 2 * C::kRows * (D + 2) * 4, &cnt, &ws);
-  if (st) return st;
-  j.desc = (uint4 *)ws;
-  j.part = (float *)(j.desc + G);
-  launch_dep(kern, dim3(G), dim3(C::kThreads), smem, c->stream, j);
-  if ((st = p0_launched(c, "kv4Attn"))) return st;
-  launch_dep(kv4_attn_join_kernel<D, F32, C::kRows>, dim3(G, C::kRows), dim3(256), 0, c->stream, j);
-  return p0_launched(c, "kv4Attn join");
-}
-
-template <int D, bool F32, int NPL, int RT, int KP>
+template <int D, bool F32, int NPL, int RT, int KP, int NW>
 p0_status attn_launch(p0_ctx *c, AttnJob &j) {
-  using C = Cfg<D, F32, NPL, RT, KP>;
+  using C = Cfg<D, F32, NPL, RT, KP, NW>;
   const size_t smem = C::kSmem + ((size_t)j.v.rows + 1) * 4;
-  const auto kern = kv4_attn_kernel<D, F32, NPL, RT, KP>;
+  const auto kern = kv4_attn_kernel<D, F32, NPL, RT, KP, NW>;
   int per = 0;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, C::kThreads, smem);
@@ -953,14 +570,15 @@ p0_status attn_launch(p0_ctx *c, AttnJob &j) {
 // the sums fill the registers; four of f32 take 32 dims a warp instead of 64)
 template <int D, bool F32, int KP>
 p0_status pick(p0_ctx *c, AttnJob &j, uint32_t frags) {
-  // a page a warp pays where there may be several pages for each (the lengths are on the device: what the table and the
-  // window allow decides); with fewer, eight warps at a page are done sooner
+  // One fragment and room for many pages (the lengths are on the device: what the table and the window allow decides): four
+  // warps and a page an item, four CTAs to an SM that do not wait for one another at the barriers. 32 contexts up to 65500
+  // keys: 117 us, with eight warps and two pages 123; 8 contexts of 10 pages: 14.1 and 12.2
   const uint64_t most = j.window ? min((uint64_t)j.v.ld, (uint64_t)j.window / kPage + 2 + (j.sinks + kPage - 1) / kPage) : j.v.ld;
   if constexpr (D < 512)
-    if (frags <= 1 && most * j.v.rows * j.v.nkv >= 16ull * c->sm_count) return pages_launch<D, F32>(c, j);
-  if (frags <= 1) return attn_launch<D, F32, 8, 1, KP>(c, j);
-  if (frags == 2 || D == 512) return attn_launch<D, F32, 8, 2, KP>(c, j);
-  if constexpr (D < 512) return attn_launch<D, F32, F32 ? 4 : 8, 4, KP>(c, j);
+    if (frags <= 1 && most * j.v.rows * j.v.nkv >= 16ull * c->sm_count) return attn_launch<D, F32, 8, 1, 1, 4>(c, j);
+  if (frags <= 1) return attn_launch<D, F32, 8, 1, KP, 8>(c, j);
+  if (frags == 2 || D == 512) return attn_launch<D, F32, 8, 2, KP, 8>(c, j);
+  if constexpr (D < 512) return attn_launch<D, F32, F32 ? 4 : 8, 4, KP, 8>(c, j);
   return P0_OK;
 }
 
