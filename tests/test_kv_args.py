@@ -126,3 +126,11 @@ def test_ref_beam_by_hand():
     parent, token, score, fin = R.beam(x, np.array([0.0, -1.0], np.float32), 1, 2, 0)
     assert parent.tolist() == [0, 1] and token.tolist() == [0, 0] and fin.tolist() == [1, 1]
     assert np.allclose(score, [np.log(0.5), -1 + np.log(0.9)])
+
+
+def test_beam_search_refuses_its_width():
+    from p0pc0rn_b200 import beam
+    cfg = {"beams": 9, "D": 512, "NH": 4, "NKV": 1, "hd": 128, "FF": 512, "vocab": 64, "kinds": ["full"], "eos": 0}
+    for m in (0, 9):
+        with pytest.raises(ValueError, match="1 to 8"):
+            beam.BeamSearch(None, {**cfg, "beams": m}, None, 64)
