@@ -597,6 +597,7 @@ extern "C" p0_status p0_kv4_attn(p0_ctx *c, const p0_kv4_attn_args *a) {
   if ((st = kv_rows(c, a->q, a->n, a->nh, a->kv.D, a->type, op, "q", &j.q))) return st;
   if ((st = kv_rows(c, a->out, a->n, a->nh, a->kv.D, a->type, op, "out", &j.out))) return st;
   j.hpg = a->nh / a->kv.nkv;
+  j.units = a->kv.nkv;
   const uint32_t most = a->kv.table_ld * kPage;          // no position is that large, so positions and bounds fit 31 bits
   j.window = a->window < most ? a->window : 0u;          // a longer window hides nothing
   j.sinks = a->sinks < most ? a->sinks : most;

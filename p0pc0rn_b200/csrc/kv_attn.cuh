@@ -8,7 +8,7 @@
 struct AttnJob {
   KvView v;
   KvRows q, out;
-  uint32_t hpg, window, sinks;
+  uint32_t hpg, window, sinks, units;   // units: of a row block (KV heads; times the parts that an output row is cut into)
   float scale;
   uint32_t *err;
   float *part;        // [grid][2][rows of a block][D + 2]
@@ -51,7 +51,7 @@ __device__ __forceinline__ void warp_sums(uint32_t *v, uint32_t n) {
 }
 
 // Work. The query rows that share a KV head (new tokens x query heads of its group) form blocks of RB; a unit is one row
-// block of one sequence and KV head, its items are the runs of PP pages that any of its rows sees (one item where there are
+// block of one sequence and KV head (or part of its output), its items are the runs of PP pages that any of its rows sees (one item where there are
 // none: zeros are to be written), after E items that stand for what beginning and ending a unit costs. pre[b] = items
 // before sequence b; [rows + 1] shared words. Every thread of the CTA.
 template <uint32_t RB, uint32_t PP, uint32_t E>
@@ -68,7 +68,7 @@ __device__ __forceinline__ void plan_items(const AttnJob &j, uint32_t *pre) {
       uint32_t lo;
       const uint32_t T = kv_tokens(j.v, b, lo);
       Span s;
-      pre[b + 1] = T ? unit_items<RB, PP, E>(j, kv_len(j.v, b), T, 0, s) * j.v.nkv : 0u;
+      pre[b + 1] = T ? unit_items<RB, PP, E>(j, kv_len(j.v, b), T, 0, s) * j.units : 0u;
     }
   } else {                                 // a warp each
     for (uint32_t b = threadIdx.x >> 5; b < R; b += blockDim.x >> 5) {
@@ -80,7 +80,7 @@ __device__ __forceinline__ void plan_items(const AttnJob &j, uint32_t *pre) {
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) items += __shfl_xor_sync(0xffffffffu, items, o);
-      if ((threadIdx.x & 31u) == 0) pre[b + 1] = items * j.v.nkv;
+      if ((threadIdx.x & 31u) == 0) pre[b + 1] = items * j.units;
     }
   }
   if (threadIdx.x == 0) pre[0] = 0u;
@@ -100,7 +100,7 @@ __device__ __forceinline__ uint32_t find_sequence(const uint32_t *pre, uint32_t 
 
 struct Unit {
   uint32_t first, T, len, rows;      // of its sequence: first token of the call, new tokens, length, query rows
-  uint32_t r0, head, begin, n;       // first row, KV head, first item and items
+  uint32_t r0, head, begin, n;       // first row, KV head (times parts, plus part), first item and items
   Span s;
 };
 // the unit of item `at` of sequence b: row blocks in order, each with its KV heads in order. A whole warp.
@@ -110,13 +110,13 @@ __device__ __forceinline__ Unit find_unit(const AttnJob &j, const uint32_t *pre,
   u.T = kv_tokens(j.v, b, u.first);
   u.len = kv_len(j.v, b);
   u.rows = u.T * j.hpg;
-  const uint32_t lane = threadIdx.x & 31u, nkv = j.v.nkv;
+  const uint32_t lane = threadIdx.x & 31u, units = j.units;
   uint32_t base = pre[b];
   for (uint32_t r = 0; r < u.rows; r += 32u * RB) {
     const uint32_t r0 = r + lane * RB;
     Span s;
     const uint32_t n = r0 < u.rows ? unit_items<RB, PP, E>(j, u.len, u.T, r0, s) : 0u;
-    uint32_t sum = n * nkv;
+    uint32_t sum = n * units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -127,7 +127,7 @@ __device__ __forceinline__ Unit find_unit(const AttnJob &j, const uint32_t *pre,
       const int k = __ffs(hit) - 1;
       u.r0 = r + k * RB;
       u.n = __shfl_sync(0xffffffffu, n, k);
-      base += __shfl_sync(0xffffffffu, sum, k) - u.n * nkv;
+      base += __shfl_sync(0xffffffffu, sum, k) - u.n * units;
       u.head = (at - base) / u.n;
       u.begin = base + u.head * u.n;
       unit_items<RB, PP, E>(j, u.len, u.T, u.r0, u.s);

@@ -23,20 +23,23 @@
 namespace {
 
 constexpr uint32_t kRB = 256, kCR = 128, kPP = 2;   // query rows of a block and of a CTA, pages of a key tile
-constexpr uint32_t kE = 4;                   // a unit's beginning and end cost about as much as four key tiles
-constexpr int kSoft = 256, kThreads = kSoft + 64;   // warps 0-7: softmax (0-3 the tile's first page, 4-7 its second); 8: copies; 9: MMAs
+constexpr uint32_t kE = 2;                   // a unit's beginning and end cost about as much as two key tiles
+constexpr int kSoft = 256, kThreads = kSoft + 128;   // warps 0-7: softmax (0-3 the tile's first page, 4-7 its second); 8: copies; 9: MMAs; 10, 11: q
 
 template <int D>
 struct Cfg {
   static constexpr uint32_t kKB = D / 64;                      // 64-dim blocks of K
-  static constexpr uint32_t kStage = D * 128;                  // of the ring: a page of K, or half of V's dims of two pages
+  static constexpr uint32_t kParts = D == 512 ? 2 : 1, kDV = D / kParts;   // parts of an output row; dims of one
+  static constexpr uint32_t kNK = D == 512 ? 4 : 1, kNV = D == 512 ? 2 : 1;   // stages of a K and of a V tile
+  static constexpr uint32_t kStage = D * 128 / kNK;            // of the ring: (a quarter of the dims of) a page of K; half of V's dims of two pages (one)
   static constexpr uint32_t kQ = kKB * 16384;
-  static constexpr int kStages = D == 256 ? 4 : 8;
+  static constexpr int kStages = D == 512 ? 5 : D == 256 ? 4 : 8;
   static constexpr uint32_t kSlot = D * 256;                   // a page of one head in f16: K blocks, then V
   static constexpr uint32_t kOut = 32 * 80;                    // a warp's 32 x 32 f16 of the output, rows padded to 80 bytes
   // tensor memory: O at 0, then P and S, 64 and 128 columns a buffer
-  static constexpr uint32_t kSB = D == 256 ? 1 : 2, kColS = 256, kColP = D == 256 ? 384 : 128;
-  static constexpr uint32_t kSmem = 1024 + kQ + kStages * kStage + 8 * kOut;
+  static constexpr uint32_t kSB = kDV == 256 ? 1 : 2, kColS = 256, kColP = kDV == 256 ? 384 : 128;
+  static constexpr uint32_t kStg = D == 512 ? 0 : kQ + kStages * kStage;   // the output on its way; D = 512: in q's place
+  static constexpr uint32_t kSmem = 1024 + kQ + kStages * kStage + (kStg ? 8 * kOut : 0);
 };
 
 // The pages of sequence b that the call sees, in order: those of the span over all its tokens. exo[b] = pages before it.
@@ -75,26 +78,29 @@ __global__ void __launch_bounds__(kET) kv4_widen_kernel(AttnJob j) {
     const auto there = [&](uint32_t k) { return ok && key0 + k < s.end && (key0 + k >= s.first_pos || key0 + k < j.sinks); };
     if (!(w2 & 1u)) {
       // K: a thread turns one word (8 dims of a key) into 16 bytes; 8 lanes make a key's 128-byte row of a block
-      constexpr uint32_t U = 64u * (D / 8) / kET;
-      uint32_t x[U], sm[U];
+      constexpr uint32_t N = 64u * (D / 8) / kET, U = N < 8 ? N : 8;
+#pragma unroll 1
+      for (uint32_t n0 = 0; n0 < N; n0 += U) {
+        uint32_t x[U], sm[U];
 #pragma unroll
-      for (uint32_t n = 0; n < U; n++) {
-        const uint32_t e = n * kET + threadIdx.x, c = e & 7u, key = (e >> 3) & 63u, g = (e >> 9) * 2u + (c >> 2);
-        x[n] = *reinterpret_cast<const uint32_t *>(rec + g * 1280u + key * 16u + (c & 3u) * 4u);
-        sm[n] = *reinterpret_cast<const uint32_t *>(rec + g * 1280u + 1024u + key * 4u);
-      }
-#pragma unroll
-      for (uint32_t n = 0; n < U; n++) {
-        const uint32_t e = n * kET + threadIdx.x, c = e & 7u, key = (e >> 3) & 63u, blk = e >> 9;
-        uint4 o = make_uint4(0u, 0u, 0u, 0u);
-        if (there(key)) {
-          const uint32_t s2 = __byte_perm(sm[n], 0, 0x1010), mn2 = __byte_perm(sm[n], 0, 0x3232), y = x[n] >> 4;
-          o.x = kv_deq2(__byte_perm(x[n], y, 0x4400), s2, mn2);   // byte i: dims 2i, 2i + 1
-          o.y = kv_deq2(__byte_perm(x[n], y, 0x5511), s2, mn2);
-          o.z = kv_deq2(__byte_perm(x[n], y, 0x6622), s2, mn2);
-          o.w = kv_deq2(__byte_perm(x[n], y, 0x7733), s2, mn2);
+        for (uint32_t n = 0; n < U; n++) {
+          const uint32_t e = (n0 + n) * kET + threadIdx.x, c = e & 7u, key = (e >> 3) & 63u, g = (e >> 9) * 2u + (c >> 2);
+          x[n] = *reinterpret_cast<const uint32_t *>(rec + g * 1280u + key * 16u + (c & 3u) * 4u);
+          sm[n] = *reinterpret_cast<const uint32_t *>(rec + g * 1280u + 1024u + key * 4u);
         }
-        *reinterpret_cast<uint4 *>(to + blk * 8192u + key * 128u + ((c ^ (key & 7u)) * 16u)) = o;
+#pragma unroll
+        for (uint32_t n = 0; n < U; n++) {
+          const uint32_t e = (n0 + n) * kET + threadIdx.x, c = e & 7u, key = (e >> 3) & 63u, blk = e >> 9;
+          uint4 o = make_uint4(0u, 0u, 0u, 0u);
+          if (there(key)) {
+            const uint32_t s2 = __byte_perm(sm[n], 0, 0x1010), mn2 = __byte_perm(sm[n], 0, 0x3232), y = x[n] >> 4;
+            o.x = kv_deq2(__byte_perm(x[n], y, 0x4400), s2, mn2);   // byte i: dims 2i, 2i + 1
+            o.y = kv_deq2(__byte_perm(x[n], y, 0x5511), s2, mn2);
+            o.z = kv_deq2(__byte_perm(x[n], y, 0x6622), s2, mn2);
+            o.w = kv_deq2(__byte_perm(x[n], y, 0x7733), s2, mn2);
+          }
+          *reinterpret_cast<uint4 *>(to + blk * 8192u + key * 128u + ((c ^ (key & 7u)) * 16u)) = o;
+        }
       }
     } else {
       // V: a thread turns the words of 8 keys (the same 8 dims) into 8 dims' 16-byte runs of 8 keys
@@ -160,22 +166,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   constexpr int NS = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t *qs = smem, *ring = smem + C::kQ, *stg = ring + NS * C::kStage;
+  uint8_t *qs = smem, *ring = smem + C::kQ, *stg = smem + C::kStg;
   uint32_t *pre = reinterpret_cast<uint32_t *>(smem_raw + C::kSmem), *exo = pre + j.v.rows + 1;
-  // full / empty: the ring; other: the odd CTA's stage has landed; sfull: S of a tile is there, sread: both CTAs have read it;
-  // pfull: both CTAs' P is there; odone: P V of a tile is done (each by buffer)
-  __shared__ __align__(8) uint64_t full[NS], empty[NS], other[NS], sfull[2], sread[2], pfull[2], odone[2], mdone;
+  // full / empty: the ring (the even CTA's is full when the odd one's is, too); sfull: S of a tile is there, sread: both CTAs have read it;
+  // pfull: both CTAs' P is there; odone: P V of a tile is done (each by buffer); qfull: both CTAs' q of a unit is there; qdone:
+  // its last S is; ofree: this CTA's output of a unit has left q's place
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], sfull[2], sread[2], pfull[2], odone[2], qfull, qdone, ofree, mdone;
   __shared__ uint32_t tmem_slot, abort_word;
-  __shared__ float mx2[2][2][kCR], l2[2][kCR];   // [tile parity][half of the tile][row]
-  __shared__ uint64_t qrow[kCR], orow[kCR];      // the rows' places in q and out
+  __shared__ float mx2[2][2][kCR], l2[2][2][kCR];   // [tile, unit parity][half of the tile][row]
   volatile uint32_t *abort_flag = &abort_word;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = tc::cluster_rank(), run = blockIdx.x >> 1;
   const uint32_t hpg = j.hpg, nkv = j.v.nkv, R = j.v.rows, W = j.window, S = j.sinks;
   if (tid == 0) {
     for (int i = 0; i < NS; i++) {
-      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&full[i], rank ? 1 : 2);
       tc::mbar_init(&empty[i], 1);
-      tc::mbar_init(&other[i], 1);
     }
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(&sfull[i], 1);
@@ -183,6 +188,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
       tc::mbar_init(&pfull[i], 2 * kSoft / 32);
       tc::mbar_init(&odone[i], 1);
     }
+    tc::mbar_init(&qfull, 4);
+    tc::mbar_init(&qdone, 1);
+    tc::mbar_init(&ofree, kSoft / 32);
     tc::mbar_init(&mdone, 1);
     abort_word = 0u;
     tc::fence_mbar_init();
@@ -201,11 +209,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   if (tid == 0 && rank == 0) j.desc[run] = make_uint4(0u, 0u, 0u, 0u);
   const uint32_t lo = run < G ? (uint32_t)((uint64_t)total * run / G) : 0u, hi = run < G ? (uint32_t)((uint64_t)total * (run + 1) / G) : 0u;
   uint32_t b = lo < hi ? find_sequence(pre, R, lo) : 0u;
-  uint32_t st = 0, tile = 0;   // ring stages and key tiles so far (each role counts its own uses alike)
+  uint32_t st = 0, sp = 0, tile = 0, unit = 0;   // the ring's stage and how often it came round; key tiles and units with tiles so far (each role counts its own uses alike)
   const float c = fabsf(j.scale) * 1.44269504088896340736f;
   const uint32_t flip = j.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale turns q around, so that maxima stay maxima
   // A wait that gives up sets the CTA's abort word, after which all its waits give up at once; every warp still walks the
-  // same units and barriers to the end
+  // same units to the end. Nothing stops between units: the next one's K, q and first S run under this one's end
+  const auto next = [&]() {
+    if (++st == (uint32_t)NS) st = 0u, sp++;
+  };
   for (uint32_t at = lo; at < hi;) {
     while (pre[b + 1] <= at) b++;
     const Unit u = find_unit<kRB, kPP, kE>(j, pre, b, at);
@@ -214,40 +225,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
     at = u.begin + end;
     if (from == to) continue;   // this run holds none of the unit's tiles
     const uint32_t tiles = s.n ? to - from : 0u;
+    const uint32_t head = u.head / C::kParts, oh = u.head % C::kParts;   // KV head, part of the output's dims
     const uint32_t rc = u.r0 + rank * kCR, nrow = rc < u.rows ? min(kCR, u.rows - rc) : 0u;   // this CTA's rows
     if (warp == 8) {
       // ------------------------------------------------------------ copies
       const Span all = whole_span(j, b);
-      const uint8_t *base = j.wide + ((uint64_t)exo[b] * nkv + u.head) * C::kSlot;
+      const uint8_t *base = j.wide + ((uint64_t)exo[b] * nkv + head) * C::kSlot;
       const auto slot = [&](uint32_t i) {   // page i of the unit's span (an odd last tile repeats its first page)
         const uint32_t jp = page_at(s, min(i, s.n - 1u)), k = jp < all.sink_pages ? jp : all.sink_pages + (jp - all.from);
         return base + (uint64_t)k * nkv * C::kSlot;
       };
       const auto stage = [&]() -> uint8_t * {
-        if (!tc::mbar_wait(&empty[st % NS], ((st / NS) & 1u) ^ 1u, abort_flag, j.err, 0x4b1u, P0_SPIN_LIMIT)) return nullptr;
-        tc::mbar_expect_tx(&full[st % NS], C::kStage);
-        return ring + (st % NS) * C::kStage;
+        if (!tc::mbar_wait(&empty[st], (sp & 1u) ^ 1u, abort_flag, j.err, 0x4b1u, P0_SPIN_LIMIT)) return nullptr;
+        tc::mbar_expect_tx(&full[st], C::kStage);
+        return ring + st * C::kStage;
       };
       const auto load_k = [&](uint32_t i) {
-        uint8_t *d = stage();
-        if (!d) return false;
-        bulk_load(d, slot(2u * i + rank), C::kStage, &full[st % NS]);
-        st++;
+        const uint8_t *from = slot(2u * i + rank);
+        for (uint32_t x = 0; x < C::kNK; x++) {
+          uint8_t *d = stage();
+          if (!d) return false;
+          bulk_load(d, from + x * C::kStage, C::kStage, &full[st]);
+          next();
+        }
         return true;
       };
       const auto load_v = [&](uint32_t i) {
-        uint8_t *d = stage();
-        if (!d) return false;
-        for (uint32_t h = 0; h < 2; h++)
-          bulk_load(d + h * (C::kStage / 2), slot(2u * i + h) + D * 128 + rank * (C::kStage / 2), C::kStage / 2, &full[st % NS]);
-        st++;
+        constexpr uint32_t half = C::kDV * 64;   // bytes of this CTA's dims of a page
+        for (uint32_t h = 0; h < 2;) {
+          uint8_t *d = stage();
+          if (!d) return false;
+          for (uint32_t k = 0; k < 2 / C::kNV; k++, h++)
+            bulk_load(d + k * half, slot(2u * i + h) + D * 128 + (oh * 2u + rank) * half, half, &full[st]);
+          next();
+        }
         return true;
       };
-      bool ok = true;
-      if (lane == 0 && tiles) ok = load_k(from);   // ahead of the barrier: under the previous unit's end
-      __syncwarp();
-      tc::cluster_sync();
-      if (lane == 0 && ok)
+      if (lane == 0 && tiles && load_k(from))
         for (uint32_t i = 0; i < tiles; i++) {
           if (i + 1 < tiles && !load_k(from + i + 1)) break;
           if (!load_v(from + i)) break;
@@ -256,101 +270,131 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
     } else if (warp == 9) {
       // ------------------------------------------------------------ the pair's MMAs (even CTA), word of what landed (odd CTA)
       const auto tell = [&]() {
-        const bool ok = tc::mbar_wait(&full[st % NS], (st / NS) & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
-        if (ok) tc::mbar_arrive_rank(&other[st % NS], 0);
-        st++;
+        const bool ok = tc::mbar_wait(&full[st], sp & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
+        if (ok) tc::mbar_arrive_rank(&full[st], 0);
+        next();
         return ok;
       };
-      bool told = tiles && rank == 1;
-      if (lane == 0 && told) told = tell();   // the first K, as it was issued, ahead of the barrier
-      __syncwarp();
-      tc::cluster_sync();
-      tc::fence_after();
       if (lane == 0 && rank == 1) {
-        for (uint32_t i = 1; i < 2u * tiles && told; i++) told = tell();
+        for (uint32_t i = 0; i < (C::kNK + C::kNV) * tiles && tell(); i++) {}
       } else if (lane == 0 && tiles) {
-        constexpr uint32_t is = tc::idesc_f16_f32(256, 128), iv = tc::idesc_f16_f32(256, D);
+        constexpr uint32_t is = tc::idesc_f16_f32(256, 128), iv = tc::idesc_f16_f32(256, C::kDV);
         const auto arrived = [&]() {
-          const bool ok = tc::mbar_wait(&full[st % NS], (st / NS) & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT) &&
-                          tc::mbar_wait(&other[st % NS], (st / NS) & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
-          tc::fence_after();
-          return ok;
+          return tc::mbar_wait(&full[st], sp & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
         };
-        const auto scores = [&](uint32_t t) {
-          if (!arrived()) return false;
-          const uint32_t sb = t % C::kSB, dst = tmem + C::kColS + sb * 128u, ks = tc::smem_u32(ring + (st % NS) * C::kStage), q0 = tc::smem_u32(qs);
+        const auto part_of = [](uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); };   // within shared memory: no carry out of the address
+        const auto scores = [&](uint32_t t) {   // over S of tile t - kSB
+          const uint32_t o = t - C::kSB;
+          if (!arrived()) return false;   // the waits that are over first: what follows the last one is in the tensor core's way
+          if (t >= C::kSB && !tc::mbar_wait(&sread[o % C::kSB], (o / C::kSB) & 1u, abort_flag, j.err, 0x4b9u, P0_SPIN_LIMIT)) return false;
+          tc::fence_after();
+          const uint32_t sb = t % C::kSB, dst = tmem + C::kColS + sb * 128u;
+          constexpr uint32_t per = C::kKB / C::kNK;   // 64-dim blocks of a stage
+#pragma unroll 1
+          for (uint32_t y = 0; y < C::kNK; y++) {
+            if (y) {
+              if (!arrived()) return false;
+              tc::fence_after();
+            }
+            const uint64_t kd = tc::desc_sw128(tc::smem_u32(ring + st * C::kStage)), qd = tc::desc_sw128(tc::smem_u32(qs) + y * per * 16384u);
 #pragma unroll
-          for (uint32_t x = 0; x < C::kKB * 4u; x++)
-            tc::mma_ss_f16_pair(dst, tc::desc_sw128(q0 + (x >> 2) * 16384u + (x & 3u) * 32u), tc::desc_sw128(ks + (x >> 2) * 8192u + (x & 3u) * 32u), is, x != 0u);
-          tc::mma_commit_pair(&empty[st % NS]);
-          st++;
-          tc::mma_commit_pair(&sfull[sb]);
+            for (uint32_t x = 0; x < per * 4u; x++)
+              tc::mma_ss_f16_pair(dst, part_of(qd, (x >> 2) * 16384u + (x & 3u) * 32u), part_of(kd, (x >> 2) * 8192u + (x & 3u) * 32u), is, (y | x) != 0u);
+            if (y + 1 == C::kNK) tc::mma_commit_pair(&sfull[sb]);
+            tc::mma_commit_pair(&empty[st]);
+            next();
+          }
+          if (t + 1u == tile + tiles) tc::mma_commit_pair(&qdone);
           return true;
         };
-        bool ok = scores(tile);
+        bool ok = tc::mbar_wait_cluster(&qfull, unit & 1u, abort_flag, j.err, 0x4bcu, P0_SPIN_LIMIT) && scores(tile);
         for (uint32_t i = 0; i < tiles && ok; i++) {
           const uint32_t t = tile + i;
-          if (i + 1 < tiles) {   // over S of tile t + 1 - kSB (i + 1 >= kSB: of this unit, or read before its end)
-            const uint32_t o = t + 1u - C::kSB;
-            if (i + 1 >= C::kSB && !(ok = tc::mbar_wait(&sread[o % C::kSB], (o / C::kSB) & 1u, abort_flag, j.err, 0x4b9u, P0_SPIN_LIMIT))) break;
-            tc::fence_after();
-            if (!(ok = scores(t + 1))) break;
-          }
+          if (i + 1 < tiles && !(ok = scores(t + 1))) break;
+          if (!(ok = arrived())) break;
           if (!(ok = tc::mbar_wait(&pfull[t & 1u], (t >> 1) & 1u, abort_flag, j.err, 0x4b4u, P0_SPIN_LIMIT))) break;
           tc::fence_after();
-          if (!(ok = arrived())) break;
-          const uint32_t pa = tmem + C::kColP + (t & 1u) * 64u, vs = tc::smem_u32(ring + (st % NS) * C::kStage);
+          const uint32_t pa = tmem + C::kColP + (t & 1u) * 64u;
+#pragma unroll 1
+          for (uint32_t y = 0; y < C::kNV; y++) {
+            constexpr uint32_t steps = 8 / C::kNV;   // of 16 keys
+            if (y) {
+              if (!(ok = arrived())) break;
+              tc::fence_after();
+            }
+            const uint64_t vd = tc::desc_sw128(tc::smem_u32(ring + st * C::kStage));
 #pragma unroll
-          for (uint32_t x = 0; x < 8u; x++)
-            tc::mma_ts_f16_pair(tmem, pa + x * 8u, tc::desc_sw128(vs + (x >> 2) * (C::kStage / 2) + (x & 3u) * 32u), iv, (i | x) != 0u);
-          tc::mma_commit_pair(&empty[st % NS]);
-          st++;
-          tc::mma_commit_pair(&odone[t & 1u]);
+            for (uint32_t x = 0; x < steps; x++)
+              tc::mma_ts_f16_pair(tmem, pa + (y * steps + x) * 8u, part_of(vd, (x >> 2) * (C::kDV * 64u) + (x & 3u) * 32u), iv, (i | y | x) != 0u);
+            if (y + 1 == C::kNV) tc::mma_commit_pair(&odone[t & 1u]);
+            tc::mma_commit_pair(&empty[st]);
+            next();
+          }
+          if (!ok) break;
         }
       }
       __syncwarp();
-    } else {
-      // ------------------------------------------------------------ q rows, swizzled (a warp reads a row at a time); zeros beyond
-      asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");   // the previous unit's rows are written
-      if (tid < kCR) {
-        const uint32_t row = rc + tid, tok = row / hpg;
-        qrow[tid] = (uint64_t)(u.first + tok) * j.q.ld + (uint64_t)(u.head * hpg + row - tok * hpg) * j.q.ldh;
-        orow[tid] = (uint64_t)(u.first + tok) * j.out.ld + (uint64_t)(u.head * hpg + row - tok * hpg) * j.out.ldh;
-      }
-      asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
-      {
-        constexpr uint32_t CH = D / 8, RW = CH < 32 ? 32 / CH : 1, PASS = kCR / (8 * RW);   // 16-byte chunks of a row, rows of a warp's pass
-        const uint32_t d8 = lane % CH, rr = lane / CH;
-        const __half *qb = reinterpret_cast<const __half *>(j.q.base) + d8 * 8u;
-        uint4 x[PASS];
+    } else if (warp >= 10) {
+      // ------------------------------------------------------------ q rows, swizzled (a warp reads a row or more at a time); zeros beyond
+      bool ok = true;
+      if (unit && tiles) ok = tc::mbar_wait(&qdone, (unit - 1u) & 1u, abort_flag, j.err, 0x4bdu, P0_SPIN_LIMIT);
+      if (!C::kStg && unit && tiles) ok = ok && tc::mbar_wait(&ofree, (unit - 1u) & 1u, abort_flag, j.err, 0x4beu, P0_SPIN_LIMIT);
+      if (__all_sync(0xffffffffu, ok && tiles)) {
+        // a warp takes 64 of the rows, RW at a time, 16 bytes a lane; each lane works out the places of two
+        constexpr uint32_t CH = D < 256 ? D / 8 : 32, RW = 32 / CH, N = 64 / RW;
+        const uint32_t r0 = (warp & 1u) * 64u;
+        uint64_t place[2];
 #pragma unroll
-        for (uint32_t p = 0; p < PASS; p++) {
-          const uint32_t r = (p * 8u + warp) * RW + rr;
-          x[p] = make_uint4(0u, 0u, 0u, 0u);
-          if (r < nrow) {
-            const __half *q = qb + qrow[r];
-            if (j.q.wide) {
-              x[p] = *reinterpret_cast<const uint4 *>(q);
-            } else {
-              uint32_t w[4];
+        for (uint32_t i = 0; i < 2; i++) {
+          const uint32_t row = rc + r0 + 32u * i + lane, tok = row / hpg;
+          place[i] = (uint64_t)(u.first + tok) * j.q.ld + (uint64_t)(head * hpg + row - tok * hpg) * j.q.ldh;
+        }
+#pragma unroll 2
+        for (uint32_t n0 = 0; n0 < N; n0 += 4) {
+          uint64_t at4[4];
 #pragma unroll
-              for (int i = 0; i < 4; i++) w[i] = (uint32_t)__half_as_ushort(q[2 * i]) | ((uint32_t)__half_as_ushort(q[2 * i + 1]) << 16);
-              x[p] = make_uint4(w[0], w[1], w[2], w[3]);
+          for (uint32_t n = 0; n < 4; n++) {
+            const uint32_t r = (n0 + n) * RW + lane / CH;
+            at4[n] = __shfl_sync(0xffffffffu, (n0 + n) * RW < 32u ? place[0] : place[1], r & 31u);
+          }
+#pragma unroll
+          for (uint32_t n = 0; n < 4; n++) {
+            const uint32_t row = r0 + (n0 + n) * RW + lane / CH;
+            const bool there = row < nrow;
+            const __half *q = reinterpret_cast<const __half *>(j.q.base) + (there ? at4[n] : 0u);
+#pragma unroll
+            for (uint32_t d8 = lane % CH; d8 < D / 8; d8 += CH) {
+              uint8_t *to = qs + (d8 >> 3) * 16384u + row * 128u + (((d8 & 7u) ^ (row & 7u)) * 16u);
+              if (j.q.wide && !flip) {   // asynchronous; no bytes read, zeros written beyond the rows
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(to)), "l"(q + d8 * 8u), "r"(there ? 16u : 0u) : "memory");
+              } else {
+                uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                  if (there) w[i] = ((uint32_t)__half_as_ushort(q[d8 * 8u + 2 * i]) | ((uint32_t)__half_as_ushort(q[d8 * 8u + 2 * i + 1]) << 16)) ^ flip;
+                *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
             }
           }
         }
-#pragma unroll
-        for (uint32_t p = 0; p < PASS; p++) {
-          const uint32_t r = (p * 8u + warp) * RW + rr;
-          *reinterpret_cast<uint4 *>(qs + (d8 >> 3) * 16384u + r * 128u + (((d8 & 7u) ^ (r & 7u)) * 16u)) =
-              make_uint4(x[p].x ^ flip, x[p].y ^ flip, x[p].z ^ flip, x[p].w ^ flip);
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the generic writes before the MMAs' reads
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_rank(&qfull, 0);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the generic writes before the MMAs' reads
-      tc::fence_before();
-      tc::cluster_sync();
-      tc::fence_after();
+      __syncwarp();
+    } else {
       // ------------------------------------------------------------ softmax: half h of row r
+      const bool whole = from == 0 && to == nt;
+      if (!whole && from == 0 && tid == 0 && rank == 0) j.desc[run] = make_uint4(1u + run_of(u.begin + u.n - 1u, total, G), b, u.r0, u.head);
+      const auto orow = [&](uint32_t r) {   // row r's place in out
+        const uint32_t tok = (rc + r) / hpg;
+        return (uint64_t)(u.first + tok) * j.out.ld + (uint64_t)(head * hpg + rc + r - tok * hpg) * j.out.ldh + oh * C::kDV;
+      };
+      if (!tiles) {   // nothing to see: zeros
+        for (uint32_t e = tid; e < nrow * C::kDV; e += kSoft) reinterpret_cast<__half *>(j.out.base)[orow(e / C::kDV) + e % C::kDV] = __half();
+        continue;
+      }
       const uint32_t r = tid & 127u, h = tid >> 7, lanes = ((warp & 3u) * 32u) << 16;
       const int32_t pos = r < nrow ? (int32_t)(u.len - u.T + (rc + r) / hpg) : -1;
       const int32_t pos0 = (int32_t)(u.len - u.T + u.r0 / hpg), pos1 = (int32_t)s.end - 1;   // of the block
@@ -358,7 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
       const uint32_t *trow = j.v.table + (uint64_t)b * j.v.ld;
       const auto entry = [&](uint32_t i) { return 2u * i + h < s.n ? trow[page_at(s, 2u * i + h)] : P0_KV_NONE; };
       bool ok = true;
-      uint32_t next = tiles ? entry(from) : P0_KV_NONE;
+      uint32_t next = entry(from);
       for (uint32_t i = 0; i < tiles; i++) {   // a warp that gave up keeps meeting the others at the barrier
         const uint32_t t = tile + i, jp = page_at(s, min(2u * (from + i) + h, s.n - 1u));
         const bool here = next < j.v.pages;
@@ -411,7 +455,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
             ok = __all_sync(0xffffffffu, tc::mbar_wait(&odone[(t - 1u) & 1u], ((t - 1u) >> 1) & 1u, abort_flag, j.err, 0x4b7u, P0_SPIN_LIMIT));
             tc::fence_after();
 #pragma unroll 1
-            for (uint32_t d = h * (D / 2); ok && d < (h + 1u) * (D / 2); d += 32u) {
+            for (uint32_t d = h * (C::kDV / 2); ok && d < (h + 1u) * (C::kDV / 2); d += 32u) {
               uint32_t o[32];
               tc::tmem_ld32(tmem + lanes + d, o);
               tc::tmem_wait_ld();
@@ -446,33 +490,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
         __syncwarp();
         if (lane == 0) tc::mbar_arrive_peer(&pfull[t & 1u], 0);
       }
-      l2[h][r] = l;
+      l2[unit & 1u][h][r] = l;
       asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
-      l += l2[h ^ 1u][r];
-      if (ok && tiles) {
+      l += l2[unit & 1u][h ^ 1u][r];
+      if (ok) {
         const uint32_t t = tile + tiles - 1u;
         if (tiles > 1) ok = tc::mbar_wait(&odone[(t - 1u) & 1u], ((t - 1u) >> 1) & 1u, abort_flag, j.err, 0x4bau, P0_SPIN_LIMIT);
         ok = ok && tc::mbar_wait(&odone[t & 1u], (t >> 1) & 1u, abort_flag, j.err, 0x4b8u, P0_SPIN_LIMIT);
         tc::fence_after();
       }
       ok = __all_sync(0xffffffffu, ok);
-      const bool whole = from == 0 && to == nt;
-      float *part = j.part + (((uint64_t)run * 2u + (from ? 0u : 1u)) * 2u + rank) * kCR * (D + 2);   // [D][rows], then m and l
-      if (!whole && from == 0 && tid == 0 && rank == 0) j.desc[run] = make_uint4(1u + run_of(u.begin + u.n - 1u, total, G), b, u.r0, u.head);
+      float *part = j.part + (((uint64_t)run * 2u + (from ? 0u : 1u)) * 2u + rank) * kCR * (C::kDV + 2);   // [dims][rows], then m and l
       if (ok) {
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const uint64_t own = orow(r);
         uint8_t *so = stg + warp * C::kOut;
 #pragma unroll 1
-        for (uint32_t d = h * (D / 2); d < (h + 1u) * (D / 2); d += 32u) {
+        for (uint32_t d = h * (C::kDV / 2); d < (h + 1u) * (C::kDV / 2); d += 32u) {
           uint32_t o[32];
           __syncwarp();
-          if (tiles) {
-            tc::tmem_ld32(tmem + lanes + d, o);
-            tc::tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = 0u;
-          }
+          tc::tmem_ld32(tmem + lanes + d, o);
+          tc::tmem_wait_ld();
           if (!whole) {
 #pragma unroll
             for (int e = 0; e < 32; e++) part[(d + e) * kCR + r] = __uint_as_float(o[e]);
@@ -491,8 +529,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++) {
               const uint32_t row = (warp & 3u) * 32u + 8u * k + (lane >> 2);
+              const uint64_t place = __shfl_sync(0xffffffffu, own, 8u * k + (lane >> 2));
               if (row >= nrow) continue;
-              __half *out = reinterpret_cast<__half *>(j.out.base) + orow[row] + d + 8u * (lane & 3u);
+              __half *out = reinterpret_cast<__half *>(j.out.base) + place + d + 8u * (lane & 3u);
               if (j.out.wide) {
                 *reinterpret_cast<uint4 *>(out) = y[k];
               } else {
@@ -504,20 +543,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
           }
         }
         if (!whole && h == 0) {
-          part[D * kCR + r] = m;
-          part[(D + 1) * kCR + r] = l;
+          part[C::kDV * kCR + r] = m;
+          part[(C::kDV + 1) * kCR + r] = l;
         }
       }
-      tc::fence_before();   // O is read before the next unit's MMAs write it
+      tc::fence_before();   // O is read before the next unit's MMAs write it: they wait for this warp's next P
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&ofree);
     }
-    st = __shfl_sync(0xffffffffu, st, 0);   // the issuing lane's count
+    st = __shfl_sync(0xffffffffu, st, 0);   // the issuing lane's
+    sp = __shfl_sync(0xffffffffu, sp, 0);
     tile += tiles;
+    unit += tiles != 0u;
   }
   __syncthreads();
   if (abort_word && lane == 0) {   // a wait gave up (j.err says which): nothing may be in flight when the CTA leaves. Bounded
     volatile uint32_t never = 0;
     if (warp == 8)
-      for (uint32_t i = st > (uint32_t)NS ? st - NS : 0; i < st; i++) tc::mbar_wait(&full[i % NS], (i / NS) & 1u, &never, j.err, 0x4b2u, P0_SPIN_LIMIT);
+      for (uint32_t i = 0; i < (uint32_t)NS; i++)
+        if (sp || i < st) tc::mbar_wait(&full[i], (i < st ? sp : sp - 1u) & 1u, &never, j.err, 0x4b2u, P0_SPIN_LIMIT);
     if (warp == 9 && rank == 0) {
       tc::mma_commit_pair(&mdone);
       tc::mbar_wait(&mdone, 0, &never, j.err, 0x4b5u, P0_SPIN_LIMIT);
@@ -532,47 +576,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   }
 }
 
-// joins the parts of a unit that several runs share: CTA (run, 32 dims, 128 of the rows), a thread per row. M = max m, o = sum
+// joins the parts of a unit that several runs share: CTA (run, 8 dims, 128 of the rows), a thread per row. M = max m, o = sum
 // 2^(m - M) acc / sum 2^(m - M) l, in run order
 template <int D>
 __global__ void __launch_bounds__(kCR) kv4_prompt_join_kernel(AttnJob j) {
   dep_enter();
   const uint4 w = j.desc[blockIdx.x];
   if (!w.x) return;
-  const uint32_t r = threadIdx.x, d0 = blockIdx.y * 32u, rank = blockIdx.z, b = w.y, r0 = w.z + rank * kCR, head = w.w, hpg = j.hpg;
+  constexpr uint32_t DV = Cfg<D>::kDV;
+  const uint32_t r = threadIdx.x, d0 = blockIdx.y * 8u, rank = blockIdx.z, b = w.y, r0 = w.z + rank * kCR, hpg = j.hpg;
+  const uint32_t head = w.w / Cfg<D>::kParts, oh = w.w % Cfg<D>::kParts;
   uint32_t first;
   const uint32_t T = kv_tokens(j.v, b, first), n = w.x - blockIdx.x;
   if (r0 + r >= T * hpg) return;
-  const auto part = [&](uint32_t i) { return j.part + (((uint64_t)(blockIdx.x + i) * 2u + (i ? 0u : 1u)) * 2u + rank) * kCR * (D + 2) + r; };
+  const auto part = [&](uint32_t i) { return j.part + (((uint64_t)(blockIdx.x + i) * 2u + (i ? 0u : 1u)) * 2u + rank) * kCR * (DV + 2) + r; };
   float M = -INFINITY;
-#pragma unroll 4
-  for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part(i)[D * kCR]);
+#pragma unroll 8
+  for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part(i)[DV * kCR]);
   const float ref = M == -INFINITY ? 0.0f : M;
-  float acc[32], sum = 0.0f;
+  float acc[8], sum = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 32; e++) acc[e] = 0.0f;
-#pragma unroll 2
+  for (int e = 0; e < 8; e++) acc[e] = 0.0f;
+#pragma unroll 4
   for (uint32_t i = 0; i < n; i++) {
     const float *p = part(i);
-    float x[32];
+    float x[8];
 #pragma unroll
-    for (int e = 0; e < 32; e++) x[e] = p[(d0 + e) * kCR];
-    const float f = exp2f(p[D * kCR] - ref);
-    sum = fmaf(f, p[(D + 1) * kCR], sum);
+    for (int e = 0; e < 8; e++) x[e] = p[(d0 + e) * kCR];
+    const float f = exp2f(p[DV * kCR] - ref);
+    sum = fmaf(f, p[(DV + 1) * kCR], sum);
 #pragma unroll
-    for (int e = 0; e < 32; e++) acc[e] = fmaf(f, x[e], acc[e]);
+    for (int e = 0; e < 8; e++) acc[e] = fmaf(f, x[e], acc[e]);
   }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  __half *out = reinterpret_cast<__half *>(j.out.base) + (uint64_t)(first + (r0 + r) / hpg) * j.out.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.out.ldh + d0;
-  uint32_t y[16];
+  __half *out = reinterpret_cast<__half *>(j.out.base) + (uint64_t)(first + (r0 + r) / hpg) * j.out.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.out.ldh + oh * DV + d0;
+  uint32_t y[4];
 #pragma unroll
-  for (int e = 0; e < 16; e++) y[e] = pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  for (int e = 0; e < 4; e++) y[e] = pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
   if (j.out.wide) {
-#pragma unroll
-    for (int e = 0; e < 4; e++) reinterpret_cast<uint4 *>(out)[e] = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+    *reinterpret_cast<uint4 *>(out) = make_uint4(y[0], y[1], y[2], y[3]);
   } else {
 #pragma unroll
-    for (int e = 0; e < 32; e++) out[e] = __ushort_as_half((unsigned short)(y[e / 2] >> (16 * (e & 1))));
+    for (int e = 0; e < 8; e++) out[e] = __ushort_as_half((unsigned short)(y[e / 2] >> (16 * (e & 1))));
   }
 }
 
@@ -581,9 +626,10 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
   using C = Cfg<D>;
   const uint32_t R = j.v.rows, G = (uint32_t)c->sm_count / 2;
   const size_t smem = C::kSmem + ((size_t)R + 1) * 8;
+  j.units = j.v.nkv * C::kParts;
   uint32_t *cnt;
   void *ws;
-  const size_t desc = ((size_t)G * sizeof(uint4) + 255) / 256 * 256, parts = ((size_t)G * 2 * kRB * (D + 2) * 4 + 255) / 256 * 256;
+  const size_t desc = ((size_t)G * sizeof(uint4) + 255) / 256 * 256, parts = ((size_t)G * 2 * kRB * (C::kDV + 2) * 4 + 255) / 256 * 256;
   p0_status st = p0_workspace(c, 0, desc + parts + wide_bytes, &cnt, &ws);
   if (st) return st;
   j.desc = (uint4 *)ws;
@@ -596,7 +642,7 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
   if ((st = p0_launched(c, "kv4Attn pages"))) return st;
   launch_dep(kern, dim3(2 * G), dim3(kThreads), smem, c->stream, j);
   if ((st = p0_launched(c, "kv4Attn prompt"))) return st;
-  launch_dep(kv4_prompt_join_kernel<D>, dim3(G, D / 32, 2), dim3(kCR), 0, c->stream, j);
+  launch_dep(kv4_prompt_join_kernel<D>, dim3(G, C::kDV / 8, 2), dim3(kCR), 0, c->stream, j);
   return p0_launched(c, "kv4Attn join");
 }
 
@@ -607,11 +653,12 @@ p0_status kv4_attn_prompt(p0_ctx *c, AttnJob &j, bool *taken) {
   const uint64_t rows = (uint64_t)j.v.n * j.hpg, D = j.v.D;
   if (rows / j.v.rows < 64) return P0_OK;
   const uint64_t wide = (uint64_t)j.v.rows * j.v.ld * j.v.nkv * D * 256;
-  if (wide > (4ull << 30) || j.v.rows > 256 || D == 512) return P0_OK;
+  if (wide > (4ull << 30) || j.v.rows > 256) return P0_OK;
   *taken = true;
   switch (D) {
     case 64: return prompt_launch<64>(c, j, wide);
     case 128: return prompt_launch<128>(c, j, wide);
-    default: return prompt_launch<256>(c, j, wide);
+    case 256: return prompt_launch<256>(c, j, wide);
+    default: return prompt_launch<512>(c, j, wide);
   }
 }

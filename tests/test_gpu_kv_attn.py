@@ -115,6 +115,8 @@ PROMPTS = [
     ([2000, 300], [600, 300], 6, 2, 128, 300, 4, 0.0),
     ([1100, 900], [700, 64], 16, 4, 64, 0, 0, 0.0),
     ([100, 20, 640], [130, 30, 100], 8, 1, 64, 90, 1, 2.0),          # sequences shorter than their tokens: rows that see nothing
+    ([1500, 64, 700], [400, 64, 40], 8, 1, 512, 0, 0, 0.0),          # 512 dims: the output in two parts
+    ([1300, 30], [300, 60], 4, 2, 512, 250, 70, -0.5),
 ]
 
 
