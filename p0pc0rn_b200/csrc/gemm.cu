@@ -19,12 +19,11 @@
 // A persistent form of the same GEMM (gemm_q4_ps, below) serves q4 calls with a store epilogue and short K: one CTA
 // per SM walks the tiles with two accumulators in tensor memory and the dequantised weights in shared memory, so a
 // tile's epilogue runs under the next tile's main loop.
-#include <cuda.h>
 #include <cstdlib>
 #include <cuda_fp16.h>
-#include <cudaTypedefs.h>
 
 #include "internal.h"
+#include "launch.cuh"
 #include "tc.cuh"
 
 namespace {
@@ -995,17 +994,6 @@ __global__ void deq_dump_q8(const uint8_t *W, uint32_t rows, uint32_t cols, uint
   uint32_t *o = reinterpret_cast<uint32_t *>(out + (size_t)row * cols + (size_t)hh * 32u);
 #pragma unroll
   for (int i = 0; i < 16; i++) o[i] = r[i];
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (!fn) {
-    void *f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      fn = (PFN_cuTensorMapEncodeTiled_v12000)f;
-  }
-  return fn;
 }
 
 const char *gepi_name(uint32_t e) {

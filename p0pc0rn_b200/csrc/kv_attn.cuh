@@ -10,6 +10,7 @@ struct AttnJob {
   KvRows q, out;
   uint32_t hpg, window, sinks, units;   // units: of a row block (KV heads; times the parts that an output row is cut into)
   float scale;
+  bool qbox;          // the prompt form: q has a tensor map
   uint32_t *err;
   float *part;        // [grid][2][rows of a block][D + 2]
   uint4 *desc;        // [grid]: (1 + last run, b, first row, KV head) of the unit that this run begins and others end

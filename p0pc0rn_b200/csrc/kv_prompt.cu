@@ -24,7 +24,7 @@ namespace {
 
 constexpr uint32_t kRB = 256, kCR = 128, kPP = 2;   // query rows of a block and of a CTA, pages of a key tile
 constexpr uint32_t kE = 2;                   // a unit's beginning and end cost about as much as two key tiles
-constexpr int kSoft = 256, kThreads = kSoft + 128;   // warps 0-7: softmax (0-3 the tile's first page, 4-7 its second); 8: copies; 9: MMAs; 10, 11: q
+constexpr int kSoft = 256, kThreads = kSoft + 128;   // warps 0-7: softmax (0-3 the tile's first page, 4-7 its second); 8: copies; 9: S; 10: P V; 11: q
 
 template <int D>
 struct Cfg {
@@ -33,7 +33,7 @@ struct Cfg {
   static constexpr uint32_t kNK = D == 512 ? 4 : 1, kNV = D == 512 ? 2 : 1;   // stages of a K and of a V tile
   static constexpr uint32_t kStage = D * 128 / kNK;            // of the ring: (a quarter of the dims of) a page of K; half of V's dims of two pages (one)
   static constexpr uint32_t kQ = kKB * 16384;
-  static constexpr int kStages = D == 512 ? 5 : D == 256 ? 4 : 8;
+  static constexpr int kSK = D == 512 ? 3 : D == 256 ? 2 : 4, kSV = D >= 256 ? 2 : 4, kStages = kSK + kSV;   // stages of the rings of K and V
   static constexpr uint32_t kSlot = D * 256;                   // a page of one head in f16: K blocks, then V
   static constexpr uint32_t kOut = 32 * 80;                    // a warp's 32 x 32 f16 of the output, rows padded to 80 bytes
   // tensor memory: O at 0, then P and S, 64 and 128 columns a buffer
@@ -140,6 +140,12 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
                "r"(bytes), "r"(tc::smem_u32(bar))
                : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(void *dst, const void *tmap, uint64_t *bar, int32_t c0, int32_t c1, int32_t c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(tc::smem_u32(dst)),
+      "l"(tmap), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -160,18 +166,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 }
 
 template <int D>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnJob j) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnJob j, const __grid_constant__ CUtensorMap qm) {
   dep_enter();
   using C = Cfg<D>;
-  constexpr int NS = C::kStages;
+  constexpr int NS = C::kStages, SK = C::kSK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *qs = smem, *ring = smem + C::kQ, *stg = smem + C::kStg;
   uint32_t *pre = reinterpret_cast<uint32_t *>(smem_raw + C::kSmem), *exo = pre + j.v.rows + 1;
-  // full / empty: the ring (the even CTA's is full when the odd one's is, too); sfull: S of a tile is there, sread: both CTAs have read it;
+  // full / empty: the stages, K's before V's (the even CTA's is full when the odd one's is, too); sfull: S of a tile is there, sread: both CTAs have read it;
   // pfull: both CTAs' P is there; odone: P V of a tile is done (each by buffer); qfull: both CTAs' q of a unit is there; qdone:
   // its last S is; ofree: this CTA's output of a unit has left q's place
-  __shared__ __align__(8) uint64_t full[NS], empty[NS], sfull[2], sread[2], pfull[2], odone[2], qfull, qdone, ofree, mdone;
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], sfull[2], sread[2], pfull[2], odone[2], qfull, qland, qdone, ofree, mdone[2];
   __shared__ uint32_t tmem_slot, abort_word;
   __shared__ float mx2[2][2][kCR], l2[2][2][kCR];   // [tile, unit parity][half of the tile][row]
   volatile uint32_t *abort_flag = &abort_word;
@@ -188,10 +194,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
       tc::mbar_init(&pfull[i], 2 * kSoft / 32);
       tc::mbar_init(&odone[i], 1);
     }
-    tc::mbar_init(&qfull, 4);
+    tc::mbar_init(&qfull, 2);
+    tc::mbar_init(&qland, 1);
     tc::mbar_init(&qdone, 1);
     tc::mbar_init(&ofree, kSoft / 32);
-    tc::mbar_init(&mdone, 1);
+    tc::mbar_init(&mdone[0], 1);
+    tc::mbar_init(&mdone[1], 1);
     abort_word = 0u;
     tc::fence_mbar_init();
   }
@@ -209,14 +217,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   if (tid == 0 && rank == 0) j.desc[run] = make_uint4(0u, 0u, 0u, 0u);
   const uint32_t lo = run < G ? (uint32_t)((uint64_t)total * run / G) : 0u, hi = run < G ? (uint32_t)((uint64_t)total * (run + 1) / G) : 0u;
   uint32_t b = lo < hi ? find_sequence(pre, R, lo) : 0u;
-  uint32_t st = 0, sp = 0, tile = 0, unit = 0;   // the ring's stage and how often it came round; key tiles and units with tiles so far (each role counts its own uses alike)
+  uint32_t tile = 0, unit = 0;   // key tiles and units with tiles so far
+  struct Ring {                  // the stage to use next, how often they came round (each role counts its own uses alike)
+    uint32_t i = 0, round = 0;
+    __device__ __forceinline__ void next(uint32_t n) {
+      if (++i == n) i = 0u, round++;
+    }
+  } rk, rv;
   const float c = fabsf(j.scale) * 1.44269504088896340736f;
-  const uint32_t flip = j.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale turns q around, so that maxima stay maxima
+  const bool flip = j.scale < 0.0f;   // a negative scale turns S around, so that maxima stay maxima
   // A wait that gives up sets the CTA's abort word, after which all its waits give up at once; every warp still walks the
   // same units to the end. Nothing stops between units: the next one's K, q and first S run under this one's end
-  const auto next = [&]() {
-    if (++st == (uint32_t)NS) st = 0u, sp++;
-  };
   for (uint32_t at = lo; at < hi;) {
     while (pre[b + 1] <= at) b++;
     const Unit u = find_unit<kRB, kPP, kE>(j, pre, b, at);
@@ -235,143 +246,128 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
         const uint32_t jp = page_at(s, min(i, s.n - 1u)), k = jp < all.sink_pages ? jp : all.sink_pages + (jp - all.from);
         return base + (uint64_t)k * nkv * C::kSlot;
       };
-      const auto stage = [&]() -> uint8_t * {
-        if (!tc::mbar_wait(&empty[st], (sp & 1u) ^ 1u, abort_flag, j.err, 0x4b1u, P0_SPIN_LIMIT)) return nullptr;
-        tc::mbar_expect_tx(&full[st], C::kStage);
-        return ring + st * C::kStage;
-      };
-      const auto load_k = [&](uint32_t i) {
-        const uint8_t *from = slot(2u * i + rank);
-        for (uint32_t x = 0; x < C::kNK; x++) {
-          uint8_t *d = stage();
-          if (!d) return false;
-          bulk_load(d, from + x * C::kStage, C::kStage, &full[st]);
-          next();
+      if (lane == 0 && tiles) {   // whichever ring has a free stage
+        constexpr uint32_t half = C::kDV * 64, per = 2 / C::kNV;   // bytes of this CTA's dims of a page, pages of a stage
+        const uint32_t nk = tiles * C::kNK, nv = tiles * C::kNV;
+        for (uint32_t ik = 0, iv = 0, spins = 0; (ik < nk || iv < nv) && !*abort_flag;) {
+          bool idle = true;
+          if (ik < nk && tc::mbar_test(&empty[rk.i], (rk.round & 1u) ^ 1u)) {
+            tc::mbar_expect_tx(&full[rk.i], C::kStage);
+            bulk_load(ring + rk.i * C::kStage, slot(2u * (from + ik / C::kNK) + rank) + ik % C::kNK * C::kStage, C::kStage, &full[rk.i]);
+            rk.next(SK);
+            ik++;
+            idle = false;
+          }
+          if (iv < nv && tc::mbar_test(&empty[SK + rv.i], (rv.round & 1u) ^ 1u)) {
+            tc::mbar_expect_tx(&full[SK + rv.i], C::kStage);
+            for (uint32_t k = 0; k < per; k++)
+              bulk_load(ring + (SK + rv.i) * C::kStage + k * half, slot(2u * from + iv * per + k) + D * 128 + (oh * 2u + rank) * half, half, &full[SK + rv.i]);
+            rv.next(C::kSV);
+            iv++;
+            idle = false;
+          }
+          spins = idle ? spins + 1u : 0u;
+          if (spins == P0_SPIN_LIMIT) {
+            *abort_flag = 1u;
+            atomicOr(j.err, 0x4b1u);
+          }
         }
-        return true;
-      };
-      const auto load_v = [&](uint32_t i) {
-        constexpr uint32_t half = C::kDV * 64;   // bytes of this CTA's dims of a page
-        for (uint32_t h = 0; h < 2;) {
-          uint8_t *d = stage();
-          if (!d) return false;
-          for (uint32_t k = 0; k < 2 / C::kNV; k++, h++)
-            bulk_load(d + k * half, slot(2u * i + h) + D * 128 + (oh * 2u + rank) * half, half, &full[st]);
-          next();
-        }
-        return true;
-      };
-      if (lane == 0 && tiles && load_k(from))
-        for (uint32_t i = 0; i < tiles; i++) {
-          if (i + 1 < tiles && !load_k(from + i + 1)) break;
-          if (!load_v(from + i)) break;
-        }
+      }
       __syncwarp();
-    } else if (warp == 9) {
-      // ------------------------------------------------------------ the pair's MMAs (even CTA), word of what landed (odd CTA)
-      const auto tell = [&]() {
-        const bool ok = tc::mbar_wait(&full[st], sp & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
-        if (ok) tc::mbar_arrive_rank(&full[st], 0);
-        next();
-        return ok;
-      };
+    } else if (warp == 9 || warp == 10) {
+      // ------------------------------------------------------------ the pair's MMAs (even CTA), word of what landed (odd CTA): S by one
+      // warp, P V by another. What a thread issues after a wait comes a few hundred cycles late; with a thread each, S and P V hide that
+      // for one another. The waits that are over come first
+      const auto landed = [&](uint32_t i, uint32_t round) { return tc::mbar_wait(&full[i], round & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT); };
+      const auto part_of = [](uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); };   // within shared memory: no carry out of the address
       if (lane == 0 && rank == 1) {
-        for (uint32_t i = 0; i < (C::kNK + C::kNV) * tiles && tell(); i++) {}
-      } else if (lane == 0 && tiles) {
-        constexpr uint32_t is = tc::idesc_f16_f32(256, 128), iv = tc::idesc_f16_f32(256, C::kDV);
-        const auto arrived = [&]() {
-          return tc::mbar_wait(&full[st], sp & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
-        };
-        const auto part_of = [](uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); };   // within shared memory: no carry out of the address
-        const auto scores = [&](uint32_t t) {   // over S of tile t - kSB
-          const uint32_t o = t - C::kSB;
-          if (!arrived()) return false;   // the waits that are over first: what follows the last one is in the tensor core's way
-          if (t >= C::kSB && !tc::mbar_wait(&sread[o % C::kSB], (o / C::kSB) & 1u, abort_flag, j.err, 0x4b9u, P0_SPIN_LIMIT)) return false;
-          tc::fence_after();
-          const uint32_t sb = t % C::kSB, dst = tmem + C::kColS + sb * 128u;
-          constexpr uint32_t per = C::kKB / C::kNK;   // 64-dim blocks of a stage
+        Ring &g = warp == 9 ? rk : rv;
+        const uint32_t n = tiles * (warp == 9 ? C::kNK : C::kNV), size = warp == 9 ? SK : C::kSV, base = warp == 9 ? 0u : SK;
+        for (uint32_t i = 0; i < n && landed(base + g.i, g.round); i++) {
+          tc::mbar_arrive_rank(&full[base + g.i], 0);
+          g.next(size);
+        }
+      } else if (lane == 0 && warp == 9 && tiles) {
+        constexpr uint32_t is = tc::idesc_f16_f32(256, 128), per = C::kKB / C::kNK;   // 64-dim blocks of a stage
+        bool ok = tc::mbar_wait_cluster(&qfull, unit & 1u, abort_flag, j.err, 0x4bcu, P0_SPIN_LIMIT);
+        for (uint32_t t = tile; t < tile + tiles && ok; t++) {   // over S of tile t - kSB
+          const uint32_t o = t - C::kSB, sb = t % C::kSB, dst = tmem + C::kColS + sb * 128u;
 #pragma unroll 1
           for (uint32_t y = 0; y < C::kNK; y++) {
-            if (y) {
-              if (!arrived()) return false;
-              tc::fence_after();
-            }
-            const uint64_t kd = tc::desc_sw128(tc::smem_u32(ring + st * C::kStage)), qd = tc::desc_sw128(tc::smem_u32(qs) + y * per * 16384u);
+            if (!(ok = landed(rk.i, rk.round))) break;
+            if (y == 0 && t >= C::kSB && !(ok = tc::mbar_wait(&sread[o % C::kSB], (o / C::kSB) & 1u, abort_flag, j.err, 0x4b9u, P0_SPIN_LIMIT))) break;
+            tc::fence_after();
+            const uint64_t kd = tc::desc_sw128(tc::smem_u32(ring + rk.i * C::kStage)), qd = tc::desc_sw128(tc::smem_u32(qs) + y * per * 16384u);
 #pragma unroll
             for (uint32_t x = 0; x < per * 4u; x++)
               tc::mma_ss_f16_pair(dst, part_of(qd, (x >> 2) * 16384u + (x & 3u) * 32u), part_of(kd, (x >> 2) * 8192u + (x & 3u) * 32u), is, (y | x) != 0u);
             if (y + 1 == C::kNK) tc::mma_commit_pair(&sfull[sb]);
-            tc::mma_commit_pair(&empty[st]);
-            next();
+            tc::mma_commit_pair(&empty[rk.i]);
+            rk.next(SK);
           }
-          if (t + 1u == tile + tiles) tc::mma_commit_pair(&qdone);
-          return true;
-        };
-        bool ok = tc::mbar_wait_cluster(&qfull, unit & 1u, abort_flag, j.err, 0x4bcu, P0_SPIN_LIMIT) && scores(tile);
-        for (uint32_t i = 0; i < tiles && ok; i++) {
-          const uint32_t t = tile + i;
-          if (i + 1 < tiles && !(ok = scores(t + 1))) break;
-          if (!(ok = arrived())) break;
-          if (!(ok = tc::mbar_wait(&pfull[t & 1u], (t >> 1) & 1u, abort_flag, j.err, 0x4b4u, P0_SPIN_LIMIT))) break;
-          tc::fence_after();
+        }
+        if (ok) tc::mma_commit_pair(&qdone);
+      } else if (lane == 0 && warp == 10 && tiles) {
+        constexpr uint32_t iv = tc::idesc_f16_f32(256, C::kDV), steps = 8 / C::kNV;   // of 16 keys
+        bool ok = true;
+        for (uint32_t t = tile; t < tile + tiles && ok; t++) {
           const uint32_t pa = tmem + C::kColP + (t & 1u) * 64u;
 #pragma unroll 1
           for (uint32_t y = 0; y < C::kNV; y++) {
-            constexpr uint32_t steps = 8 / C::kNV;   // of 16 keys
-            if (y) {
-              if (!(ok = arrived())) break;
-              tc::fence_after();
-            }
-            const uint64_t vd = tc::desc_sw128(tc::smem_u32(ring + st * C::kStage));
+            if (!(ok = landed(SK + rv.i, rv.round))) break;
+            if (y == 0 && !(ok = tc::mbar_wait(&pfull[t & 1u], (t >> 1) & 1u, abort_flag, j.err, 0x4b4u, P0_SPIN_LIMIT))) break;
+            tc::fence_after();
+            const uint64_t vd = tc::desc_sw128(tc::smem_u32(ring + (SK + rv.i) * C::kStage));
 #pragma unroll
             for (uint32_t x = 0; x < steps; x++)
-              tc::mma_ts_f16_pair(tmem, pa + (y * steps + x) * 8u, part_of(vd, (x >> 2) * (C::kDV * 64u) + (x & 3u) * 32u), iv, (i | y | x) != 0u);
+              tc::mma_ts_f16_pair(tmem, pa + (y * steps + x) * 8u, part_of(vd, (x >> 2) * (C::kDV * 64u) + (x & 3u) * 32u), iv, (t != tile) | (y | x) != 0u);
             if (y + 1 == C::kNV) tc::mma_commit_pair(&odone[t & 1u]);
-            tc::mma_commit_pair(&empty[st]);
-            next();
+            tc::mma_commit_pair(&empty[SK + rv.i]);
+            rv.next(C::kSV);
           }
-          if (!ok) break;
         }
       }
       __syncwarp();
-    } else if (warp >= 10) {
-      // ------------------------------------------------------------ q rows, swizzled (a warp reads a row or more at a time); zeros beyond
+    } else if (warp == 11) {
+      // ------------------------------------------------------------ q rows, as K's: blocks of 64 dims, swizzled rows of 128 bytes
       bool ok = true;
       if (unit && tiles) ok = tc::mbar_wait(&qdone, (unit - 1u) & 1u, abort_flag, j.err, 0x4bdu, P0_SPIN_LIMIT);
       if (!C::kStg && unit && tiles) ok = ok && tc::mbar_wait(&ofree, (unit - 1u) & 1u, abort_flag, j.err, 0x4beu, P0_SPIN_LIMIT);
-      if (__all_sync(0xffffffffu, ok && tiles)) {
-        // a warp takes 64 of the rows, RW at a time, 16 bytes a lane; each lane works out the places of two
-        constexpr uint32_t CH = D < 256 ? D / 8 : 32, RW = 32 / CH, N = 64 / RW;
-        const uint32_t r0 = (warp & 1u) * 64u;
-        uint64_t place[2];
+      ok = __all_sync(0xffffffffu, ok && tiles);
+      if (ok && j.qbox) {          // by tensor copies; rows of other sequences beyond this one's are not looked at
+        if (lane == 0) {
+          uint64_t *bar = rank ? &qland : &qfull;
+          tc::mbar_expect_tx(bar, C::kQ);
+          for (uint32_t k = 0; k < C::kKB; k++)
+            tma_load_3d(qs + k * 16384u, &qm, bar, (int32_t)(k * 64u), (int32_t)(head * hpg + rc % hpg), (int32_t)(u.first + rc / hpg));
+          if (rank && tc::mbar_wait(&qland, unit & 1u, abort_flag, j.err, 0x4bfu, P0_SPIN_LIMIT)) tc::mbar_arrive_rank(&qfull, 0);
+        }
+      } else if (ok) {             // RW rows at a time, 16 bytes a lane; each lane works out the places of four. Zeros beyond the rows
+        constexpr uint32_t CH = D < 256 ? D / 8 : 32, RW = 32 / CH;
+        uint64_t place[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 2; i++) {
-          const uint32_t row = rc + r0 + 32u * i + lane, tok = row / hpg;
+        for (uint32_t i = 0; i < 4; i++) {
+          const uint32_t row = rc + 32u * i + lane, tok = row / hpg;
           place[i] = (uint64_t)(u.first + tok) * j.q.ld + (uint64_t)(head * hpg + row - tok * hpg) * j.q.ldh;
         }
-#pragma unroll 2
-        for (uint32_t n0 = 0; n0 < N; n0 += 4) {
-          uint64_t at4[4];
 #pragma unroll
-          for (uint32_t n = 0; n < 4; n++) {
-            const uint32_t r = (n0 + n) * RW + lane / CH;
-            at4[n] = __shfl_sync(0xffffffffu, (n0 + n) * RW < 32u ? place[0] : place[1], r & 31u);
-          }
-#pragma unroll
-          for (uint32_t n = 0; n < 4; n++) {
-            const uint32_t row = r0 + (n0 + n) * RW + lane / CH;
+        for (uint32_t g = 0; g < 4; g++) {
+#pragma unroll 4
+          for (uint32_t r0 = 0; r0 < 32; r0 += RW) {
+            const uint32_t row = 32u * g + r0 + lane / CH;
             const bool there = row < nrow;
-            const __half *q = reinterpret_cast<const __half *>(j.q.base) + (there ? at4[n] : 0u);
+            const uint64_t at = __shfl_sync(0xffffffffu, place[g], r0 + lane / CH);
+            const __half *q = reinterpret_cast<const __half *>(j.q.base) + (there ? at : 0u);
 #pragma unroll
             for (uint32_t d8 = lane % CH; d8 < D / 8; d8 += CH) {
               uint8_t *to = qs + (d8 >> 3) * 16384u + row * 128u + (((d8 & 7u) ^ (row & 7u)) * 16u);
-              if (j.q.wide && !flip) {   // asynchronous; no bytes read, zeros written beyond the rows
+              if (j.q.wide) {
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(to)), "l"(q + d8 * 8u), "r"(there ? 16u : 0u) : "memory");
               } else {
                 uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                  if (there) w[i] = ((uint32_t)__half_as_ushort(q[d8 * 8u + 2 * i]) | ((uint32_t)__half_as_ushort(q[d8 * 8u + 2 * i + 1]) << 16)) ^ flip;
+                  if (there) w[i] = (uint32_t)__half_as_ushort(q[d8 * 8u + 2 * i]) | ((uint32_t)__half_as_ushort(q[d8 * 8u + 2 * i + 1]) << 16);
                 *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
               }
             }
@@ -419,6 +415,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
           tc::fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive_peer(&sread[t % C::kSB], 0);   // the even CTA's MMAs wait for both
+          if (flip)
+#pragma unroll
+            for (int e = 0; e < 64; e++) x[e >> 5][e & 31] ^= 0x80000000u;
           // keys that this row does not see; a page that the whole block sees needs no look
           const int32_t k0 = (int32_t)(jp * kPage);
           if (!(here && k0 + 63 <= pos0 && (!W || k0 > pos1 - (int32_t)W || (uint32_t)k0 + 63u < S))) {
@@ -551,8 +550,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&ofree);
     }
-    st = __shfl_sync(0xffffffffu, st, 0);   // the issuing lane's
-    sp = __shfl_sync(0xffffffffu, sp, 0);
     tile += tiles;
     unit += tiles != 0u;
   }
@@ -560,11 +557,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   if (abort_word && lane == 0) {   // a wait gave up (j.err says which): nothing may be in flight when the CTA leaves. Bounded
     volatile uint32_t never = 0;
     if (warp == 8)
-      for (uint32_t i = 0; i < (uint32_t)NS; i++)
-        if (sp || i < st) tc::mbar_wait(&full[i], (i < st ? sp : sp - 1u) & 1u, &never, j.err, 0x4b2u, P0_SPIN_LIMIT);
-    if (warp == 9 && rank == 0) {
-      tc::mma_commit_pair(&mdone);
-      tc::mbar_wait(&mdone, 0, &never, j.err, 0x4b5u, P0_SPIN_LIMIT);
+      for (uint32_t i = 0; i < (uint32_t)NS; i++) {
+        const Ring &g = i < SK ? rk : rv;
+        const uint32_t n = i < SK ? i : i - SK;
+        if (g.round || n < g.i) tc::mbar_wait(&full[i], (n < g.i ? g.round : g.round - 1u) & 1u, &never, j.err, 0x4b2u, P0_SPIN_LIMIT);
+      }
+    if (warp == 11 && j.qbox && unit) tc::mbar_wait(rank ? &qland : &qfull, (unit - 1u) & 1u, &never, j.err, 0x4b2u, P0_SPIN_LIMIT);
+    if ((warp == 9 || warp == 10) && rank == 0) {
+      tc::mma_commit_pair(&mdone[warp - 9]);
+      tc::mbar_wait(&mdone[warp - 9], 0, &never, j.err, 0x4b5u, P0_SPIN_LIMIT);
     }
   }
   __syncwarp();
@@ -636,11 +637,21 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
   j.part = (float *)((uint8_t *)ws + desc);
   j.wide = (uint8_t *)ws + desc + parts;
   const auto kern = kv4_prompt_kernel<D>;
+  // q as [tokens][heads][dims]: where 128 rows are whole tokens' heads, or some of one token's, a block is a box of it
+  CUtensorMap qm = {};
+  const auto encode = tensor_map_encoder();
+  if (encode && j.q.wide && (j.hpg & (j.hpg - 1u)) == 0u) {
+    const uint32_t heads = j.hpg < kCR ? j.hpg : kCR;
+    const cuuint64_t size[3] = {(cuuint64_t)D, (cuuint64_t)j.hpg * j.v.nkv, j.v.n}, stride[2] = {(cuuint64_t)j.q.ldh * 2u, (cuuint64_t)j.q.ld * 2u};
+    const cuuint32_t box[3] = {64, heads, kCR / heads}, one[3] = {1, 1, 1};
+    j.qbox = encode(&qm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<uint8_t *>(j.q.base), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  }
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) { cudaGetLastError(); return p0_fail(c, P0_EDEVICE, "kv4Attn: the prompt kernel does not fit this device"); }
   launch_dep(kv4_widen_kernel<D>, dim3((unsigned)c->sm_count * 4u), dim3(kET), ((size_t)R + 1) * 4, c->stream, j);
   if ((st = p0_launched(c, "kv4Attn pages"))) return st;
-  launch_dep(kern, dim3(2 * G), dim3(kThreads), smem, c->stream, j);
+  launch_dep(kern, dim3(2 * G), dim3(kThreads), smem, c->stream, j, qm);
   if ((st = p0_launched(c, "kv4Attn prompt"))) return st;
   launch_dep(kv4_prompt_join_kernel<D>, dim3(G, C::kDV / 8, 2), dim3(kCR), 0, c->stream, j);
   return p0_launched(c, "kv4Attn join");

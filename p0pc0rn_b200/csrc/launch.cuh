@@ -1,8 +1,10 @@
 // launch.cuh -- programmatic dependent launch for the small operator kernels: every kernel is launched so that it may
 // start while the kernel ahead of it is still running; it waits for that kernel (griddepcontrol.wait: all prerequisite
 // grids complete, their writes visible) before it reads anything, then lets the kernel after it launch at once. Without
-// such a launch both are no-ops.
+// such a launch both are no-ops. And the driver's encoder of tensor maps.
 #pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 __device__ __forceinline__ void dep_enter() {
@@ -24,4 +26,16 @@ cudaError_t launch_dep(Kern k, dim3 grid, dim3 block, size_t smem, cudaStream_t 
   cfg.attrs = at;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
+// cuTensorMapEncodeTiled, or null
+inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (!fn) {
+    void *f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = (PFN_cuTensorMapEncodeTiled_v12000)f;
+  }
+  return fn;
 }
