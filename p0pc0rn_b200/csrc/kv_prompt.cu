@@ -23,7 +23,7 @@
 namespace {
 
 constexpr uint32_t kRB = 256, kCR = 128, kPP = 2;   // query rows of a block and of a CTA, pages of a key tile
-constexpr uint32_t kE = 2;                   // a unit's beginning and end cost about as much as two key tiles
+constexpr uint32_t kE = 4;                   // a unit's beginning and end cost about as much as four key tiles
 constexpr int kSoft = 256, kThreads = kSoft + 128;   // warps 0-7: softmax (0-3 the tile's first page, 4-7 its second); 8: copies; 9: S; 10: P V; 11: q
 
 template <int D>
@@ -146,6 +146,8 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const void *tmap, uint64_
       "l"(tmap), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
+// bits 0 .. n - 1
+__device__ __forceinline__ uint64_t first_bits(int32_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -167,7 +169,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 
 template <int D>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_prompt_kernel(AttnJob j, const __grid_constant__ CUtensorMap qm) {
-  dep_enter();
   using C = Cfg<D>;
   constexpr int NS = C::kStages, SK = C::kSK;
   extern __shared__ uint8_t smem_raw[];
@@ -212,6 +213,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   tc::fence_before();
   tc::cluster_sync();
   tc::fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp == 8) asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t tmem = tmem_slot;
   const uint32_t total = pre[R], runs = gridDim.x >> 1, G = min(runs, max(total, 1u));
   if (tid == 0 && rank == 0) j.desc[run] = make_uint4(0u, 0u, 0u, 0u);
@@ -228,9 +231,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   const bool flip = j.scale < 0.0f;   // a negative scale turns S around, so that maxima stay maxima
   // A wait that gives up sets the CTA's abort word, after which all its waits give up at once; every warp still walks the
   // same units to the end. Nothing stops between units: the next one's K, q and first S run under this one's end
+  Unit u;
   for (uint32_t at = lo; at < hi;) {
-    while (pre[b + 1] <= at) b++;
-    const Unit u = find_unit<kRB, kPP, kE>(j, pre, b, at);
+    if (at == lo || pre[b + 1] <= at) {
+      while (pre[b + 1] <= at) b++;
+      u = find_unit<kRB, kPP, kE>(j, pre, b, at);
+    } else {   // the next one of this sequence
+      u.begin += u.n;
+      if (++u.head == j.units) {
+        u.head = 0;
+        u.r0 += kRB;
+        u.n = unit_items<kRB, kPP, kE>(j, u.len, u.T, u.r0, u.s);
+      }
+    }
     const Span &s = u.s;
     const uint32_t from = max(at - u.begin, kE) - kE, nt = u.n - kE, end = min(hi - u.begin, u.n), to = max(end, kE) - kE;
     at = u.begin + end;
@@ -424,13 +437,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
             // keys up to `gone` are behind the window, those below `sink` are kept all the same
             const int32_t last = here ? pos - k0 : -1, gone = W ? pos - (int32_t)W - k0 : -1;
             const int32_t sink = S > (uint32_t)k0 ? (int32_t)min(S - (uint32_t)k0, kPage) : 0;
+            const uint64_t see = first_bits(last + 1) & (~first_bits(gone + 1) | first_bits(sink));
 #pragma unroll
-            for (int q = 0; q < 2; q++)
+            for (int q = 0; q < 2; q++) {
+              const uint32_t bits = (uint32_t)(see >> (32 * q));
 #pragma unroll
-              for (int e = 0; e < 32; e++) {
-                const int32_t k = q * 32 + e;
-                if (!(k <= last && (k > gone || k < sink))) x[q][e] = 0xff800000u;
-              }
+              for (int e = 0; e < 32; e++)
+                if (!(bits >> e & 1u)) x[q][e] = 0xff800000u;
+            }
           }
           float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
