@@ -216,7 +216,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 8) asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t tmem = tmem_slot;
-  const uint32_t total = pre[R], runs = gridDim.x >> 1, G = min(runs, max(total, 1u));
+  const uint32_t total = pre[R], runs = gridDim.x >> 1, G = min(runs, max(total / 2u, 1u));   // two tiles at least: parts cost more
   if (tid == 0 && rank == 0) j.desc[run] = make_uint4(0u, 0u, 0u, 0u);
   const uint32_t lo = run < G ? (uint32_t)((uint64_t)total * run / G) : 0u, hi = run < G ? (uint32_t)((uint64_t)total * (run + 1) / G) : 0u;
   uint32_t b = lo < hi ? find_sequence(pre, R, lo) : 0u;
@@ -591,37 +591,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   }
 }
 
-// joins the parts of a unit that several runs share: CTA (run, 8 dims, 128 of the rows), a thread per row. M = max m, o = sum
-// 2^(m - M) acc / sum 2^(m - M) l, in run order
-template <int D>
-__global__ void __launch_bounds__(kCR) kv4_prompt_join_kernel(AttnJob j) {
+// joins the parts of a unit that several runs share: CTA (run, 8 dims, 128 of the rows), a thread per row and every kJoin-th part,
+// then those in order. M = max m, o = sum 2^(m - M) acc / sum 2^(m - M) l
+template <int D, uint32_t kJoin>
+__global__ void __launch_bounds__(kCR *kJoin) kv4_prompt_join_kernel(AttnJob j) {
   dep_enter();
   const uint4 w = j.desc[blockIdx.x];
   if (!w.x) return;
   constexpr uint32_t DV = Cfg<D>::kDV;
-  const uint32_t r = threadIdx.x, d0 = blockIdx.y * 8u, rank = blockIdx.z, b = w.y, r0 = w.z + rank * kCR, hpg = j.hpg;
-  const uint32_t head = w.w / Cfg<D>::kParts, oh = w.w % Cfg<D>::kParts;
+  __shared__ float got[kJoin][10][kCR];
+  const uint32_t r = threadIdx.x % kCR, g = threadIdx.x / kCR, d0 = blockIdx.y * 8u, rank = blockIdx.z, b = w.y, r0 = w.z + rank * kCR, hpg = j.hpg;
+  const uint32_t head = w.w / Cfg<D>::kParts, oh = w.w % Cfg<D>::kParts, n = w.x - blockIdx.x;
   uint32_t first;
-  const uint32_t T = kv_tokens(j.v, b, first), n = w.x - blockIdx.x;
-  if (r0 + r >= T * hpg) return;
+  const uint32_t T = kv_tokens(j.v, b, first);
+  const bool here = r0 + r < T * hpg;
   const auto part = [&](uint32_t i) { return j.part + (((uint64_t)(blockIdx.x + i) * 2u + (i ? 0u : 1u)) * 2u + rank) * kCR * (DV + 2) + r; };
-  float M = -INFINITY;
-#pragma unroll 8
-  for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part(i)[DV * kCR]);
-  const float ref = M == -INFINITY ? 0.0f : M;
-  float acc[8], sum = 0.0f;
+  float M = -INFINITY, acc[8], sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; e++) acc[e] = 0.0f;
+  if (here) {
+#pragma unroll 8
+    for (uint32_t i = g; i < n; i += kJoin) M = fmaxf(M, part(i)[DV * kCR]);
+    const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll 4
-  for (uint32_t i = 0; i < n; i++) {
-    const float *p = part(i);
-    float x[8];
+    for (uint32_t i = g; i < n; i += kJoin) {
+      const float *p = part(i);
+      float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = p[(d0 + e) * kCR];
-    const float f = exp2f(p[DV * kCR] - ref);
-    sum = fmaf(f, p[(DV + 1) * kCR], sum);
+      for (int e = 0; e < 8; e++) x[e] = p[(d0 + e) * kCR];
+      const float f = exp2f(p[DV * kCR] - ref);
+      sum = fmaf(f, p[(DV + 1) * kCR], sum);
 #pragma unroll
-    for (int e = 0; e < 8; e++) acc[e] = fmaf(f, x[e], acc[e]);
+      for (int e = 0; e < 8; e++) acc[e] = fmaf(f, x[e], acc[e]);
+    }
+  }
+  if (g) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) got[g][e][r] = acc[e];
+    got[g][8][r] = sum;
+    got[g][9][r] = M;
+  }
+  __syncthreads();
+  if (g || !here) return;
+  float all = M;
+#pragma unroll
+  for (uint32_t i = 1; i < kJoin; i++) all = fmaxf(all, got[i][9][r]);
+  const float ref = all == -INFINITY ? 0.0f : all, f0 = exp2f(M - ref);
+  sum *= f0;
+#pragma unroll
+  for (int e = 0; e < 8; e++) acc[e] *= f0;
+#pragma unroll
+  for (uint32_t i = 1; i < kJoin; i++) {
+    const float f = exp2f(got[i][9][r] - ref);
+    sum = fmaf(f, got[i][8][r], sum);
+#pragma unroll
+    for (int e = 0; e < 8; e++) acc[e] = fmaf(f, got[i][e][r], acc[e]);
   }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   __half *out = reinterpret_cast<__half *>(j.out.base) + (uint64_t)(first + (r0 + r) / hpg) * j.out.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.out.ldh + oh * DV + d0;
@@ -667,7 +691,11 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
   if ((st = p0_launched(c, "kv4Attn pages"))) return st;
   launch_dep(kern, dim3(2 * G), dim3(kThreads), smem, c->stream, j, qm);
   if ((st = p0_launched(c, "kv4Attn prompt"))) return st;
-  launch_dep(kv4_prompt_join_kernel<D>, dim3(G, C::kDV / 8, 2), dim3(kCR), 0, c->stream, j);
+  // four threads a row where units are in many parts (16 rows' heads of 30000 keys, D = 256: 57 us with one, 45 with four), one
+  // where they are in two or three (3 x 2048 of 5003 tokens: 110 with one, 126 with four)
+  const uint64_t units = ((uint64_t)j.v.n * j.hpg / kRB + 1u) * j.units;
+  if (units * 4u <= G) launch_dep(kv4_prompt_join_kernel<D, 4>, dim3(G, C::kDV / 8, 2), dim3(kCR * 4), 0, c->stream, j);
+  else launch_dep(kv4_prompt_join_kernel<D, 1>, dim3(G, C::kDV / 8, 2), dim3(kCR), 0, c->stream, j);
   return p0_launched(c, "kv4Attn join");
 }
 
@@ -676,7 +704,7 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
 p0_status kv4_attn_prompt(p0_ctx *c, AttnJob &j, bool *taken) {
   *taken = false;
   const uint64_t rows = (uint64_t)j.v.n * j.hpg, D = j.v.D;
-  if (rows / j.v.rows < 64) return P0_OK;
+  if (rows / j.v.rows < (D == 512 ? 128 : 64)) return P0_OK;
   const uint64_t wide = (uint64_t)j.v.rows * j.v.ld * j.v.nkv * D * 256;
   if (wide > (4ull << 30) || j.v.rows > 256) return P0_OK;
   *taken = true;
