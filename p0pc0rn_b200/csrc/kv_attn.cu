@@ -566,8 +566,9 @@ p0_status attn_launch(p0_ctx *c, AttnJob &j) {
   return p0_launched(c, "kv4Attn join");
 }
 
-// fragments per block: one, two or four, so that a page is dequantised for as many rows at once as there are (at D = 512 two:
-// the sums fill the registers; four of f32 take 32 dims a warp instead of 64)
+// fragments per block: one, two or four, so that a page is dequantised for as many rows at once as there are. Four of f32 take 32
+// dims a warp instead of 64. At D = 512 one: with two, a warp's sums leave one CTA an SM, and dequantising twice on two is as fast
+// or faster (4 sequences of 8000 keys, 32 rows a KV head: f32 58 us with two, 57 with one; f16 53 and 47)
 template <int D, bool F32, int KP>
 p0_status pick(p0_ctx *c, AttnJob &j, uint32_t frags) {
   // One fragment and room for many pages (the lengths are on the device: what the table and the window allow decides): four
@@ -576,10 +577,11 @@ p0_status pick(p0_ctx *c, AttnJob &j, uint32_t frags) {
   const uint64_t most = j.window ? min((uint64_t)j.v.ld, (uint64_t)j.window / kPage + 2 + (j.sinks + kPage - 1) / kPage) : j.v.ld;
   if constexpr (D < 512)
     if (frags <= 1 && most * j.v.rows * j.v.nkv >= 16ull * c->sm_count) return attn_launch<D, F32, 8, 1, 1, 4>(c, j);
-  if (frags <= 1) return attn_launch<D, F32, 8, 1, KP, 8>(c, j);
-  if (frags == 2 || D == 512) return attn_launch<D, F32, 8, 2, KP, 8>(c, j);
-  if constexpr (D < 512) return attn_launch<D, F32, F32 ? 4 : 8, 4, KP, 8>(c, j);
-  return P0_OK;
+  if constexpr (D < 512) {
+    if (frags == 2) return attn_launch<D, F32, 8, 2, KP, 8>(c, j);
+    if (frags > 2) return attn_launch<D, F32, F32 ? 4 : 8, 4, KP, 8>(c, j);
+  }
+  return attn_launch<D, F32, 8, 1, KP, 8>(c, j);
 }
 
 }  // namespace
