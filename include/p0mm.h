@@ -325,7 +325,8 @@ p0_status p0_attn_dec(p0_ctx *ctx, const p0_attn_dec_args *a);
  * State on the device: table u32 [rows][table_ld], the page of each sequence's tokens 64 j .. 64 j + 63 (an entry >=
  * pages, e.g. P0_KV_NONE, is no page: its tokens are not there), len u32 [rows] (a length beyond 64 * table_ld counts as
  * that), and ref u32 [pages], how many table entries (and holders of the caller's own) refer to each page.
- * Offsets of table and len in u32. rows <= 1024, D 64, 128, 256 or 512; pool_off, page_stride 16-byte aligned.
+ * Offsets of table and len in u32. rows <= 1024, nkv <= 1024, table_ld <= 2^23, tokens of a call <= 2^28, D 64, 128, 256 or 512;
+ * pool_off, page_stride 16-byte aligned.
  * Everything is read when the call's kernels run, so a call's arguments stay valid from step to step. The operators keep
  * their scratch in the context's workspace: calls of one context run in stream order, also after p0_set_stream only if
  * the caller orders the streams; the first call of a size may grow it (which waits for the stream), so it should not sit

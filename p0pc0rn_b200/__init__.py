@@ -4,7 +4,8 @@ The product is the C-ABI library libp0mm.so (include/p0mm.h; CUDA kernels under 
 and mirrors the reference's operator surface with the same argument objects and error messages:
   gemv / gemvM (engine/llm/lops.js, engine/llm/lops_spec.js) and gemm (engine/ops/gemm.js),
 over Gpu buffers (engine/core/gpu.js), plus the quantisers packQ4 / packQ8 (engine/kcheck.js:22-53) on the device;
-the decode-path operators around the GEMV (embed, normadd, qkrope, attnDec, argmax / argmaxM, dhead); and the
+the decode-path operators around the GEMV (embed, normadd, qkrope, attnDec, argmax / argmaxM, dhead); a paged 4-bit KV
+cache for many sequences (kv4Put, kv4Get, kv4Attn, kvStep, kvCompact) with beam search's selection (beamSelect); and the
 weight-pack store (p0pc0rn_b200.store, engine/core/store.js) that uploads pack shards into device buffers.
 """
 from .gpu import Buffer, Gpu, P0Error, createGpu, version  # noqa: F401

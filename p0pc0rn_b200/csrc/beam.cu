@@ -10,6 +10,8 @@
 // grows, so every candidate above the k-th best c has been kept; candidates that round to the very same c as the k-th best
 // may not have been, and where that can be (a part's last kept one ties with it) the merge looks the row's logits up again
 // in index order.
+// 128 rows of 262144 logits, 8 beams: 33.8 us, 4.0 TB/s; the scan's instructions and the merge's launch stand before the
+// bytes. 4 rows of 4099: 8.7 us, two launches.
 #include "internal.h"
 #include "launch.cuh"
 

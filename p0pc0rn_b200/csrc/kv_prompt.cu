@@ -7,17 +7,29 @@
 // The second is attention over tiles of 128 keys (two pages) for 256 query rows (of one KV head: tokens x its query heads)
 // by a pair of CTAs, each with 128 of the rows. The pair's MMAs (cta_group::2) read half of K and V from either CTA's
 // shared memory: a CTA loads one of the two pages of K and half of V's dims, half the bytes out of L2 that a CTA on its
-// own would need for the same rows, and the ring holds two tiles of D = 256. In each CTA one warp issues the bulk copies,
-// one the pair's MMAs (the odd CTA's tells the even one's what has landed), eight hold half a row (64 keys) per thread:
+// own would need for the same rows, and the rings hold two tiles of D = 256. In each CTA one warp issues the copies of K and
+// V, one those of q, two the pair's MMAs (the odd CTA's tell the even one's what has landed), eight hold half a row (64
+// keys) per thread:
 //   S_j = Q K_j^T     tcgen05.mma, 256 x 128 x D, f32 in tensor memory: S_j+1 runs while softmax_j computes, as soon as it has
-//                     read S_j (D = 256: one buffer) or S_j-1 (two)
-//   P_j = 2^(S_j c - m)   the row's maximum by its two threads through shared memory; f16 in tensor memory, two buffers
+//                     read S_j (256 dims and more: one buffer) or S_j-1 (two)
+//   P_j = 2^(S_j c - m)   the row's maximum by its two threads through shared memory; f16 in tensor memory (an operand's type:
+//                     a rounding of 2^-11 of each P, as the output's own), two buffers
 //   O  += P_j V_j     tcgen05.mma with P from tensor memory
 // Nothing in tensor memory is written while an MMA that was not waited for may read it (MMAs of different shapes or
 // accumulators have no order among themselves).
 // m is the row's maximum as of the last time O was rescaled: P may grow to 2^8 (harmless in f16 and f32) before O, in
 // tensor memory, is read and written again, which then happens in few tiles.
+// At 512 dims O does not fit: a unit is a row block and half of the output's dims, S is computed for each half, 1.5 times
+// the products of a whole.
 // Work is cut into equal runs of key tiles as in kv_attn.cuh, one per pair; a unit's parts meet in the join kernel.
+//
+// What bounds it: an MMA of 128 columns occupies the issuing thread for 84 cycles (64 of them at the tensor core's rate), one of 256
+// columns 128, and what a thread issues after a wait that is already over comes 150 cycles late: S and P V by one thread took
+// 4100 cycles a tile of 256 dims, by a thread each 2800, the softmax's chain (load 64 scores, maximum, barrier, exponentials, store P)
+// with one S buffer. A unit's end (the last P V, output through shared memory) costs another 6000 to 8000 cycles, under which the
+// next unit's K, q and first S run; the widening takes 7 us, the join of parts 8 to 10. 3 sequences with 2048 new of up to
+// 5003 tokens, 8 heads of 256 dims: 110 us, 0.98 PFLOP/s (125 in long runs at the power limit); 4 with 1500 of 6001, 16 heads of 128 on 4, window 1024: 133 us,
+// 0.34 PFLOP/s (units of 9 tiles); 2048 of 6000, 8 heads of 512: 250 us, 0.67 PFLOP/s.
 #include "kv_attn.cuh"
 
 namespace {
@@ -701,6 +713,10 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
 
 }  // namespace
 
+// Taken where the sequences have 64 query rows a KV head on average (128 at 512 dims): one sequence of 1200 keys, 64 rows of 256
+// dims, 22 us against 32 of the form for few rows; 24 of 6000 keys, 70 against 76; 32 rows of 1200 keys, 23 against 19. (One
+// sequence of 30000 keys and 64 rows: 57 against 50; 512 dims, 24 of 6000, 64 rows: 165 against 114, 256 rows: 152 against 269.)
+// And where all pages of the table as f16 take no more than 4 GB.
 p0_status kv4_attn_prompt(p0_ctx *c, AttnJob &j, bool *taken) {
   *taken = false;
   const uint64_t rows = (uint64_t)j.v.n * j.hpg, D = j.v.D;
