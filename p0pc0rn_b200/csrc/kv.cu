@@ -141,25 +141,39 @@ __device__ __forceinline__ void load8(const uint8_t *base, uint64_t at, float (&
   }
 }
 
-// The codes clamp(rint(fl(d / s)), 0, 15) of 8 values d = fl(x - mn) as a word, with r = fl(1 / s). d * r is within two units in
+// The codes clamp(rint(fl(d / s)), 0, 15) of 8 values d = fl(x - mn) as a word, with r = fl(1 / s). d * r is within three units in
 // the last place of the quotient, so it rounds to the same whole number unless it lies next to a half, and then the divisions
-// decide. y + 1.5 * 2^23 rounds y to a whole number, half to even, and holds it in its low bits.
+// decide. d * r + 1.5 * 2^23 rounds it to a whole number, half to even, and holds that in its low bits; what the upper bits add up
+// to, shifted, is taken off at the end.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float mn, float s, float r) {
   constexpr float kRound = 12582912.0f;
+  constexpr uint32_t kBits = 0x4b400000u;   // of kRound
   uint32_t word = 0;
   float off = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(x[e], mn), r), 0.0f), 15.0f), t = __fadd_rn(y, kRound);
-    off = fmaxf(off, fabsf(__fsub_rn(y, __fsub_rn(t, kRound))));
-    word |= (__float_as_uint(t) & 15u) << (4 * e);
+  for (int e = 7; e >= 0; e--) {
+    const float d = __fsub_rn(x[e], mn), t = __fmaf_rn(d, r, kRound);
+    off = fmaxf(off, fabsf(__fmaf_rn(d, r, -__fsub_rn(t, kRound))));
+    word = (word << 4) + __float_as_uint(fminf(fmaxf(t, kRound), kRound + 15.0f));
   }
-  if (off > 0.4999f) {
+  word -= kBits + (kBits << 4) + (kBits << 8);
+  if (!(off <= 0.4999f)) {
     word = 0;
 #pragma unroll
     for (int e = 0; e < 8; e++) word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], mn), s)), 0.0f), 15.0f) << (4 * e);
   }
   return word;
+}
+// the smaller, the larger; NaN where one of them is
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float c;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
 }
 
 // per 32 dims: mn = f16(min), s = f16((max - mn) / 15) (0 -> 1), q = clamp(rhe((x - mn) / s), 0, 15), every step rounded
@@ -183,15 +197,13 @@ __global__ void __launch_bounds__(kT) kv4_put_kernel(RowsJob j) {
 #pragma unroll
     for (uint32_t i = 0; i < kGroups; i++) {
       if (g0 + i >= p.g1) break;
-      float lo = kHold, hi = -kHold;
-      bool fine = true;
+      float lo = x[i][0], hi = lo;
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        fine = fine && fabsf(x[i][e]) <= kHold;
-        lo = fminf(lo, x[i][e]);
-        hi = fmaxf(hi, x[i][e]);
+      for (int e = 1; e < 8; e++) {
+        lo = min_nan(lo, x[i][e]);
+        hi = max_nan(hi, x[i][e]);
       }
-      if (!fine) {   // held at +-60000, NaN as 0
+      if (!(lo >= -kHold && hi <= kHold)) {   // held at +-60000, NaN as 0
         lo = kHold;
         hi = -kHold;
 #pragma unroll
@@ -211,7 +223,7 @@ __global__ void __launch_bounds__(kT) kv4_put_kernel(RowsJob j) {
       const float mn = __half2float(mnh);
       __half sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, mn), 15.0f));
       if (__half2float(sh) == 0.0f) sh = __float2half_rn(1.0f);
-      const float s = __half2float(sh), inv = __fdiv_rn(1.0f, s);
+      const float s = __half2float(sh), inv = __frcp_rn(s);
       const uint32_t word = codes_of(x[i], mn, s, inv);
       if (rec) {
         uint8_t *to = rec + (g0 + i) * 1280u;

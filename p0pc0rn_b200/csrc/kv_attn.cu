@@ -150,39 +150,51 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
     }
     // the rows' positions and q fragments
     if (tid < (uint32_t)RB) rpos[tid] = tid < nrow ? (int32_t)(len - T + (r0 + tid) / hpg) : -1;
-    for (uint32_t e = tid; e < RT * (D / 16) * 32u; e += C::kThreads) {
-      const uint32_t ln = e & 31u, step = (e >> 5) % (D / 16), rt = (e >> 5) / (D / 16);
-      const uint32_t wi = step >> 1, l4 = ln & 3u;   // the lane's K word wi; its codes d0, +4, +1, +5
-      const uint32_t d0 = (D >= 128 ? ((wi >> 2) * 4u + l4) * 32u + (wi & 3u) * 8u : l4 * 16u + wi * 8u) + (step & 1u) * 2u;
-      float x[2][4];
+    {
+      constexpr uint32_t all = RT * (D / 16) * 32, E = (all + C::kThreads - 1) / C::kThreads, H = F32 ? 1 : 2;   // a thread's, all on their way before one is used
+      const bool wide = j.q.wide;
+      uint2 x[E][H][2];   // dims d0, + 1 and + 4, + 5 (f16: the low words)
 #pragma unroll
-      for (int half = 0; half < (F32 ? 1 : 2); half++) {
-        const uint32_t r = rt * RR + (ln >> 2) + 8u * half;
-        if (r < nrow) {
-          const uint64_t o = (uint64_t)(first + (r0 + r) / hpg) * j.q.ld + (uint64_t)(head * hpg + (r0 + r) % hpg) * j.q.ldh + d0;
-          if (F32) {
-            const float *q = reinterpret_cast<const float *>(j.q.base) + o;
-            x[half][0] = q[0]; x[half][1] = q[4]; x[half][2] = q[1]; x[half][3] = q[5];
-          } else {
-            const __half *q = reinterpret_cast<const __half *>(j.q.base) + o;
-            x[half][0] = __half2float(q[0]); x[half][1] = __half2float(q[4]); x[half][2] = __half2float(q[1]); x[half][3] = __half2float(q[5]);
+      for (uint32_t i = 0; i < E; i++) {
+        const uint32_t e = i * C::kThreads + tid, ln = e & 31u, step = (e >> 5) % (D / 16), rt = (e >> 5) / (D / 16);
+        const uint32_t wi = step >> 1, l4 = ln & 3u;   // the lane's K word wi; its codes d0, +4, +1, +5
+        const uint32_t d0 = (D >= 128 ? ((wi >> 2) * 4u + l4) * 32u + (wi & 3u) * 8u : l4 * 16u + wi * 8u) + (step & 1u) * 2u;
+#pragma unroll
+        for (uint32_t half = 0; half < H; half++) {
+          const uint32_t r = rt * RR + (ln >> 2) + 8u * half, tok = (r0 + r) / hpg;
+          x[i][half][0] = x[i][half][1] = make_uint2(0u, 0u);
+          if (r >= nrow || e >= all) continue;
+          const uint64_t o = (uint64_t)(first + tok) * j.q.ld + (uint64_t)(head * hpg + r0 + r - tok * hpg) * j.q.ldh + d0;
+#pragma unroll
+          for (uint32_t k = 0; k < 2; k++) {
+            if (F32) {
+              const uint32_t *q = reinterpret_cast<const uint32_t *>(j.q.base) + o + 4u * k;
+              x[i][half][k] = wide ? *reinterpret_cast<const uint2 *>(q) : make_uint2(q[0], q[1]);
+            } else {
+              const uint16_t *q = reinterpret_cast<const uint16_t *>(j.q.base) + o + 4u * k;
+              x[i][half][k].x = wide ? *reinterpret_cast<const uint32_t *>(q) : q[0] | ((uint32_t)q[1] << 16);
+            }
           }
-        } else {
-          x[half][0] = x[half][1] = x[half][2] = x[half][3] = 0.0f;
         }
       }
-      uint4 f;
-      f.x = pack2(x[0][0], x[0][1]);
-      f.z = pack2(x[0][2], x[0][3]);
-      if (F32) {   // rows + 8: what f16 leaves of the same rows
-        const float2 h0 = __half22float2(*reinterpret_cast<const __half2 *>(&f.x)), h1 = __half22float2(*reinterpret_cast<const __half2 *>(&f.z));
-        f.y = pack2(x[0][0] - h0.x, x[0][1] - h0.y);
-        f.w = pack2(x[0][2] - h1.x, x[0][3] - h1.y);
-      } else {
-        f.y = pack2(x[1][0], x[1][1]);
-        f.w = pack2(x[1][2], x[1][3]);
+#pragma unroll
+      for (uint32_t i = 0; i < E; i++) {
+        uint4 f;
+        if (F32) {   // rows + 8: what f16 leaves of the same rows
+          const float2 a = make_float2(__uint_as_float(x[i][0][0].x), __uint_as_float(x[i][0][1].x)), c = make_float2(__uint_as_float(x[i][0][0].y), __uint_as_float(x[i][0][1].y));
+          f.x = pack2(a.x, a.y);
+          f.z = pack2(c.x, c.y);
+          const float2 h0 = __half22float2(*reinterpret_cast<const __half2 *>(&f.x)), h1 = __half22float2(*reinterpret_cast<const __half2 *>(&f.z));
+          f.y = pack2(a.x - h0.x, a.y - h0.y);
+          f.w = pack2(c.x - h1.x, c.y - h1.y);
+        } else {
+          f.x = __byte_perm(x[i][0][0].x, x[i][0][1].x, 0x5410);
+          f.z = __byte_perm(x[i][0][0].x, x[i][0][1].x, 0x7632);
+          f.y = __byte_perm(x[i][H - 1][0].x, x[i][H - 1][1].x, 0x5410);
+          f.w = __byte_perm(x[i][H - 1][0].x, x[i][H - 1][1].x, 0x7632);
+        }
+        if (all % C::kThreads == 0 || i * C::kThreads + tid < all) qf[i * C::kThreads + tid] = f;
       }
-      qf[e] = f;
     }
     __syncthreads();
     // this warp's dims and keys in P V
@@ -488,7 +500,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnJob j) {
   dep_enter();
   constexpr int L = D / 4, K = 256 / L > 0 ? 256 / L : 1;   // lanes per row (4 dims each), parts at a time
   __shared__ float4 acc[K][L];
-  __shared__ float ms[256], sums[K];
+  __shared__ float sums[K];
   const uint4 u = j.desc[blockIdx.x];
   const uint32_t r = blockIdx.y;
   if (!u.x) return;
@@ -500,19 +512,16 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnJob j) {
   const auto part = [&](uint32_t i) {
     return j.part + ((uint64_t)(blockIdx.x + i) * 2u + (i ? 0u : 1u)) * RB * (D + 2) + (uint64_t)r * (D + 2);
   };
-  float M = -INFINITY;
-  for (uint32_t i = threadIdx.x; i < n; i += 256) M = fmaxf(M, part(i)[D]);
-  ms[threadIdx.x] = M;
-  __syncthreads();
-  for (int s = 128; s > 0; s >>= 1) {
-    if ((int)threadIdx.x < s) ms[threadIdx.x] = fmaxf(ms[threadIdx.x], ms[threadIdx.x + s]);
-    __syncthreads();
-  }
-  M = ms[0];
+  float M = -INFINITY;   // each warp for itself
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x & 31u; i < n; i += 32) M = fmaxf(M, part(i)[D]);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
   const float ref = M == -INFINITY ? 0.0f : M;
   const uint32_t k = threadIdx.x / L, e = threadIdx.x % L;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
+#pragma unroll 4
   for (uint32_t i = k; i < n; i += K) {
     const float *p = part(i);
     const float w = F32 ? expf(p[D] - ref) : exp2f(p[D] - ref);
