@@ -286,10 +286,13 @@ __global__ void __launch_bounds__(kT) kv4_get_kernel(RowsJob j) {
 // ---------------------------------------------------------------- kvStep / kvCompact: the plans
 // One cluster of kPC CTAs plans a call in phases with cluster barriers between them; the page copies follow in a second
 // kernel from the list that the plan leaves in the workspace. Counts are integer sums, so their order does not matter.
-// 64 sequences of 9000 tokens, 26 layers (16 MB of tails): 13.3 us; 8 small ones: 9.9 us, of which the barriers and two
+// 64 sequences of 9000 tokens, 26 layers (16 MB of tails): 13.3 us; 8 small ones: 6.3 us, of which two
 // launches are most. Compacting 160 MB of pages: 60.6 us, 51 of them the copies at the copy rate.
 constexpr uint32_t kPC = 8, kPT = 1024;
 constexpr uint32_t kNone = P0_KV_NONE;
+// One CTA plans a step, the counts in shared memory, where no thread has more than a few entries: 8 sequences of 3011 tokens, 200
+// pages: 6.3 us, by a cluster 9.2; 16 of 20000, 3000 pages: 10.4 and 10.2; 64 of 9000, 2300 pages: 15.4 and 13.6
+constexpr uint32_t kOnePages = 4096, kOneEntries = 4096;
 
 __device__ __forceinline__ uint32_t plan_tid() { return blockIdx.x * kPT + threadIdx.x; }
 
@@ -333,16 +336,24 @@ __device__ __forceinline__ bool page_dead(uint32_t j, uint32_t n, uint32_t windo
   return window && first + kPage - 1 + window <= n && first >= sinks;
 }
 
-__global__ void __cluster_dims__(kPC, 1, 1) __launch_bounds__(kPT) kv_step_plan(StepJob j) {
+// NC CTAs: one, which keeps the counts in shared memory, where the state is small, or a cluster
+template <uint32_t NC>
+__device__ __forceinline__ void step_plan(const StepJob &j) {
   dep_enter();
   // per row: the parent (kNone: an empty row), its length, the new length, and (first needed page rank << 1 | copies
   // its tail)
   extern __shared__ uint32_t sm[];
   const uint32_t R = j.v.rows, ld = j.v.ld, P = j.v.pages;
   uint32_t *par = sm, *lp = sm + R, *to = sm + 2 * R, *want = sm + 3 * R, *first = sm + 4 * R;
+  uint32_t *rc = NC == 1 ? sm + 5 * R : j.to_ref;   // the counts as they become
   __shared__ uint32_t red[32], too_long;
-  const uint32_t tid = plan_tid(), all = kPC * kPT;
-  for (uint32_t p = tid; p < P; p += all) j.to_ref[p] = j.ref[p];
+  const uint32_t tid = plan_tid(), all = NC * kPT;
+  const auto meet = [] {
+    if (NC == 1) __syncthreads();
+    else tc::cluster_sync();
+  };
+  const auto count = [&](uint32_t p) { return NC == 1 ? rc[p] : __ldcg(&rc[p]); };
+  for (uint32_t p = tid; p < P; p += all) rc[p] = j.ref[p];
   if (threadIdx.x == 0) too_long = 0u;
   for (uint32_t i = threadIdx.x; i < R; i += kPT) first[i] = kNone;
   __syncthreads();
@@ -369,12 +380,11 @@ __global__ void __cluster_dims__(kPC, 1, 1) __launch_bounds__(kPT) kv_step_plan(
     const uint32_t incl = cta_scan(w, red, total);
     if (i < R) want[i] = (incl - w) << 1 | copies;
   }
-  __syncthreads();
-  tc::cluster_sync();   // to_ref holds the old counts
+  meet();   // rc holds the old counts
   // the table without the new pages, and the counts that follow from it: an entry that a row keeps in place changes
   // nothing
   for (uint64_t e = tid; e < (uint64_t)R * ld; e += all) {
-    const uint32_t i = (uint32_t)(e / ld), p = (uint32_t)(e % ld);
+    const uint32_t i = (uint32_t)e / ld, p = (uint32_t)e - i * ld;
     const uint32_t n = kv_len(j.v, i);
     uint32_t a = p < (n + kPage - 1) / kPage ? j.v.table[e] : kNone, b = kNone;
     if (a >= P) a = kNone;
@@ -383,25 +393,28 @@ __global__ void __cluster_dims__(kPC, 1, 1) __launch_bounds__(kPT) kv_step_plan(
       if (b >= P || page_dead(p, lp[i], j.window, j.sinks) || ((want[i] & 1u) && p == lp[i] / kPage)) b = kNone;
     }
     if (a != b) {
-      if (a != kNone) atomicSub(&j.to_ref[a], 1u);
-      if (b != kNone) atomicAdd(&j.to_ref[b], 1u);
+      if (a != kNone) atomicSub(&rc[a], 1u);
+      if (b != kNone) atomicAdd(&rc[b], 1u);
     }
     j.to_table[e] = b;
   }
-  tc::cluster_sync();
+  meet();
   // free pages: each CTA counts its share, then gives out the lowest ones in the order of the rows' needs
-  const uint32_t per = (P + kPC - 1) / kPC, lo = min(P, blockIdx.x * per), hi = min(P, lo + per);
+  const uint32_t per = (P + NC - 1) / NC, lo = min(P, blockIdx.x * per), hi = min(P, lo + per);
   uint32_t mine = 0;
-  for (uint32_t p = lo + threadIdx.x; p < hi; p += kPT) mine += __ldcg(&j.to_ref[p]) == 0u;
+  for (uint32_t p = lo + threadIdx.x; p < hi; p += kPT) mine += count(p) == 0u;
   uint32_t share;
   cta_scan(mine, red, share);
-  if (threadIdx.x == 0) j.cnt[blockIdx.x] = share;
-  tc::cluster_sync();
-  uint32_t before = 0, left = 0;
-  for (uint32_t k = 0; k < kPC; k++) {
-    const uint32_t s = __ldcg(&j.cnt[k]);
-    if (k < blockIdx.x) before += s;
-    left += s;
+  uint32_t before = 0, left = share;
+  if (NC > 1) {
+    if (threadIdx.x == 0) j.cnt[blockIdx.x] = share;
+    meet();
+    left = 0;
+    for (uint32_t k = 0; k < NC; k++) {
+      const uint32_t s = __ldcg(&j.cnt[k]);
+      if (k < blockIdx.x) before += s;
+      left += s;
+    }
   }
   const bool ok = !too_long && total <= left;
   if (!ok) {   // all or nothing: the state as it was
@@ -433,7 +446,7 @@ __global__ void __cluster_dims__(kPC, 1, 1) __launch_bounds__(kPT) kv_step_plan(
   }
   for (uint32_t p0 = lo; p0 < hi && before < total; p0 += kPT) {
     const uint32_t p = p0 + threadIdx.x;
-    const bool fr = p < hi && __ldcg(&j.to_ref[p]) == 0u;
+    const bool fr = p < hi && count(p) == 0u;
     uint32_t here;
     const uint32_t k = before + cta_scan(fr ? 1u : 0u, red, here) - 1u;
     if (fr && k < total) {
@@ -450,11 +463,18 @@ __global__ void __cluster_dims__(kPC, 1, 1) __launch_bounds__(kPT) kv_step_plan(
         at += (lp[a] + kPage - 1) / kPage;
       }
       j.to_table[(uint64_t)a * ld + at] = p;
-      j.to_ref[p] = 1u;
+      rc[p] = 1u;
     }
     before += here;
   }
+  if (NC == 1) {
+    __syncthreads();
+    for (uint32_t p = tid; p < P; p += all) j.to_ref[p] = rc[p];
+  }
 }
+
+__global__ void __launch_bounds__(kPT) kv_step_plan_one(StepJob j) { step_plan<1>(j); }
+__global__ void __cluster_dims__(kPC, 1, 1) __launch_bounds__(kPT) kv_step_plan(StepJob j) { step_plan<kPC>(j); }
 
 struct CompactJob {
   KvView v;
@@ -620,7 +640,8 @@ p0_status p0_kv_step(p0_ctx *c, const p0_kv_step_args *a) {
   if ((st = p0_workspace(c, 0, 256 + R * sizeof(uint2), &cnt, &ws))) return st;
   j.cnt = (uint32_t *)ws;
   j.list = (uint2 *)((uint8_t *)ws + 256);
-  launch_dep(kv_step_plan, dim3(kPC), dim3(kPT), (size_t)R * 5 * 4, c->stream, j);
+  if (P <= kOnePages && E <= kOneEntries) launch_dep(kv_step_plan_one, dim3(1), dim3(kPT), (size_t)(R * 5 + P) * 4, c->stream, j);
+  else launch_dep(kv_step_plan, dim3(kPC), dim3(kPT), (size_t)R * 5 * 4, c->stream, j);
   if ((st = p0_launched(c, op))) return st;
   if (!parent) return P0_OK;   // without parents no row has a second child: there is nothing to copy
   const uint64_t runs = (j.v.stride / 16 + kCopyT * kCopyU - 1) / (kCopyT * kCopyU);
