@@ -192,6 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   // its last S is; ofree: this CTA's output of a unit has left q's place
   __shared__ __align__(8) uint64_t full[NS], empty[NS], sfull[2], sread[2], pfull[2], odone[2], qfull, qland, qdone, ofree, mdone[2];
   __shared__ uint32_t tmem_slot, abort_word;
+  __shared__ Unit units[kThreads / 32];
   __shared__ float mx2[2][2][kCR], l2[2][2][kCR];   // [tile, unit parity][half of the tile][row]
   volatile uint32_t *abort_flag = &abort_word;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = tc::cluster_rank(), run = blockIdx.x >> 1;
@@ -243,20 +244,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   const bool flip = j.scale < 0.0f;   // a negative scale turns S around, so that maxima stay maxima
   // A wait that gives up sets the CTA's abort word, after which all its waits give up at once; every warp still walks the
   // same units to the end. Nothing stops between units: the next one's K, q and first S run under this one's end
-  Unit u;
+  Unit &u = units[warp];   // in shared memory: what a tile does not need stays out of the registers
   for (uint32_t at = lo; at < hi;) {
-    if (at == lo || pre[b + 1] <= at) {
-      while (pre[b + 1] <= at) b++;
-      u = find_unit<kRB, kPP, kE>(j, pre, b, at);
-    } else {   // the next one of this sequence
-      u.begin += u.n;
-      if (++u.head == j.units) {
-        u.head = 0;
-        u.r0 += kRB;
-        u.n = unit_items<kRB, kPP, kE>(j, u.len, u.T, u.r0, u.s);
+    Span s;
+    {
+      Unit w;
+      if (at == lo || pre[b + 1] <= at) {
+        while (pre[b + 1] <= at) b++;
+        w = find_unit<kRB, kPP, kE>(j, pre, b, at);
+      } else {   // the next one of this sequence
+        w = u;
+        w.begin += w.n;
+        if (++w.head == j.units) {
+          w.head = 0;
+          w.r0 += kRB;
+          w.n = unit_items<kRB, kPP, kE>(j, w.len, w.T, w.r0, w.s);
+        }
       }
+      s = w.s;
+      __syncwarp();
+      if (lane == 0) u = w;
+      __syncwarp();
     }
-    const Span &s = u.s;
     const uint32_t from = max(at - u.begin, kE) - kE, nt = u.n - kE, end = min(hi - u.begin, u.n), to = max(end, kE) - kE;
     at = u.begin + end;
     if (from == to) continue;   // this run holds none of the unit's tiles
@@ -436,7 +445,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
           tc::fence_after();
           tc::tmem_ld32(sc + 64u * h, x[0]);
           tc::tmem_ld32(sc + 64u * h + 32u, x[1]);
+          // meanwhile: P of tile t - 2 has been used (before that it lies in a unit whose end was waited for)
+          if (i > 1 && !tc::mbar_wait(&odone[t & 1u], ((t >> 1) - 1u) & 1u, abort_flag, j.err, 0x4bbu, P0_SPIN_LIMIT)) ok = false;
           tc::tmem_wait_ld();
+          tc::fence_after();
           tc::fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive_peer(&sread[t % C::kSB], 0);   // the even CTA's MMAs wait for both
@@ -468,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
         }
         mx2[t & 1u][h][r] = mx;
         asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
-        if (!ok) continue;
+        if (!(ok = __all_sync(0xffffffffu, ok))) continue;
         mx = fmaxf(mx, mx2[t & 1u][h ^ 1u][r]);
         // O follows a maximum that has grown by more than 2^8 (or that is a row's first)
         const bool grow = mx > m + 8.0f;
@@ -489,11 +501,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
               tmem_st32(tmem + lanes + d, o);
             }
           }
-        }
-        if (i > 1) {   // P of tile t - 2 has been used (before that it lies in a unit whose end was waited for)
-          ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(&odone[t & 1u], ((t >> 1) - 1u) & 1u, abort_flag, j.err, 0x4bbu, P0_SPIN_LIMIT));
-          if (!ok) continue;
-          tc::fence_after();
         }
         const float ref = m == -INFINITY ? 0.0f : m;
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
