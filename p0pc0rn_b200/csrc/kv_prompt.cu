@@ -226,6 +226,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
   tc::fence_before();
   tc::cluster_sync();
   tc::fence_after();
+  // This kernel starts when every CTA of the widening one has passed its own wait, so all that came before that one is done: lengths,
+  // tables, q and the workspace are read and written while it still runs. Only the widened pages are waited for, by the warp that
+  // copies them; every CTA has that warp, so this kernel does not end before the other
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 8) asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t tmem = tmem_slot;

@@ -130,6 +130,26 @@ def test_prompt(g, lens, counts, nh, nkv, D, window, sinks, scale):
     check(got, c, q, counts, nh, "f16", window, sinks, float(np.float32(scale or 1.0)), ref=R.attention_prompt)
 
 
+@pytest.mark.parametrize("D,nh,nkv,lay,out_lay,scale", [
+    (64, 8, 1, (8 * 72 + 8, 72, 16), (8 * 72, 72, 8), 0.4),          # rows apart, 16 bytes at a time
+    (128, 6, 2, (6 * 136, 136, 8), (0, 0, 0), -0.3),                 # three heads a group: no box of 128 rows
+    (256, 4, 2, (4 * 257 + 3, 257, 5), (4 * 259 + 1, 259, 3), -0.2), # odd offsets and strides, a negative scale
+    (512, 4, 1, (4 * 513, 513, 1), (0, 0, 2), 0.0),
+    (64, 256, 1, (0, 0, 0), (0, 0, 0), 0.0),                         # more heads a group than a block has rows
+    (128, 2, 2, (128, 128 * 330, 0), (128, 128 * 330, 0), 0.0),      # head-major rows
+])
+def test_prompt_strides(g, D, nh, nkv, lay, out_lay, scale):
+    rng = np.random.default_rng(17 + D)
+    lens, counts = ([700, 300, 80], [200, 30, 100]) if nh < 256 else ([300, 70], [5, 2])
+    c = R.Cache(rng, lens, nkv, D)
+    c.fill_fast(rng)
+    q = (rng.standard_normal((sum(counts), nh, D)) * (3.0 / D ** 0.5)).astype(np.float16)
+    got = run(g, c, q, counts, nh, "f16", 90, 3, scale, lay=lay, out_lay=out_lay)
+    check(got, c, q, counts, nh, "f16", 90, 3, float(np.float32(scale or 1.0)), ref=R.attention_prompt)
+    again = run(g, c, q, counts, nh, "f16", 90, 3, scale, lay=lay, out_lay=out_lay)
+    assert np.array_equal(again.view(np.uint16), got.view(np.uint16))
+
+
 @pytest.mark.parametrize("D", [64, 256])
 @pytest.mark.parametrize("T", [1, 400])
 def test_attn_growing_scores(g, D, T):
