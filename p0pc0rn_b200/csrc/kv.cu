@@ -81,22 +81,22 @@ struct RowsJob {
   uint8_t *rec;         // the pool again, writable for kv4Put
   KvRows k, vv;
   uint32_t runs;        // of groups: warps per 8 tokens, head and K or V
-  uint64_t warps;       // of the whole call
+  uint32_t warps;       // of the whole call
 };
 
 struct Place { uint32_t g0, g1, vsel, head, tok, word; bool in; };
-__device__ __forceinline__ Place place_of(const RowsJob &j, uint64_t w) {
+__device__ __forceinline__ Place place_of(const RowsJob &j, uint32_t w) {
   const uint32_t lane = threadIdx.x & 31u, G = j.v.D / 32u;
   Place p;
-  const uint32_t run = (uint32_t)(w % j.runs);
+  const uint32_t run = w % j.runs;
   p.g0 = G * run / j.runs;
   p.g1 = G * (run + 1) / j.runs;
   w /= j.runs;
-  p.vsel = (uint32_t)(w & 1u);
+  p.vsel = w & 1u;
   w >>= 1;
-  p.head = (uint32_t)(w % j.v.nkv);
+  p.head = w % j.v.nkv;
   w /= j.v.nkv;
-  p.tok = (uint32_t)w * 8u + (lane >> 2);
+  p.tok = w * 8u + (lane >> 2);
   p.word = lane & 3u;
   p.in = p.tok < j.v.n;
   return p;
@@ -181,7 +181,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 template <bool F16, bool WIDE>
 __global__ void __launch_bounds__(kT) kv4_put_kernel(RowsJob j) {
   dep_enter();
-  const uint64_t w = ((uint64_t)blockIdx.x * kT + threadIdx.x) / 32u;
+  const uint32_t w = blockIdx.x * (kT / 32) + threadIdx.x / 32u;
   if (w >= j.warps) return;
   const Place p = place_of(j, w);
   const KvRows &r = p.vsel ? j.vv : j.k;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kT) kv4_put_kernel(RowsJob j) {
 template <bool F16, bool WIDE>
 __global__ void __launch_bounds__(kT) kv4_get_kernel(RowsJob j) {
   dep_enter();
-  const uint64_t w = ((uint64_t)blockIdx.x * kT + threadIdx.x) / 32u;
+  const uint32_t w = blockIdx.x * (kT / 32) + threadIdx.x / 32u;
   if (w >= j.warps) return;
   const Place p = place_of(j, w);
   if (!p.in) return;
@@ -576,9 +576,9 @@ p0_status rows_call(p0_ctx *c, const p0_kv4_rows_args *a, bool put) {
   // a warp takes four groups; where there are few tokens, one
   const uint64_t eights = (uint64_t)((a->n + 7) / 8) * a->kv.nkv * 2, G = a->kv.D / 32;
   j.runs = (uint32_t)(eights < 8u * (uint32_t)c->sm_count ? G : (G + kGroups - 1) / kGroups);
-  j.warps = eights * j.runs;
-  const uint64_t grid = (j.warps + kT / 32 - 1) / (kT / 32);
-  if (grid > 0x7fffffffu) return p0_fail(c, P0_EINVAL, "%s: %u tokens in one call", op, a->n);
+  const uint64_t warps = eights * j.runs, grid = (warps + kT / 32 - 1) / (kT / 32);
+  j.warps = (uint32_t)warps;
+  if (warps > 0xffffff00u) return p0_fail(c, P0_EINVAL, "%s: %u tokens in one call", op, a->n);
   const bool f16 = a->type == P0_F16, wide = j.k.wide && j.vv.wide;
   cudaSetDevice(c->device);
   auto go = [&](auto kern) { launch_dep(kern, dim3((unsigned)grid), dim3(kT), 0, c->stream, j); };
