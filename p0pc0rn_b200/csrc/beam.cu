@@ -3,15 +3,15 @@
 //   lse_b = log sum_v exp(x[b, v]),  c[b, v] = score[b] + (x[b, v] - lse_b),  the k largest c, ties to the lowest b * V + v
 // One pass over the logits (they are the only traffic that counts: 4 bytes per candidate). A CTA takes a part of a row, 4096
 // logits (a chunk) at a time in registers, and keeps per thread the running (max, sum exp), per thread and chunk the maximum
-// in shared memory: five instructions a logit. The (k + 1)-th largest of the threads' maxima is a bound that k + 1 logits
+// in shared memory: six instructions a logit. The (k + 1)-th largest of the threads' maxima is a bound that k + 1 logits
 // reach; the few (thread, chunk) pairs whose maximum reaches it are read again (out of L2), and what reaches it is ranked.
 // Where equal logits make the list too long, the CTA goes over its part again with keys that order equal values too.
 // A second kernel merges: lse per row, then the group's k best among the kept ones. Within a row c does not decrease as x
 // grows, so every candidate above the k-th best c has been kept; candidates that round to the very same c as the k-th best
 // may not have been, and where that can be (a part's last kept one ties with it) the merge looks the row's logits up again
 // in index order.
-// 128 rows of 262144 logits, 8 beams: 33.8 us, 4.0 TB/s; the scan's instructions and the merge's launch stand before the
-// bytes. 4 rows of 4099: 8.7 us, two launches.
+// 128 rows of 262144 logits, 8 beams: 32.4 us, 4.1 TB/s; the scan's instructions (half the issue slots), each part's ranking and
+// the merge's launch stand before the bytes. 4 rows of 4099: 8.7 us, two launches.
 #include "internal.h"
 #include "launch.cuh"
 
@@ -85,7 +85,14 @@ struct BeamJob {
 // a thread's logits of a chunk; -inf beyond V
 template <bool WIDE>
 __device__ __forceinline__ void load_chunk(const float *x, uint32_t base, uint32_t V, float (&v)[kPer]) {
-  if (WIDE) {
+  if (WIDE && base + kChunk <= V) {   // a whole chunk: no looks at V
+    const float4 *p = reinterpret_cast<const float4 *>(x + base) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kPer / 4; i++) {
+      const float4 f = __ldcs(p + i * kT);
+      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    }
+  } else if (WIDE) {
 #pragma unroll
     for (int i = 0; i < kPer / 4; i++) {
       const uint32_t at = base + (i * kT + threadIdx.x) * 4u;
@@ -146,6 +153,7 @@ __global__ void __launch_bounds__(kT, 4) beam_scan_kernel(BeamJob j) {
   // m: the thread's maximum so far, s: its sum of exp(x - m). A NaN or +inf makes s, its row's lse and every c NaN
   float m = -INFINITY, s = 0.0f, v[kPer], next[kPer];
   load_chunk<WIDE>(x, c0 * kChunk, j.V, next);
+#pragma unroll 2   // the two buffers change places without moves
   for (uint32_t ch = c0; ch < c1; ch++) {
 #pragma unroll
     for (int i = 0; i < kPer; i++) v[i] = next[i];

@@ -71,8 +71,9 @@ constexpr int kT = 256;
 // ---------------------------------------------------------------- kv4Put / kv4Get
 // A warp takes 8 consecutive tokens of one head's K or V and a run of its groups of 32 dims (a lane: one token's code word, 8
 // dims), so that it finds the tokens' places once, reads or writes whole runs of 32 values and, where the tokens are
-// neighbours in a page, 128 contiguous bytes of codes. 8192 tokens of 2 heads of 256, f32: 20.4 us, 2.7 TB/s, bound by the
-// latency of the places and the divisions' instructions; 8 tokens: 5.3 us, the launch.
+// neighbours in a page, 128 contiguous bytes of codes. 8192 tokens of 2 heads of 256, f32: 19.0 us, 2.9 TB/s, bound by
+// each warp's chain of instructions (f16, half the bytes, takes as long): places, extent, rounded division, codes. 8 tokens: 5.1 us,
+// the launch.
 constexpr float kHold = 60000.0f;   // 15 * f16(range / 15) + f16(-60000) stays finite in f16
 constexpr uint32_t kGroups = 4;     // groups whose values a lane holds at a time
 
@@ -286,8 +287,8 @@ __global__ void __launch_bounds__(kT) kv4_get_kernel(RowsJob j) {
 // ---------------------------------------------------------------- kvStep / kvCompact: the plans
 // One cluster of kPC CTAs plans a call in phases with cluster barriers between them; the page copies follow in a second
 // kernel from the list that the plan leaves in the workspace. Counts are integer sums, so their order does not matter.
-// 64 sequences of 9000 tokens, 26 layers (16 MB of tails): 13.3 us; 8 small ones: 6.3 us, of which two
-// launches are most. Compacting 160 MB of pages: 60.6 us, 51 of them the copies at the copy rate.
+// 64 sequences of 9000 tokens, 26 layers (16 MB of tails): 12.9 us; 8 small ones: 6.2 us, of which two
+// launches are most. Compacting 160 MB of pages: 59 us, 51 of them the copies at the copy rate.
 constexpr uint32_t kPC = 8, kPT = 1024;
 constexpr uint32_t kNone = P0_KV_NONE;
 // One CTA plans a step, the counts in shared memory, where no thread has more than a few entries: 8 sequences of 3011 tokens, 200

