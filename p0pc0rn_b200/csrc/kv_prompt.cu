@@ -34,6 +34,7 @@
 
 namespace {
 
+constexpr uint32_t kDrain = 1u << 16;                // polls for what is in flight when a wait has given up: copies and MMAs end in microseconds
 constexpr uint32_t kRB = 256, kCR = 128, kPP = 2;   // query rows of a block and of a CTA, pages of a key tile
 constexpr uint32_t kE = 4;                   // a unit's beginning and end cost about as much as four key tiles
 constexpr int kSoft = 256, kThreads = kSoft + 128;   // warps 0-7: softmax (0-3 the tile's first page, 4-7 its second); 8: copies; 9: S; 10: P V; 11: q
@@ -596,12 +597,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
       for (uint32_t i = 0; i < (uint32_t)NS; i++) {
         const Ring &g = i < SK ? rk : rv;
         const uint32_t n = i < SK ? i : i - SK;
-        if (g.round || n < g.i) tc::mbar_wait(&full[i], (n < g.i ? g.round : g.round - 1u) & 1u, &never, j.err, 0x4b2u, P0_SPIN_LIMIT);
+        never = 0;   // each one is waited for
+        if (g.round || n < g.i) tc::mbar_wait(&full[i], (n < g.i ? g.round : g.round - 1u) & 1u, &never, j.err, 0x4b2u, kDrain);
       }
-    if (warp == 11 && j.qbox && unit) tc::mbar_wait(rank ? &qland : &qfull, (unit - 1u) & 1u, &never, j.err, 0x4b2u, P0_SPIN_LIMIT);
+    if (warp == 11 && j.qbox && unit) tc::mbar_wait(rank ? &qland : &qfull, (unit - 1u) & 1u, &never, j.err, 0x4b2u, kDrain);
     if ((warp == 9 || warp == 10) && rank == 0) {
       tc::mma_commit_pair(&mdone[warp - 9]);
-      tc::mbar_wait(&mdone[warp - 9], 0, &never, j.err, 0x4b5u, P0_SPIN_LIMIT);
+      tc::mbar_wait(&mdone[warp - 9], 0, &never, j.err, 0x4b5u, kDrain);
     }
   }
   __syncwarp();
