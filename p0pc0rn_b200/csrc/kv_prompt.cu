@@ -584,6 +584,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
         }
       }
       tc::fence_before();   // O is read before the next unit's MMAs write it: they wait for this warp's next P
+      if (!C::kStg) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the output stood in q's place: before q's next copy
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&ofree);
     }

@@ -150,6 +150,19 @@ def test_prompt_strides(g, D, nh, nkv, lay, out_lay, scale):
     assert np.array_equal(again.view(np.uint16), got.view(np.uint16))
 
 
+def test_prompt_units_in_a_row_d512(g):
+    # several whole units after one another in every run, where the output of one stands in the place of the next one's q
+    rng = np.random.default_rng(31)
+    lens, counts, nh = [300, 270, 256, 290] * 3, [256, 200, 256, 100] * 3, 16
+    c = R.Cache(rng, lens, nh, 512)
+    c.fill_fast(rng)
+    q = (rng.standard_normal((sum(counts), nh, 512)) * (3.0 / 512 ** 0.5)).astype(np.float16)
+    got = run(g, c, q, counts, nh, "f16")
+    check(got, c, q, counts, nh, "f16", ref=R.attention_prompt)
+    for _ in range(20):
+        assert np.array_equal(run(g, c, q, counts, nh, "f16").view(np.uint16), got.view(np.uint16))
+
+
 @pytest.mark.parametrize("D", [64, 256])
 @pytest.mark.parametrize("T", [1, 400])
 def test_attn_growing_scores(g, D, T):
