@@ -316,7 +316,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
       // ------------------------------------------------------------ the pair's MMAs (even CTA), word of what landed (odd CTA): S by one
       // warp, P V by another. What a thread issues after a wait comes a few hundred cycles late; with a thread each, S and P V hide that
       // for one another. The waits that are over come first
-      const auto landed = [&](uint32_t i, uint32_t round) { return tc::mbar_wait(&full[i], round & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT); };
+      const auto landed = [&](uint32_t i, uint32_t round) {   // the even CTA's barriers are completed by the odd one, too: acquire over the pair
+        return rank ? tc::mbar_wait(&full[i], round & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT)
+                    : tc::mbar_wait_cluster(&full[i], round & 1u, abort_flag, j.err, 0x4b3u, P0_SPIN_LIMIT);
+      };
       const auto part_of = [](uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); };   // within shared memory: no carry out of the address
       if (lane == 0 && rank == 1) {
         Ring &g = warp == 9 ? rk : rv;

@@ -163,6 +163,20 @@ def test_prompt_units_in_a_row_d512(g):
         assert np.array_equal(run(g, c, q, counts, nh, "f16").view(np.uint16), got.view(np.uint16))
 
 
+@pytest.mark.parametrize("D,nh,nkv", [(64, 16, 8), (128, 16, 4), (256, 8, 4)])
+def test_prompt_same_bits(g, D, nh, nkv):
+    # many tiles and units a run: what either CTA of a pair copied is there when the pair's products read it, each time
+    rng = np.random.default_rng(32 + D)
+    lens, counts = [1100, 700, 900, 1000], [300, 520, 410, 256]
+    c = R.Cache(rng, lens, nkv, D)
+    c.fill_fast(rng)
+    q = (rng.standard_normal((sum(counts), nh, D)) * (3.0 / D ** 0.5)).astype(np.float16)
+    got = run(g, c, q, counts, nh, "f16")
+    check(got, c, q, counts, nh, "f16", ref=R.attention_prompt)
+    for _ in range(20):
+        assert np.array_equal(run(g, c, q, counts, nh, "f16").view(np.uint16), got.view(np.uint16))
+
+
 @pytest.mark.parametrize("D", [64, 256])
 @pytest.mark.parametrize("T", [1, 400])
 def test_attn_growing_scores(g, D, T):
