@@ -22,6 +22,7 @@ p0_status kv_view(p0_ctx *c, const p0_kv &kv, bool layer, const char *op, KvView
   if (!stride) return p0_fail(c, P0_EINVAL, "%s: the page stride is missing", op);
   if (stride < need) return p0_fail(c, P0_EINVAL, "%s: page stride %llu below the layer's %llu bytes", op, (unsigned long long)stride, (unsigned long long)need);
   if (stride > (1ull << 40)) return p0_fail(c, P0_EINVAL, "%s: page stride %llu", op, (unsigned long long)stride);
+  if (kv.pages - 1 > (~0ull - need) / stride) return p0_fail(c, P0_EINVAL, "%s: %u pages of %llu bytes pass 64 bits", op, kv.pages, (unsigned long long)stride);
   P0Range rp, rt, rl;
   p0_status st;
   if ((st = p0_range(c, kv.pool, kv.pool_off, (uint64_t)(kv.pages - 1) * stride + need, op, "pool", &rp))) return st;

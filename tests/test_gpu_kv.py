@@ -280,3 +280,19 @@ def test_refusals(g):
     with pytest.raises(p0.P0Error, match="must not lie over"):
         p0.kvCompact(g, {"kv": kv, "ref": {"buf": ref}, "to": {"table": to["table"], "ref": {"buf": ref}}, "stat": {"buf": stat}})
     g.done()
+
+
+def test_refuses_pools_beyond_64_bits(g):
+    # (pages - 1) * stride wraps to 0 here: the pool would seem to fit its buffer
+    rng = np.random.default_rng(7)
+    c = R.Cache(rng, [100], 1, 64)
+    bufs, kv = kv_args(g, c)
+    huge = {**kv, "pages": (1 << 24) + 1, "pool": {"buf": bufs["pool"], "stride": 1 << 40}}
+    x = g.buffer(64 * 4)
+    with pytest.raises(p0.P0Error, match="pass 64 bits"):
+        p0.kv4Put(g, {"kv": huge, "k": {"buf": x}, "v": {"buf": x}, "type": "f32", "n": 1, "T": 1})
+    with pytest.raises(p0.P0Error, match="pass 64 bits"):
+        p0.kv4Attn(g, {"kv": huge, "q": {"buf": x}, "out": {"buf": x}, "type": "f32", "nh": 1, "n": 1, "T": 1})
+    with pytest.raises(p0.P0Error, match="pool range"):              # the largest that does not wrap is still beyond the buffer
+        p0.kv4Put(g, {"kv": {**huge, "pages": 1 << 24}, "k": {"buf": x}, "v": {"buf": x}, "type": "f32", "n": 1, "T": 1})
+    g.done()
