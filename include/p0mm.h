@@ -361,7 +361,8 @@ p0_status p0_kv4_get(p0_ctx *ctx, const p0_kv4_rows_args *a);
 /* kv4Attn: attention of the n newest tokens (laid out over the sequences as for kv4Put) with nh query heads, query head
  * h reading KV head h / (nh / nkv): out = softmax over the visible keys of scale * (q . k), times v. The token at
  * position p sees key j <= p if window is 0, j > p - window or j < sinks. A token that sees nothing gives zeros. What
- * the memory of unseen keys holds does not matter. scale 0 = 1. type P0_F32: q, out f32, computed to about 2^-22;
+ * the memory of unseen keys holds does not matter. Tokens of no sequence keep what out held; a cu (it should not decrease)
+ * that gives the sequences more than n tokens between them computes nothing. scale 0 = 1. type P0_F32: q, out f32, computed to about 2^-22;
  * P0_F16: q, out f16, P rounded to f16. */
 typedef struct {
   p0_kv kv;

@@ -17,7 +17,7 @@ struct KvView {
 };
 
 // the tokens [lo, lo + count) of the call that belong to sequence b. A cu that decreases or passes n gives no tokens
-// out of range.
+// out of range (it may give a token to several sequences: claims_fit).
 __device__ __forceinline__ uint32_t kv_tokens(const KvView &v, uint32_t b, uint32_t &lo) {
   uint32_t hi;
   if (v.cu) {

@@ -51,6 +51,21 @@ __device__ __forceinline__ void warp_sums(uint32_t *v, uint32_t n) {
   }
 }
 
+// Sequences that claim more than the call's n tokens between them (a cu that goes up and down) claim some twice. The host
+// counts work for n tokens, so such a call has none. A whole warp
+__device__ __forceinline__ bool claims_fit(const KvView &view) {
+  if (!view.cu) return true;
+  uint64_t claimed = 0;
+#pragma unroll 1
+  for (uint32_t b = threadIdx.x & 31u; b < view.rows; b += 32) {
+    uint32_t lo;
+    claimed += kv_tokens(view, b, lo);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) claimed += __shfl_xor_sync(0xffffffffu, claimed, o);
+  return claimed <= view.n;
+}
+
 // Work. The query rows that share a KV head (new tokens x query heads of its group) form blocks of RB; a unit is one row
 // block of one sequence and KV head (or part of its output), its items are the runs of PP pages that any of its rows sees (one item where there are
 // none: zeros are to be written), after E items that stand for what beginning and ending a unit costs. pre[b] = items
@@ -86,7 +101,11 @@ __device__ __forceinline__ void plan_items(const AttnJob &j, uint32_t *pre) {
   }
   if (threadIdx.x == 0) pre[0] = 0u;
   __syncthreads();
-  if (threadIdx.x < 32) warp_sums(pre + 1, R);
+  if (threadIdx.x < 32) {
+    if (claims_fit(j.v)) warp_sums(pre + 1, R);
+    else
+      for (uint32_t b = threadIdx.x; b < R; b += 32) pre[b + 1] = 0u;
+  }
   __syncthreads();
 }
 // the last b with pre[b] <= at (a sequence with items of its own, or one before it)

@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kET) kv4_widen_kernel(AttnJob j) {
   dep_enter();
   extern __shared__ uint32_t exo[];
   plan_pages(j, exo);
-  const uint32_t total = exo[j.v.rows], nkv = j.v.nkv;
+  const uint32_t total = claims_fit(j.v) ? exo[j.v.rows] : 0u, nkv = j.v.nkv;
   constexpr uint32_t part = D / 32 * 1280;
   uint32_t b = 0;
   for (uint64_t w2 = blockIdx.x; w2 < (uint64_t)total * nkv * 2u; w2 += gridDim.x) {   // K, or V, of a page and head

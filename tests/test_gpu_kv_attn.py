@@ -297,6 +297,26 @@ def test_attn_cu_out_of_order(g):
     check(got[2:], c2, q[2:], [8], 2, "f32")                         # sequence 1 has tokens 2 .. 9, the others none
 
 
+@pytest.mark.parametrize("type_,R_,n", [("f32", 1024, 40), ("f16", 1024, 40), ("f16", 200, 13000)])
+def test_attn_cu_up_and_down(g, type_, R_, n):
+    # 0, n, 0, n, ...: half of the sequences claim every token. More than the call has: nothing is computed (few rows, and prompts)
+    rng = np.random.default_rng(33)
+    c = R.Cache(rng, [70], 1, 64)
+    c.fill_fast(rng)
+    c.table, c.lens = np.repeat(c.table, R_, 0), np.full(R_, 70, np.uint32)
+    _, kv = kv_args(g, c)
+    dt = np.float32 if type_ == "f32" else np.float16
+    q, o = g.upload(np.ones(n * 64, dt)), g.upload(np.full(n * 64, -77, dt))
+    cu = np.tile(np.array([0, n], np.uint32), R_)[:R_ + 1]
+    p0.kv4Attn(g, {"kv": kv, "q": {"buf": q}, "out": {"buf": o}, "type": type_, "nh": 1, "n": n, "cu": {"buf": g.upload(cu)}})
+    g.done()
+    assert np.all(g.read(o, 0, n * 64 * dt().itemsize, dt) == -77)
+    cu = np.minimum(np.arange(R_ + 1) * (n // R_ + 1), n).astype(np.uint32)
+    p0.kv4Attn(g, {"kv": kv, "q": {"buf": q}, "out": {"buf": o}, "type": type_, "nh": 1, "n": n, "cu": {"buf": g.upload(cu)}})
+    g.done()
+    assert not np.any(g.read(o, 0, n * 64 * dt().itemsize, dt) == -77)   # every token of a sequence is written
+
+
 def test_attn_refusals(g):
     rng = np.random.default_rng(14)
     c = R.Cache(rng, [100, 70], 2, 64)
