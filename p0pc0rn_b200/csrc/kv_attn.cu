@@ -23,7 +23,8 @@
 // launches and their latencies: 8 contexts in a window of 512, 11.3 us. 4 x 8 tokens, 8190 keys, 8 f32 heads on 2 of 512: 54 us.
 //
 // Precision. f32 queries and outputs: q and P are split into f16 high and low parts (about 22 bits) in rows r and r + 8
-// of the fragments; each item's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
+// of the fragments; a row of q is brought to [2^14, 2^15) by a power of two first, which its scores give back, so that
+// neither part leaves f16's range for any f32 q; each item's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
 // f16 matrix operand), 16 rows per fragment.
 #include "kv_attn.cuh"
 
@@ -58,6 +59,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 __device__ __forceinline__ uint32_t lds_u32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
+
+// The power of two that brings a row whose largest |q| has these bits to [2^14, 2^15), and its inverse; rows below 2^-112
+// as if they reached it, so that both are normal numbers
+__device__ __forceinline__ float row_up(uint32_t bits) { return __uint_as_float((268u - max(bits >> 23, 15u)) << 23); }
+__device__ __forceinline__ float row_down(uint32_t bits) { return __uint_as_float((max(bits >> 23, 15u) - 14u) << 23); }
 
 constexpr uint32_t kRec = 1312;   // a K record's place in shared memory
 
@@ -95,6 +101,7 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
   __shared__ uint32_t abort_flag, page_ok[NS][KP];
   __shared__ __align__(16) float wmax[RB][NW], wsum[RB][NW];
   __shared__ int32_t rpos[RB];
+  __shared__ uint32_t qmax[RB];   // f32: the largest |q| of a row, as bits
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g4 = lane >> 2, t4 = lane & 3u;
   const uint32_t hpg = j.hpg, R = j.v.rows, W = j.window, S = j.sinks;
   if (tid == 0) {
@@ -102,13 +109,14 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
     abort_flag = 0u;
     tc::fence_mbar_init();
   }
+  if (F32 && tid < (uint32_t)RB) qmax[tid] = 0u;
   plan_items<RB, KP, 0>(j, pre);
   const uint32_t total = pre[R], G = min(gridDim.x, max(total, 1u));   // no run is empty
   if (tid == 0) j.desc[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
   if (blockIdx.x >= G) return;
   const uint32_t lo = (uint32_t)((uint64_t)total * blockIdx.x / G), hi = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / G);
   uint32_t b = find_sequence(pre, R, lo);
-  const float scale = F32 ? j.scale : j.scale * 1.44269504088896340736f;   // f16: scores and maxima in powers of two
+  const float log2_scale = j.scale * 1.44269504088896340736f;   // f16: scores and maxima in powers of two
   const auto ex = [](float x) { return exp2_fast(F32 ? x * 1.44269504088896340736f : x); };
   uint32_t at = lo, it = 0;   // item; items through the ring so far
   while (at < hi) {
@@ -177,11 +185,26 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
           }
         }
       }
+      if (F32) {   // a thread's rows are g4 of its fragments
+#pragma unroll
+        for (uint32_t i = 0; i < E; i++) {
+          float mx = 0.0f;   // of the numbers
+#pragma unroll
+          for (uint32_t k = 0; k < 2; k++) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[i][0][k].x)), fabsf(__uint_as_float(x[i][0][k].y))));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const uint32_t rt = (i * C::kThreads + tid) / (32u * (D / 16));
+          if (t4 == 0 && rt < (uint32_t)RT) atomicMax(&qmax[rt * RR + g4], __float_as_uint(mx));
+        }
+        __syncthreads();
+      }
 #pragma unroll
       for (uint32_t i = 0; i < E; i++) {
         uint4 f;
         if (F32) {   // rows + 8: what f16 leaves of the same rows
-          const float2 a = make_float2(__uint_as_float(x[i][0][0].x), __uint_as_float(x[i][0][1].x)), c = make_float2(__uint_as_float(x[i][0][0].y), __uint_as_float(x[i][0][1].y));
+          const uint32_t rt = min((i * C::kThreads + tid) / (32u * (D / 16)), (uint32_t)RT - 1u);
+          const float up = row_up(qmax[rt * RR + g4]);
+          const float2 a = make_float2(__uint_as_float(x[i][0][0].x) * up, __uint_as_float(x[i][0][1].x) * up), c = make_float2(__uint_as_float(x[i][0][0].y) * up, __uint_as_float(x[i][0][1].y) * up);
           f.x = pack2(a.x, a.y);
           f.z = pack2(c.x, c.y);
           const float2 h0 = __half22float2(*reinterpret_cast<const __half2 *>(&f.x)), h1 = __half22float2(*reinterpret_cast<const __half2 *>(&f.z));
@@ -206,8 +229,10 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
     constexpr int RH = F32 ? 1 : 2;   // rows of a lane per fragment: g4 (and g4 + 8)
     float o[RT][NPL][4], m[RT][RH], l[RT][RH];
     int32_t pos[RT][RH];
+    float scale[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
+      scale[rt] = F32 ? j.scale * row_down(qmax[rt * RR + g4]) : log2_scale;
 #pragma unroll
       for (int i = 0; i < NPL; i++)
 #pragma unroll
@@ -289,7 +314,7 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
 #pragma unroll
           for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) x[rt][nt][h][e] = (F32 ? sc[rt][nt][e] + sc[rt][nt][e + 2] : sc[rt][nt][2 * h + e]) * scale;
+            for (int e = 0; e < 2; e++) x[rt][nt][h][e] = (F32 ? sc[rt][nt][e] + sc[rt][nt][e + 2] : sc[rt][nt][2 * h + e]) * scale[rt];
           if (!plain) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -421,6 +446,7 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
         if (t4 == 0) wsum[rt * RR + g4 + 8 * h][warp] = t;
       }
     __syncthreads();
+    if (F32 && tid < (uint32_t)RB) qmax[tid] = 0u;   // every thread has its rows' scales; before the next unit's barriers
     // ---- the key shares of O meet in the first one, through the ring (no copy is in flight)
 #pragma unroll 1
     for (int k = 1; k < C::kKs; k++) {

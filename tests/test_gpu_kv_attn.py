@@ -297,6 +297,46 @@ def test_attn_cu_out_of_order(g):
     check(got[2:], c2, q[2:], [8], 2, "f32")                         # sequence 1 has tokens 2 .. 9, the others none
 
 
+@pytest.mark.parametrize("D,T,nh", [(64, 1, 8), (256, 1, 8), (128, 6, 4), (256, 8, 8), (512, 4, 4)])
+@pytest.mark.parametrize("size", [2.0 ** 17, 3e9, 2.0 ** 100, 1e-6, 3e-12, 2.0 ** -105])
+def test_attn_f32_queries_of_any_size(g, D, T, nh, size):
+    # q far outside f16's range, and the scale that makes ordinary scores of it; rows of sizes of their own, a row of zeros, one
+    # element that stands out (its keys' dim is small)
+    rng = np.random.default_rng(34 + D)
+    c = R.Cache(rng, [700, 90], 1, D)
+    c.fill_fast(rng)
+    scale = float(np.float32(1.0 / size))
+    q = rng.standard_normal((2 * T, nh, D)) * (3.0 / D ** 0.5)
+    q[0, 1] *= 2.0 ** -9
+    q[0, 2] = 0.0
+    q[-1, 3] *= 8.0
+    q[-1, 0, 5] = 40.0
+    q = (q * size).astype(np.float32)
+    check(run(g, c, q, [T, T], nh, "f32", scale=scale), c, q, [T, T], nh, "f32", scale=scale, ref=R.attention_prompt)
+
+
+def test_attn_f32_queries_beyond_f16(g):
+    # a query beyond 65504 in a dim where every key is 0: its scores are the other dims'
+    rng = np.random.default_rng(35)
+    c = R.Cache(rng, [200], 1, 64)
+    c.fill_fast(rng)
+    for page in c.table[0, :4]:
+        rec = c.pool[page, :1280]
+        rec[0:1024:16] &= 0xF0                                       # K's dim 0: code 0
+        sm = np.ascontiguousarray(rec[1024:]).view(np.float16).reshape(64, 2)
+        sm[:, 1] = 0.0                                               # and minimum 0
+        rec[1024:] = sm.view(np.uint8).reshape(-1)
+    q = (rng.standard_normal((1, 4, 64)) * 0.3).astype(np.float32)
+    q[0, :, 0] = [65520.0, -7e4, 1e9, 6e4]
+    got = run(g, c, q, [1], 4, "f32")
+    assert np.isfinite(got).all()
+    want, spread, size = R.attention(c, q, [1], 4)
+    # the low part of the other dims is held to 2^-25 at a row's largest of 2^14 or more: 2^-39 of it
+    lost = np.abs(q).max(-1) * 2.0 ** -38 * 64 * 4.0
+    tol = R.attention_bound(spread, size, want, 64, 5, False) + 2 * lost[..., None] * spread
+    assert np.all(np.abs(got - want) <= tol)
+
+
 @pytest.mark.parametrize("type_,R_,n", [("f32", 1024, 40), ("f16", 1024, 40), ("f16", 200, 13000)])
 def test_attn_cu_up_and_down(g, type_, R_, n):
     # 0, n, 0, n, ...: half of the sequences claim every token. More than the call has: nothing is computed (few rows, and prompts)
