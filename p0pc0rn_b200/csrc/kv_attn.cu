@@ -24,8 +24,9 @@
 //
 // Precision. f32 queries and outputs: q and P are split into f16 high and low parts (about 22 bits) in rows r and r + 8
 // of the fragments; a row of q is brought to [2^14, 2^15) by a power of two first, which its scores give back, so that
-// neither part leaves f16's range for any f32 q; each item's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
-// f16 matrix operand), 16 rows per fragment.
+// neither part leaves f16's range for any f32 q; P is held as 2^15 P, as its sum l is, for the same reason: parts that f16
+// does not hold lie below 2^-40 (P <= 1), and a long tail of small P counts in the output as it does in l; each item's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
+// f16 matrix operand; as 2^15 P, too), 16 rows per fragment.
 #include "kv_attn.cuh"
 
 namespace {
@@ -65,6 +66,7 @@ __device__ __forceinline__ uint32_t lds_u32(const uint8_t *p) { return *reinterp
 __device__ __forceinline__ float row_up(uint32_t bits) { return __uint_as_float((268u - max(bits >> 23, 15u)) << 23); }
 __device__ __forceinline__ float row_down(uint32_t bits) { return __uint_as_float((max(bits >> 23, 15u) - 14u) << 23); }
 
+constexpr float kPUp = 32768.0f;   // P in [0, 1] uses f16's whole range
 constexpr uint32_t kRec = 1312;   // a K record's place in shared memory
 
 template <int D, bool F32, int NPL, int RT, int KP, int NW>
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy into this slot
         }
       }
-      // ---- P = exp(x - m), into shared memory as f16 (f32: high and low parts)
+      // ---- P = 2^15 exp(x - m), into shared memory as f16 (f32: high and low parts)
 #pragma unroll
       for (int rt = 0; rt < RT; rt++) {
         float keep[RH];
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
           uint8_t *row = ps + (rt * 16 + g4 + 8 * h) * C::kPRow;
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
-            const float p0 = ex(x[rt][nt][h][0] - ref), p1 = ex(x[rt][nt][h][1] - ref);
+            const float p0 = ex(x[rt][nt][h][0] - ref) * kPUp, p1 = ex(x[rt][nt][h][1] - ref) * kPUp;
             l[rt][h] += p0 + p1;
             const uint32_t hi2 = pack2(p0, p1), col = ((warp * NT + nt) * 8u + 2u * t4) * 2u;
             *reinterpret_cast<uint32_t *>(row + col) = hi2;

@@ -17,8 +17,9 @@
 //   O  += P_j V_j     tcgen05.mma with P from tensor memory
 // Nothing in tensor memory is written while an MMA that was not waited for may read it (MMAs of different shapes or
 // accumulators have no order among themselves).
-// m is the row's maximum as of the last time O was rescaled: P may grow to 2^8 (harmless in f16 and f32) before O, in
-// tensor memory, is read and written again, which then happens in few tiles.
+// m is 7 less than the row's maximum as of the last time O was rescaled: P starts at 2^7 and may grow to 2^15 (f16 ends at
+// 2^16) before O, in tensor memory, is read and written again, which then happens in few tiles. P that f16 does not hold lies
+// below 2^-32 of the maximum's, so that a long tail of small P counts in O as it does in l.
 // At 512 dims O does not fit: a unit is a row block and half of the output's dims, S is computed for each half, 1.5 times
 // the products of a whole.
 // Work is cut into equal runs of key tiles as in kv_attn.cuh, one per pair; a unit's parts meet in the join kernel.
@@ -169,6 +170,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
+}
+// the same, held at 65504: scores of 2^24 and more may come out a few units above their maximum
+__device__ __forceinline__ uint32_t pack2_finite(float a, float b) {
+  uint32_t d;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
 #pragma unroll
@@ -489,11 +496,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
         asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
         if (!(ok = __all_sync(0xffffffffu, ok))) continue;
         mx = fmaxf(mx, mx2[t & 1u][h ^ 1u][r]);
-        // O follows a maximum that has grown by more than 2^8 (or that is a row's first)
-        const bool grow = mx > m + 8.0f;
+        // O follows a maximum whose P would pass 2^15 (or that is a row's first)
+        const bool grow = mx > m + 15.0f;
         if (__any_sync(0xffffffffu, grow)) {
-          const float f = grow ? exp2_fast(m - mx) : 1.0f;
-          if (grow) m = mx;
+          const float to_m = mx - 7.0f, f = grow ? exp2_fast(m - to_m) : 1.0f;
+          if (grow) m = to_m;
           l *= f;
           if (i) {
             ok = __all_sync(0xffffffffu, tc::mbar_wait(&odone[(t - 1u) & 1u], ((t - 1u) >> 1) & 1u, abort_flag, j.err, 0x4b7u, P0_SPIN_LIMIT));
@@ -519,7 +526,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) kv4_pro
             const float a = exp2_fast(fmaf(__uint_as_float(x[q][2 * e]), c, -ref)), d = exp2_fast(fmaf(__uint_as_float(x[q][2 * e + 1]), c, -ref));
             sum[2 * (e & 1)] += a;
             sum[2 * (e & 1) + 1] += d;
-            p[e] = pack2(a, d);
+            p[e] = pack2_finite(a, d);
           }
           tc::tmem_st16(pc + 32u * h + 16u * q, p);
         }

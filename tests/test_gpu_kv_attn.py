@@ -337,6 +337,40 @@ def test_attn_f32_queries_beyond_f16(g):
     assert np.all(np.abs(got - want) <= tol)
 
 
+@pytest.mark.parametrize("gap", [10.0, 13.3, 17.4])
+@pytest.mark.parametrize("type_,D,R_,T,nh,at", [("f32", 64, 1, 1, 1, 0), ("f32", 64, 1024, 1, 1, 0), ("f32", 256, 600, 1, 8, 40000), ("f32", 128, 200, 8, 4, 0),
+                                                ("f32", 512, 300, 2, 4, 7), ("f16", 64, 1024, 1, 2, 0), ("f16", 256, 200, 8, 4, 0), ("f16", 64, 127, 64, 1, 0),
+                                                ("f16", 256, 60, 70, 1, 200), ("f16", 512, 30, 130, 1, 30)])
+def test_attn_long_flat_tail(g, type_, D, R_, T, nh, at, gap):
+    # one key holds the maximum, 65499 others of one score lie `gap` below it and weigh e^-gap each: up to 3 of its 1 together.
+    # Each exp(-gap) has to reach O as it reaches the sum, though f16 by itself ends at 2^-24. The sequences are one and the same,
+    # so many that a run holds most of one's pages (each run has a maximum of its own)
+    n = 65500
+    rng = np.random.default_rng(36)
+    c = R.Cache(rng, [n], 1, D, ld=1024)
+    G = D // 32
+    rec = np.zeros((c.pages, 2, G, 1280), np.uint8)                  # codes 0: a row's value is its minimum
+    mn = np.zeros((c.pages, 2, G, 64, 2), np.float16)
+    mn[..., 0] = 1.0
+    mn[:, 1, :, :, 1] = 1.0 + 0.25 * rng.random((c.pages, G, 64))
+    top = c.table[0, at // 64], slice(None), slice(None), at % 64, 1
+    mn[top] = np.array([[1.0], [-1.0]])
+    rec[..., 1024:] = mn.reshape(c.pages, 2, G, 128).view(np.uint8)
+    c.pool[:] = rec.reshape(c.pages, -1)
+    dt = np.float32 if type_ == "f32" else np.float16
+    q = np.full((T, nh, D), gap / D, dt)
+    want, spread, size = R.attention_prompt(c, q, [T], nh)
+    # attention_bound's sums and scores; what P loses: 2^-22 of it as two halves, and 2^-40 (f32, f16) or 2^-32 (prompts) a key
+    e = (D / 16 + D / 32 + 4) * 2.0 ** -23 * size[..., None]
+    tol = (2 * e + 2.0 ** -20 + (c.ld + 8) * 2.0 ** -23) * spread + n * 2.0 ** (-32 if T * nh >= 64 else -40) * 2
+    if type_ == "f16":
+        tol += 2.0 ** -11 * spread + 2.0 ** -11 * np.abs(want)
+    c.table, c.lens = np.repeat(c.table, R_, 0), np.full(R_, n, np.uint32)
+    got = run(g, c, np.tile(q, (R_, 1, 1)), [T] * R_, nh, type_).reshape(R_, T, nh, D)
+    err = np.abs(got.astype(np.float64) - want)
+    assert np.all(err <= tol), float((err / tol).max())
+
+
 @pytest.mark.parametrize("type_,R_,n", [("f32", 1024, 40), ("f16", 1024, 40), ("f16", 200, 13000)])
 def test_attn_cu_up_and_down(g, type_, R_, n):
     # 0, n, 0, n, ...: half of the sequences claim every token. More than the call has: nothing is computed (few rows, and prompts)
