@@ -324,7 +324,8 @@ p0_status p0_attn_dec(p0_ctx *ctx, const p0_attn_dec_args *a);
  * all layers' parts (0 = one layer's); a layer's view has its part's place in the page as pool_off.
  * State on the device: table u32 [rows][table_ld], the page of each sequence's tokens 64 j .. 64 j + 63 (an entry >=
  * pages, e.g. P0_KV_NONE, is no page: its tokens are not there), len u32 [rows] (a length beyond 64 * table_ld counts as
- * that), and ref u32 [pages], how many table entries (and holders of the caller's own) refer to each page.
+ * that), and ref u32 [pages], how many table entries (and holders of the caller's own) refer to each page; entries beyond a
+ * length count, too (where there is no page, the table holds P0_KV_NONE from the start).
  * Offsets of table and len in u32. rows <= 1024, nkv <= 1024, table_ld <= 2^23, tokens of a call <= 2^28, D 64, 128, 256 or 512;
  * pool_off, page_stride 16-byte aligned.
  * Everything is read when the call's kernels run, so a call's arguments stay valid from step to step. The operators keep
@@ -376,7 +377,9 @@ p0_status p0_kv4_attn(p0_ctx *ctx, const p0_kv4_attn_args *a);
 
 /* kvStep: one step of every sequence: fork, reorder or free (parent), give back what the window has passed, extend (add).
  * New sequence i continues old sequence parent[i] (u32 [rows]; absent: i; >= rows: it is empty, its pages are given
- * back) with length n = len[parent[i]]. It refers to the parent's pages, without those whose every token lies outside the
+ * back) with length n = len[parent[i]]. A length may have been lowered since the last step (tokens taken back, e.g. drafts
+ * that were not accepted; not below a length that it was forked at, whose pages others share): the pages that only tokens
+ * beyond it needed are given back. The new sequence refers to the parent's pages, without those whose every token lies outside the
  * window of position n and behind the first `sinks` (window 0: all are kept). If n is not a multiple of 64, the last page
  * stays with the parent's first child; every further child gets a copy of it (all layers: page_stride bytes). Then
  * add[i] (u32 [rows]; absent: addn) tokens are appended: new pages for those beyond the last page. Pages are taken from

@@ -384,11 +384,10 @@ __device__ __forceinline__ void step_plan(const StepJob &j) {
   }
   meet();   // rc holds the old counts
   // the table without the new pages, and the counts that follow from it: an entry that a row keeps in place changes
-  // nothing
+  // nothing. Old entries beyond a length (it may have been lowered) are references as well, and end here
   for (uint64_t e = tid; e < (uint64_t)R * ld; e += all) {
     const uint32_t i = (uint32_t)e / ld, p = (uint32_t)e - i * ld;
-    const uint32_t n = kv_len(j.v, i);
-    uint32_t a = p < (n + kPage - 1) / kPage ? j.v.table[e] : kNone, b = kNone;
+    uint32_t a = j.v.table[e], b = kNone;
     if (a >= P) a = kNone;
     if (par[i] != kNone && p < (lp[i] + kPage - 1) / kPage) {
       b = j.v.table[(uint64_t)par[i] * ld + p];

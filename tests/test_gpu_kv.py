@@ -230,6 +230,48 @@ def test_step_many_random(g):
     assert np.array_equal(np.bincount(used, minlength=pages), ref)
 
 
+def lowered_step(table, lens, ref, pages, *a):
+    """R.step of a state whose tables may hold pages beyond the lengths: those are references, which the step ends"""
+    clean, counts = table.copy(), ref.astype(np.int64)
+    for b, n in enumerate(lens):
+        for j in range(-(-int(n) // R.PAGE), table.shape[1]):
+            if clean[b, j] < pages:
+                counts[clean[b, j]] -= 1
+                clean[b, j] = R.NONE
+    got = R.step(clean, lens, counts.astype(np.uint32), pages, *a)
+    return got if got[3][0] == 0 else (table, lens, ref, (got[3][0], int((ref == 0).sum())), [])
+
+
+@pytest.mark.parametrize("spare", [60, 6000])                        # one CTA plans, and a cluster
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4)])
+def test_step_after_a_lowered_length(g, spare, window, sinks):
+    # rounds of: every row takes up to 200 drafted tokens, keeps some of them, and goes on; rows end and fork now and then. No page
+    # is lost: the counts are the table's at every step
+    rng = np.random.default_rng(21)
+    table, ln, ref, pages = batch(rng, [300, 65], [(3, 2), (3, 0)], 30, spare)
+    rows = len(ln)
+    pool = rng.integers(0, 256, (pages, 32), dtype=np.uint8)
+    for step in range(14):
+        parent = np.arange(rows)
+        if step % 4 == 3:
+            parent = np.where(rng.random(rows) < 0.2, R.NONE, rng.integers(0, rows, rows))
+        add = rng.integers(0, 200, rows) if step != 9 else np.full(rows, 64 * 30)   # once more than the tables hold: nothing changes
+        want = lowered_step(table, ln, ref, pages, parent, add, window, sinks)
+        got = run_step(g, table, ln, ref, pages, 32, pool, parent=parent, add=add, window=window, sinks=sinks)
+        assert (want[3][0] != 0) == (step == 9)
+        assert got[3] == want[3]
+        for s, d in want[4]:
+            pool[d] = pool[s]
+        for a, b in zip(got[:3], want[:3]):
+            assert np.array_equal(a, b)
+        assert np.array_equal(got[4], pool)
+        before, (table, ln, ref) = ln, want[:3]
+        assert np.array_equal(np.bincount(table[table < pages], minlength=pages), ref)
+        if step != 9:                                                # the drafts that are not accepted: never below the length before
+            keep = rng.integers(0, add + 1)
+            ln = np.where(ln >= add, ln - np.minimum(add, ln) + keep, ln).astype(np.uint32)
+
+
 @pytest.mark.parametrize("seed,pages,live,rows", [(0, 1, 0.0, 1), (1, 1, 1.0, 2), (2, 300, 0.5, 7), (3, 5000, 0.3, 33), (4, 20011, 0.9, 3), (5, 64, 1.0, 4)])
 def test_compact(g, seed, pages, live, rows):
     rng = np.random.default_rng(seed)
