@@ -704,8 +704,16 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
   uint32_t *cnt;
   void *ws;
   const size_t desc = ((size_t)G * sizeof(uint4) + 255) / 256 * 256, parts = ((size_t)G * 2 * kRB * (C::kDV + 2) * 4 + 255) / 256 * 256;
-  p0_status st = p0_workspace(c, 0, desc + parts + wide_bytes, &cnt, &ws);
+  // in place and with the output in parts, a unit writes where another reads q: both work from a copy
+  const bool in_place = C::kParts > 1 && j.q.base == j.out.base;
+  const uint64_t q_bytes = ((uint64_t)(j.v.n - 1) * j.q.ld + (uint64_t)(j.hpg * j.v.nkv - 1) * j.q.ldh + D) * 2u;
+  p0_status st = p0_workspace(c, 0, desc + parts + wide_bytes + (in_place ? q_bytes : 0u), &cnt, &ws);
   if (st) return st;
+  if (in_place) {
+    uint8_t *copy = (uint8_t *)ws + desc + parts + wide_bytes;
+    if ((st = p0_cuda(c, cudaMemcpyAsync(copy, j.q.base, q_bytes, cudaMemcpyDeviceToDevice, c->stream), "kv4Attn in place"))) return st;
+    j.q.base = copy;
+  }
   j.desc = (uint4 *)ws;
   j.part = (float *)((uint8_t *)ws + desc);
   j.wide = (uint8_t *)ws + desc + parts;

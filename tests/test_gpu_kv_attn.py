@@ -337,6 +337,41 @@ def test_attn_f32_queries_beyond_f16(g):
     assert np.all(np.abs(got - want) <= tol)
 
 
+@pytest.mark.parametrize("type_", ["f32", "f16"])
+@pytest.mark.parametrize("lens,counts,nh,nkv,D,lay", [
+    ([900, 130, 40], [1, 1, 1], 8, 1, 256, (0, 0, 0)),
+    ([700, 300], [40, 9], 4, 2, 128, (4 * 130, 130, 3)),
+    ([700, 300, 90], [300, 200, 90], 8, 2, 256, (0, 0, 0)),
+    ([700, 300, 90], [300, 200, 90], 8, 4, 512, (0, 0, 0)),          # prompts of 512 dims: the output in two parts
+    ([700, 300], [300, 200], 4, 4, 512, (4 * 513, 513, 1)),
+    ([700, 300], [300, 200], 2, 2, 512, (512, 512 * 501, 0)),
+])
+def test_attn_in_place(g, type_, lens, counts, nh, nkv, D, lay):
+    # out = q gives what a call with an output of its own gives
+    rng = np.random.default_rng(37)
+    c = R.Cache(rng, lens, nkv, D)
+    c.fill_fast(rng)
+    n = sum(counts)
+    q = (rng.standard_normal((n, nh, D)) * (3.0 / D ** 0.5)).astype(np.float32 if type_ == "f32" else np.float16)
+    want = run(g, c, q, counts, nh, type_, 200, 3, lay=lay, out_lay=lay)
+    check(want, c, q, counts, nh, type_, 200, 3, ref=R.attention_prompt)
+    ld, ldh, off = lay[0] or nh * D, lay[1] or D, lay[2]
+    at = off + np.arange(n)[:, None, None] * ld + np.arange(nh)[None, :, None] * ldh + np.arange(D)
+    host = np.full(at.max() + 1, -77, q.dtype)
+    host[at] = q
+    _, kv = kv_args(g, c)
+    x = g.upload(host)
+    rows = {"buf": x, "off": off, "ld": ld, "ldh": ldh}
+    cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    new = {"T": counts[0]} if len(set(counts)) == 1 else {"cu": {"buf": g.upload(cu)}}
+    p0.kv4Attn(g, {"kv": kv, "q": rows, "out": rows, "type": type_, "nh": nh, "n": n, "window": 200, "sinks": 3, **new})
+    g.done()
+    got = g.read(x, 0, host.nbytes, q.dtype)
+    assert np.array_equal(got[at].view(np.uint8), want.view(np.uint8))
+    got[at] = -77
+    assert np.all(got == -77)
+
+
 @pytest.mark.parametrize("gap", [10.0, 13.3, 17.4])
 @pytest.mark.parametrize("type_,D,R_,T,nh,at", [("f32", 64, 1, 1, 1, 0), ("f32", 64, 1024, 1, 1, 0), ("f32", 256, 600, 1, 8, 40000), ("f32", 128, 200, 8, 4, 0),
                                                 ("f32", 512, 300, 2, 4, 7), ("f16", 64, 1024, 1, 2, 0), ("f16", 256, 200, 8, 4, 0), ("f16", 64, 127, 64, 1, 0),
