@@ -163,5 +163,5 @@ __device__ __forceinline__ Unit find_unit(const AttnJob &j, const uint32_t *pre,
 // runs end where total * (c + 1) / G does: the run of item i
 __device__ __forceinline__ uint32_t run_of(uint32_t i, uint32_t total, uint32_t G) { return (uint32_t)((((uint64_t)i + 1u) * G - 1u) / total); }
 
-// the prompt form (kv_prompt.cu): f16, many new tokens; P0_OK with *taken = false where it does not serve the call
+// the prompt form (kv_prompt.cu): f16, many new tokens; P0_OK with *taken = false, and j as it was, where it does not serve the call
 p0_status kv4_attn_prompt(p0_ctx *c, AttnJob &j, bool *taken);

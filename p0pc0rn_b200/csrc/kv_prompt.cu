@@ -695,20 +695,35 @@ __global__ void __launch_bounds__(kCR *kJoin) kv4_prompt_join_kernel(AttnJob j) 
   }
 }
 
+// whether the workspace has this much scratch, or the device the memory for it (as far as one can tell before asking): the one that
+// is there is not given up in vain
+bool room_for(p0_ctx *c, uint64_t scratch) {
+  const uint64_t need = c->ws_cnt_bytes + scratch;
+  if (need <= c->ws_bytes) return true;
+  size_t left = 0, all = 0;
+  if (cudaMemGetInfo(&left, &all) != cudaSuccess) { cudaGetLastError(); return true; }
+  return need + (16ull << 20) <= (uint64_t)left + c->ws_bytes;
+}
+
+// *taken stays false where there is no memory for the pages as f16: the form for few rows needs none
 template <int D>
-p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
+p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes, bool *taken) {
   using C = Cfg<D>;
   const uint32_t R = j.v.rows, G = (uint32_t)c->sm_count / 2;
   const size_t smem = C::kSmem + ((size_t)R + 1) * 8;
-  j.units = j.v.nkv * C::kParts;
   uint32_t *cnt;
   void *ws;
   const size_t desc = ((size_t)G * sizeof(uint4) + 255) / 256 * 256, parts = ((size_t)G * 2 * kRB * (C::kDV + 2) * 4 + 255) / 256 * 256;
   // in place and with the output in parts, a unit writes where another reads q: both work from a copy
   const bool in_place = C::kParts > 1 && j.q.base == j.out.base;
   const uint64_t q_bytes = ((uint64_t)(j.v.n - 1) * j.q.ld + (uint64_t)(j.hpg * j.v.nkv - 1) * j.q.ldh + D) * 2u;
-  p0_status st = p0_workspace(c, 0, desc + parts + wide_bytes + (in_place ? q_bytes : 0u), &cnt, &ws);
+  const uint64_t scratch = desc + parts + wide_bytes + (in_place ? q_bytes : 0u);
+  if (!room_for(c, scratch)) return P0_OK;
+  p0_status st = p0_workspace(c, 0, scratch, &cnt, &ws);
+  if (st == P0_ENOMEM) return P0_OK;
+  *taken = true;
   if (st) return st;
+  j.units = j.v.nkv * C::kParts;
   if (in_place) {
     uint8_t *copy = (uint8_t *)ws + desc + parts + wide_bytes;
     if ((st = p0_cuda(c, cudaMemcpyAsync(copy, j.q.base, q_bytes, cudaMemcpyDeviceToDevice, c->stream), "kv4Attn in place"))) return st;
@@ -747,18 +762,23 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes) {
 // Taken where the sequences have 64 query rows a KV head on average (128 at 512 dims): one sequence of 1200 keys, 64 rows of 256
 // dims, 22 us against 32 of the form for few rows; 24 of 6000 keys, 70 against 76; 32 rows of 1200 keys, 23 against 19. (One
 // sequence of 30000 keys and 64 rows: 57 against 50; 512 dims, 24 of 6000, 64 rows: 165 against 114, 256 rows: 152 against 269.)
-// And where all pages of the table as f16 take no more than 4 GB.
+// And where the pages that the call may see take no more than 4 GB as f16: of each sequence all that its table row holds, or with a
+// window those of the sinks, of the window before its first new token, and of its new tokens (T / 64 and a page's ends more).
 p0_status kv4_attn_prompt(p0_ctx *c, AttnJob &j, bool *taken) {
   *taken = false;
-  const uint64_t rows = (uint64_t)j.v.n * j.hpg, D = j.v.D;
-  if (rows / j.v.rows < (D == 512 ? 128 : 64)) return P0_OK;
-  const uint64_t wide = (uint64_t)j.v.rows * j.v.ld * j.v.nkv * D * 256;
-  if (wide > (4ull << 30) || j.v.rows > 256) return P0_OK;
-  *taken = true;
+  const uint64_t rows = (uint64_t)j.v.n * j.hpg, D = j.v.D, R = j.v.rows;
+  if (rows / R < (D == 512 ? 128 : 64) || R > 256) return P0_OK;
+  uint64_t pages = R * j.v.ld;
+  if (j.window) {
+    const uint64_t seen = R * ((j.sinks + kPage - 1) / kPage + j.window / kPage + 3u) + j.v.n / kPage;
+    if (seen < pages) pages = seen;
+  }
+  const uint64_t wide = pages * j.v.nkv * D * 256;
+  if (wide > (4ull << 30)) return P0_OK;
   switch (D) {
-    case 64: return prompt_launch<64>(c, j, wide);
-    case 128: return prompt_launch<128>(c, j, wide);
-    case 256: return prompt_launch<256>(c, j, wide);
-    default: return prompt_launch<512>(c, j, wide);
+    case 64: return prompt_launch<64>(c, j, wide, taken);
+    case 128: return prompt_launch<128>(c, j, wide, taken);
+    case 256: return prompt_launch<256>(c, j, wide, taken);
+    default: return prompt_launch<512>(c, j, wide, taken);
   }
 }

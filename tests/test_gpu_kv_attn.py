@@ -372,6 +372,44 @@ def test_attn_in_place(g, type_, lens, counts, nh, nkv, D, lay):
     assert np.all(got == -77)
 
 
+def test_prompt_without_memory_for_wide_pages(g):
+    # a device too full for the pages as f16 (2 GB here): the call is served by the form for few rows (two launches), and by the
+    # other one (three) once there is room
+    import torch
+    rng = np.random.default_rng(38)
+    c = R.Cache(rng, [400, 130], 1, 256, ld=16384)
+    c.fill_fast(rng)
+    counts = [80, 80]
+    q = (rng.standard_normal((160, 2, 256)) * (3.0 / 256 ** 0.5)).astype(np.float16)
+    own = p0.Gpu(0)
+    try:
+        check(run(own, c, q, counts, 2, "f16", 100, 3), c, q, counts, 2, "f16", 100, 3, ref=R.attention_prompt)
+        full = own.buffer(torch.cuda.mem_get_info()[0] - (1 << 30), "what fills the device")
+        for launches in (2, 2, 3):
+            if launches == 3:
+                own.free(full)
+            before = own.stats["dispatches"]
+            got = run(own, c, q, counts, 2, "f16")
+            assert own.stats["dispatches"] - before == launches
+            check(got, c, q, counts, 2, "f16", ref=R.attention_prompt)
+    finally:
+        own.close()
+
+
+def test_prompt_window_in_a_wide_table(g):
+    # what the window lets a call see bounds the pages held as f16, not what the table could hold
+    rng = np.random.default_rng(39)
+    lens, counts = [3000, 500, 64, 900], [300, 200, 64, 1]
+    c = R.Cache(rng, lens, 1, 64, ld=70000)
+    c.fill_fast(rng)
+    q = (rng.standard_normal((sum(counts), 2, 64)) * (3.0 / 8)).astype(np.float16)
+    before = g.stats["dispatches"]
+    got = run(g, c, q, counts, 2, "f16", 130, 70)
+    assert g.stats["dispatches"] - before == 3
+    want, spread, size = R.attention_prompt(c, q, counts, 2, 130, 70)
+    assert np.all(np.abs(got - want) <= R.attention_bound(spread, size, want, 64, 50, True))
+
+
 @pytest.mark.parametrize("gap", [10.0, 13.3, 17.4])
 @pytest.mark.parametrize("type_,D,R_,T,nh,at", [("f32", 64, 1, 1, 1, 0), ("f32", 64, 1024, 1, 1, 0), ("f32", 256, 600, 1, 8, 40000), ("f32", 128, 200, 8, 4, 0),
                                                 ("f32", 512, 300, 2, 4, 7), ("f16", 64, 1024, 1, 2, 0), ("f16", 256, 200, 8, 4, 0), ("f16", 64, 127, 64, 1, 0),
