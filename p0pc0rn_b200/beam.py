@@ -19,6 +19,7 @@ from . import ops
 from .decode import KP, model_sizes
 
 PAGE = L.P0_KV_PAGE
+LOG = 4096                  # steps whose shortages a cache holds before it looks at them
 
 
 class PagedCache:
@@ -30,7 +31,9 @@ class PagedCache:
         self.pool = g.buffer(pages * layers * self.part, "kv pages")
         none = np.full(rows * max_pages, L.P0_KV_NONE, np.uint32)
         self.state = [{"table": g.upload(none), "len": g.buffer(rows * 4), "ref": g.buffer(pages * 4)} for _ in range(2)]
-        self.now, self.stat = 0, g.buffer(16, "stat")
+        self.now, self.moved = 0, g.buffer(16, "moved")
+        # what each step was short of, and left free: kept until ran_short() has looked at it
+        self.log, self.steps, self.first_short = g.buffer(8 * LOG, "steps"), 0, 0
 
     def view(self, layer=0):
         s = self.state[self.now]
@@ -39,22 +42,34 @@ class PagedCache:
 
     def step(self, **a):
         """kvStep into the other state, which becomes the current one"""
+        if self.steps and self.steps % LOG == 0:
+            self.ran_short()
         to = self.state[1 - self.now]
         kv = self.view()
-        ops.kvStep(self.g, {"kv": kv, "ref": {"buf": self.state[self.now]["ref"]}, "to": {k: {"buf": to[k]} for k in to}, "stat": {"buf": self.stat}, **a})
+        stat = self.g.wrap(self.log.ptr + 8 * (self.steps % LOG), 8, "stat")
+        ops.kvStep(self.g, {"kv": kv, "ref": {"buf": self.state[self.now]["ref"]}, "to": {k: {"buf": to[k]} for k in to}, "stat": {"buf": stat}, **a})
+        self.g.free(stat)
+        self.steps += 1
         self.now = 1 - self.now
 
     def compact(self):
         """the pages in use into the lowest ones"""
         s, to = self.state[self.now], self.state[1 - self.now]
         ops.kvCompact(self.g, {"kv": self.view(), "ref": {"buf": s["ref"]}, "to": {"table": {"buf": to["table"]}, "ref": {"buf": to["ref"]}},
-                               "stat": {"buf": self.stat}})
+                               "stat": {"buf": self.moved}})
         self.g.copy(s["len"], 0, to["len"], 0, self.rows * 4)
         self.now = 1 - self.now
 
     def short(self):
-        """pages that the last step was short of (0: none; its state is then the one before it). Waits for the device"""
-        return int(self.g.read(self.stat, 0, 4, np.uint32)[0])
+        """pages that the last step was short of (0: none; its state is otherwise the one before it). Waits for the device"""
+        return int(self.g.read(self.log, 8 * ((self.steps - 1) % LOG), 4, np.uint32)[0]) if self.steps else 0
+
+    def ran_short(self):
+        """pages that a step was short of, however long ago (0: no step was). Waits for the device"""
+        if not self.first_short and self.steps:
+            logged = self.g.read(self.log, 0, 8 * min(self.steps, LOG), np.uint32)[0::2]   # beyond LOG steps: of some that were looked at before
+            self.first_short = int(logged[logged != 0][0]) if logged.any() else 0
+        return self.first_short
 
 
 class BeamSearch:
@@ -161,8 +176,8 @@ class BeamSearch:
         """(sequences, best first, without the prompt; scores; finished). A finished hypothesis goes on with eos"""
         M = self.cfg["beams"]
         for c in self.cache.values():
-            if c.short():
-                raise RuntimeError("the cache is short of %d pages" % c.short())
+            if c.ran_short():
+                raise RuntimeError("the cache is short of %d pages" % c.ran_short())
         h = self.g.read(self.b["hist"], 0, 2 * M * 4 * self.chosen, np.uint32).reshape(self.chosen, 2, M)
         score = self.g.read(self.b["score"], 0, 4 * M, np.float32)
         out = []
