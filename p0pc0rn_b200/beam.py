@@ -72,6 +72,12 @@ class PagedCache:
         return self.first_short
 
 
+    def close(self, tables=True):
+        """gives back the pages and, with tables, the states (which can be read until then)"""
+        for b in [self.pool, self.log, self.moved] + ([b for s in self.state for b in s.values()] if tables else []):
+            self.g.free(b)
+
+
 class BeamSearch:
     """cfg as p0pc0rn_b200.decode's, plus beams (<= 8), eos, sinks (default 0); model m as decode_token's"""
 
@@ -96,10 +102,15 @@ class BeamSearch:
         g.write(self.b["score"], np.array([0.0] + [-np.inf] * (M - 1), np.float32))
 
     def close(self):
+        """gives back the buffers and the caches' pages; the caches' tables, lengths and counts stay until PagedCache.close()"""
         for r in self.rows:
             for w in r.values():
                 self.g.free(w)
         self.rows = []
+        for b in self.b.values():
+            self.g.free(b)
+        for c in self.cache.values():
+            c.close(tables=False)
 
     def _layers(self, ids):
         """one token of every row (ids: a device buffer) at position self.pos - 1 of the current caches"""

@@ -65,3 +65,18 @@ def test_result_refuses_after_a_shortage(g, model):
         s.result()
     g.done()
     s.close()
+
+
+def test_close_gives_the_memory_back(g, model):
+    before, held = g.stats["alive"], len(g.bufs)
+    s = beam.BeamSearch(g, CFG, model, 160)
+    s.prompt([3])
+    s.step()
+    s.close()
+    tables = sum(b.size for c in s.cache.values() for st in c.state for b in st.values())
+    assert g.stats["alive"] - before == tables                       # the caches' states can still be read
+    for c in s.cache.values():
+        assert g.read(c.state[c.now]["len"], 0, 4, np.uint32)[0] == 2
+        c.close()
+    assert g.stats["alive"] == before and len(g.bufs) == held
+    s.close()                                                        # again: nothing left to do
