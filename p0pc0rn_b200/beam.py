@@ -164,8 +164,12 @@ class BeamSearch:
         self.pos += 1
 
     def prompt(self, tokens):
-        """the prompt's tokens through row 0, then the first selection"""
+        """the prompt's tokens through row 0, then the first selection. Once: the other rows are empty until then"""
         M = self.cfg["beams"]
+        if self.pos:
+            raise ValueError("the search has its prompt")
+        if not 1 <= len(tokens) <= self.max_pos:
+            raise ValueError("a prompt of %d tokens: 1 to %d" % (len(tokens), self.max_pos))
         self.g.write(self.b["add"], np.array([1] + [0] * (M - 1), np.uint32))
         ids = self.g.upload(np.repeat(np.asarray(tokens, np.uint32)[:, None], M, 1))
         one = [self.g.wrap(ids.ptr + 4 * M * i, 4 * M, "ids") for i in range(len(tokens))]

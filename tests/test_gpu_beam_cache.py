@@ -80,3 +80,19 @@ def test_close_gives_the_memory_back(g, model):
         c.close()
     assert g.stats["alive"] == before and len(g.bufs) == held
     s.close()                                                        # again: nothing left to do
+
+
+def test_prompts_that_are_refused(g, model):
+    # without a token there is nothing to select from; a second prompt would write over the rows' last tokens
+    s = beam.BeamSearch(g, CFG, model, 160)
+    for tokens in ([], [5] * 161):
+        with pytest.raises(ValueError, match="a prompt of %d tokens" % len(tokens)):
+            s.prompt(tokens)
+    s.prompt([3, 9])
+    want = s.result()
+    with pytest.raises(ValueError, match="has its prompt"):
+        s.prompt([4])
+    got = s.result()
+    assert got[0] == want[0] and np.array_equal(got[1], want[1])
+    g.done()
+    s.close()
