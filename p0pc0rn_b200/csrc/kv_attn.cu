@@ -27,6 +27,8 @@
 // neither part leaves f16's range for any f32 q; P is held as 2^15 P, as its sum l is, for the same reason: parts that f16
 // does not hold lie below 2^-40 (P <= 1), and a long tail of small P counts in the output as it does in l; each item's P V is summed from zero and added in f32. f16: q as it is, P rounded to f16 once (as any
 // f16 matrix operand; as 2^15 P, too), 16 rows per fragment.
+#include <cstdlib>
+
 #include "kv_attn.cuh"
 
 namespace {
@@ -120,7 +122,7 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
   uint32_t b = find_sequence(pre, R, lo);
   const float log2_scale = j.scale * 1.44269504088896340736f;   // f16: scores and maxima in powers of two
   const auto ex = [](float x) { return exp2_fast(F32 ? x * 1.44269504088896340736f : x); };
-  uint32_t at = lo, it = 0;   // item; items through the ring so far
+  uint32_t at = lo, it = 0, started = 0;   // item; items through the ring so far; items whose copies were started (warp 0's)
   while (at < hi) {
     while (pre[b + 1] <= at) b++;
     const Unit u = find_unit<RB, KP, 0>(j, pre, b, at);
@@ -140,6 +142,8 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
     };
     uint32_t ahead = P0_KV_NONE;
     const auto issue = [&](uint32_t i) {
+      if (__any_sync(0xffffffffu, *(volatile uint32_t *)&abort_flag)) return;   // the slot's last copies may still be on their way
+      started = it + i + 1u;
       const uint32_t st = (it + i) % NS, p = ahead;
       const bool have = p < j.v.pages;
       const uint32_t n_k = __popc(__ballot_sync(0xffffffffu, have && cr < C::kRecs)), n_v = __popc(__ballot_sync(0xffffffffu, have && cr == C::kRecs));
@@ -250,7 +254,7 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
     bool lost = false;
     for (uint32_t i = 0; i < steps; i++) {
       const uint32_t st = (it + i) % NS, pi = (from + i) * KP;
-      if (!tc::mbar_wait(&full[st], ((it + i) / NS) & 1u, &abort_flag, j.err, 0x4a1u, P0_SPIN_LIMIT)) lost = true;
+      if (!tc::mbar_wait(&full[st], ((it + i) / NS) & 1u, &abort_flag, j.err, 0x4a1u, j.polls)) lost = true;
       const uint8_t *stage = ring + st * C::kStage;
       uint32_t key0[KP], ok[KP];
 #pragma unroll
@@ -431,9 +435,10 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
             for (int e = 0; e < 4; e++) o[rt][nt][e] += c[rt][nt][e];
       }
     }
-    if (__syncthreads_or(lost)) {   // a copy did not arrive in time: j.err says so. Let the copies in flight land before the CTA leaves
-      for (uint32_t i = 0; i < steps; i++)
-        for (uint32_t k = 0; k < (1u << 16) && !tc::mbar_try(&full[(it + i) % NS], ((it + i) / NS) & 1u); k++) {}
+    if (__syncthreads_or(lost)) {   // a copy did not arrive in time: j.err says so. The copies in flight, each slot's last, land before
+      if (warp == 0)                // the CTA leaves: a slot's wait is bounded, too
+        for (uint32_t i = started > (uint32_t)NS ? started - NS : 0u; i < started; i++)
+          for (uint32_t k = 0; k < (1u << 16) && !tc::mbar_try(&full[i % NS], (i / NS) & 1u); k++) {}
       return;
     }
     it += steps;
@@ -644,6 +649,8 @@ extern "C" p0_status p0_kv4_attn(p0_ctx *c, const p0_kv4_attn_args *a) {
   j.sinks = a->sinks < most ? a->sinks : most;
   j.scale = a->scale != 0.0f ? a->scale : 1.0f;
   j.err = c->d_err;
+  const char *polls = getenv("P0MM_KV4_POLLS");   // for tests of what follows a wait that gives up
+  j.polls = polls ? (uint32_t)strtoul(polls, nullptr, 10) : P0_SPIN_LIMIT;
   // the kernels count query rows and items (pages of row blocks) in 32 bits
   const uint64_t rows = (uint64_t)a->n * j.hpg;
   if (rows > 0x7fffffffu || (rows / 8 + a->kv.rows + 1) * a->kv.nkv * a->kv.table_ld > 0xffffffffull)

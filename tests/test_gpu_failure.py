@@ -47,3 +47,28 @@ def test_wait_selftest_rejects_bad_limits(g):
     for polls in (0, (1 << 20) + 1):
         with pytest.raises(p0.P0Error, match="polls"):
             g.wait_selftest(polls)
+
+
+@pytest.mark.parametrize("type_", ["f32", "f16"])
+@pytest.mark.parametrize("lens,T,nh,D", [([9000, 700, 30], 1, 8, 256), ([40000] * 4, 1, 2, 64), ([3000, 200], 7, 4, 128), ([2000, 900], 5, 4, 512)])
+def test_attention_gives_up_and_context_stays_usable(g, type_, lens, T, nh, D, monkeypatch):
+    # every wait of kv4Attn for its copies gives up at once, while they are on their way: the call reports it, and the next one is right
+    from . import kv_ref as R
+    from .test_gpu_kv import kv_args
+    from .test_gpu_kv_attn import check, run
+    rng = np.random.default_rng(40 + D)
+    c = R.Cache(rng, lens, 1, D)
+    c.fill_fast(rng)
+    n, dt = T * len(lens), np.float32 if type_ == "f32" else np.float16
+    q = (rng.standard_normal((n, nh, D)) * (3.0 / D ** 0.5)).astype(dt)
+    _, kv = kv_args(g, c)
+    qb, o = g.upload(q), g.buffer(q.nbytes)
+    a = {"kv": kv, "q": {"buf": qb}, "out": {"buf": o}, "type": type_, "nh": nh, "n": n, "T": T}
+    for _ in range(3):
+        monkeypatch.setenv("P0MM_KV4_POLLS", "0")
+        p0.kv4Attn(g, a)
+        with pytest.raises(p0.P0Error, match="0x4a1") as ei:
+            g.done(10000)
+        assert ei.value.status == L.P0_ETIMEOUT
+        monkeypatch.delenv("P0MM_KV4_POLLS")
+        check(run(g, c, q, [T] * len(lens), nh, type_), c, q, [T] * len(lens), nh, type_)
