@@ -410,6 +410,20 @@ def test_prompt_window_in_a_wide_table(g):
     assert np.all(np.abs(got - want) <= R.attention_bound(spread, size, want, 64, 50, True))
 
 
+@pytest.mark.parametrize("type_", ["f32", "f16"])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("T,nh,nkv", [(7, 8, 1), (9, 12, 2), (3, 7, 1)])
+def test_attn_fragments_at_once(g, type_, D, T, nh, nkv):
+    # 56, 54 and 21 rows a KV head: up to four fragments of rows on each dequantised page, the last ones not full
+    rng = np.random.default_rng(41 + D)
+    lens = [900, 64, 333, 7]
+    c = R.Cache(rng, lens, nkv, D)
+    c.fill_fast(rng)
+    q = (rng.standard_normal((4 * T, nh, D)) * (3.0 / D ** 0.5)).astype(np.float32 if type_ == "f32" else np.float16)
+    for window, sinks in ((0, 0), (100, 66)):
+        check(run(g, c, q, [T] * 4, nh, type_, window, sinks), c, q, [T] * 4, nh, type_, window, sinks, ref=R.attention_prompt)
+
+
 @pytest.mark.parametrize("gap", [10.0, 13.3, 17.4])
 @pytest.mark.parametrize("type_,D,R_,T,nh,at", [("f32", 64, 1, 1, 1, 0), ("f32", 64, 1024, 1, 1, 0), ("f32", 256, 600, 1, 8, 40000), ("f32", 128, 200, 8, 4, 0),
                                                 ("f32", 512, 300, 2, 4, 7), ("f16", 64, 1024, 1, 2, 0), ("f16", 256, 200, 8, 4, 0), ("f16", 64, 127, 64, 1, 0),
