@@ -91,7 +91,7 @@ struct Cfg {
 };
 
 template <int D, bool F32, int NPL, int RT, int KP, int NW>
-__global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel(AttnJob j) {
+__global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel(AttnJob j, uint32_t polls) {
   dep_enter();
   using C = Cfg<D, F32, NPL, RT, KP, NW>;
   constexpr int NT = C::kNt, RR = C::kRowsPer, RB = C::kRows, NS = C::kStages;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(NW * 32, RT > 1 ? 1 : 16 / NW) kv4_attn_kernel
     bool lost = false;
     for (uint32_t i = 0; i < steps; i++) {
       const uint32_t st = (it + i) % NS, pi = (from + i) * KP;
-      if (!tc::mbar_wait(&full[st], ((it + i) / NS) & 1u, &abort_flag, j.err, 0x4a1u, j.polls)) lost = true;
+      if (!tc::mbar_wait(&full[st], ((it + i) / NS) & 1u, &abort_flag, j.err, 0x4a1u, polls)) lost = true;
       const uint8_t *stage = ring + st * C::kStage;
       uint32_t key0[KP], ok[KP];
 #pragma unroll
@@ -604,7 +604,9 @@ p0_status attn_launch(p0_ctx *c, AttnJob &j) {
   if (st) return st;
   j.desc = (uint4 *)ws;
   j.part = (float *)(j.desc + G);
-  launch_dep(kern, dim3(G), dim3(C::kThreads), smem, c->stream, j);
+  const char *limit = getenv("P0MM_KV4_POLLS");   // for tests of what follows a wait that gives up
+  const uint32_t polls = limit ? (uint32_t)strtoul(limit, nullptr, 10) : P0_SPIN_LIMIT;
+  launch_dep(kern, dim3(G), dim3(C::kThreads), smem, c->stream, j, polls);
   if ((st = p0_launched(c, "kv4Attn"))) return st;
   launch_dep(kv4_attn_join_kernel<D, F32, C::kRows>, dim3(G, C::kRows), dim3(256), 0, c->stream, j);
   return p0_launched(c, "kv4Attn join");
@@ -649,8 +651,6 @@ extern "C" p0_status p0_kv4_attn(p0_ctx *c, const p0_kv4_attn_args *a) {
   j.sinks = a->sinks < most ? a->sinks : most;
   j.scale = a->scale != 0.0f ? a->scale : 1.0f;
   j.err = c->d_err;
-  const char *polls = getenv("P0MM_KV4_POLLS");   // for tests of what follows a wait that gives up
-  j.polls = polls ? (uint32_t)strtoul(polls, nullptr, 10) : P0_SPIN_LIMIT;
   // the kernels count query rows and items (pages of row blocks) in 32 bits
   const uint64_t rows = (uint64_t)a->n * j.hpg;
   if (rows > 0x7fffffffu || (rows / 8 + a->kv.rows + 1) * a->kv.nkv * a->kv.table_ld > 0xffffffffull)

@@ -11,7 +11,7 @@ struct AttnJob {
   uint32_t hpg, window, sinks, units;   // units: of a row block (KV heads; times the parts that an output row is cut into)
   float scale;
   bool qbox;          // the prompt form: q has a tensor map
-  uint32_t *err, polls;   // polls: after which the waits of the form for few rows give up
+  uint32_t *err;
   float *part;        // [grid][2][rows of a block][D + 2]
   uint4 *desc;        // [grid]: (1 + last run, b, first row, KV head) of the unit that this run begins and others end
   uint8_t *wide;      // the prompt form: pages as f16 tiles
