@@ -362,10 +362,11 @@ p0_status p0_kv4_get(p0_ctx *ctx, const p0_kv4_rows_args *a);
 /* kv4Attn: attention of the n newest tokens (laid out over the sequences as for kv4Put) with nh query heads, query head
  * h reading KV head h / (nh / nkv): out = softmax over the visible keys of scale * (q . k), times v. The token at
  * position p sees key j <= p if window is 0, j > p - window or j < sinks. A token that sees nothing gives zeros. What
- * the memory of unseen keys holds does not matter. Tokens of no sequence keep what out held; a cu (it should not decrease)
- * that gives the sequences more than n tokens between them computes nothing. out may be q itself (with q's offset and
- * strides); otherwise they share no element. scale 0 = 1. Scores are held in f32. type P0_F32: q, out f32, q to about 2^-22 of
- * the row's largest |q|, P to about 2^-22; P0_F16: q, out f16, P rounded to f16.
+ * the memory of keys that no token of the call sees holds does not matter; the others' values are finite, as kv4Put writes
+ * them. Tokens of no sequence keep what out held; a cu (it should not decrease) that gives the sequences more than n tokens
+ * between them computes nothing. out may be q itself (with q's offset and strides); otherwise they share no element. scale
+ * 0 = 1. Scores are held in f32. type P0_F32: q, out f32, q to about 2^-22 of the row's largest |q|, P to about 2^-22; P0_F16:
+ * q, out f16, P rounded to f16.
  * f16 calls with many new tokens hold the pages that they may see (whole table rows, or what window and sinks let them
  * see) as f16 in the context's workspace, 256 * D bytes a page and KV head, up to 4 GB, which it then keeps; beyond that, or
  * where the device has no such memory left, they are computed without, more slowly. */

@@ -11,7 +11,8 @@ hypotheses at once, on the device from one step to the next.
 Layers of one kind (full, sliding) share a page table; a page holds every layer of the kind. Sliding layers see the last
 `window` tokens and the first `sinks`; kvStep gives back the pages that no later token sees. The prompt goes through row 0
 alone (the other rows are empty: nothing is stored or seen for them); the first selection then forks it to every row.
-Nothing is read back but the chosen (parent, token) pairs at the end, from which the sequences follow."""
+Nothing is read back but the chosen (parent, token) pairs at the end, from which the sequences follow, and what the steps
+were short of (then, and every LOG steps)."""
 import numpy as np
 
 from . import _lib as L

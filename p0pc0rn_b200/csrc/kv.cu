@@ -72,9 +72,10 @@ constexpr int kT = 256;
 // ---------------------------------------------------------------- kv4Put / kv4Get
 // A warp takes 8 consecutive tokens of one head's K or V and a run of its groups of 32 dims (a lane: one token's code word, 8
 // dims), so that it finds the tokens' places once, reads or writes whole runs of 32 values and, where the tokens are
-// neighbours in a page, 128 contiguous bytes of codes. 8192 tokens of 2 heads of 256, f32: 19.0 us, 2.9 TB/s, bound by
-// each warp's chain of instructions (f16, half the bytes, takes as long): places, extent, rounded division, codes. 8 tokens: 5.1 us,
-// the launch.
+// neighbours in a page, 128 contiguous bytes of codes. 8192 tokens of 2 heads of 256: kv4Put of f32 13.6 us, 2.9 TB/s (f16, half the
+// bytes read: 11.8), kv4Get to f16 6.7 us, 3.3 TB/s. kv4Put has 5 warps a scheduler (72 registers) and uses 53 % of the issue slots; of
+// the cycles between a warp's instructions 36 % are waits for its loads, 20 % for the instruction before (places, extent, rounded
+// division, codes: a chain). kv4Get: 51 % and 10 warps, half the cycles waits for loads. 8 tokens: 4.5 us each, the launch.
 constexpr float kHold = 60000.0f;   // 15 * f16(range / 15) + f16(-60000) stays finite in f16
 constexpr uint32_t kGroups = 4;     // groups whose values a lane holds at a time
 

@@ -18,9 +18,11 @@
 //   S = Q K^T   a warp takes 8 or 16 of the item's keys
 //   P = exp(S - m) through shared memory, m over all warps
 //   O += P V    a warp takes 64 (or 32) dims and a share of the keys; the shares meet when the unit ends
-// The instructions per code, about 2 for each of K and V, bound a batch of long contexts (3500 warp instructions a page of 256
-// dims, 2.2 a cycle): 32 contexts up to 65500 keys, 8 f32 heads on one of 256, 112 us, 3.1 TB/s of records, 57 % of the issue slots. Small calls are two
-// launches and their latencies: 8 contexts in a window of 512, 11.3 us. 4 x 8 tokens, 8190 keys, 8 f32 heads on 2 of 512: 54 us.
+// A batch of long contexts is bound by the instructions per code, about 2 for each of K and V (3500 warp instructions a page of 256
+// dims, 2.2 a cycle), and by what 16 warps an SM, as many as their registers allow, leave of the issue slots: the two barriers an
+// item are a quarter of the cycles between a warp's instructions. 32 contexts up to 65500 keys, 8 f32 heads on one of 256: 114 us,
+// 3.1 TB/s of records, 56 % of the issue slots. Small calls are two launches, with grids for the whole GPU, and their latencies: 8
+// contexts in a window of 512, 11.7 us. 4 x 8 tokens, 8190 keys, 8 f32 heads on 2 of 512: 55 us.
 //
 // Precision. f32 queries and outputs: q and P are split into f16 high and low parts (about 22 bits) in rows r and r + 8
 // of the fragments; a row of q is brought to [2^14, 2^15) by a power of two first, which its scores give back, so that
@@ -619,7 +621,8 @@ template <int D, bool F32, int KP>
 p0_status pick(p0_ctx *c, AttnJob &j, uint32_t frags) {
   // One fragment and room for many pages (the lengths are on the device: what the table and the window allow decides): four
   // warps and a page an item, four CTAs to an SM that do not wait for one another at the barriers. 32 contexts up to 65500
-  // keys: 117 us, with eight warps and two pages 123 (112 since); 8 contexts of 10 pages: 14.1 and 12.2
+  // keys: 117 us, with eight warps and two pages 123 (114 since); 8 contexts of 10 pages: 14.1 and 12.2, which is what short
+  // contexts in wide tables lose
   const uint64_t most = j.window ? min((uint64_t)j.v.ld, (uint64_t)j.window / kPage + 2 + (j.sinks + kPage - 1) / kPage) : j.v.ld;
   if constexpr (D < 512)
     if (frags <= 1 && most * j.v.rows * j.v.nkv >= 16ull * c->sm_count) return attn_launch<D, F32, 8, 1, 1, 4>(c, j);

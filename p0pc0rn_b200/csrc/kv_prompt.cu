@@ -29,8 +29,8 @@
 // 4100 cycles a tile of 256 dims, by a thread each 2800, the softmax's chain (load 64 scores, maximum, barrier, exponentials, store P)
 // with one S buffer. A unit's end (the last P V, output through shared memory) costs another 6000 to 8000 cycles, under which the
 // next unit's K, q and first S run; the widening takes 7 us, the join of parts 8 to 10. 3 sequences with 2048 new of up to
-// 5003 tokens, 8 heads of 256 dims: 110 us, 0.98 PFLOP/s (125 in long runs at the power limit); 4 with 1500 of 6001, 16 heads of 128 on 4, window 1024: 127 us,
-// 0.35 PFLOP/s (units of 9 tiles); 2048 of 6000, 8 heads of 512: 250 us, 0.67 PFLOP/s.
+// 5003 tokens, 8 heads of 256 dims: 119 us, 0.91 PFLOP/s (132 in long runs at the power limit); 4 with 1500 of 6001, 16 heads of 128 on 4, window 1024: 131 us,
+// 0.34 PFLOP/s (units of 9 tiles); 2048 of 6000, 8 heads of 512: 246 us, 0.68 PFLOP/s. Where the compiler places the code decides 5 % of these.
 #include "kv_attn.cuh"
 
 namespace {
@@ -761,7 +761,7 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes, bool *taken)
 
 // Taken where the sequences have 64 query rows a KV head on average (128 at 512 dims): one sequence of 1200 keys, 64 rows of 256
 // dims, 22 us against 32 of the form for few rows; 24 of 6000 keys, 70 against 76; 32 rows of 1200 keys, 23 against 19. (One
-// sequence of 30000 keys and 64 rows: 57 against 50; 512 dims, 24 of 6000, 64 rows: 165 against 114, 256 rows: 152 against 269.)
+// sequence of 30000 keys and 64 rows: 46 against 50; 512 dims, 24 of 6000, 64 rows: 165 against 114, 256 rows: 152 against 269.)
 // And where the pages that the call may see take no more than 4 GB as f16: of each sequence all that its table row holds, or with a
 // window those of the sinks, of the window before its first new token, and of its new tokens (T / 64 and a page's ends more).
 p0_status kv4_attn_prompt(p0_ctx *c, AttnJob &j, bool *taken) {

@@ -1,7 +1,8 @@
 // launch.cuh -- programmatic dependent launch for the small operator kernels: every kernel is launched so that it may
 // start while the kernel ahead of it is still running; it waits for that kernel (griddepcontrol.wait: all prerequisite
-// grids complete, their writes visible) before it reads anything, then lets the kernel after it launch at once. Without
-// such a launch both are no-ops. And the encoder of tensor maps.
+// grids complete, their writes visible) before it reads anything, then lets the kernel after it launch at once (dep_enter;
+// one kernel does it in parts of its own: kv4_prompt_kernel reads early what the kernel before the last one left, and one warp
+// of each CTA waits for the last one). Without such a launch both are no-ops. And the encoder of tensor maps.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
