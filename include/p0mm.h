@@ -424,6 +424,71 @@ typedef struct {
 } p0_beam_args;
 p0_status p0_beam_select(p0_ctx *ctx, const p0_beam_args *a);
 
+/* ---------------------------------------------------------------------------------------------- matrices in 8 bits */
+/* Activations and weights in e4m3 with an f32 scale for each block of 128, for matmuls that the tensor cores bound (prompts, DiT
+ * blocks): twice the products a second of f16, half its activation bytes. No counterpart in the reference (its activations are f16).
+ * A matrix of R rows and K columns: codes u8, element (r, k) at off + r * ld + k (ld 0 = K up to a multiple of 16; off and ld
+ * multiples of 16 bytes from a 16-byte aligned buffer), and scales f32 at s_off (floats) of s. A code stands for its e4m3 value times
+ * its block's scale. A block is
+ *   P0_F8_ROW   128 columns of a row, scale [k / 128][r], rows of s_ld >= R (0 = R up to a multiple of 4): activations
+ *   P0_F8_TILE  128 x 128, scale [r / 128][k / 128], rows of s_ld >= K / 128 rounded up (0 = that): weights
+ * (the last block of a row or column may be short). Quantised per block: a = its largest |x|, at least 2^-100 and at most the largest f32,
+ * s = a / 448, code = e4m3(x * (448 / a)), each step rounded to nearest in f32, halves to even; NaN becomes the code of NaN and does not
+ * count for a; an infinity becomes +-448. Codes beyond column K of a row and scales beyond R are never read nor written. */
+enum { P0_F8_ROW = 0, P0_F8_TILE = 1 };
+#define P0_F8_MAX_D 16384u
+typedef struct {
+  p0_buf buf; uint64_t off; uint32_t ld;
+  p0_buf s; uint64_t s_off; uint32_t s_ld;
+} p0_f8;
+
+/* packF8: M rows of K values (type P0_F32 or P0_F16; value (m, k) at x_off + m * x_ld + k in elements, x_ld 0 = K) -> y, in blocks of
+ * `block`. x and y share no byte. */
+typedef struct {
+  p0_buf x; uint64_t x_off; uint32_t x_ld;
+  uint32_t type, M, K, block;
+  p0_f8 y;
+} p0_pack_f8_args;
+p0_status p0_pack_f8(p0_ctx *ctx, const p0_pack_f8_args *a);
+
+/* normF8: the residual's addition and a root-mean-square norm, per row m < M of D <= P0_F8_MAX_D, with codes as the output:
+ *   tv = sum over j < t_n (0 = 1) of t[t_off + j * t_ld + m * t_ldm + i]   in order, f32 (t absent: 0; t_ldm 0 = D, t_ld 0 = M * t_ldm)
+ *   tv = tv * rsqrt(mean tv^2 + eps) * pw[pw_off + i]                      if pw is given (the norm behind a sublayer, as in normadd)
+ *   h  = (x + tv) * scale                                                  rounded to `type`: the new stream
+ *   st[st_off + m] = r = rsqrt(mean h^2 + eps)                             (st optional), of the rounded h
+ *   y  = codes of (h * r) * w[w_off + i]                                   in blocks of P0_F8_ROW
+ * x and h: rows of `type`, at off + m * ld + i in elements (ld 0 = D); h absent: x itself is updated. t: rows of t_type. eps 0 =
+ * 1e-6; scale has no default here (1 adds plainly). Nothing written lies over anything else, but h may be x's rows exactly. */
+typedef struct {
+  p0_buf x; uint64_t x_off; uint32_t x_ld, type;
+  p0_buf t; uint64_t t_off, t_ld; uint32_t t_ldm, t_type, t_n;
+  p0_buf pw; uint32_t pw_off;
+  p0_buf h; uint64_t h_off; uint32_t h_ld;
+  p0_buf w; uint32_t w_off;
+  p0_f8 y;
+  p0_buf st; uint32_t st_off;
+  uint32_t M, D;
+  float eps, scale;
+} p0_norm_f8_args;
+p0_status p0_norm_f8(p0_ctx *ctx, const p0_norm_f8_args *a);
+
+/* gemmF8: Y[m, n] = sum_k X[m, k] * W[n, k] of the values that x (M rows of K, P0_F8_ROW) and w (N rows of K, P0_F8_TILE) stand for:
+ * the products of a block of 128 k are summed in the tensor cores' f32, then scaled and added up in f32.
+ *   P0_F8EPI_F16, _F32      y: rows of f16 or f32, element (m, n) at y.off + m * y.ld + n (elements, y.ld 0 = N; y.s not used);
+ *                           with bv: + bv[bv_off + n] before the rounding
+ *   P0_F8EPI_SWIGLU, _GEGLU y: codes (P0_F8_ROW) of act(X W^T) * (X U^T), u as w; act = silu or the tanh form of gelu, in f32
+ * The operator needs no packed form of its own: x, w and u are read as packF8 and normF8 write them. y shares no byte with the inputs.
+ * Gated calls with few tokens keep M * N floats in the context's workspace; the first call of a size may grow it (which waits for the
+ * stream), so it should not sit inside a stream capture. */
+enum { P0_F8EPI_F16 = 0, P0_F8EPI_F32 = 1, P0_F8EPI_SWIGLU = 2, P0_F8EPI_GEGLU = 3 };
+typedef struct {
+  p0_f8 x, w, u;
+  uint32_t M, N, K, epi;
+  p0_buf bv; uint32_t bv_off;
+  p0_f8 y;
+} p0_gemm_f8_args;
+p0_status p0_gemm_f8(p0_ctx *ctx, const p0_gemm_f8_args *a);
+
 /* ---------------------------------------------------------------------------------------------- quantiser */
 /* packQ4 (engine/kcheck.js:22-38) on the device, bit for bit: W f32 [N][ldw] at w_off (bytes) -> q4g32a.t64 records
  * (N*K*5/8 bytes) at out_off. N % 64 == 0, K % 32 == 0. The dequantised value of code q is q*s + mn. */

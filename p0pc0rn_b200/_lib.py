@@ -20,7 +20,10 @@ ACT = {"silu": 0, "gelu": 1}
 XPRO = {"f16": 0, "lnmod": 1, "rms": 2}
 P0_ROPE_INTER, P0_ROPE_HALF = 0, 1
 TYPE = {"f32": 0, "f16": 1}
+F8BLOCK = {"row": 0, "tile": 1}
+F8EPI = {"f16": 0, "f32": 1, "swiglu": 2, "geglu": 3}
 P0_KV_PAGE, P0_KV_NONE = 64, 0xffffffff
+P0_F8_MAX_D = 16384
 
 # every symbol include/p0mm.h declares
 EXPORTS = ["p0_init", "p0_destroy", "p0_set_stream", "p0_set_overlap", "p0_last_error", "p0_stats", "p0_buffer", "p0_wrap", "p0_upload", "p0_read",
@@ -28,7 +31,8 @@ EXPORTS = ["p0_init", "p0_destroy", "p0_set_stream", "p0_set_overlap", "p0_last_
            "p0_dequant_f16", "p0_version", "p0_argmaxM", "p0_embed", "p0_normadd", "p0_dhead",
            "p0_upload_file", "p0_qkrope", "p0_attn_dec", "p0_wait_selftest",
            "p0_chain_begin", "p0_chain_end", "p0_chain_run", "p0_chain_info", "p0_chain_free", "p0_copy",
-           "p0_kv4_put", "p0_kv4_get", "p0_kv4_attn", "p0_kv_step", "p0_kv_compact", "p0_beam_select"]
+           "p0_kv4_put", "p0_kv4_get", "p0_kv4_attn", "p0_kv_step", "p0_kv_compact", "p0_beam_select",
+           "p0_pack_f8", "p0_norm_f8", "p0_gemm_f8"]
 P0_NOALLOC_SCRATCH_BYTES = 16 << 20   # include/p0mm.h
 P0_OVERLAP_WEIGHTS = 1
 P0_NOALLOC_COUNTER_BYTES = 64 << 10
@@ -130,6 +134,26 @@ class p0_beam_args(ctypes.Structure):
                 ("V", _u32), ("eos", _u32), ("parent", p0_buf), ("token", p0_buf), ("score_out", p0_buf), ("fin_out", p0_buf)]
 
 
+class p0_f8(ctypes.Structure):
+    _fields_ = [("buf", p0_buf), ("off", ctypes.c_uint64), ("ld", _u32), ("s", p0_buf), ("s_off", ctypes.c_uint64), ("s_ld", _u32)]
+
+
+class p0_pack_f8_args(ctypes.Structure):
+    _fields_ = [("x", p0_buf), ("x_off", ctypes.c_uint64), ("x_ld", _u32), ("type", _u32), ("M", _u32), ("K", _u32), ("block", _u32), ("y", p0_f8)]
+
+
+class p0_norm_f8_args(ctypes.Structure):
+    _fields_ = [("x", p0_buf), ("x_off", ctypes.c_uint64), ("x_ld", _u32), ("type", _u32), ("t", p0_buf), ("t_off", ctypes.c_uint64),
+                ("t_ld", ctypes.c_uint64), ("t_ldm", _u32), ("t_type", _u32), ("t_n", _u32), ("pw", p0_buf), ("pw_off", _u32), ("h", p0_buf),
+                ("h_off", ctypes.c_uint64), ("h_ld", _u32), ("w", p0_buf), ("w_off", _u32), ("y", p0_f8), ("st", p0_buf), ("st_off", _u32), ("M", _u32),
+                ("D", _u32), ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
+class p0_gemm_f8_args(ctypes.Structure):
+    _fields_ = [("x", p0_f8), ("w", p0_f8), ("u", p0_f8), ("M", _u32), ("N", _u32), ("K", _u32), ("epi", _u32), ("bv", p0_buf), ("bv_off", _u32),
+                ("y", p0_f8)]
+
+
 _lib = None
 
 
@@ -182,6 +206,9 @@ def load():
     L.p0_kv_step.argtypes = [vp, ctypes.POINTER(p0_kv_step_args)]
     L.p0_kv_compact.argtypes = [vp, ctypes.POINTER(p0_kv_compact_args)]
     L.p0_beam_select.argtypes = [vp, ctypes.POINTER(p0_beam_args)]
+    L.p0_pack_f8.argtypes = [vp, ctypes.POINTER(p0_pack_f8_args)]
+    L.p0_norm_f8.argtypes = [vp, ctypes.POINTER(p0_norm_f8_args)]
+    L.p0_gemm_f8.argtypes = [vp, ctypes.POINTER(p0_gemm_f8_args)]
     L.p0_version.restype = ctypes.c_char_p
     for name in EXPORTS:
         if name != "p0_version":

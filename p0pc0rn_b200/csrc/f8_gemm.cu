@@ -1,0 +1,187 @@
+// f8_gemm.cu -- gemmF8: products of matrices in 8 bits. The entry point, and the form for few tokens.
+//
+// Y[m, n] = sum over blocks b of 128 k:  xs[b, m] * ws[n / 128, b] * sum_{k in b} xc[m, k] wc[n, k].
+//
+// Few tokens: bound by the weights' bytes. A CTA computes 16 weight rows; its warps take blocks of k in turn, a lane loads 16
+// bytes of two rows at a time straight into the fragments of mma.sync.m16n8k32 (e4m3, f32 sums): the order of k inside a
+// fragment is free as long as both operands share it, so 16 consecutive bytes serve two instructions. Tokens are the n side,
+// loaded the same way. Each block's sums are scaled and added in f32; the warps' parts meet in shared memory, in order.
+#include "f8.cuh"
+
+namespace {
+
+constexpr int kT = 256, kW = kT / 32;
+
+struct GemmJob {
+  F8Mat x, w, u;
+  const float *bv;
+  uint8_t *y;              // f16 or f32 rows of y_ld
+  uint64_t y_ld;
+  uint32_t M, N, K, KB, epi;
+};
+
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// codes k .. k + 15 of a row of K (a 16-byte boundary); zeros beyond it
+__device__ __forceinline__ uint4 codes16(const uint8_t *row, uint32_t k, uint32_t K) {
+  if (k + 16u <= K) return *reinterpret_cast<const uint4 *>(row + k);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  for (uint32_t i = 0; k + i < K; i++) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3u));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// NT: groups of 8 tokens; MATS: 2 with u
+template <int NT, int MATS>
+__global__ void __launch_bounds__(kT) f8_few_kernel(GemmJob j) {
+  dep_enter();
+  constexpr int kOut = NT * 128;                 // outputs of a matrix: token * 16 + row
+  __shared__ float red[kW][MATS * kOut];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, c = lane & 3u;
+  const uint32_t nblk = (j.N + 15u) / 16u, n0 = blockIdx.x % nblk * 16u, m0 = blockIdx.x / nblk * (8u * NT);
+  float acc[MATS][NT][4];
+#pragma unroll
+  for (int a = 0; a < MATS; a++)
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[a][t][i] = 0.0f;
+  const uint64_t r0 = min(n0 + g, j.N - 1u), r1 = min(n0 + g + 8u, j.N - 1u);   // rows beyond the last: their sums are not stored
+  for (uint32_t kb = warp; kb < j.KB; kb += kW) {
+    const uint32_t k = kb * kF8Block + c * 16u;
+    uint4 x[NT][2];
+    float xs[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const uint32_t m = m0 + t * 8u + g;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        x[t][h] = m < j.M ? codes16(j.x.q + (uint64_t)m * j.x.ld, k + h * 64u, j.K) : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t mc = m0 + t * 8u + 2u * c + h;
+        xs[t][h] = mc < j.M ? j.x.s[(uint64_t)kb * j.x.s_ld + mc] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < MATS; a++) {
+      const F8Mat &w = a ? j.u : j.w;
+      uint4 w0[2], w1[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        w0[h] = codes16(w.q + r0 * w.ld, k + h * 64u, j.K);
+        w1[h] = codes16(w.q + r1 * w.ld, k + h * 64u, j.K);
+      }
+      const float ws = w.s[(uint64_t)(n0 / kF8Block) * w.s_ld + kb];
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          mma_e4m3(d, w0[h].x, w1[h].x, w0[h].y, w1[h].y, x[t][h].x, x[t][h].y);
+          mma_e4m3(d, w0[h].z, w1[h].z, w0[h].w, w1[h].w, x[t][h].z, x[t][h].w);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[a][t][i] = fmaf(d[i], xs[t][i & 1] * ws, acc[a][t][i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < MATS; a++)
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) red[warp][a * kOut + (t * 8 + 2 * c + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[a][t][i];
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < kOut; e += kT) {
+    const uint32_t m = m0 + e / 16u, n = n0 + e % 16u;
+    if (m >= j.M || n >= j.N) continue;
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kW; w++) y += red[w][e];
+    if (MATS == 2) {
+      float u = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kW; w++) u += red[w][(MATS - 1) * kOut + e];
+      y = f8_gate(y, j.epi) * u;
+    } else if (j.bv) {
+      y += j.bv[n];
+    }
+    const uint64_t at = (uint64_t)m * j.y_ld + n;
+    if (j.epi == P0_F8EPI_F16) reinterpret_cast<__half *>(j.y)[at] = __float2half_rn(y);
+    else reinterpret_cast<float *>(j.y)[at] = y;
+  }
+}
+
+p0_status few_launch(p0_ctx *c, const GemmJob &j, const char *op) {
+  const uint32_t nblk = (j.N + 15u) / 16u;
+  const bool gated = j.epi >= P0_F8EPI_SWIGLU;
+  auto go = [&](auto kern, uint32_t tok) {
+    launch_dep(kern, dim3((unsigned)(nblk * ((j.M + tok - 1u) / tok))), dim3(kT), 0, c->stream, j);
+  };
+  if (j.M <= 8) gated ? go(f8_few_kernel<1, 2>, 8) : go(f8_few_kernel<1, 1>, 8);
+  else if (j.M <= 16) gated ? go(f8_few_kernel<2, 2>, 16) : go(f8_few_kernel<2, 1>, 16);
+  else gated ? go(f8_few_kernel<4, 2>, 32) : go(f8_few_kernel<4, 1>, 32);
+  return p0_launched(c, op);
+}
+
+}  // namespace
+
+extern "C" p0_status p0_gemm_f8(p0_ctx *c, const p0_gemm_f8_args *a) {
+  if (!c || !a) return P0_EINVAL;
+  const char *op = "gemmF8";
+  if (a->epi > P0_F8EPI_GEGLU) return p0_fail(c, P0_EINVAL, "%s: epilogue %u", op, a->epi);
+  const bool gated = a->epi >= P0_F8EPI_SWIGLU;
+  if (gated && !a->u.buf.id) return p0_fail(c, P0_EINVAL, "%s: a gated epilogue needs u", op);
+  if (!gated && a->u.buf.id) return p0_fail(c, P0_EINVAL, "%s: u without a gated epilogue", op);
+  if (gated && a->bv.id) return p0_fail(c, P0_EINVAL, "%s: bv with a gated epilogue", op);
+  if (!a->M || !a->N) return P0_OK;
+  if (!a->K) return p0_fail(c, P0_EINVAL, "%s: K is 0", op);
+  const uint64_t M = a->M, N = a->N, K = a->K;
+  if (K > (1u << 24) || N > (1u << 24) || M > (1u << 24) || ((N + 15) / 16) * ((M + 7) / 8) >= (1ull << 31))
+    return p0_fail(c, P0_EINVAL, "%s: M %u, N %u, K %u", op, a->M, a->N, a->K);
+  GemmJob j{};
+  j.M = a->M;
+  j.N = a->N;
+  j.K = a->K;
+  j.KB = (a->K + kF8Block - 1) / kF8Block;
+  j.epi = a->epi;
+  p0_status st;
+  if ((st = f8_view(c, a->x, M, K, false, op, "x", &j.x))) return st;
+  if ((st = f8_view(c, a->w, N, K, true, op, "w", &j.w))) return st;
+  if (gated && (st = f8_view(c, a->u, N, K, true, op, "u", &j.u))) return st;
+  F8Mat y{};
+  uint64_t yn, ysn = 0;
+  if (gated) {
+    if ((st = f8_view(c, a->y, M, N, false, op, "y", &y))) return st;
+    yn = f8_code_bytes(y, M, N);
+    ysn = f8_scale_bytes(y, M, N, false);
+  } else {
+    const uint8_t *p;
+    uint32_t ld;
+    const uint32_t type = a->epi == P0_F8EPI_F16 ? P0_F16 : P0_F32;
+    if ((st = f8_rows(c, a->y.buf, a->y.off, a->y.ld, M, N, type, op, "y", &p, &ld, nullptr))) return st;
+    j.y = (uint8_t *)p;
+    j.y_ld = ld;
+    yn = ((M - 1) * ld + N) * (type == P0_F16 ? 2 : 4);
+  }
+  P0Range rb;
+  if ((st = p0_range(c, a->bv, (uint64_t)a->bv_off * 4, N * 4, op, "bv", &rb, true))) return st;
+  if ((uintptr_t)rb.base % 4) return p0_fail(c, P0_EALIGN, "%s: bv must be 4-byte aligned", op);
+  j.bv = (const float *)rb.base;
+  const void *yp = gated ? (const void *)y.q : (const void *)j.y;
+  const auto over = [&](const void *p, uint64_t n) { return f8_meet(yp, yn, p, n) || (ysn && f8_meet(y.s, ysn, p, n)); };
+  if (over(j.x.q, f8_code_bytes(j.x, M, K)) || over(j.x.s, f8_scale_bytes(j.x, M, K, false)) || over(j.w.q, f8_code_bytes(j.w, N, K)) ||
+      over(j.w.s, f8_scale_bytes(j.w, N, K, true)) || (gated && (over(j.u.q, f8_code_bytes(j.u, N, K)) || over(j.u.s, f8_scale_bytes(j.u, N, K, true)))) ||
+      (j.bv && over(j.bv, N * 4)) || (gated && f8_meet(y.q, yn, y.s, ysn)))
+    return p0_fail(c, P0_EINVAL, "%s: y must not lie over the inputs", op);
+  DeviceGuard guard(c->device);
+  if (!gated) return few_launch(c, j, op);
+  uint32_t *cnt;
+  void *ws;
+  if ((st = p0_workspace(c, 0, M * N * 4, &cnt, &ws))) return st;
+  j.y = (uint8_t *)ws;
+  j.y_ld = N;
+  if ((st = few_launch(c, j, op))) return st;
+  return f8_pack_rows(c, (const float *)ws, N, a->M, a->N, y, op);
+}

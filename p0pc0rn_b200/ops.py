@@ -301,7 +301,63 @@ def beamSelect(g, a):
     bound(beamSelect, g, a)()
 
 
+# ---------------------------------------------------------------- matrices in 8 bits
+def _f8(m):
+    sc = (m or {}).get("s") or {}
+    m = m or {}
+    return L.p0_f8(_b(m), int(m.get("off") or 0), int(m.get("ld") or 0), _b(sc), int(sc.get("off") or 0), int(sc.get("ld") or 0))
+
+
+def _o(o, k="off"):
+    return int((o or {}).get(k) or 0)
+
+
+def _pack_f8_args(a):
+    x, block = a["x"], a.get("block") or "row"
+    if block not in L.F8BLOCK:
+        raise P0Error(L.P0_EINVAL, "packF8: block %s" % block)
+    return L.p0_pack_f8_args(handle(x["buf"]), _o(x), _o(x, "ld"), _type(a, "packF8"), int(a["M"]), int(a["K"]), L.F8BLOCK[block], _f8(a["y"]))
+
+
+def _norm_f8_args(a):
+    x, t, pw, h, w, st, scale = a["x"], a.get("t"), a.get("pw"), a.get("h"), a["w"], a.get("st"), a.get("scale")
+    return L.p0_norm_f8_args(handle(x["buf"]), _o(x), _o(x, "ld"), _type(a, "normF8"), _b(t), _o(t), _o(t, "ld"), _o(t, "ldm"), _type(t or {}, "normF8"),
+                             _o(t, "n"), _b(pw), _o(pw), _b(h), _o(h), _o(h, "ld"), handle(w["buf"]), _o(w), _f8(a["y"]), _b(st), _o(st), int(a["M"]),
+                             int(a["D"]), float(a.get("eps") or 0.0), 1.0 if scale is None else float(scale))
+
+
+def _gemm_f8_args(a):
+    epi, bv = a.get("epi") or "f16", a.get("bv")
+    if epi not in L.F8EPI:
+        raise P0Error(L.P0_EINVAL, "gemmF8: epilogue %s" % epi)
+    return L.p0_gemm_f8_args(_f8(a["x"]), _f8(a["w"]), _f8(a.get("u")), int(a["M"]), int(a["N"]), int(a["K"]), L.F8EPI[epi], _b(bv), _o(bv), _f8(a["y"]))
+
+
+def packF8(g, a):
+    """a = {x: {buf, off, ld}, type ('f32' | 'f16'), M, K, block ('row' | 'tile'), y}: values as e4m3 codes with a scale for
+    each 128 columns of a row (activations) or each 128 x 128 tile (weights). y = {buf, off, ld, s: {buf, off, ld}} is a matrix
+    in 8 bits (p0_f8 in include/p0mm.h)."""
+    bound(packF8, g, a)()
+
+
+def normF8(g, a):
+    """a = {x: {buf, off, ld}, type, t: {buf, off, type, n, ld, ldm} (optional), pw: {buf, off} (optional), h: {buf, off, ld}
+    (default: x itself), w: {buf, off}, y, st: {buf, off} (optional), M, D, eps, scale (default 1)}: h = (x + t) * scale, t
+    summed over n partial rows and with pw normed first; y = the codes of rms(h) * w, st = the rows' rstd"""
+    bound(normF8, g, a)()
+
+
+def gemmF8(g, a):
+    """a = {x, w, u (gated only), M, N, K, epi, bv: {buf, off} (optional), y}: x [M][K] in blocks of rows times w [N][K] in
+    tiles, all matrices in 8 bits. epi 'f16' (default) | 'f32': y = {buf, off, ld} of that type; 'swiglu' | 'geglu': y = the
+    codes of act(x w^T) * (x u^T)"""
+    bound(gemmF8, g, a)()
+
+
 _BOUND = {
+    packF8: ("p0_pack_f8", _pack_f8_args),
+    normF8: ("p0_norm_f8", _norm_f8_args),
+    gemmF8: ("p0_gemm_f8", _gemm_f8_args),
     kv4Put: ("p0_kv4_put", lambda a: _kv4_rows_args(a, "kv4Put")),
     kv4Get: ("p0_kv4_get", lambda a: _kv4_rows_args(a, "kv4Get")),
     kv4Attn: ("p0_kv4_attn", _kv4_attn_args),
