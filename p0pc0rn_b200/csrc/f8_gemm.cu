@@ -6,19 +6,11 @@
 // bytes of two rows at a time straight into the fragments of mma.sync.m16n8k32 (e4m3, f32 sums): the order of k inside a
 // fragment is free as long as both operands share it, so 16 consecutive bytes serve two instructions. Tokens are the n side,
 // loaded the same way. Each block's sums are scaled and added in f32; the warps' parts meet in shared memory, in order.
-#include "f8.cuh"
+#include "f8_gemm.cuh"
 
 namespace {
 
 constexpr int kT = 256, kW = kT / 32;
-
-struct GemmJob {
-  F8Mat x, w, u;
-  const float *bv;
-  uint8_t *y;              // f16 or f32 rows of y_ld
-  uint64_t y_ld;
-  uint32_t M, N, K, KB, epi;
-};
 
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -176,6 +168,7 @@ extern "C" p0_status p0_gemm_f8(p0_ctx *c, const p0_gemm_f8_args *a) {
       (j.bv && over(j.bv, N * 4)) || (gated && f8_meet(y.q, yn, y.s, ysn)))
     return p0_fail(c, P0_EINVAL, "%s: y must not lie over the inputs", op);
   DeviceGuard guard(c->device);
+  if (M > 64) return f8_tc_launch(c, j, y, op);
   if (!gated) return few_launch(c, j, op);
   uint32_t *cnt;
   void *ws;
