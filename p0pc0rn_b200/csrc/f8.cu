@@ -1,66 +1,69 @@
 // f8.cu -- packF8 (values to e4m3 codes with a scale for each block of 128) and normF8 (residual, RMS norm, codes).
 //
-// Both are bound by memory. Half a warp holds a row's block of 128 columns, eight to a lane: 16-byte loads of f16 (two of f32),
-// the block's maximum by four shuffles, 8-byte stores of codes.
+// Both are bound by memory. Eight lanes hold a row's block of 128 columns, sixteen to a lane (columns 8 l .. and 64 + 8 l ..): 16-byte
+// loads of f16 (two of f32), the block's maximum by three shuffles, 8-byte stores of codes. What a block costs besides (two rounded
+// divisions, its place) is shared by sixteen columns a lane.
 #include "f8.cuh"
 
 namespace {
 
 constexpr int kT = 256;
 
+// eight columns as they lie in memory, and as f32
+template <bool F16>
+struct Raw {
+  uint4 w[F16 ? 1 : 2];
+};
 struct Vals {
   float v[8];
 };
-// x[k .. k + 7] of a row of K; zeros beyond it
+// x[k .. k + 7] of a row of K; zeros beyond it. WIDE: rows start on 16-byte boundaries
 template <bool F16, bool WIDE>
-__device__ __forceinline__ Vals load8(const void *row, uint32_t k, uint32_t K) {
-  Vals r;
+__device__ __forceinline__ Raw<F16> load8(const void *row, uint32_t k, uint32_t K) {
+  Raw<F16> r;
   if (WIDE && k + 8u <= K) {
-    if (F16) {
-      const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __half *>(row) + k);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        r.v[2 * i] = f.x;
-        r.v[2 * i + 1] = f.y;
-      }
-    } else {
-      const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(row) + k);
-      const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(row) + k + 4);
-      r.v[0] = a.x, r.v[1] = a.y, r.v[2] = a.z, r.v[3] = a.w, r.v[4] = b.x, r.v[5] = b.y, r.v[6] = b.z, r.v[7] = b.w;
-    }
+    const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(row) + (uint64_t)k * (F16 ? 2u : 4u));
+    r.w[0] = p[0];
+    if (!F16) r.w[F16 ? 0 : 1] = p[1];
   } else {
+    uint32_t w[8];
 #pragma unroll
     for (uint32_t i = 0; i < 8; i++)
-      r.v[i] = k + i >= K ? 0.0f : F16 ? __half2float(reinterpret_cast<const __half *>(row)[k + i]) : reinterpret_cast<const float *>(row)[k + i];
+      w[i] = k + i >= K ? 0u : F16 ? (uint32_t)reinterpret_cast<const uint16_t *>(row)[k + i] : reinterpret_cast<const uint32_t *>(row)[k + i];
+    if (F16) {
+      r.w[0] = make_uint4(w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16));
+    } else {
+      r.w[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      r.w[F16 ? 0 : 1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
   }
   return r;
 }
-template <bool F16, bool WIDE>
-__device__ __forceinline__ void store8(void *row, uint32_t k, uint32_t K, const Vals &x) {
-  if (WIDE && k + 8u <= K) {
-    if (F16) {
-      uint32_t w[4];
+template <bool F16>
+__device__ __forceinline__ Vals vals(const Raw<F16> &r) {
+  Vals x;
+  const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[F16 ? 0 : 1].x, r.w[F16 ? 0 : 1].y, r.w[F16 ? 0 : 1].z, r.w[F16 ? 0 : 1].w};
+  if (F16) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const __half2 h = __floats2half2_rn(x.v[2 * i], x.v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t *>(&h);
-      }
-      *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(row) + k) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      float *p = reinterpret_cast<float *>(row) + k;
-      *reinterpret_cast<float4 *>(p) = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
-      *reinterpret_cast<float4 *>(p + 4) = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+    for (int i = 0; i < 4; i++) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      x.v[2 * i] = f.x;
+      x.v[2 * i + 1] = f.y;
     }
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 8; i++)
-      if (k + i < K) {
-        if (F16) reinterpret_cast<__half *>(row)[k + i] = __float2half_rn(x.v[i]);
-        else reinterpret_cast<float *>(row)[k + i] = x.v[i];
-      }
+    for (int i = 0; i < 8; i++) x.v[i] = __uint_as_float(w[i]);
   }
+  return x;
+}
+template <bool F16>
+__device__ __forceinline__ void store8(void *row, uint32_t k, uint32_t K, const Vals &x) {
+#pragma unroll
+  for (uint32_t i = 0; i < 8; i++)
+    if (k + i < K) {
+      if (F16) reinterpret_cast<__half *>(row)[k + i] = __float2half_rn(x.v[i]);
+      else reinterpret_cast<float *>(row)[k + i] = x.v[i];
+    }
 }
 // codes of x[k .. k + 7]; rows of codes start on 16-byte boundaries
 __device__ __forceinline__ void store_codes(uint8_t *row, uint32_t k, uint32_t K, const Vals &x, float inv) {
@@ -80,10 +83,10 @@ __device__ __forceinline__ float max8(const Vals &x) {
   for (int i = 0; i < 8; i++) a = fmaxf(a, fabsf(x.v[i]));   // fmaxf leaves NaN aside
   return a;
 }
-// the maximum over half a warp
-__device__ __forceinline__ float half_max(float a) {
+// the maximum over eight lanes
+__device__ __forceinline__ float eight_max(float a) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  for (int o = 4; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
   return a;
 }
 
@@ -92,29 +95,37 @@ struct PackJob {
   const uint8_t *x;
   uint64_t ld;
   uint32_t M, K, KB, units;   // units = M * KB
+  uint32_t magic;             // u / KB = umulhi(u, magic) (+ 1 where the remainder says so) for u < 2^31
   F8Mat y;
 };
 template <bool F16, bool WIDE>
 __global__ void __launch_bounds__(kT) f8_pack_rows_kernel(PackJob j) {
   dep_enter();
-  constexpr uint32_t U = 4;   // blocks of a half warp on their way at once
-  const uint32_t l = threadIdx.x & 15u, es = F16 ? 2u : 4u, halves = gridDim.x * (kT / 16);
-  for (uint64_t u0 = blockIdx.x * (kT / 16) + (threadIdx.x >> 4); __any_sync(0xffffffffu, u0 < j.units); u0 += (uint64_t)halves * U) {
-    Vals x[U];
+  constexpr uint32_t U = F16 ? 4 : 2;   // blocks of eight lanes on their way at once: 128 bytes a lane
+  const uint32_t l = threadIdx.x & 7u, es = F16 ? 2u : 4u, eights = gridDim.x * (kT / 8);
+  for (uint64_t u0 = blockIdx.x * (kT / 8) + (threadIdx.x >> 3); __any_sync(0xffffffffu, u0 < j.units); u0 += (uint64_t)eights * U) {
+    Raw<F16> x[U][2];
     uint32_t m[U], kb[U];
 #pragma unroll
     for (uint32_t i = 0; i < U; i++) {
-      const uint64_t u = u0 + (uint64_t)i * halves;
+      const uint64_t u = u0 + (uint64_t)i * eights;
       const bool here = u < j.units;
-      m[i] = here ? (uint32_t)u / j.KB : 0u;
-      kb[i] = here ? (uint32_t)u - m[i] * j.KB : j.KB;   // beyond the row: zeros, nothing stored
-      x[i] = load8<F16, WIDE>(j.x + (uint64_t)m[i] * j.ld * es, kb[i] * kF8Block + l * 8u, j.K);
+      uint32_t d = j.KB == 1u ? (uint32_t)u : __umulhi((uint32_t)u, j.magic);
+      if ((uint32_t)u - d * j.KB >= j.KB) d++;
+      m[i] = here ? d : 0u;
+      kb[i] = here ? (uint32_t)u - d * j.KB : j.KB;   // beyond the row: zeros, nothing stored
+      const uint8_t *row = j.x + (uint64_t)m[i] * j.ld * es;
+#pragma unroll
+      for (uint32_t g = 0; g < 2; g++) x[i][g] = load8<F16, WIDE>(row, kb[i] * kF8Block + g * 64u + l * 8u, j.K);
     }
 #pragma unroll
     for (uint32_t i = 0; i < U; i++) {
-      const float a = f8_hold(half_max(max8(x[i])));
+      const Vals v[2] = {vals<F16>(x[i][0]), vals<F16>(x[i][1])};
+      const float a = f8_hold(eight_max(fmaxf(max8(v[0]), max8(v[1]))));
       if (kb[i] == j.KB) continue;
-      store_codes(j.y.q + (uint64_t)m[i] * j.y.ld, kb[i] * kF8Block + l * 8u, j.K, x[i], __fdiv_rn(448.0f, a));
+      const float inv = __fdiv_rn(448.0f, a);
+#pragma unroll
+      for (uint32_t g = 0; g < 2; g++) store_codes(j.y.q + (uint64_t)m[i] * j.y.ld, kb[i] * kF8Block + g * 64u + l * 8u, j.K, v[g], inv);
       if (l == 0) j.y.s[(uint64_t)kb[i] * j.y.s_ld + m[i]] = __fdiv_rn(a, 448.0f);
     }
   }
@@ -127,7 +138,7 @@ __global__ void __launch_bounds__(kT) f8_pack_tiles_kernel(PackJob j) {
   __shared__ float red[kT / 32];
   const uint32_t l = threadIdx.x & 15u, es = F16 ? 2u : 4u, nb = blockIdx.x / j.KB, kb = blockIdx.x % j.KB;
   const uint32_t k = kb * kF8Block + l * 8u;
-  Vals x[8];
+  Raw<F16> x[8];
 #pragma unroll
   for (uint32_t i = 0; i < 8; i++) {
     const uint32_t m = nb * kF8Block + i * 16u + (threadIdx.x >> 4);
@@ -135,8 +146,9 @@ __global__ void __launch_bounds__(kT) f8_pack_tiles_kernel(PackJob j) {
   }
   float a = 0.0f;
 #pragma unroll
-  for (uint32_t i = 0; i < 8; i++) a = fmaxf(a, max8(x[i]));
-  a = half_max(a);
+  for (uint32_t i = 0; i < 8; i++) a = fmaxf(a, max8(vals<F16>(x[i])));
+  a = eight_max(a);
+  a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 8));
   a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 16));
   if ((threadIdx.x & 31u) == 0) red[threadIdx.x >> 5] = a;
   __syncthreads();
@@ -147,119 +159,263 @@ __global__ void __launch_bounds__(kT) f8_pack_tiles_kernel(PackJob j) {
 #pragma unroll
   for (uint32_t i = 0; i < 8; i++) {
     const uint32_t m = nb * kF8Block + i * 16u + (threadIdx.x >> 4);
-    if (m < j.M) store_codes(j.y.q + (uint64_t)m * j.y.ld, k, j.K, x[i], inv);
+    if (m < j.M) store_codes(j.y.q + (uint64_t)m * j.y.ld, k, j.K, vals<F16>(x[i]), inv);
   }
   if (threadIdx.x == 0) j.y.s[(uint64_t)nb * j.y.s_ld + kb] = __fdiv_rn(a, 448.0f);
 }
 
 // ---------------------------------------------------------------- normF8
 // tv = the sum of the partial rows in order; with pw: tv * rsqrt(mean tv^2 + eps) * pw; h = (x + tv) * scale, rounded to the
-// stream's type; st = rsqrt(mean h^2 + eps); codes of (h * st) * w. A row is held in registers by blockDim.x threads, NB blocks
-// to a half warp; blockDim.y rows a CTA.
+// stream's type; st = rsqrt(mean h^2 + eps); codes of (h * st) * w. blockDim.x threads hold a row, 16 columns each, and take rows in
+// turn (blockDim.y of them a CTA). Rows that start on 16 bytes come through shared memory (RING): every thread copies (cp.async) what
+// it will read itself, up to two rows ahead, so that nothing waits for another thread and no register holds what is on its way. With the
+// next row in registers instead, few CTAs fit an SM (190 us for 32760 rows of 2240 in f16), and loads of the weights, which return in
+// order behind the next row's, held up each row.
 struct NormJob {
   const uint8_t *x, *t;
   uint8_t *h;
   const float *pw, *w;
   float *st;
   uint64_t x_ld, t_ld, t_ldm, h_ld;
-  uint32_t parts, M, D;
+  uint32_t parts, M, D, nbuf;   // nbuf: rows that a thread has room for
   float eps, scale;
-  bool store;
+  bool store, wsm;              // wsm: the norms' weights are kept in shared memory
   F8Mat y;
 };
-// the sum of one float per thread over a row's threads
+// the sum of one float per thread over a row's threads; red: a place for its warps that no sum since the last but one has used
 __device__ __forceinline__ float row_sum(float v, float *red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   const uint32_t warps = blockDim.x >> 5;
-  if (warps == 1) return v;
-  float *r = red + threadIdx.y * warps;
-  if ((threadIdx.x & 31u) == 0) r[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.0f;
-  for (uint32_t i = 0; i < warps; i++) s += r[i];
-  return s;
+  if (warps == 1u) return v;
+  if ((threadIdx.x & 31u) == 0) red[threadIdx.x >> 5] = v;
+  asm volatile("bar.sync %0, %1;" ::"r"(1u + threadIdx.y), "r"(blockDim.x) : "memory");
+  // the warps' sums, one a lane, by the same tree in every warp
+  v = (threadIdx.x & 31u) < warps ? red[threadIdx.x & 31u] : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
-template <bool XF16, bool TF16, bool WIDE, int NB>
-__global__ void __launch_bounds__(1024) f8_norm_kernel(NormJob j) {
-  dep_enter();
-  __shared__ float red[2][32];
-  const uint32_t l = threadIdx.x & 15u, half = threadIdx.x >> 4, halves = blockDim.x >> 4;
-  const uint32_t m = blockIdx.x * blockDim.y + threadIdx.y;
-  const bool here = m < j.M;
-  const uint32_t mr = here ? m : j.M - 1u, D = here ? j.D : 0u;   // a row beyond the last one: nothing is read or stored
-  const uint8_t *xr = j.x + (uint64_t)mr * j.x_ld * (XF16 ? 2u : 4u);
-  Vals h[NB], tv[NB];
+__device__ __forceinline__ void copy16(uint4 *dst, const uint8_t *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+// x += t, times scale, rounded to f16 where the stream has that type; what is stored of it
+template <bool F16>
+__device__ __forceinline__ Raw<F16> settle(Vals &x, const Vals &t, float scale) {
+  Raw<F16> r;
+  uint32_t w[8];
 #pragma unroll
-  for (int b = 0; b < NB; b++) h[b] = load8<XF16, WIDE>(xr, (half + b * halves) * kF8Block + l * 8u, D);
+  for (int i = 0; i < 8; i++) x.v[i] = __fadd_rn(x.v[i], t.v[i]);
+  if (scale != 1.0f)
 #pragma unroll
-  for (int b = 0; b < NB; b++) tv[b] = Vals{};
-  for (uint32_t p = 0; p < j.parts; p++) {
-    const uint8_t *tr = j.t + ((uint64_t)p * j.t_ld + (uint64_t)mr * j.t_ldm) * (TF16 ? 2u : 4u);
+    for (int i = 0; i < 8; i++) x.v[i] = __fmul_rn(x.v[i], scale);
+  if (F16) {
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-      const Vals t = load8<TF16, WIDE>(tr, (half + b * halves) * kF8Block + l * 8u, D);
-#pragma unroll
-      for (int i = 0; i < 8; i++) tv[b].v[i] += t.v[i];
+    for (int i = 0; i < 4; i++) {
+      const __half2 h = __floats2half2_rn(x.v[2 * i], x.v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+      const float2 f = __half22float2(h);
+      x.v[2 * i] = f.x;
+      x.v[2 * i + 1] = f.y;
     }
+    r.w[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = __float_as_uint(x.v[i]);
+    r.w[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    r.w[F16 ? 0 : 1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
-  if (j.pw) {
+  return r;
+}
+enum { kScalar = 0, kDirect = 1, kRing = 2 };   // rows that start anywhere; on 16 bytes, loaded as they are needed; ahead
+template <bool XF16, bool TF16, int MODE, bool POST>
+__global__ void __launch_bounds__(MODE == kDirect ? 512 : 1024) f8_norm_kernel(NormJob j) {
+  dep_enter();
+  constexpr bool RING = MODE == kRing, WIDE = MODE != kScalar;
+  constexpr uint32_t xs = XF16 ? 2 : 4, ts = TF16 ? 2 : 4, XC = xs, TC = ts;   // 16 columns are as many chunks of 16 bytes as a value has bytes
+  extern __shared__ uint4 sm[];
+  __shared__ float red[3][64];   // of each sum in turn, [row of the CTA][warp]
+  const uint32_t l = threadIdx.x & 7u, kb = threadIdx.x >> 3, k0 = kb * kF8Block + l * 8u, step = gridDim.x * blockDim.y;
+  const uint32_t T = blockDim.x * blockDim.y;
+  const bool in[2] = {k0 < j.D, k0 + 64u < j.D};   // where rows start on 16 bytes, D is a multiple of 8
+  uint32_t turn = 0;
+  const auto place = [&]() {
+    float *p = red[turn] + threadIdx.y * (blockDim.x >> 5);
+    turn = turn == 2u ? 0u : turn + 1u;
+    return p;
+  };
+  // shared memory: places of rows [x | t], each warp's 512 columns together, then (wsm) [chunk][thread of a row] of w and pw. Columns beyond D stay zeros
+  const uint32_t lane = threadIdx.x & 31u, wx = (threadIdx.x >> 5) * 32u * XC, wt = blockDim.x * XC + (threadIdx.x >> 5) * 32u * TC;   // a warp's chunks of a place
+  uint4 *const own = sm + threadIdx.y * blockDim.x * (XC + TC), *const wat = sm + (RING ? j.nbuf * (XC + TC) * T : 0u) + threadIdx.x;
+  if (RING) {
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    for (uint32_t c = threadIdx.y * blockDim.x + threadIdx.x; c < j.nbuf * (XC + TC) * T; c += T) sm[c] = zero;
+    if (j.wsm && threadIdx.y == 0)
+#pragma unroll
+      for (uint32_t g = 0; g < 2; g++) {
+        Raw<false> w = load8<false, true>(j.w, k0 + g * 64u, j.D);
+        wat[2u * g * blockDim.x] = w.w[0], wat[(2u * g + 1u) * blockDim.x] = w.w[1];
+        if (!POST) continue;
+        w = load8<false, true>(j.pw, k0 + g * 64u, j.D);
+        wat[(4u + 2u * g) * blockDim.x] = w.w[0], wat[(5u + 2u * g) * blockDim.x] = w.w[1];
+      }
+    __syncthreads();
+  }
+  Raw<false> wr[2] = {}, pr[2] = {};   // kDirect: the norms' weights
+  if (MODE == kDirect)
+#pragma unroll
+    for (uint32_t g = 0; g < 2; g++) {
+      wr[g] = load8<false, true>(j.w, k0 + g * 64u, j.D);
+      if (POST) pr[g] = load8<false, true>(j.pw, k0 + g * 64u, j.D);
+    }
+  // 8 values of f32 weights, of group g
+  const auto weights = [&](const float *w, uint32_t chunk, uint32_t g) {
+    if (MODE == kDirect) return vals<false>(chunk ? pr[g] : wr[g]);
+    Raw<false> r;
+    if (RING && j.wsm) r.w[0] = wat[(chunk + 2u * g) * blockDim.x], r.w[1] = wat[(chunk + 2u * g + 1u) * blockDim.x];
+    else r = load8<false, WIDE>(w, k0 + g * 64u, j.D);
+    return vals<false>(r);
+  };
+  uint32_t m = blockIdx.x * blockDim.y + threadIdx.y, mf = m;   // the row to work on, to fetch
+  uint32_t into = 0, from = 0;                                  // their places
+  const uint32_t cx = (threadIdx.x >> 5) * 512u + lane * (16u / xs), ct = (threadIdx.x >> 5) * 512u + lane * (16u / ts);   // columns of a lane's first chunks
+  const uint8_t *xf = j.x + ((uint64_t)m * j.x_ld + cx) * xs, *tf = j.t + ((uint64_t)m * j.t_ldm + ct) * ts;
+  const auto fetch = [&]() {
+    if (mf < j.M) {
+      uint4 *to = own + into * (XC + TC) * T;
+#pragma unroll
+      for (uint32_t c = 0; c < XC; c++)
+        if (cx + c * (512u / xs) < j.D) copy16(to + wx + c * 32u + lane, xf + c * 512u);
+      if (j.parts)
+#pragma unroll
+        for (uint32_t c = 0; c < TC; c++)
+          if (ct + c * (512u / ts) < j.D) copy16(to + wt + c * 32u + lane, tf + c * 512u);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    into = into + 1u == j.nbuf ? 0u : into + 1u;
+    mf += step;
+    xf += (uint64_t)step * j.x_ld * xs;
+    tf += (uint64_t)step * j.t_ldm * ts;
+  };
+  if (RING)
+    for (uint32_t i = 0; i + 1u < j.nbuf; i++) fetch();
+  uint8_t *hp = j.h + ((uint64_t)m * j.h_ld + k0) * xs, *yp = j.y.q + (uint64_t)m * j.y.ld;
+  for (; m < j.M; m += step, hp += (uint64_t)step * j.h_ld * xs, yp += (uint64_t)step * j.y.ld) {   // the threads of a row go together
+    Vals h[2], tv[2];
+    if (RING) {
+      fetch();
+      if (j.nbuf == 3u) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else if (j.nbuf == 2u) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();   // a warp's lanes copied for one another
+      const uint4 *at = own + from * (XC + TC) * T;
+      from = from + 1u == j.nbuf ? 0u : from + 1u;
+#pragma unroll
+      for (uint32_t g = 0; g < 2; g++) {
+        Raw<XF16> x;
+        Raw<TF16> t;
+#pragma unroll
+        for (uint32_t c = 0; c < XC / 2; c++) x.w[c] = at[wx + (lane >> 3) * (8u * XC) + g * (4u * XC) + l * (XC / 2) + c];
+        h[g] = vals<XF16>(x);
+        tv[g] = Vals{};
+        if (!j.parts) continue;
+#pragma unroll
+        for (uint32_t c = 0; c < TC / 2; c++) t.w[c] = at[wt + (lane >> 3) * (8u * TC) + g * (4u * TC) + l * (TC / 2) + c];
+        tv[g] = vals<TF16>(t);
+      }
+    } else {
+#pragma unroll
+      for (uint32_t g = 0; g < 2; g++) {
+        h[g] = vals<XF16>(load8<XF16, WIDE>(j.x + (uint64_t)m * j.x_ld * xs, k0 + g * 64u, j.D));
+        tv[g] = j.parts ? vals<TF16>(load8<TF16, WIDE>(j.t + (uint64_t)m * j.t_ldm * ts, k0 + g * 64u, j.D)) : Vals{};
+      }
+    }
+    for (uint32_t p = 1; p < j.parts; p++)
+#pragma unroll
+      for (uint32_t g = 0; g < 2; g++) {
+        const Vals t = vals<TF16>(load8<TF16, WIDE>(j.t + ((uint64_t)p * j.t_ld + (uint64_t)m * j.t_ldm) * ts, k0 + g * 64u, j.D));
+#pragma unroll
+        for (int i = 0; i < 8; i++) tv[g].v[i] += t.v[i];
+      }
+    if (POST) {
+      float s = 0.0f;
+#pragma unroll
+      for (uint32_t g = 0; g < 2; g++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) s = fmaf(tv[g].v[i], tv[g].v[i], s);
+      const float rs = rsqrtf(row_sum(s, place()) / (float)j.D + j.eps);
+#pragma unroll
+      for (uint32_t g = 0; g < 2; g++) {
+        const Vals w = weights(j.pw, 4, g);
+#pragma unroll
+        for (int i = 0; i < 8; i++) tv[g].v[i] = __fmul_rn(__fmul_rn(tv[g].v[i], rs), w.v[i]);
+      }
+    }
     float s = 0.0f;
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+    for (uint32_t g = 0; g < 2; g++) {
+      const Raw<XF16> r = settle<XF16>(h[g], tv[g], j.scale);
 #pragma unroll
-      for (int i = 0; i < 8; i++) s = fmaf(tv[b].v[i], tv[b].v[i], s);
-    const float rs = rsqrtf(row_sum(s, red[0]) / (float)j.D + j.eps);
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      const Vals w = load8<false, WIDE>(j.pw, (half + b * halves) * kF8Block + l * 8u, D);
-#pragma unroll
-      for (int i = 0; i < 8; i++) tv[b].v[i] = __fmul_rn(__fmul_rn(tv[b].v[i], rs), w.v[i]);
+      for (int i = 0; i < 8; i++) s = fmaf(h[g].v[i], h[g].v[i], s);
+      if (!j.store) continue;
+      if (WIDE) {
+        if (!in[g]) continue;
+        uint4 *to = reinterpret_cast<uint4 *>(hp + g * 64u * xs);
+        to[0] = r.w[0];
+        if (!XF16) to[1] = r.w[XF16 ? 0 : 1];
+      } else {
+        store8<XF16>(j.h + (uint64_t)m * j.h_ld * xs, k0 + g * 64u, j.D, h[g]);
+      }
     }
-  }
-  float s = 0.0f;
+    const float st = rsqrtf(row_sum(s, place()) / (float)j.D + j.eps);
+    if (j.st && threadIdx.x == 0) j.st[m] = st;
 #pragma unroll
-  for (int b = 0; b < NB; b++) {
+    for (uint32_t g = 0; g < 2; g++) {
+      const Vals w = weights(j.w, 0, g);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      float v = __fmul_rn(__fadd_rn(h[b].v[i], tv[b].v[i]), j.scale);
-      if (XF16) v = __half2float(__float2half_rn(v));
-      h[b].v[i] = v;
-      s = fmaf(v, v, s);
+      for (int i = 0; i < 8; i++) h[g].v[i] = __fmul_rn(__fmul_rn(h[g].v[i], st), w.v[i]);
     }
-    if (j.store) store8<XF16, WIDE>(j.h + (uint64_t)mr * j.h_ld * (XF16 ? 2u : 4u), (half + b * halves) * kF8Block + l * 8u, D, h[b]);
-  }
-  const float st = rsqrtf(row_sum(s, red[1]) / (float)j.D + j.eps);
-  if (here && j.st && threadIdx.x == 0) j.st[m] = st;
+    const float a = f8_hold(eight_max(fmaxf(max8(h[0]), max8(h[1])))), inv = __fdiv_rn(448.0f, a);
+    if (in[0]) {
 #pragma unroll
-  for (int b = 0; b < NB; b++) {
-    const uint32_t kb = half + b * halves, k = kb * kF8Block + l * 8u;
-    const Vals w = load8<false, WIDE>(j.w, k, D);
-#pragma unroll
-    for (int i = 0; i < 8; i++) h[b].v[i] = __fmul_rn(__fmul_rn(h[b].v[i], st), w.v[i]);
-    const float a = f8_hold(half_max(max8(h[b])));
-    if (kb * kF8Block >= D) continue;
-    store_codes(j.y.q + (uint64_t)mr * j.y.ld, k, D, h[b], __fdiv_rn(448.0f, a));
-    if (l == 0) j.y.s[(uint64_t)kb * j.y.s_ld + m] = __fdiv_rn(a, 448.0f);
+      for (uint32_t g = 0; g < 2; g++) store_codes(yp, k0 + g * 64u, j.D, h[g], inv);
+    }
+    if (l == 0 && in[0]) j.y.s[(uint64_t)kb * j.y.s_ld + m] = __fdiv_rn(a, 448.0f);
+    __syncwarp();
   }
+  if (RING) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <bool XF16, bool TF16, bool WIDE>
-void norm_launch(p0_ctx *c, const NormJob &j) {
-  // a step of blockDim.x threads covers 8 columns a thread. Few rows: as many threads a row as it has columns for. Many: two blocks
-  // a half warp, rows of up to 512 columns several a CTA
-  const uint32_t D = j.D;
-  const bool few = j.M <= 2u * (uint32_t)c->sm_count;
-  const uint32_t nb = D > 8192 || (!few && D > 256) ? 2u : 1u;
-  const uint32_t T = ((D + 8u * nb - 1u) / (8u * nb) + 31u) / 32u * 32u, R = T <= 64 && !few ? 256u / T : 1u;
-  const dim3 grid((j.M + R - 1u) / R), block(T, R);
-  auto go = [&](auto kern) { launch_dep(kern, grid, block, 0, c->stream, j); };
-  if (nb == 1) go(f8_norm_kernel<XF16, TF16, WIDE, 1>);
-  else go(f8_norm_kernel<XF16, TF16, WIDE, 2>);
+template <bool XF16, bool TF16>
+p0_status norm_launch(p0_ctx *c, NormJob &j, bool wide, const char *op) {
+  // several rows a CTA where they are short; as many CTAs as an SM holds, each with its rows in turn
+  const uint32_t T = (j.D + 511u) / 512u * 32u, R = T <= 160u ? 320u / T : 1u, ctas = (j.M + R - 1u) / R;
+  const uint32_t row = T * R * 16u * ((XF16 ? 2u : 4u) + (TF16 ? 2u : 4u)), ws = T * 64u * (j.pw ? 2u : 1u);
+  uint32_t per = 1024u / (T * R), smem = 0;
+  const auto go = [&](auto kern, dim3 grid, dim3 block) {
+    const cudaError_t e = smem > 40u * 1024u ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+    if (e != cudaSuccess) return p0_cuda(c, e, op);
+    launch_dep(kern, grid, block, smem, c->stream, j);
+    return p0_launched(c, op);
+  };
+  if (!wide) return j.pw ? go(f8_norm_kernel<XF16, TF16, kScalar, true>, dim3(ctas), dim3(T, R)) : go(f8_norm_kernel<XF16, TF16, kScalar, false>, dim3(ctas), dim3(T, R));
+  if (j.M <= (uint32_t)c->sm_count && T <= 512u)
+    return j.pw ? go(f8_norm_kernel<XF16, TF16, kDirect, true>, dim3(j.M), dim3(T)) : go(f8_norm_kernel<XF16, TF16, kDirect, false>, dim3(j.M), dim3(T));
+  // room for three rows where it does not cost CTAs, two else; one for the longest in f32
+  const uint32_t all = 220u * 1024u;
+  j.wsm = row + ws <= all;
+  const uint32_t w = j.wsm ? ws : 0u;
+  j.nbuf = (3u * row + w) * per <= all ? 3u : 2u * row + w <= all ? 2u : 1u;
+  smem = j.nbuf * row + w;
+  if (per > all / smem) per = all / smem;
+  const uint32_t fit = (uint32_t)c->sm_count * per;
+  return j.pw ? go(f8_norm_kernel<XF16, TF16, kRing, true>, dim3(ctas < fit ? ctas : fit), dim3(T, R))
+              : go(f8_norm_kernel<XF16, TF16, kRing, false>, dim3(ctas < fit ? ctas : fit), dim3(T, R));
 }
 
-void pack_rows_launch(p0_ctx *c, const PackJob &j, bool f16, bool wide) {
-  const uint64_t want = ((uint64_t)j.units + kT / 16 - 1) / (kT / 16), most = (uint64_t)c->sm_count * 8u;
+void pack_rows_launch(p0_ctx *c, PackJob j, bool f16, bool wide) {
+  j.magic = (uint32_t)((1ull << 32) / j.KB);   // one too small at most
+  const uint64_t want = ((uint64_t)j.units + kT / 8 - 1) / (kT / 8), most = (uint64_t)c->sm_count * 8u;
   const dim3 grid((unsigned)(want < most ? want : most));
   auto go = [&](auto kern) { launch_dep(kern, grid, dim3(kT), 0, c->stream, j); };
   if (f16) wide ? go(f8_pack_rows_kernel<true, true>) : go(f8_pack_rows_kernel<true, false>);
@@ -306,7 +462,7 @@ p0_status f8_view(p0_ctx *c, const p0_f8 &m, uint64_t rows, uint64_t cols, bool 
 }
 
 p0_status f8_pack_rows(p0_ctx *c, const float *x, uint64_t ld, uint32_t M, uint32_t K, const F8Mat &y, const char *op) {
-  PackJob j{(const uint8_t *)x, ld, M, K, (K + kF8Block - 1) / kF8Block, 0, y};
+  PackJob j{(const uint8_t *)x, ld, M, K, (K + kF8Block - 1) / kF8Block, 0, 0, y};
   j.units = M * j.KB;
   pack_rows_launch(c, j, false, ld % 4 == 0);
   return p0_launched(c, op);
@@ -412,17 +568,11 @@ p0_status p0_norm_f8(p0_ctx *c, const p0_norm_f8_args *a) {
   j.M = a->M;
   j.D = a->D;
   j.eps = a->eps != 0.0f ? a->eps : 1e-6f;
-  wide = wide && w1 && w2 && (uintptr_t)j.w % 16 == 0 && (uintptr_t)j.pw % 16 == 0;
+  wide = wide && w1 && w2 && (uintptr_t)j.w % 16 == 0 && (uintptr_t)j.pw % 16 == 0 && D % 8 == 0;
   DeviceGuard guard(c->device);
   const bool xf = a->type == P0_F16, tf = a->t_type == P0_F16;
-  if (wide) {
-    if (xf) tf ? norm_launch<true, true, true>(c, j) : norm_launch<true, false, true>(c, j);
-    else tf ? norm_launch<false, true, true>(c, j) : norm_launch<false, false, true>(c, j);
-  } else {
-    if (xf) tf ? norm_launch<true, true, false>(c, j) : norm_launch<true, false, false>(c, j);
-    else tf ? norm_launch<false, true, false>(c, j) : norm_launch<false, false, false>(c, j);
-  }
-  return p0_launched(c, op);
+  if (xf) return tf ? norm_launch<true, true>(c, j, wide, op) : norm_launch<true, false>(c, j, wide, op);
+  return tf ? norm_launch<false, true>(c, j, wide, op) : norm_launch<false, false>(c, j, wide, op);
 }
 
 }  // extern "C"

@@ -6,6 +6,8 @@
 // bytes of two rows at a time straight into the fragments of mma.sync.m16n8k32 (e4m3, f32 sums): the order of k inside a
 // fragment is free as long as both operands share it, so 16 consecutive bytes serve two instructions. Tokens are the n side,
 // loaded the same way. Each block's sums are scaled and added in f32; the warps' parts meet in shared memory, in order.
+#include <cstdlib>
+
 #include "f8_gemm.cuh"
 
 namespace {
@@ -168,7 +170,10 @@ extern "C" p0_status p0_gemm_f8(p0_ctx *c, const p0_gemm_f8_args *a) {
       (j.bv && over(j.bv, N * 4)) || (gated && f8_meet(y.q, yn, y.s, ysn)))
     return p0_fail(c, P0_EINVAL, "%s: y must not lie over the inputs", op);
   DeviceGuard guard(c->device);
-  if (M > 64) return f8_tc_launch(c, j, y, op);
+  const char *ev = getenv("P0MM_F8");   // tuning and tests: the form
+  const char form = ev && (ev[0] == 'f' || ev[0] == 'm' || ev[0] == 't') ? ev[0] : M > 64 ? 't' : 'f';
+  if (form == 't') return f8_tc_launch(c, j, y, op);
+  if (form == 'm') return f8_mid_launch(c, j, y, op);
   if (!gated) return few_launch(c, j, op);
   uint32_t *cnt;
   void *ws;

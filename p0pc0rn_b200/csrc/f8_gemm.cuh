@@ -12,3 +12,5 @@ struct GemmJob {
 
 // the form for many tokens (f8_tc.cu); y: where the codes of a gated call go
 p0_status f8_tc_launch(p0_ctx *c, const GemmJob &j, const F8Mat &y, const char *op);
+// where tokens or tiles are few (f8_mid.cu)
+p0_status f8_mid_launch(p0_ctx *c, const GemmJob &j, const F8Mat &y, const char *op);
