@@ -443,7 +443,7 @@ typedef struct {
 } p0_f8;
 
 /* packF8: M rows of K values (type P0_F32 or P0_F16; value (m, k) at x_off + m * x_ld + k in elements, x_ld 0 = K) -> y, in blocks of
- * `block`. x and y share no byte. */
+ * `block`. x, y's codes and its scales lie apart, each from its first byte to its last. */
 typedef struct {
   p0_buf x; uint64_t x_off; uint32_t x_ld;
   uint32_t type, M, K, block;
@@ -458,7 +458,8 @@ p0_status p0_pack_f8(p0_ctx *ctx, const p0_pack_f8_args *a);
  *   st[st_off + m] = r = rsqrt(mean h^2 + eps)                             (st optional), of the rounded h
  *   y  = codes of (h * r) * w[w_off + i]                                   in blocks of P0_F8_ROW
  * x and h: rows of `type`, at off + m * ld + i in elements (ld 0 = D); h absent: x itself is updated. t: rows of t_type. eps 0 =
- * 1e-6; scale has no default here (1 adds plainly). Nothing written lies over anything else, but h may be x's rows exactly. */
+ * 1e-6; scale has no default here (1 adds plainly). What is written lies apart from everything else, each from
+ * its first byte to its last, but h may be x's rows exactly. */
 typedef struct {
   p0_buf x; uint64_t x_off; uint32_t x_ld, type;
   p0_buf t; uint64_t t_off, t_ld; uint32_t t_ldm, t_type, t_n;
@@ -477,9 +478,8 @@ p0_status p0_norm_f8(p0_ctx *ctx, const p0_norm_f8_args *a);
  *   P0_F8EPI_F16, _F32      y: rows of f16 or f32, element (m, n) at y.off + m * y.ld + n (elements, y.ld 0 = N; y.s not used);
  *                           with bv: + bv[bv_off + n] before the rounding
  *   P0_F8EPI_SWIGLU, _GEGLU y: codes (P0_F8_ROW) of act(X W^T) * (X U^T), u as w; act = silu or the tanh form of gelu, in f32
- * The operator needs no packed form of its own: x, w and u are read as packF8 and normF8 write them. y shares no byte with the inputs.
- * Gated calls with few tokens keep M * N floats in the context's workspace; the first call of a size may grow it (which waits for the
- * stream), so it should not sit inside a stream capture. */
+ * The operator needs no packed form of its own: x, w and u are read as packF8 and normF8 write them. y lies apart from the inputs.
+ * None of the three uses the context's workspace: they may be captured, and captured graphs may run side by side. */
 enum { P0_F8EPI_F16 = 0, P0_F8EPI_F32 = 1, P0_F8EPI_SWIGLU = 2, P0_F8EPI_GEGLU = 3 };
 typedef struct {
   p0_f8 x, w, u;

@@ -461,13 +461,6 @@ p0_status f8_view(p0_ctx *c, const p0_f8 &m, uint64_t rows, uint64_t cols, bool 
   return P0_OK;
 }
 
-p0_status f8_pack_rows(p0_ctx *c, const float *x, uint64_t ld, uint32_t M, uint32_t K, const F8Mat &y, const char *op) {
-  PackJob j{(const uint8_t *)x, ld, M, K, (K + kF8Block - 1) / kF8Block, 0, 0, y};
-  j.units = M * j.KB;
-  pack_rows_launch(c, j, false, ld % 4 == 0);
-  return p0_launched(c, op);
-}
-
 extern "C" {
 
 p0_status p0_pack_f8(p0_ctx *c, const p0_pack_f8_args *a) {

@@ -48,9 +48,6 @@ inline uint64_t f8_scale_bytes(const F8Mat &m, uint64_t rows, uint64_t cols, boo
   const uint64_t kb = (cols + kF8Block - 1) / kF8Block, nb = (rows + kF8Block - 1) / kF8Block;
   return tile ? ((nb - 1) * m.s_ld + kb) * 4 : ((kb - 1) * m.s_ld + rows) * 4;
 }
-// packs rows of f32 in the context's stream (gemmF8's gated results on their way to codes)
-p0_status f8_pack_rows(p0_ctx *c, const float *x, uint64_t ld, uint32_t M, uint32_t K, const F8Mat &y, const char *op);
-
 __device__ __forceinline__ float f8_hold(float a) { return fminf(fmaxf(a, 0x1p-100f), 3.402823466e38f); }
 // two values to two e4m3 codes, round to nearest even, held at +-448; lo in the low byte
 __device__ __forceinline__ uint32_t f8_codes2(float lo, float hi) {
@@ -59,8 +56,3 @@ __device__ __forceinline__ uint32_t f8_codes2(float lo, float hi) {
   return r;
 }
 __device__ __forceinline__ uint32_t f8_codes4(float a, float b, float c, float d) { return f8_codes2(a, b) | (f8_codes2(c, d) << 16); }
-// the gate of a gated epilogue: silu, or the tanh form of gelu as x * sigmoid(2 z), z = sqrt(2 / pi) (x + 0.044715 x^3)
-__device__ __forceinline__ float f8_gate(float x, uint32_t epi) {
-  const float z = epi == P0_F8EPI_SWIGLU ? x : 1.5957691216057308f * fmaf(0.044715f * x, x * x, x);
-  return __fdividef(x, 1.0f + __expf(-z));
-}

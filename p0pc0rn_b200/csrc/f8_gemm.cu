@@ -6,8 +6,6 @@
 // bytes of two rows at a time straight into the fragments of mma.sync.m16n8k32 (e4m3, f32 sums): the order of k inside a
 // fragment is free as long as both operands share it, so 16 consecutive bytes serve two instructions. Tokens are the n side,
 // loaded the same way. Each block's sums are scaled and added in f32; the warps' parts meet in shared memory, in order.
-#include <cstdlib>
-
 #include "f8_gemm.cuh"
 
 namespace {
@@ -15,7 +13,7 @@ namespace {
 constexpr int kT = 256, kW = kT / 32;
 
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -27,80 +25,66 @@ __device__ __forceinline__ uint4 codes16(const uint8_t *row, uint32_t k, uint32_
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// NT: groups of 8 tokens; MATS: 2 with u
-template <int NT, int MATS>
+// NT: groups of 8 tokens
+template <int NT>
 __global__ void __launch_bounds__(kT) f8_few_kernel(GemmJob j) {
   dep_enter();
-  constexpr int kOut = NT * 128;                 // outputs of a matrix: token * 16 + row
-  __shared__ float red[kW][MATS * kOut];
+  constexpr int kOut = NT * 128;   // token * 16 + row
+  __shared__ float red[kW][kOut];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, c = lane & 3u;
-  const uint32_t nblk = (j.N + 15u) / 16u, n0 = blockIdx.x % nblk * 16u, m0 = blockIdx.x / nblk * (8u * NT);
-  float acc[MATS][NT][4];
+  const uint32_t n0 = blockIdx.x * 16u;
+  float acc[NT][4];
 #pragma unroll
-  for (int a = 0; a < MATS; a++)
+  for (int t = 0; t < NT; t++)
 #pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) acc[a][t][i] = 0.0f;
+    for (int i = 0; i < 4; i++) acc[t][i] = 0.0f;
   const uint64_t r0 = min(n0 + g, j.N - 1u), r1 = min(n0 + g + 8u, j.N - 1u);   // rows beyond the last: their sums are not stored
+#pragma unroll 2
   for (uint32_t kb = warp; kb < j.KB; kb += kW) {
     const uint32_t k = kb * kF8Block + c * 16u;
     uint4 x[NT][2];
     float xs[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const uint32_t m = m0 + t * 8u + g;
+      const uint32_t m = t * 8u + g;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         x[t][h] = m < j.M ? codes16(j.x.q + (uint64_t)m * j.x.ld, k + h * 64u, j.K) : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t mc = m0 + t * 8u + 2u * c + h;
+        const uint32_t mc = t * 8u + 2u * c + h;
         xs[t][h] = mc < j.M ? j.x.s[(uint64_t)kb * j.x.s_ld + mc] : 0.0f;
       }
     }
+    uint4 w0[2], w1[2];
 #pragma unroll
-    for (int a = 0; a < MATS; a++) {
-      const F8Mat &w = a ? j.u : j.w;
-      uint4 w0[2], w1[2];
+    for (int h = 0; h < 2; h++) {
+      w0[h] = codes16(j.w.q + r0 * j.w.ld, k + h * 64u, j.K);
+      w1[h] = codes16(j.w.q + r1 * j.w.ld, k + h * 64u, j.K);
+    }
+    const float ws = j.w.s[(uint64_t)(n0 / kF8Block) * j.w.s_ld + kb];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        w0[h] = codes16(w.q + r0 * w.ld, k + h * 64u, j.K);
-        w1[h] = codes16(w.q + r1 * w.ld, k + h * 64u, j.K);
+        mma_e4m3(d, w0[h].x, w1[h].x, w0[h].y, w1[h].y, x[t][h].x, x[t][h].y);
+        mma_e4m3(d, w0[h].z, w1[h].z, w0[h].w, w1[h].w, x[t][h].z, x[t][h].w);
       }
-      const float ws = w.s[(uint64_t)(n0 / kF8Block) * w.s_ld + kb];
 #pragma unroll
-      for (int t = 0; t < NT; t++) {
-        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          mma_e4m3(d, w0[h].x, w1[h].x, w0[h].y, w1[h].y, x[t][h].x, x[t][h].y);
-          mma_e4m3(d, w0[h].z, w1[h].z, w0[h].w, w1[h].w, x[t][h].z, x[t][h].w);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[a][t][i] = fmaf(d[i], xs[t][i & 1] * ws, acc[a][t][i]);
-      }
+      for (int i = 0; i < 4; i++) acc[t][i] = fmaf(d[i], xs[t][i & 1] * ws, acc[t][i]);
     }
   }
 #pragma unroll
-  for (int a = 0; a < MATS; a++)
+  for (int t = 0; t < NT; t++)
 #pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) red[warp][a * kOut + (t * 8 + 2 * c + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[a][t][i];
+    for (int i = 0; i < 4; i++) red[warp][(t * 8 + 2 * c + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[t][i];
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < kOut; e += kT) {
-    const uint32_t m = m0 + e / 16u, n = n0 + e % 16u;
+    const uint32_t m = e / 16u, n = n0 + e % 16u;
     if (m >= j.M || n >= j.N) continue;
     float y = 0.0f;
 #pragma unroll
     for (int w = 0; w < kW; w++) y += red[w][e];
-    if (MATS == 2) {
-      float u = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kW; w++) u += red[w][(MATS - 1) * kOut + e];
-      y = f8_gate(y, j.epi) * u;
-    } else if (j.bv) {
-      y += j.bv[n];
-    }
+    if (j.bv) y += j.bv[n];
     const uint64_t at = (uint64_t)m * j.y_ld + n;
     if (j.epi == P0_F8EPI_F16) reinterpret_cast<__half *>(j.y)[at] = __float2half_rn(y);
     else reinterpret_cast<float *>(j.y)[at] = y;
@@ -108,14 +92,9 @@ __global__ void __launch_bounds__(kT) f8_few_kernel(GemmJob j) {
 }
 
 p0_status few_launch(p0_ctx *c, const GemmJob &j, const char *op) {
-  const uint32_t nblk = (j.N + 15u) / 16u;
-  const bool gated = j.epi >= P0_F8EPI_SWIGLU;
-  auto go = [&](auto kern, uint32_t tok) {
-    launch_dep(kern, dim3((unsigned)(nblk * ((j.M + tok - 1u) / tok))), dim3(kT), 0, c->stream, j);
-  };
-  if (j.M <= 8) gated ? go(f8_few_kernel<1, 2>, 8) : go(f8_few_kernel<1, 1>, 8);
-  else if (j.M <= 16) gated ? go(f8_few_kernel<2, 2>, 16) : go(f8_few_kernel<2, 1>, 16);
-  else gated ? go(f8_few_kernel<4, 2>, 32) : go(f8_few_kernel<4, 1>, 32);
+  const dim3 grid((j.N + 15u) / 16u);
+  if (j.M <= 8) launch_dep(f8_few_kernel<1>, grid, dim3(kT), 0, c->stream, j);
+  else launch_dep(f8_few_kernel<2>, grid, dim3(kT), 0, c->stream, j);
   return p0_launched(c, op);
 }
 
@@ -170,16 +149,8 @@ extern "C" p0_status p0_gemm_f8(p0_ctx *c, const p0_gemm_f8_args *a) {
       (j.bv && over(j.bv, N * 4)) || (gated && f8_meet(y.q, yn, y.s, ysn)))
     return p0_fail(c, P0_EINVAL, "%s: y must not lie over the inputs", op);
   DeviceGuard guard(c->device);
-  const char *ev = getenv("P0MM_F8");   // tuning and tests: the form
-  const char form = ev && (ev[0] == 'f' || ev[0] == 'm' || ev[0] == 't') ? ev[0] : M > 64 ? 't' : 'f';
-  if (form == 't') return f8_tc_launch(c, j, y, op);
-  if (form == 'm') return f8_mid_launch(c, j, y, op);
-  if (!gated) return few_launch(c, j, op);
-  uint32_t *cnt;
-  void *ws;
-  if ((st = p0_workspace(c, 0, M * N * 4, &cnt, &ws))) return st;
-  j.y = (uint8_t *)ws;
-  j.y_ld = N;
-  if ((st = few_launch(c, j, op))) return st;
-  return f8_pack_rows(c, (const float *)ws, N, a->M, a->N, y, op);
+  // RULE
+  if (!gated && ((M <= 8 && j.KB <= 64) || (M <= 16 && N <= 4096 && j.KB <= 32))) return few_launch(c, j, op);
+  if (gated ? M <= 64 : M <= 128 || f8_mid_parts(c, j.M, j.N, j.KB) > 1) return f8_mid_launch(c, j, y, op);
+  return f8_tc_launch(c, j, y, op);
 }

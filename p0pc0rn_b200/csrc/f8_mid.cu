@@ -9,13 +9,13 @@
 // token's 128 columns, adds the S parts in order (over distributed shared memory) and stores them; of a gated call it knows all 128
 // columns of the block of codes.
 #include "f8_gemm.cuh"
-#include "tc.cuh"
 
 namespace {
 
+using namespace f8tc;
+
 constexpr uint32_t kW = 128 * 128;        // a stage's rows of one matrix
 constexpr uint32_t kScales = 4;           // groups of blocks whose scales are on their way
-constexpr uint32_t kDrain = 1u << 16;     // polls for what is in flight when a wait has given up
 
 template <int TN, int MATS>
 struct Cfg {
@@ -36,11 +36,6 @@ struct MidJob {
   uint32_t *err;
 };
 
-__device__ __forceinline__ bool elect() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(p));
-  return p != 0u;
-}
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -64,25 +59,6 @@ __device__ __forceinline__ float4 remote4(const void *p, uint32_t rank) {
                : "memory");
   return v;
 }
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *err, uint32_t code) {
-  return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort, err, code, P0_SPIN_LIMIT));
-}
-
-// for two phases: a wait that is over costs its latency, here once for both
-__device__ __forceinline__ bool warp_wait_two(uint64_t *x, uint32_t px, uint64_t *y, uint32_t py, volatile uint32_t *abort, uint32_t *err, uint32_t code) {
-  bool ok = false;
-  for (uint32_t i = 0; i < P0_SPIN_LIMIT; i++) {
-    const bool a = tc::mbar_try(x, px), b = tc::mbar_try(y, py);
-    if (a && b) { ok = true; break; }
-    if (*abort) break;
-  }
-  if (!ok && !*abort) {
-    *abort = 1u;
-    atomicOr(err, code);
-  }
-  return __all_sync(0xffffffffu, ok);
-}
-
 template <int TN, int MATS>
 __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     f8_mid_kernel(MidJob q, const __grid_constant__ CUtensorMap xm, const __grid_constant__ CUtensorMap wm, const __grid_constant__ CUtensorMap um) {
@@ -116,6 +92,12 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     tc::fence_mbar_init();
   }
   if (warp == 0) {
+    if (elect()) {   // the maps are this launch's own
+      tc::prefetch_tmap(&wm);
+      tc::prefetch_tmap(&xm);
+      if (MATS == 2) tc::prefetch_tmap(&um);
+    }
+    __syncwarp();
     tc::tmem_alloc(&tmem_slot, C::kCols);
     tc::tmem_relinquish();
   }
@@ -130,7 +112,7 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     // ------------------------------------------------------------ copies
     for (uint32_t kb = k_lo; kb < k_hi; kb++) {
       const uint32_t i = kb - k_lo, s = i % NS;
-      if (!(ok = warp_wait(&empty[s], (i / NS & 1u) ^ 1u, abort_flag, q.err, 0x8a1u))) break;
+      if (i >= NS && !(ok = warp_wait(&empty[s], (i / NS & 1u) ^ 1u, abort_flag, q.err, 0x8a1u))) break;
       if (elect()) {
         uint8_t *to = ring + s * C::kStage;
         tc::mbar_expect_tx(&full[s], C::kStage);
@@ -280,66 +262,58 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     }
 #pragma unroll
     for (uint32_t i = 0; i < U; i++) {
-    const uint32_t t = t0 + i * stride;
-    if (t >= mend) break;
-    float (&v)[MATS][4] = sums[i];
-    const uint32_t n = n0 + lane * 4u, m = m0 + t;
-    if (MATS == 2) {
-      float a = 0.0f;
+      const uint32_t t = t0 + i * stride;
+      if (t >= mend) break;
+      float (&v)[MATS][4] = sums[i];
+      const uint32_t n = n0 + lane * 4u, m = m0 + t;
+      if (MATS == 2) {
+        float a = 0.0f;
 #pragma unroll
-      for (uint32_t e = 0; e < 4; e++) {
-        v[0][e] = n + e < j.N ? f8_gate(v[0][e], j.epi) * v[MATS - 1][e] : 0.0f;
-        a = fmaxf(a, fabsf(v[0][e]));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-      a = f8_hold(a);
-      const float inv = __fdiv_rn(448.0f, a);
-      const uint32_t codes = f8_codes4(v[0][0] * inv, v[0][1] * inv, v[0][2] * inv, v[0][3] * inv);
-      uint8_t *to = q.y.q + (uint64_t)m * q.y.ld + n;
-      if (n + 4u <= j.N) *reinterpret_cast<uint32_t *>(to) = codes;
-      else
-        for (uint32_t e = 0; n + e < j.N; e++) to[e] = (uint8_t)(codes >> (8 * e));
-      if (lane == 0) q.y.s[(uint64_t)nb * q.y.s_ld + m] = __fdiv_rn(a, 448.0f);
-    } else {
-      const uint64_t to = (uint64_t)m * j.y_ld + n;
-      if (j.bv)
-#pragma unroll
-        for (uint32_t e = 0; e < 4; e++)
-          if (n + e < j.N) v[0][e] += j.bv[n + e];
-      if (j.epi == P0_F8EPI_F16) {
-        __half *y = reinterpret_cast<__half *>(j.y) + to;
-        if (q.wide && n + 4u <= j.N) {
-          const __half2 lo = __floats2half2_rn(v[0][0], v[0][1]), hi = __floats2half2_rn(v[0][2], v[0][3]);
-          *reinterpret_cast<uint2 *>(y) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-        } else {
-#pragma unroll
-          for (uint32_t e = 0; e < 4; e++)
-            if (n + e < j.N) y[e] = __float2half_rn(v[0][e]);
+        for (uint32_t e = 0; e < 4; e++) {
+          v[0][e] = n + e < j.N ? f8_gate(v[0][e], j.epi) * v[MATS - 1][e] : 0.0f;
+          a = fmaxf(a, fabsf(v[0][e]));
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        a = f8_hold(a);
+        const float inv = __fdiv_rn(448.0f, a);
+        const uint32_t codes = f8_codes4(v[0][0] * inv, v[0][1] * inv, v[0][2] * inv, v[0][3] * inv);
+        uint8_t *to = q.y.q + (uint64_t)m * q.y.ld + n;
+        if (n + 4u <= j.N) *reinterpret_cast<uint32_t *>(to) = codes;
+        else
+          for (uint32_t e = 0; n + e < j.N; e++) to[e] = (uint8_t)(codes >> (8 * e));
+        if (lane == 0) q.y.s[(uint64_t)nb * q.y.s_ld + m] = __fdiv_rn(a, 448.0f);
       } else {
-        float *y = reinterpret_cast<float *>(j.y) + to;
-        if (q.wide && n + 4u <= j.N) {
-          *reinterpret_cast<float4 *>(y) = make_float4(v[0][0], v[0][1], v[0][2], v[0][3]);
-        } else {
+        const uint64_t to = (uint64_t)m * j.y_ld + n;
+        if (j.bv)
 #pragma unroll
           for (uint32_t e = 0; e < 4; e++)
-            if (n + e < j.N) y[e] = v[0][e];
+            if (n + e < j.N) v[0][e] += j.bv[n + e];
+        if (j.epi == P0_F8EPI_F16) {
+          __half *y = reinterpret_cast<__half *>(j.y) + to;
+          if (q.wide && n + 4u <= j.N) {
+            const __half2 lo = __floats2half2_rn(v[0][0], v[0][1]), hi = __floats2half2_rn(v[0][2], v[0][3]);
+            *reinterpret_cast<uint2 *>(y) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+          } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++)
+              if (n + e < j.N) y[e] = __float2half_rn(v[0][e]);
+          }
+        } else {
+          float *y = reinterpret_cast<float *>(j.y) + to;
+          if (q.wide && n + 4u <= j.N) {
+            *reinterpret_cast<float4 *>(y) = make_float4(v[0][0], v[0][1], v[0][2], v[0][3]);
+          } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++)
+              if (n + e < j.N) y[e] = v[0][e];
+          }
         }
       }
-    }
     }
   }
   __syncwarp();
   if (S > 1u) tc::cluster_sync();   // no CTA leaves while another may read its parts
-}
-
-bool code_map(CUtensorMap *m, const F8Mat &a, uint64_t rows, uint64_t cols, uint32_t box_rows) {
-  const auto encode = tensor_map_encoder();
-  const cuuint64_t size[2] = {cols, rows}, stride[1] = {a.ld};
-  const cuuint32_t box[2] = {128, box_rows}, one[2] = {1, 1};
-  return encode && encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a.q, size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int TN, int MATS>
@@ -365,7 +339,19 @@ p0_status launch(p0_ctx *c, const MidJob &q, uint32_t tiles, const CUtensorMap &
   return p0_launched(c, op);
 }
 
+uint32_t tokens_of(uint32_t M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
+
 }  // namespace
+
+// as many CTAs as there are SMs, two blocks of k each at least; clusters of eight wait long for their SMs (128 tokens, N = K = 2048: 23.5 us
+// against 9.0 with four)
+uint32_t f8_mid_parts(const p0_ctx *c, uint32_t M, uint32_t N, uint32_t KB) {
+  const uint32_t TN = tokens_of(M);
+  const uint64_t tiles = (uint64_t)((N + 127u) / 128u) * ((M + TN - 1u) / TN);
+  uint32_t S = 1;
+  while (S < 4u && tiles * S * 2u <= (uint64_t)c->sm_count && KB >= S * 4u) S *= 2u;
+  return S;
+}
 
 p0_status f8_mid_launch(p0_ctx *c, const GemmJob &j, const F8Mat &y, const char *op) {
   const bool gated = j.epi >= P0_F8EPI_SWIGLU;
@@ -374,18 +360,22 @@ p0_status f8_mid_launch(p0_ctx *c, const GemmJob &j, const F8Mat &y, const char 
   q.err = c->d_err;
   const uint32_t es = j.epi == P0_F8EPI_F16 ? 2 : 4;
   q.wide = (uintptr_t)j.y % (4 * es) == 0 && j.y_ld % 4 == 0;
-  const uint32_t TN = j.M <= 16 ? 16 : j.M <= 32 ? 32 : j.M <= 64 ? 64 : 128, tiles = q.nblk * ((j.M + TN - 1u) / TN);
-  // as many CTAs as there are SMs, two blocks of k each at least
-  q.S = 1;
-  while (q.S < 8u && tiles * q.S * 2u <= (uint32_t)c->sm_count && j.KB >= q.S * 4u) q.S *= 2u;
+  const uint32_t TN = tokens_of(j.M), tiles = q.nblk * ((j.M + TN - 1u) / TN);
+  q.S = f8_mid_parts(c, j.M, j.N, j.KB);
+  const auto map = [&](CUtensorMap *m, const F8Mat &a, uint64_t rows, uint32_t box) {
+    return f8_box_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.q, rows, j.K, a.ld, box);
+  };
   CUtensorMap xm, wm, um = {};
-  if (!code_map(&xm, j.x, j.M, j.K, TN) || !code_map(&wm, j.w, j.N, j.K, 128) || (gated && !code_map(&um, j.u, j.N, j.K, 128)))
+  if (!map(&xm, j.x, j.M, TN) || !map(&wm, j.w, j.N, 128) || (gated && !map(&um, j.u, j.N, 128)))
     return p0_fail(c, P0_EDEVICE, "%s: tensor map encode failed", op);
-  const auto go = [&](auto one, auto two) { return gated ? two() : one(); };
+  if (gated) {   // up to 64 tokens
+    if (TN == 16) return launch<16, 2>(c, q, tiles, xm, wm, um, op);
+    return TN == 32 ? launch<32, 2>(c, q, tiles, xm, wm, um, op) : launch<64, 2>(c, q, tiles, xm, wm, um, op);
+  }
   switch (TN) {
-    case 16: return go([&] { return launch<16, 1>(c, q, tiles, xm, wm, um, op); }, [&] { return launch<16, 2>(c, q, tiles, xm, wm, um, op); });
-    case 32: return go([&] { return launch<32, 1>(c, q, tiles, xm, wm, um, op); }, [&] { return launch<32, 2>(c, q, tiles, xm, wm, um, op); });
-    case 64: return go([&] { return launch<64, 1>(c, q, tiles, xm, wm, um, op); }, [&] { return launch<64, 2>(c, q, tiles, xm, wm, um, op); });
-    default: return go([&] { return launch<128, 1>(c, q, tiles, xm, wm, um, op); }, [&] { return launch<128, 2>(c, q, tiles, xm, wm, um, op); });
+    case 16: return launch<16, 1>(c, q, tiles, xm, wm, um, op);
+    case 32: return launch<32, 1>(c, q, tiles, xm, wm, um, op);
+    case 64: return launch<64, 1>(c, q, tiles, xm, wm, um, op);
+    default: return launch<128, 1>(c, q, tiles, xm, wm, um, op);
   }
 }

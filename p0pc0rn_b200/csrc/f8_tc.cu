@@ -6,14 +6,14 @@
 // tensor memory, and eight warps add the block's sums, scaled, to the tile's in their registers: 128 columns of a token to a thread,
 // each times xs[b, m] * ws[n / 128, b]. While a tile's results are stored, the next tile's first two blocks are computed.
 #include "f8_gemm.cuh"
-#include "tc.cuh"
 
 namespace {
+
+using namespace f8tc;
 
 constexpr uint32_t kSums = 256, kThreads = kSums + 128;   // warps 0: copies; 1: MMAs; 2: what landed; 3: none (a warpgroup changes its registers as one); 4-11: sums
 constexpr uint32_t kBox = 128 * 128, kHalf = 64 * 128, kStage = kBox + 2 * kHalf;
 constexpr uint32_t kOut = 2 * 32 * 128;   // a warp's results on their way: two boxes of 32 rows of 128 bytes
-constexpr uint32_t kDrain = 1u << 16;     // polls for what is in flight when a wait has given up
 constexpr uint32_t kGroup = 8;            // row tiles whose x stays in L2 while the columns pass
 template <bool GATED>
 struct Cfg {
@@ -29,13 +29,6 @@ struct TcJob {
   uint32_t *err;
 };
 
-// one lane of a converged warp. What it issues to the tensor core and the copy engine costs a few cycles each; under a condition on the
-// lane's number the compiler cannot tell that there is one lane, and the same loop took 1050 cycles a block instead of 830
-__device__ __forceinline__ bool elect() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(p));
-  return p != 0u;
-}
 // a 2D tile into this CTA's shared memory, its bytes counted by the even CTA's barrier
 __device__ __forceinline__ void tma_load_pair(void *dst, const void *tmap, uint32_t bar, int32_t c0, int32_t c1) {
   asm volatile(
@@ -94,25 +87,6 @@ __device__ __forceinline__ uint64_t twice(float f) {
   return r;
 }
 
-// a warp's waits: every lane returns the same
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *err, uint32_t code) {
-  return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort, err, code, P0_SPIN_LIMIT));
-}
-// for two phases (y may be null): a wait that is over costs its latency, here once for both
-__device__ __forceinline__ bool warp_wait_two(uint64_t *x, uint32_t px, uint64_t *y, uint32_t py, volatile uint32_t *abort, uint32_t *err, uint32_t code) {
-  bool ok = false;
-  for (uint32_t i = 0; i < P0_SPIN_LIMIT; i++) {
-    const bool a = tc::mbar_try(x, px), b = !y || tc::mbar_try(y, py);
-    if (a && b) { ok = true; break; }
-    if (*abort) break;
-  }
-  if (!ok && !*abort) {
-    *abort = 1u;
-    atomicOr(err, code);
-  }
-  return __all_sync(0xffffffffu, ok);
-}
-
 // tile t: its row and column of tiles. Column by column within groups of kGroup rows
 __device__ __forceinline__ uint2 tile_at(const TcJob &q, uint32_t t) {
   const uint32_t per = kGroup * q.nt, grp = t / per, r0 = grp * kGroup, rows = min(kGroup, q.mt - r0), in = t - grp * per;
@@ -148,6 +122,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tc::fence_mbar_init();
   }
   if (warp == 0) {
+    if (elect()) {   // the maps are this launch's own
+      tc::prefetch_tmap(&xm);
+      tc::prefetch_tmap(&wm);
+      tc::prefetch_tmap(&um);
+    }
+    __syncwarp();
     tc::tmem_alloc_pair(&tmem_slot, 512);
     tc::tmem_relinquish_pair();
   }
@@ -402,15 +382,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-// a matrix of bytes (codes) or of results, in boxes of rows of 128 bytes
-bool box_map(CUtensorMap *m, CUtensorMapDataType type, uint32_t es, const void *base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
-  const auto encode = tensor_map_encoder();
-  const cuuint64_t size[2] = {cols, rows}, stride[1] = {ld * es};
-  const cuuint32_t box[2] = {128 / es, box_rows}, one[2] = {1, 1};
-  return encode && encode(m, type, 2, const_cast<void *>(base), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 }  // namespace
 
 p0_status f8_tc_launch(p0_ctx *c, const GemmJob &j, const F8Mat &y, const char *op) {
@@ -421,12 +392,12 @@ p0_status f8_tc_launch(p0_ctx *c, const GemmJob &j, const F8Mat &y, const char *
   q.tiles = q.mt * q.nt;
   q.err = c->d_err;
   CUtensorMap xm, wm, um = {};   // um: u, or the results
-  if (!box_map(&xm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, j.x.q, j.M, j.K, j.x.ld, 128) || !box_map(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, j.w.q, j.N, j.K, j.w.ld, 64) ||
-      (gated && !box_map(&um, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, j.u.q, j.N, j.K, j.u.ld, 64)))
+  if (!f8_box_map(&xm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, j.x.q, j.M, j.K, j.x.ld, 128) || !f8_box_map(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, j.w.q, j.N, j.K, j.w.ld, 64) ||
+      (gated && !f8_box_map(&um, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, j.u.q, j.N, j.K, j.u.ld, 64)))
     return p0_fail(c, P0_EDEVICE, "%s: tensor map encode failed", op);
   const uint32_t es = f16 ? 2 : 4;
   if (gated) q.wide = (uintptr_t)y.q % 32 == 0 && y.ld % 32 == 0;
-  else q.wide = (uintptr_t)j.y % 16 == 0 && j.y_ld * es % 16 == 0 && box_map(&um, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es, j.y, j.M, j.N, j.y_ld, 32);
+  else q.wide = (uintptr_t)j.y % 16 == 0 && j.y_ld * es % 16 == 0 && f8_box_map(&um, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es, j.y, j.M, j.N, j.y_ld, 32);
   const auto kern = gated ? f8_tc_kernel<true> : f8_tc_kernel<false>;
   const uint32_t smem = gated ? Cfg<true>::kSmem : Cfg<false>::kSmem, pairs = (uint32_t)c->sm_count / 2u;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
