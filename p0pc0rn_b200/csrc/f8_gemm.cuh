@@ -71,4 +71,18 @@ __device__ __forceinline__ bool warp_wait_two(uint64_t *x, uint32_t px, uint64_t
   return __all_sync(0xffffffffu, ok);
 }
 
+// pairs of f32 in 64 bits: the instructions that take two at once leave issue slots (and instruction fetches) to others
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t twice(float f) { return pair(__float_as_uint(f), __float_as_uint(f)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void fma2(uint64_t &a, uint64_t d, uint64_t f) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(d), "l"(f)); }
+
 }  // namespace f8tc

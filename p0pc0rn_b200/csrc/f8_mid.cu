@@ -19,7 +19,8 @@ constexpr uint32_t kScales = 4;           // groups of blocks whose scales are o
 
 template <int TN, int MATS>
 struct Cfg {
-  static constexpr uint32_t kThreads = 128 + 128 * MATS;   // warps 0: copies; 1: MMAs; 2: scales; 3: none; then four a matrix: sums
+  static constexpr uint32_t kParts = TN == 128 ? 2 : 1;    // of a matrix's tokens: 64 at most to a thread
+  static constexpr uint32_t kSets = MATS * kParts, kThreads = 128 + 128 * kSets;   // warps 0: copies; 1: MMAs; 2: scales; 3: none; then four a part: sums
   static constexpr uint32_t kStage = MATS * kW + TN * 128, kFit = 200u * 1024 / kStage, kStages = kFit < 6 ? kFit : 6;
   static constexpr uint32_t kTile = TN * 512;              // a matrix's sums as f32
   static constexpr uint32_t kG = TN < 64 ? 64 / TN : 1;    // blocks of a group: its sums are waited for and read at once
@@ -81,11 +82,11 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     }
     for (uint32_t i = 0; i < kScales; i++) {
       tc::mbar_init(&sfull[i], 32);
-      tc::mbar_init(&sread[i], 4 * MATS);
+      tc::mbar_init(&sread[i], 4 * C::kSets);
     }
     for (uint32_t i = 0; i < 2; i++) {
       tc::mbar_init(&dfull[i], 1);
-      tc::mbar_init(&dread[i], 4 * MATS);
+      tc::mbar_init(&dread[i], 4 * C::kSets);
     }
     tc::mbar_init(&mdone, 1);
     abort_word = 0u;
@@ -128,8 +129,7 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     constexpr uint32_t idesc = tc::idesc_f16_f32(128, TN);   // e4m3 has the format number 0, too
     for (uint32_t kb = k_lo; kb < k_hi; kb++) {
       const uint32_t i = kb - k_lo, s = i % NS, grp = i / G, b = grp & 1u, in = i % G;
-      if (in == 0u && grp >= 2u && !(ok = warp_wait(&dread[b], ((grp >> 1) - 1u) & 1u, abort_flag, q.err, 0x8a3u))) break;
-      if (!(ok = warp_wait(&full[s], i / NS & 1u, abort_flag, q.err, 0x8a2u))) break;
+      if (!(ok = warp_wait_two(&full[s], i / NS & 1u, in == 0u && grp >= 2u ? &dread[b] : nullptr, ((grp >> 1) - 1u) & 1u, abort_flag, q.err, 0x8a2u))) break;
       tc::fence_after();
       if (elect()) {
         const uint64_t xd = tc::desc_sw128(tc::smem_u32(ring + s * C::kStage + MATS * kW));
@@ -159,14 +159,18 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= 4) {
-    // ------------------------------------------------------------ sums: row r of matrix a
-    const uint32_t a = (warp >> 2) - 1u, r = (warp & 3u) * 32u + lane, base = tmem + (((warp & 3u) * 32u) << 16) + a * G * TN;
+    // ------------------------------------------------------------ sums: row r of matrix a, tokens t0 .. t0 + TW - 1
+    constexpr uint32_t TW = TN / C::kParts;
+    const uint32_t set = (warp >> 2) - 1u, a = set / C::kParts, t0 = set % C::kParts * TW, r = (warp & 3u) * 32u + lane;
+    const uint32_t base = tmem + (((warp & 3u) * 32u) << 16) + a * G * TN + t0;
     const float *ws = a ? j.u.s + (uint64_t)nb * j.u.s_ld : j.w.s + (uint64_t)nb * j.w.s_ld;
-    float acc[TN], w[G], wn[G];
+    uint64_t acc[TW / 2];   // pairs of tokens
+    float w[G], wn[G];
 #pragma unroll
-    for (int e = 0; e < TN; e++) acc[e] = 0.0f;
+    for (int e = 0; e < TW / 2; e++) acc[e] = 0ull;
 #pragma unroll
     for (uint32_t g = 0; g < G; g++) wn[g] = k_lo + g < k_hi ? ws[k_lo + g] : 0.0f;
+    bool hot = false;   // the next group's sums and scales were seen
     for (uint32_t kb = k_lo, grp = 0; kb < k_hi; kb += G, grp++) {
       const uint32_t s = grp % kScales, b = grp & 1u;
 #pragma unroll
@@ -174,29 +178,28 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
         w[g] = wn[g];
         if (kb + G + g < k_hi) wn[g] = ws[kb + G + g];
       }
-      if (!(ok = warp_wait_two(&dfull[b], (grp >> 1) & 1u, &sfull[s], grp / kScales & 1u, abort_flag, q.err, 0x8a5u))) break;
+      if (!__all_sync(0xffffffffu, hot) && !(ok = warp_wait_two(&dfull[b], (grp >> 1) & 1u, &sfull[s], grp / kScales & 1u, abort_flag, q.err, 0x8a5u))) break;
       tc::fence_after();
 #pragma unroll
-      for (uint32_t c0 = 0; c0 < G * TN; c0 += 64u) {
+      for (uint32_t c0 = 0; c0 < G * TW; c0 += 64u) {
         uint32_t d[2][32];
         tc::tmem_ld32(base + b * MATS * G * TN + c0, d[0]);
         tc::tmem_ld32(base + b * MATS * G * TN + c0 + 32u, d[1]);
         tc::tmem_wait_ld();
-        if (c0 + 64u == G * TN) {
+        if (c0 + 64u == G * TW) {
           tc::fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&dread[b]);
+          hot = tc::mbar_test(&dfull[b ^ 1u], ((grp + 1u) >> 1) & 1u) && tc::mbar_test(&sfull[(grp + 1u) % kScales], (grp + 1u) / kScales & 1u);
         }
 #pragma unroll
         for (uint32_t e = 0; e < 64u; e += 4u) {
-          const uint32_t g = (c0 + e) / TN, t = (c0 + e) % TN;
+          const uint32_t g = (c0 + e) / TW, t = (c0 + e) % TW;
           if (G > 1u && kb + g >= k_hi) break;   // a last group may be short
-          const float4 x = *reinterpret_cast<const float4 *>(&scales[s][c0 + e]);
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&scales[s][t0 + c0 + e]);
           const uint32_t *v = &d[e >> 5][e & 31u];
-          acc[t] = fmaf(__uint_as_float(v[0]), x.x * w[g], acc[t]);
-          acc[t + 1] = fmaf(__uint_as_float(v[1]), x.y * w[g], acc[t + 1]);
-          acc[t + 2] = fmaf(__uint_as_float(v[2]), x.z * w[g], acc[t + 2]);
-          acc[t + 3] = fmaf(__uint_as_float(v[3]), x.w * w[g], acc[t + 3]);
+          fma2(acc[t / 2], pair(v[0], v[1]), mul2(x.x, twice(w[g])));
+          fma2(acc[t / 2 + 1], pair(v[2], v[3]), mul2(x.y, twice(w[g])));
         }
       }
       __syncwarp();
@@ -204,9 +207,14 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     }
     // the last block's sums were waited for, so every copy has landed and every MMA has read it: the ring is free
     if (ok) {
-      float *to = reinterpret_cast<float *>(ring + a * C::kTile) + r;
+      float *to = reinterpret_cast<float *>(ring + a * C::kTile) + t0 * 128u + r;
 #pragma unroll
-      for (int e = 0; e < TN; e++) to[e * 128] = acc[e];
+      for (int e = 0; e < TW / 2; e++) {
+        float lo, hi;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(acc[e]));
+        to[2 * e * 128] = lo;
+        to[(2 * e + 1) * 128] = hi;
+      }
     }
   }
   __syncthreads();

@@ -79,14 +79,6 @@ __device__ __forceinline__ void tmem_ld64(uint32_t t, uint64_t (&d)[32]) {
       : "r"(t)
       : "memory");
 }
-// two f32 FMAs: a += d * (f, f)
-__device__ __forceinline__ void fma2(uint64_t &a, uint64_t d, uint64_t f) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(d), "l"(f)); }
-__device__ __forceinline__ uint64_t twice(float f) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(f));
-  return r;
-}
-
 // tile t: its row and column of tiles. Column by column within groups of kGroup rows
 __device__ __forceinline__ uint2 tile_at(const TcJob &q, uint32_t t) {
   const uint32_t per = kGroup * q.nt, grp = t / per, r0 = grp * kGroup, rows = min(kGroup, q.mt - r0), in = t - grp * per;
