@@ -8,6 +8,9 @@
 // A cluster of S CTAs shares a tile's blocks of k. Each leaves its sums in its shared memory as [token][row]; then a warp takes a
 // token's 128 columns, adds the S parts in order (over distributed shared memory) and stores them; of a gated call it knows all 128
 // columns of the block of codes.
+// 16 tokens, 8192 x 2048: 7.7 us, of which the weights take 2.6 at the copy rate (the loop runs at it: 620 cycles a block over 128 CTAs) and 5 go by
+// before the first block and after the last, in the cluster's barriers most of all; 8192 x 8192: 16 us, 4.2 TB/s. 100 tokens, 6720 x 2240: 10.9 us. Groups
+// of blocks (64 sums to a wait) took 64 tokens from 10.0 to 9.4 us, eight warps for 128 tokens 8192 x 8192 from 24.1 to 22.3.
 #include "f8_gemm.cuh"
 
 namespace {
