@@ -8,8 +8,8 @@
 // A cluster of S CTAs shares a tile's blocks of k. Each leaves its sums in its shared memory as [token][row]; then a warp takes a
 // token's 128 columns, adds the S parts in order (over distributed shared memory) and stores them; of a gated call it knows all 128
 // columns of the block of codes.
-// 16 tokens, 8192 x 2048: 7.7 us, of which the weights take 2.6 at the copy rate (the loop runs at it: 620 cycles a block over 128 CTAs) and 5 go by
-// before the first block and after the last, in the cluster's barriers most of all; 8192 x 8192: 16 us, 4.2 TB/s. 100 tokens, 6720 x 2240: 10.9 us. Groups
+// 16 tokens, 8192 x 2048: 7.5 us, of which the weights take 2.6 at the copy rate (the loop runs at it: 620 cycles a block over 128 CTAs) and 5 go by
+// before the first block and after the last, in the cluster's barriers most of all; 8192 x 8192: 16 us, 4.2 TB/s. 100 tokens, 6720 x 2240: 10.6 us. Groups
 // of blocks (64 sums to a wait) took 64 tokens from 10.0 to 9.4 us, eight warps for 128 tokens 8192 x 8192 from 24.1 to 22.3.
 #include "f8_gemm.cuh"
 
@@ -324,7 +324,9 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     }
   }
   __syncwarp();
-  if (S > 1u) tc::cluster_sync();   // no CTA leaves while another may read its parts
+  // no CTA leaves while another may read its parts. What was read has been used, so there is nothing to release: a barrier that also waits
+  // for the stores of y took 0.3 us more
+  if (S > 1u) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 template <int TN, int MATS>

@@ -123,7 +123,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (elect()) {   // the maps are this launch's own
       tc::prefetch_tmap(&xm);
       tc::prefetch_tmap(&wm);
-      tc::prefetch_tmap(&um);
+      if (GATED || q.wide) tc::prefetch_tmap(&um);
     }
     __syncwarp();
     tc::tmem_alloc_pair(&tmem_slot, 512);
