@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t even_bar(uint64_t *bar) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tc::smem_u32(bar)));
   return r;
 }
-// a 2D tile out of shared memory; what lies beyond the matrix is not stored
+// a 2D tile out of shared memory; rows beyond the matrix are not stored, nor whole 16 bytes beyond a row
 __device__ __forceinline__ void tma_store(const void *tmap, const void *src, int32_t c0, int32_t c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(tc::smem_u32(src)), "r"(c0), "r"(c1) : "memory");
 }
@@ -339,7 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               }
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
-          } else {   // rows that do not start on 16 bytes: a lane a column, row by row
+          } else {   // rows that do not start or end on 16 bytes: a lane a column, row by row
             __syncwarp();
             for (uint32_t row = 0; row < 32u && mw + row < j.M; row++)
 #pragma unroll
@@ -395,7 +395,8 @@ p0_status f8_tc_launch(p0_ctx *c, const GemmJob &j, const F8Mat &y, const char *
     return p0_fail(c, P0_EDEVICE, "%s: tensor map encode failed", op);
   const uint32_t es = f16 ? 2 : 4;
   if (gated) q.wide = (uintptr_t)y.q % 32 == 0 && y.ld % 32 == 0;
-  else q.wide = (uintptr_t)j.y % 16 == 0 && j.y_ld * es % 16 == 0 && f8_box_map(&um, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es, j.y, j.M, j.N, j.y_ld, 32);
+  // a tensor copy ends a row in whole 16 bytes: a row that ends inside of them is stored the other way, or what lies behind it would be lost
+  else q.wide = (uintptr_t)j.y % 16 == 0 && j.y_ld * es % 16 == 0 && j.N * es % 16 == 0 && f8_box_map(&um, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es, j.y, j.M, j.N, j.y_ld, 32);
   const auto kern = gated ? f8_tc_kernel<true> : f8_tc_kernel<false>;
   const uint32_t smem = gated ? Cfg<true>::kSmem : Cfg<false>::kSmem, pairs = (uint32_t)c->sm_count / 2u;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

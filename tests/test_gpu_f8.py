@@ -279,6 +279,14 @@ def test_gemm_layouts(g, M, epi, ld, off):
     run_gemm(g, M, 280, 400, epi, lay=LAY, ylay=ylay)
 
 
+@pytest.mark.parametrize("epi", ["f16", "f32", "geglu"])
+@pytest.mark.parametrize("ld,off", [(1120, 32), (1109, 3), (1116, 4)])     # rows of y on 16 bytes, on none, f32 alone
+def test_gemm_layouts_many_tokens(g, epi, ld, off):
+    M, N, K = 2100, 1101, 400
+    lay = {"x": dict(ld=464, off=48, s_ld=2107, s_off=3), "w": dict(ld=448, off=16, s_ld=9, s_off=1), "u": dict(ld=416, off=64, s_ld=4, s_off=7)}
+    run_gemm(g, M, N, K, epi, bias=epi == "f32", lay=lay, ylay=dict(ld=ld, off=off) if epi != "geglu" else dict(ld=-(-ld // 16) * 16, off=off // 16 * 16, s_ld=M + 5, s_off=off & 7))
+
+
 @pytest.mark.parametrize("M,N,K", [(1100, 1300, 700), (2100, 520, 2240), (300, 4000, 1024)])
 @pytest.mark.parametrize("epi", ["f16", "f32", "geglu"])
 def test_gemm_large(g, M, N, K, epi):
