@@ -474,7 +474,10 @@ typedef struct {
 p0_status p0_norm_f8(p0_ctx *ctx, const p0_norm_f8_args *a);
 
 /* gemmF8: Y[m, n] = sum_k X[m, k] * W[n, k] of the values that x (M rows of K, P0_F8_ROW) and w (N rows of K, P0_F8_TILE) stand for:
- * the products of a block of 128 k are summed in the tensor cores' f32, then scaled and added up in f32.
+ * the products of a block of 128 k are summed in the tensor cores' f32, then scaled and added up in f32. A block's factor is xs * ws, x's
+ * scale times w's, rounded to f32 first. Where that is below 2^-126 (or rounds to zero) a result is off by up to 2^-125 a block besides.
+ * It must stay below 2^128: a block beyond adds an infinity, or NaN if its sum is 0. Blocks of x up to 2^90 and of w up to 2^50 in magnitude
+ * stay far below; a block of x with an infinity (scale 2^119) does where w's is below 2^17.
  *   P0_F8EPI_F16, _F32      y: rows of f16 or f32, element (m, n) at y.off + m * y.ld + n (elements, y.ld 0 = N; y.s not used);
  *                           with bv: + bv[bv_off + n] before the rounding
  *   P0_F8EPI_SWIGLU, _GEGLU y: codes (P0_F8_ROW) of act(X W^T) * (X U^T), u as w; act = silu or the tanh form of gelu, in f32
