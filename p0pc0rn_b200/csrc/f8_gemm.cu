@@ -10,6 +10,8 @@
 // fragment is free as long as both operands share it, so 16 consecutive bytes serve two instructions. Tokens are the n side,
 // loaded the same way. Each block's sums are scaled and added in f32; the warps' parts meet in shared memory, in order.
 // 1 token, 2048 x 2048: 3.5 us (launch, a round trip to memory, the join); 8 tokens, 8192 x 2048: 6.2 us, 2.7 TB/s; 8192 x 8192: 16 us, 4.2 TB/s.
+#include <cstdlib>
+
 #include "f8_gemm.cuh"
 
 namespace {
@@ -123,6 +125,8 @@ extern "C" p0_status p0_gemm_f8(p0_ctx *c, const p0_gemm_f8_args *a) {
   j.K = a->K;
   j.KB = (a->K + kF8Block - 1) / kF8Block;
   j.epi = a->epi;
+  const char *limit = getenv("P0MM_F8_POLLS");   // for tests of what follows a wait that gives up
+  j.polls = limit ? (uint32_t)strtoul(limit, nullptr, 10) : P0_SPIN_LIMIT;
   p0_status st;
   if ((st = f8_view(c, a->x, M, K, false, op, "x", &j.x))) return st;
   if ((st = f8_view(c, a->w, N, K, true, op, "w", &j.w))) return st;

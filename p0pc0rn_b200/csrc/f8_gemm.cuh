@@ -9,6 +9,7 @@ struct GemmJob {
   uint8_t *y;              // f16 or f32 rows of y_ld
   uint64_t y_ld;
   uint32_t M, N, K, KB, epi;
+  uint32_t polls;          // after which the copies' waits give up. The others' limit is a constant: with an argument few tokens took 0.2 us more
 };
 
 // the form for many tokens (f8_tc.cu); y: where the codes of a gated call go
@@ -50,13 +51,14 @@ __device__ __forceinline__ bool elect() {
   return p != 0u;
 }
 // a warp's waits: every lane returns the same
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *err, uint32_t code) {
-  return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort, err, code, P0_SPIN_LIMIT));
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *err, uint32_t code, uint32_t polls) {
+  return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort, err, code, polls));
 }
 // for two phases (y may be null): a wait that is over costs its latency, here once for both
-__device__ __forceinline__ bool warp_wait_two(uint64_t *x, uint32_t px, uint64_t *y, uint32_t py, volatile uint32_t *abort, uint32_t *err, uint32_t code) {
+__device__ __forceinline__ bool warp_wait_two(uint64_t *x, uint32_t px, uint64_t *y, uint32_t py, volatile uint32_t *abort, uint32_t *err, uint32_t code,
+                                              uint32_t polls) {
   bool ok = false;
-  for (uint32_t i = 0; i < P0_SPIN_LIMIT; i++) {
+  for (uint32_t i = 0; i < polls; i++) {
     const bool a = tc::mbar_try(x, px), b = !y || tc::mbar_try(y, py);
     if (a && b) {
       ok = true;

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     // ------------------------------------------------------------ copies
     for (uint32_t kb = k_lo; kb < k_hi; kb++) {
       const uint32_t i = kb - k_lo, s = i % NS;
-      if (i >= NS && !(ok = warp_wait(&empty[s], (i / NS & 1u) ^ 1u, abort_flag, q.err, 0x8a1u))) break;
+      if (i >= NS && !(ok = warp_wait(&empty[s], (i / NS & 1u) ^ 1u, abort_flag, q.err, 0x8a1u, j.polls))) break;
       if (elect()) {
         uint8_t *to = ring + s * C::kStage;
         tc::mbar_expect_tx(&full[s], C::kStage);
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     constexpr uint32_t idesc = tc::idesc_f16_f32(128, TN);   // e4m3 has the format number 0, too
     for (uint32_t kb = k_lo; kb < k_hi; kb++) {
       const uint32_t i = kb - k_lo, s = i % NS, grp = i / G, b = grp & 1u, in = i % G;
-      if (!(ok = warp_wait_two(&full[s], i / NS & 1u, in == 0u && grp >= 2u ? &dread[b] : nullptr, ((grp >> 1) - 1u) & 1u, abort_flag, q.err, 0x8a2u))) break;
+      if (!(ok = warp_wait_two(&full[s], i / NS & 1u, in == 0u && grp >= 2u ? &dread[b] : nullptr, ((grp >> 1) - 1u) & 1u, abort_flag, q.err, 0x8a2u, P0_SPIN_LIMIT))) break;
       tc::fence_after();
       if (elect()) {
         const uint64_t xd = tc::desc_sw128(tc::smem_u32(ring + s * C::kStage + MATS * kW));
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     // ------------------------------------------------------------ x's scales
     for (uint32_t kb = k_lo, grp = 0; kb < k_hi; kb += G, grp++) {
       const uint32_t s = grp % kScales;
-      if (!(ok = warp_wait(&sread[s], (grp / kScales & 1u) ^ 1u, abort_flag, q.err, 0x8a4u))) break;
+      if (!(ok = warp_wait(&sread[s], (grp / kScales & 1u) ^ 1u, abort_flag, q.err, 0x8a4u, j.polls))) break;
 #pragma unroll
       for (uint32_t e = lane; e < G * TN; e += 32u) {
         const uint32_t k = kb + e / TN, t = e % TN;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
         w[g] = wn[g];
         if (kb + G + g < k_hi) wn[g] = ws[kb + G + g];
       }
-      if (!__all_sync(0xffffffffu, hot) && !(ok = warp_wait_two(&dfull[b], (grp >> 1) & 1u, &sfull[s], grp / kScales & 1u, abort_flag, q.err, 0x8a5u))) break;
+      if (!__all_sync(0xffffffffu, hot) && !(ok = warp_wait_two(&dfull[b], (grp >> 1) & 1u, &sfull[s], grp / kScales & 1u, abort_flag, q.err, 0x8a5u, P0_SPIN_LIMIT))) break;
       tc::fence_after();
 #pragma unroll
       for (uint32_t c0 = 0; c0 < G * TW; c0 += 64u) {
@@ -222,17 +222,18 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
   }
   __syncthreads();
   const bool failed = abort_word != 0u;
-  if (failed && lane == 0) {   // a wait gave up (q.err says which): nothing may be in flight when the CTA leaves. Bounded
+  if (failed) {   // a wait gave up (q.err says which): nothing may be in flight when the CTA leaves. Bounded
     volatile uint32_t never = 0;
-    if (warp == 0)
+    if (warp == 0 && lane == 0)
       for (uint32_t i = 0; i < NS && i < issued; i++) {
         const uint32_t last = (issued - 1u - i) / NS * NS + i;   // the last use of stage i
         never = 0;
-        tc::mbar_wait(&full[i], (last / NS) & 1u, &never, q.err, 0x8a7u, kDrain);
+        tc::mbar_wait(&full[i], (last / NS) & 1u, &never, q.err, 0x18a7u, kDrain);
       }
-    if (warp == 1) {
-      tc::mma_commit(&mdone);
-      tc::mbar_wait(&mdone, 0, &never, q.err, 0x8a8u, kDrain);
+    if (warp == 1) {   // a commit is for what its own thread issued: the elected one, as above
+      if (elect()) tc::mma_commit(&mdone);
+      __syncwarp();
+      warp_wait(&mdone, 0, &never, q.err, 0x18a8u, kDrain);
     }
   }
   __syncwarp();

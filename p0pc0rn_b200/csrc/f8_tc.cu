@@ -145,7 +145,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint2 at = tile_at(q, t);
         const int32_t m0 = (int32_t)(at.x * 256u + rank * 128u), n0 = (int32_t)((GATED ? at.y * 128u : at.y * 256u) + rank * 64u);
         for (uint32_t kb = 0; kb < j.KB; kb++) {
-          if (!(ok = warp_wait(&empty[s], (round & 1u) ^ 1u, abort_flag, q.err, 0x8f1u))) break;
+          if (!(ok = warp_wait(&empty[s], (round & 1u) ^ 1u, abort_flag, q.err, 0x8f1u, P0_SPIN_LIMIT))) break;
           if (elect()) {
             if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * kStage);
             const uint32_t bar = even_bar(&full[s]);
@@ -165,7 +165,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (uint32_t t = first; t < q.tiles && ok; t += step)
         for (uint32_t kb = 0; kb < j.KB; kb++, c++) {
           const uint64_t ad = tc::desc_sw128(tc::smem_u32(ring + s * kStage)), bd = tc::desc_sw128(tc::smem_u32(ring + s * kStage + kBox));
-          if (!(ok = warp_wait_two(&ready[s], round & 1u, c >= 2u ? &dread[c & 1u] : nullptr, ((c >> 1) - 1u) & 1u, abort_flag, q.err, 0x8f3u))) break;
+          if (!(ok = warp_wait_two(&ready[s], round & 1u, c >= 2u ? &dread[c & 1u] : nullptr, ((c >> 1) - 1u) & 1u, abort_flag, q.err, 0x8f3u, P0_SPIN_LIMIT))) break;
           tc::fence_after();
           if (elect()) {
 #pragma unroll
@@ -236,7 +236,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint64_t f[2] = {twice(x[i] * __shfl_sync(0xffffffffu, wc[0], (k0 + i) & 31u)), twice(x[i] * __shfl_sync(0xffffffffu, wc[1], (k0 + i) & 31u))};
           const bool here = k0 + i + 4u < KB;
           x[i] = j.x.s[(uint64_t)(here ? k0 + i + 4u : i) * j.x.s_ld + (here ? row : row_next)];
-          if (!__all_sync(0xffffffffu, hot)) ok = warp_wait(&dfull[c & 1u], (c >> 1) & 1u, abort_flag, q.err, 0x8f4u);
+          if (!__all_sync(0xffffffffu, hot)) ok = warp_wait(&dfull[c & 1u], (c >> 1) & 1u, abort_flag, q.err, 0x8f4u, P0_SPIN_LIMIT);
           if (!ok) break;
           tc::fence_after();
 #pragma unroll
