@@ -125,8 +125,12 @@ extern "C" p0_status p0_gemm_f8(p0_ctx *c, const p0_gemm_f8_args *a) {
   j.K = a->K;
   j.KB = (a->K + kF8Block - 1) / kF8Block;
   j.epi = a->epi;
-  const char *limit = getenv("P0MM_F8_POLLS");   // for tests of what follows a wait that gives up
-  j.polls = limit ? (uint32_t)strtoul(limit, nullptr, 10) : P0_SPIN_LIMIT;
+  j.polls[0] = j.polls[1] = P0_SPIN_LIMIT;
+  if (const char *limit = getenv("P0MM_F8_POLLS")) {   // for tests of what follows a wait that gives up: one limit, or two
+    char *odd;
+    j.polls[0] = j.polls[1] = (uint32_t)strtoul(limit, &odd, 10);
+    if (*odd == ',') j.polls[1] = (uint32_t)strtoul(odd + 1, nullptr, 10);
+  }
   p0_status st;
   if ((st = f8_view(c, a->x, M, K, false, op, "x", &j.x))) return st;
   if ((st = f8_view(c, a->w, N, K, true, op, "w", &j.w))) return st;

@@ -9,7 +9,8 @@ struct GemmJob {
   uint8_t *y;              // f16 or f32 rows of y_ld
   uint64_t y_ld;
   uint32_t M, N, K, KB, epi;
-  uint32_t polls;          // after which the copies' waits give up. The others' limit is a constant: with an argument few tokens took 0.2 us more
+  uint32_t polls[2];       // after which the copies' waits give up (of a pair's even and odd CTA). The others' limit is a constant: with an
+                           // argument few tokens took 0.2 us more
 };
 
 // the form for many tokens (f8_tc.cu); y: where the codes of a gated call go

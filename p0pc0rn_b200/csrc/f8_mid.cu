@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     // ------------------------------------------------------------ copies
     for (uint32_t kb = k_lo; kb < k_hi; kb++) {
       const uint32_t i = kb - k_lo, s = i % NS;
-      if (i >= NS && !(ok = warp_wait(&empty[s], (i / NS & 1u) ^ 1u, abort_flag, q.err, 0x8a1u, j.polls))) break;
+      if (i >= NS && !(ok = warp_wait(&empty[s], (i / NS & 1u) ^ 1u, abort_flag, q.err, 0x8a1u, j.polls[0]))) break;
       if (elect()) {
         uint8_t *to = ring + s * C::kStage;
         tc::mbar_expect_tx(&full[s], C::kStage);
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
     // ------------------------------------------------------------ x's scales
     for (uint32_t kb = k_lo, grp = 0; kb < k_hi; kb += G, grp++) {
       const uint32_t s = grp % kScales;
-      if (!(ok = warp_wait(&sread[s], (grp / kScales & 1u) ^ 1u, abort_flag, q.err, 0x8a4u, j.polls))) break;
+      if (!(ok = warp_wait(&sread[s], (grp / kScales & 1u) ^ 1u, abort_flag, q.err, 0x8a4u, j.polls[0]))) break;
 #pragma unroll
       for (uint32_t e = lane; e < G * TN; e += 32u) {
         const uint32_t k = kb + e / TN, t = e % TN;

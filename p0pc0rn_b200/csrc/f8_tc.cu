@@ -47,6 +47,19 @@ __device__ __forceinline__ uint32_t even_bar(uint64_t *bar) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tc::smem_u32(bar)));
   return r;
 }
+// a word of CTA `rank` of the pair, at this place in shared memory
+__device__ __forceinline__ void store_rank(uint32_t *p, uint32_t rank, uint32_t v) {
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n st.shared::cluster.u32 [a], %2;\n}" ::"r"(tc::smem_u32(p)), "r"(rank), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t load_rank(const uint32_t *p, uint32_t rank) {
+  uint32_t v;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.u32 %0, [a];\n}" : "=r"(v) : "r"(tc::smem_u32(p)), "r"(rank) : "memory");
+  return v;
+}
+// counts bytes on a barrier as a copy would
+__device__ __forceinline__ void complete_tx(uint64_t *bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(bytes) : "memory");
+}
 // a 2D tile out of shared memory; rows beyond the matrix are not stored, nor whole 16 bytes beyond a row
 __device__ __forceinline__ void tma_store(const void *tmap, const void *src, int32_t c0, int32_t c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(tc::smem_u32(src)), "r"(c0), "r"(c1) : "memory");
@@ -100,7 +113,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // full (even CTA's): both CTAs' rows of a stage are there; ready: that was seen; empty: its MMAs are done; dfull: a block's sums are there;
   // dread: both CTAs' warps have read them
   __shared__ __align__(8) uint64_t full[NS], ready[NS], empty[NS], dfull[2], dread[2], mdone;
-  __shared__ uint32_t tmem_slot, abort_word;
+  __shared__ uint32_t tmem_slot, abort_word, issued_word, failed_word;   // failed_word: abort_word of either CTA
   __shared__ float peak[GATED ? 2 : 1][2][GATED ? 128 : 1];   // [tile parity][half of the columns][row]
   volatile uint32_t *abort_flag = &abort_word;
   const GemmJob &j = q.j;
@@ -116,7 +129,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tc::mbar_init(&dread[i], 2 * kSums / 32);
     }
     tc::mbar_init(&mdone, 1);
-    abort_word = 0u;
+    abort_word = failed_word = 0u;
     tc::fence_mbar_init();
   }
   if (warp == 0) {
@@ -145,7 +158,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint2 at = tile_at(q, t);
         const int32_t m0 = (int32_t)(at.x * 256u + rank * 128u), n0 = (int32_t)((GATED ? at.y * 128u : at.y * 256u) + rank * 64u);
         for (uint32_t kb = 0; kb < j.KB; kb++) {
-          if (!(ok = warp_wait(&empty[s], (round & 1u) ^ 1u, abort_flag, q.err, 0x8f1u, P0_SPIN_LIMIT))) break;
+          if (round && !(ok = warp_wait(&empty[s], (round & 1u) ^ 1u, abort_flag, q.err, 0x8f1u, j.polls[rank]))) break;
           if (elect()) {
             if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * kStage);
             const uint32_t bar = even_bar(&full[s]);
@@ -158,6 +171,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (++s == NS) s = 0, round++;
         }
       }
+      if (lane == 0) issued_word = issued;
     } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- the pair's MMAs
       constexpr uint32_t idesc = tc::idesc_f16_f32(256, 256);   // e4m3 has the format number 0, too
@@ -358,22 +372,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (!GATED && q.wide && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncthreads();
-  if (abort_word && lane == 0) {   // a wait gave up (q.err says which): nothing may be in flight when the pair leaves. Bounded
-    volatile uint32_t never = 0;
-    if (warp == 0 && rank == 0)
-      for (uint32_t i = 0; i < NS && i < issued; i++) {
-        const uint32_t last = (issued - 1u - i) / NS * NS + i;   // the last use of stage i
-        never = 0;
-        tc::mbar_wait(&full[i], (last / NS) & 1u, &never, q.err, 0x8f5u, kDrain);
-      }
-    if (warp == 1 && rank == 0) {
-      tc::mma_commit_pair(&mdone);
-      tc::mbar_wait(&mdone, 0, &never, q.err, 0x8f6u, kDrain);
-    }
-  }
+  if (tid < 2 && abort_word) store_rank(&failed_word, tid, 1u);
   __syncwarp();
   tc::fence_before();
   tc::cluster_sync();   // neither CTA frees its tensor memory or exits while the other may still use it
+  if (failed_word) {    // a wait gave up (q.err says which): nothing may be in flight when the pair leaves. Both CTAs' warps have ended their loops. Bounded
+    volatile uint32_t never = 0;
+    if (warp == 0 && lane == 0 && rank == 0) {
+      const uint32_t mine = issued_word, theirs = load_rank(&issued_word, 1);
+      for (uint32_t i = 0; i < NS; i++) {
+        // uses of stage i. They differ by one at most: a stage is free again for both when its MMAs have read both CTAs' halves
+        const uint32_t a = mine > i ? (mine - 1u - i) / NS + 1u : 0u, b = theirs > i ? (theirs - 1u - i) / NS + 1u : 0u;
+        if (a > b) complete_tx(&full[i], kStage);             // the odd CTA's half was expected and does not come
+        else if (b > a) tc::mbar_expect_tx(&full[i], kStage);   // its half comes, with none from here
+        never = 0;
+        if (a || b) tc::mbar_wait(&full[i], (max(a, b) - 1u) & 1u, &never, q.err, 0x18f5u, kDrain);
+      }
+    }
+    if (warp == 1) {   // a commit is for what its own thread issued: the elected one, as above. It arrives in both CTAs
+      if (rank == 0 && elect()) tc::mma_commit_pair(&mdone);
+      __syncwarp();
+      warp_wait(&mdone, 0, &never, q.err, 0x18f6u, kDrain);
+    }
+    __syncwarp();
+    tc::cluster_sync();
+  }
   if (warp == 0) {
     tc::fence_after();
     tc::tmem_dealloc_pair(tmem, 512);
