@@ -127,6 +127,9 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
       __syncwarp();
       issued++;
     }
+    // the CTA does not leave before the last MMAs have signalled that their stages are free
+    if (ok && lane < NS && lane < issued) tc::mbar_wait(&empty[lane], ((issued - 1u - lane) / NS) & 1u, abort_flag, q.err, 0x8a6u, P0_SPIN_LIMIT);
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMAs
     constexpr uint32_t idesc = tc::idesc_f16_f32(128, TN);   // e4m3 has the format number 0, too

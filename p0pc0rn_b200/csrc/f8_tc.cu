@@ -172,6 +172,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       }
       if (lane == 0) issued_word = issued;
+      // the last MMAs signal both CTAs that their stages are free: neither leaves before that has arrived (the results take longer)
+      if (ok && lane < NS && lane < issued) tc::mbar_wait(&empty[lane], ((issued - 1u - lane) / NS) & 1u, abort_flag, q.err, 0x8f7u, P0_SPIN_LIMIT);
+      __syncwarp();
     } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- the pair's MMAs
       constexpr uint32_t idesc = tc::idesc_f16_f32(256, 256);   // e4m3 has the format number 0, too
