@@ -539,7 +539,7 @@ p0_status p0_norm_f8(p0_ctx *c, const p0_norm_f8_args *a) {
   if (a->h.id && (st = f8_rows(c, a->h, a->h_off, a->h_ld, M, D, a->type, op, "h", &h, &h_ld, &w2))) return st;
   j.h = (uint8_t *)h;
   j.h_ld = h_ld;
-  const bool in_place = h == j.x && h_ld == ld;
+  const bool in_place = h == j.x && (h_ld == ld || M == 1);   // the stride of one row is not looked at
   j.store = !in_place || j.parts || a->scale != 1.0f;
   const uint64_t hn = ((M - 1) * h_ld + D) * es;
   P0Range rw, rp, rs;
