@@ -481,6 +481,7 @@ p0_status p0_norm_f8(p0_ctx *ctx, const p0_norm_f8_args *a);
  *   P0_F8EPI_F16, _F32      y: rows of f16 or f32, element (m, n) at y.off + m * y.ld + n (elements, y.ld 0 = N; y.s not used);
  *                           with bv: + bv[bv_off + n] before the rounding
  *   P0_F8EPI_SWIGLU, _GEGLU y: codes (P0_F8_ROW) of act(X W^T) * (X U^T), u as w; act = silu or the tanh form of gelu, in f32
+ *                           (an act below 2^-119 may be 0)
  * The operator needs no packed form of its own: x, w and u are read as packF8 and normF8 write them. y lies apart from the inputs.
  * None of the three uses the context's workspace: they may be captured, and captured graphs may run side by side. */
 enum { P0_F8EPI_F16 = 0, P0_F8EPI_F32 = 1, P0_F8EPI_SWIGLU = 2, P0_F8EPI_GEGLU = 3 };

@@ -20,11 +20,12 @@ p0_status f8_mid_launch(p0_ctx *c, const GemmJob &j, const F8Mat &y, const char 
 uint32_t f8_mid_parts(const p0_ctx *c, uint32_t M, uint32_t N, uint32_t KB);
 
 // the gate of a gated epilogue: silu, or the tanh form of gelu as x * sigmoid(2 z), z = sqrt(2 / pi) (x + 0.044715 x^3)
-// e^-z = 2^hi 2^lo with hi + lo = -z log2(e) in two f32, 2^lo = 1 + lo ln 2 (lo is below 2^-17): a plain __expf's error grows with z and moved one code
-// in 60000 to its neighbour; expf and a rounded division took the gated form for many tokens from 78 to 93 us (1031 tokens, N = 8960, K = 2240)
+// e^-z = 2^hi 2^lo with hi + lo = -z log2(e) in two f32 (1.44269504 is log2(e) in f32, 1.92596303e-8 what that is too small by), 2^lo = 1 + lo ln 2 (lo is
+// below 2^-17): off by 1.25 * 2^-22, the gate by 2.5 * 2^-22, where z is exact. A plain __expf's error grows with z and moved one code in 60000
+// to its neighbour; expf and a rounded division took the gated form for many tokens from 78 to 93 us (1031 tokens, N = 8960, K = 2240)
 __device__ __forceinline__ float f8_gate(float x, uint32_t epi) {
   const float z = epi == P0_F8EPI_SWIGLU ? x : 1.5957691216057308f * fmaf(0.044715f * x, x * x, x);
-  const float zc = fminf(fmaxf(z, -88.0f), 88.0f);   // beyond it the gate is 0 (the quotient by more than 2^126) or 1
+  const float zc = fminf(fmaxf(z, -88.0f), 88.0f);   // beyond it the gate is 0 (a quotient by more than 2^126 is, from z = -87.3 on: x * gate is below 2^-119) or 1
   const float hi = -1.44269504f * zc, lo = fmaf(-1.44269504f, zc, -hi) - 1.92596303e-8f * zc;
   float p;
   asm("ex2.approx.f32 %0, %1;" : "=f"(p) : "f"(hi));
