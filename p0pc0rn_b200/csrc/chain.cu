@@ -616,7 +616,7 @@ p0_status p0_chain_run(p0_ctx *c, p0_chain *ch) {
     run.err = c->d_err;
     ChainKernel k = chain_kernel_for(ch->M);
     const size_t smem = chain_smem(ch->M, pc.nslot);
-    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    p0_smem_limit((const void *)k);
     int occ = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k, kCT, smem) != cudaSuccess || occ < 1) {
       cudaGetLastError();

@@ -227,7 +227,6 @@ __device__ __forceinline__ Raw<F16> settle(Vals &x, const Vals &t, float scale) 
   }
   return r;
 }
-constexpr uint32_t kRingMost = 220u * 1024u;   // shared memory that a CTA of kRing may ask for
 enum { kScalar = 0, kDirect = 1, kRing = 2 };   // rows that start anywhere; on 16 bytes, loaded as they are needed; ahead
 template <bool XF16, bool TF16, int MODE, bool POST>
 __global__ void __launch_bounds__(MODE == kDirect ? 512 : 1024) f8_norm_kernel(NormJob j) {
@@ -394,8 +393,7 @@ p0_status norm_launch(p0_ctx *c, NormJob &j, bool wide, const char *op) {
   const uint32_t row = T * R * 16u * ((XF16 ? 2u : 4u) + (TF16 ? 2u : 4u)), ws = T * 64u * (j.pw ? 2u : 1u);
   uint32_t per = 1024u / (T * R), smem = 0;
   const auto go = [&](auto kern, dim3 grid, dim3 block) {
-    // the limit belongs to the kernel, not to the context: always the same one, or another thread's smaller call could lower it before this launch
-    const cudaError_t e = smem ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingMost) : cudaSuccess;
+    const cudaError_t e = smem ? p0_smem_limit((const void *)kern, 768) : cudaSuccess;   // 768: red
     if (e != cudaSuccess) return p0_cuda(c, e, op);
     launch_dep(kern, grid, block, smem, c->stream, j);
     return p0_launched(c, op);
@@ -405,7 +403,7 @@ p0_status norm_launch(p0_ctx *c, NormJob &j, bool wide, const char *op) {
   if (j.M <= (uint32_t)c->sm_count && T <= 512u)
     return j.pw ? go(f8_norm_kernel<XF16, TF16, kDirect, true>, dim3(j.M), dim3(T)) : go(f8_norm_kernel<XF16, TF16, kDirect, false>, dim3(j.M), dim3(T));
   // room for three rows where it does not cost CTAs, two else; one for the longest in f32
-  const uint32_t all = kRingMost;
+  const uint32_t all = 220u * 1024u;
   j.wsm = row + ws <= all;
   const uint32_t w = j.wsm ? ws : 0u;
   j.nbuf = (3u * row + w) * per <= all ? 3u : 2u * row + w <= all ? 2u : 1u;

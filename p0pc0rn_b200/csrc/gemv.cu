@@ -444,7 +444,7 @@ cudaError_t launch_v2(const GemvParams &p, uint32_t nsplit, int sms, cudaStream_
     const uint32_t RW = rws[a];
     if (p.epi == P0_EPI_SOFTCAP && RW != 4) continue;
     V2Kernel k = v2_kernel_for(p.M, pair, RW);
-    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    p0_smem_limit((const void *)k, 0);
     int occ = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k, kThreads, smem) != cudaSuccess || occ < 1) { cudaGetLastError(); occ = 1; }
     const uint32_t slots = (uint32_t)sms * (uint32_t)occ;
@@ -470,11 +470,11 @@ template <int MT>
 cudaError_t launch_mt(const GemvParams &p, dim3 grid, size_t smem, cudaStream_t s) {
   if (p.epi == P0_EPI_GEGLU) {
     auto k = gemv_q4_v1<MT, true>;
-    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    p0_smem_limit((const void *)k, 0);
     return launch_pdl(k, grid, dim3(kThreads), smem, s, 1, p);
   } else {
     auto k = gemv_q4_v1<MT, false>;
-    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    p0_smem_limit((const void *)k, 0);
     return launch_pdl(k, grid, dim3(kThreads), smem, s, 1, p);
   }
 }

@@ -597,7 +597,7 @@ cudaError_t launch_v3(const GemvParams &p, int sms, cudaStream_t s) {
     nslot = 2;
     smem = v3_smem(p.M, G, 2, kG4Slot);
   }
-  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  p0_smem_limit((const void *)k, 0);
   const uint32_t need = S == 1 ? (ntile + kV3Warps - 1) / kV3Warps : ntile;
   uint32_t gx = (uint32_t)sms;
   if (gx > need) gx = need;

@@ -485,7 +485,7 @@ size_t v4_counter_bytes(const V4Plan &pl) { return (size_t)pl.ntile * pl.nsplit 
 cudaError_t launch_v4(const GemvParams &p, const V4Plan &pl, cudaStream_t s) {
   V4Kernel k = v4_kernel_for(p.M, pl.Gt != pl.G);
   const size_t smem = v4_smem(p.M, pl.G, pl.nslot);
-  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  p0_smem_limit((const void *)k, 0);
   return launch_pdl(k, dim3(pl.NW / kV4Warps), dim3(kV4Threads), smem, s, 1, p, pl);
 }
 

@@ -399,7 +399,7 @@ bool v5_plan(const GemvParams &p, uint32_t nsplit, int sms, V5Plan *pl) {
 cudaError_t launch_v5(const GemvParams &p, const V5Plan &pl, cudaStream_t s) {
   V5Kernel k = v5_kernel_for(p.M, pl.pair != 0, p.q8 != 0);
   const size_t smem = v5_smem(p.M, pl.nmax, p.q8 != 0);
-  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  p0_smem_limit((const void *)k, 0);
   return launch_pdl(k, dim3(pl.units * pl.CS), dim3(kV5Threads), smem, s, pl.CS, p, pl);
 }
 

@@ -90,6 +90,17 @@ inline p0_status p0_range(p0_ctx *c, p0_buf b, uint64_t off, uint64_t need, cons
   return P0_OK;
 }
 
+// Lets a kernel ask for as much dynamic shared memory as it ever may: 227 KB less its static arrays. The limit belongs to the function on the device,
+// not to a context: were it set to a call's own size, another context's smaller call, on another thread, could lower it before this call's launch
+inline cudaError_t p0_smem_limit(const void *kern, size_t statics) {
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(227u * 1024u - statics));
+}
+inline cudaError_t p0_smem_limit(const void *kern) {   // asks how much they take
+  cudaFuncAttributes at;
+  const cudaError_t e = cudaFuncGetAttributes(&at, kern);
+  return e != cudaSuccess ? e : p0_smem_limit(kern, at.sharedSizeBytes);
+}
+
 // launch bookkeeping: counts dispatches and turns launch errors into statuses
 inline p0_status p0_launched(p0_ctx *c, const char *what) {
   cudaError_t e = cudaGetLastError();

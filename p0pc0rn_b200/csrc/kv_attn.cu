@@ -595,7 +595,7 @@ p0_status attn_launch(p0_ctx *c, AttnJob &j) {
   const size_t smem = C::kSmem + ((size_t)j.v.rows + 1) * 4;
   const auto kern = kv4_attn_kernel<D, F32, NPL, RT, KP, NW>;
   int per = 0;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = p0_smem_limit((const void *)kern);
   if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, C::kThreads, smem);
   if (e != cudaSuccess || per < 1) { cudaGetLastError(); return p0_fail(c, P0_EDEVICE, "kv4Attn: the kernel does not fit this device"); }
   const uint32_t G = (uint32_t)(per * c->sm_count);

@@ -743,7 +743,7 @@ p0_status prompt_launch(p0_ctx *c, AttnJob &j, uint64_t wide_bytes, bool *taken)
     j.qbox = encode(&qm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<uint8_t *>(j.q.base), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   }
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = p0_smem_limit((const void *)kern);
   if (e != cudaSuccess) { cudaGetLastError(); return p0_fail(c, P0_EDEVICE, "kv4Attn: the prompt kernel does not fit this device"); }
   launch_dep(kv4_widen_kernel<D>, dim3((unsigned)c->sm_count * 4u), dim3(kET), ((size_t)R + 1) * 4, c->stream, j);
   if ((st = p0_launched(c, "kv4Attn pages"))) return st;

@@ -476,7 +476,7 @@ p0_status p0_normadd(p0_ctx *c, const p0_normadd_args *a) {
   const size_t smem = (size_t)D * (pre ? 12 : 4);
   cudaSetDevice(c->device);
   // above the 48 KB default the kernel opts in (its static reduction array counts against the same limit)
-  if (smem > 40u * 1024u) cudaFuncSetAttribute(normadd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 40u * 1024u) p0_smem_limit((const void *)normadd_kernel);
   launch_dep(normadd_kernel, dim3(M), dim3(kT), smem, c->stream, (const float *)rt.base, nsrc, ldp, a->mode == 0 ? (const float *)rw.base + a->w_off : nullptr,
                                              (float *)rx.base, (float *)rs.base, a->st_off, D, a->mode, eps, a->scale, pre);
   return p0_launched(c, "normadd");
@@ -535,7 +535,7 @@ p0_status p0_qkrope(p0_ctx *c, const p0_qkrope_args *a) {
   const float eps = a->eps != 0.0f ? a->eps : 1e-6f;   // lops.js:230 `a.eps || 1e-6`
   const size_t smem = (size_t)D * 4;
   cudaSetDevice(c->device);
-  if (smem > 40u * 1024u) cudaFuncSetAttribute(qkrope_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 40u * 1024u) p0_smem_limit((const void *)qkrope_kernel);
   launch_dep(qkrope_kernel, dim3(nh), dim3(kT), smem, c->stream, (const float *)rs.base, nsrc, ldp, (const float *)rn.base, (const float *)rr.base, (float *)rq.base,
                                              a->hasKV ? (__half *)rk.base : nullptr, a->hasKV ? (__half *)rv.base : nullptr, D, nq, nkv, a->pos,
                                              eps, a->qw, a->kw, a->npairs, a->rope_off, a->kvRow, a->kvLen);
@@ -562,7 +562,7 @@ p0_status p0_attn_dec(p0_ctx *c, const p0_attn_dec_args *a) {
   const size_t smem = ((size_t)nh * D + (size_t)nh * 64) * 4 + (size_t)64 * D * 2;   // q | scores | a chunk's V rows
   cudaSetDevice(c->device);
   auto go = [&](auto kern) {
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    p0_smem_limit((const void *)kern);
     launch_dep(kern, dim3(nchunk), dim3(kT), smem, c->stream, (const float *)rq.base, (const __half *)rk.base, (const __half *)rv.base, (float *)rp.base, D, nh, nkv,
                                           rows, a->kStart, a->kEnd, a->ring);
   };
