@@ -425,8 +425,8 @@ typedef struct {
 p0_status p0_beam_select(p0_ctx *ctx, const p0_beam_args *a);
 
 /* ---------------------------------------------------------------------------------------------- matrices in 8 bits */
-/* Activations and weights in e4m3 with an f32 scale for each block of 128, for matmuls that the tensor cores bound (prompts, DiT
- * blocks): twice the products a second of f16, half its activation bytes. No counterpart in the reference (its activations are f16).
+/* Activations and weights in e4m3 with an f32 scale for each block of 128, for matmuls that the tensor cores bound (the MLP of
+ * prompts, plain projections): twice the products a second of f16, half its activation bytes. No counterpart in the reference (its activations are f16).
  * A matrix of R rows and K columns: codes u8, element (r, k) at off + r * ld + k (ld 0 = K up to a multiple of 16; off and ld
  * multiples of 16 bytes from a 16-byte aligned buffer), and scales f32 at s_off (floats) of s. A code stands for its e4m3 value times
  * its block's scale. A block is

@@ -167,10 +167,13 @@ __global__ void __launch_bounds__(kT) f8_pack_tiles_kernel(PackJob j) {
 // ---------------------------------------------------------------- normF8
 // tv = the sum of the partial rows in order; with pw: tv * rsqrt(mean tv^2 + eps) * pw; h = (x + tv) * scale, rounded to the
 // stream's type; st = rsqrt(mean h^2 + eps); codes of (h * st) * w. blockDim.x threads hold a row, 16 columns each, and take rows in
-// turn (blockDim.y of them a CTA). Rows that start on 16 bytes come through shared memory (RING): every thread copies (cp.async) what
-// it will read itself, up to two rows ahead, so that nothing waits for another thread and no register holds what is on its way. With the
+// turn (blockDim.y of them a CTA). Rows that start on 16 bytes come through shared memory (RING): every warp copies (cp.async) the 512 columns that
+// it will read itself, up to two rows ahead, so that no warp waits for another one and no register holds what is on its way. Its lanes copy for one
+// another: a row's copies have landed for all of them behind one __syncwarp, and its place is overwritten behind the next. With the
 // next row in registers instead, few CTAs fit an SM (190 us for 32760 rows of 2240 in f16), and loads of the weights, which return in
-// order behind the next row's, held up each row. Now 95 us, 5.4 TB/s, at 76 % of the issue slots; 2051 rows of 1536, f32 + f16 with both norms: 13.1.
+// order behind the next row's, held up each row. Now 95 us, 5.4 TB/s, at 76 % of the issue slots (in long runs 104 at 1.81 GHz); 2051 rows of 1536, f32 +
+// f16 with both norms: 13.1; 4096 of 16384, f32 + f32, with room for one row a thread: 161, 5.4 TB/s. Rows that start anywhere, or D % 8 != 0, go value by
+// value: 4096 rows of 2241 in f16 55 us, of 2240 17.
 struct NormJob {
   const uint8_t *x, *t;
   uint8_t *h;

@@ -9,7 +9,7 @@
 // bytes of two rows at a time straight into the fragments of mma.sync.m16n8k32 (e4m3, f32 sums): the order of k inside a
 // fragment is free as long as both operands share it, so 16 consecutive bytes serve two instructions. Tokens are the n side,
 // loaded the same way. Each block's sums are scaled and added in f32; the warps' parts meet in shared memory, in order.
-// 1 token, 2048 x 2048: 3.5 us (launch, a round trip to memory, the join); 8 tokens, 8192 x 2048: 6.2 us, 2.7 TB/s; 8192 x 8192: 16 us, 4.2 TB/s.
+// 1 token, 2048 x 2048: 3.5 us (launch, a round trip to memory, the join); 8 tokens, 8192 x 2048: 6.1 us, 2.8 TB/s; 8192 x 8192: 16 us, 4.2 TB/s.
 #include <cstdlib>
 
 #include "f8_gemm.cuh"
@@ -161,10 +161,10 @@ extern "C" p0_status p0_gemm_f8(p0_ctx *c, const p0_gemm_f8_args *a) {
       (j.bv && over(j.bv, N * 4)) || (gated && f8_meet(y.q, yn, y.s, ysn)))
     return p0_fail(c, P0_EINVAL, "%s: y must not lie over the inputs", op);
   DeviceGuard guard(c->device);
-  // Up to 8 tokens and k of 8192 the form without tensor memory is the faster one (8 tokens, 8192 x 2048: 6.2 us against 7.5; 1 token, 2048 x
-  // 16384: 19 against 11), for small matrices up to 16 (2048 x 2048: 4.1 against 6.0). f8_mid.cu up to 128 tokens (128, 8192 x 2048: 11.1
-  // against 12.6 us of f8_tc.cu) and where its clusters share k, as then few of the other's tiles there are (256, 2048 x 8192: 16.7 against 32.5; 512, 4096 x
-  // 2048, where they do not: 14.4 against 12.5). Gated, with twice the stages' bytes, up to 64 (64: 14.9 against 17.1; 100: 29 against 17)
+  // Up to 8 tokens and k of 8192 the form without tensor memory is the faster one (8 tokens, 8192 x 2048: 6.1 us against 7.4; 1 token, 2048 x
+  // 16384: 19 against 14.6), for small matrices up to 16 (2048 x 2048: 4.3 against 6.0). f8_mid.cu up to 128 tokens (128, 8192 x 2048: 10.7
+  // against 12.6 us of f8_tc.cu) and where its clusters share k, as then few of the other's tiles there are (256, 2048 x 8192: 15.1 against 32.5; 512, 4096 x
+  // 2048, where they do not: 14.4 against 12.5). Gated, with twice the stages' bytes, up to 64 (64: 13.9 against 17.1; 100: 29 against 18.6)
   if (!gated && ((M <= 8 && j.KB <= 64) || (M <= 16 && N <= 4096 && j.KB <= 32))) return few_launch(c, j, op);
   if (gated ? M <= 64 : M <= 128 || f8_mid_parts(c, j.M, j.N, j.KB) > 1) return f8_mid_launch(c, j, y, op);
   return f8_tc_launch(c, j, y, op);

@@ -8,9 +8,9 @@
 // A cluster of S CTAs shares a tile's blocks of k. Each leaves its sums in its shared memory as [token][row]; then a warp takes a
 // token's 128 columns, adds the S parts in order (over distributed shared memory) and stores them; of a gated call it knows all 128
 // columns of the block of codes.
-// 16 tokens, 8192 x 2048: 7.5 us, of which the weights take 2.6 at the copy rate (the loop runs at it: 620 cycles a block over 128 CTAs) and 5 go by
-// before the first block and after the last, in the cluster's barriers most of all; 8192 x 8192: 16 us, 4.2 TB/s. 100 tokens, 6720 x 2240: 10.6 us. Groups
-// of blocks (64 sums to a wait) took 64 tokens from 10.0 to 9.4 us, eight warps for 128 tokens 8192 x 8192 from 24.1 to 22.3.
+// 16 tokens, 8192 x 2048: 7.4 us, of which the weights take 2.6 at the copy rate (the loop runs at it: 620 cycles a block over 128 CTAs) and 5 go by
+// before the first block and after the last, in the cluster's barriers most of all; 8192 x 8192: 15.6 us, 4.3 TB/s. 100 tokens, 6720 x 2240: 10.8 us. Groups
+// of blocks (64 sums to a wait) took 64 tokens from 10.0 to 9.4 us (now 8.9), eight warps for 128 tokens 8192 x 8192 from 24.1 to 22.3 (now 21.9).
 #include "f8_gemm.cuh"
 
 namespace {
@@ -283,8 +283,8 @@ __global__ void __launch_bounds__(Cfg<TN, MATS>::kThreads, 1)
         }
     };
     // Another CTA's parts are read only for tokens that there are: those are used, and so have arrived, before this warp comes to the last
-    // barrier. Where all U are there nothing is asked (100 tokens, 6720 x 2240: 10.9 us with the predicates throughout, 10.7 so; N = 8192, K = 2048
-    // with reads of absent tokens and now: 16 tokens 7.5 and 7.3, 16 gated 11.4 and 10.7, 64 plain 8.7 and 8.9)
+    // barrier. Where all U are there nothing is asked (100 tokens, 6720 x 2240: 10.9 us with the predicates throughout, 10.7 to 10.8 so; N = 8192, K = 2048
+    // with reads of absent tokens and now: 16 tokens 7.5 and 7.4, 16 gated 11.4 and 10.7, 64 plain 8.7 and 8.9)
     const bool all = S == 1u || t0 + (U - 1u) * stride < mend;
     for (uint32_t z = 0; z < S; z++) {
       if (all) add([=](const float *at, bool) { return S > 1u ? remote4(at, z) : *reinterpret_cast<const float4 *>(at); });
@@ -376,7 +376,7 @@ uint32_t tokens_of(uint32_t M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 
 }  // namespace
 
 // as many CTAs as there are SMs, two blocks of k each at least; clusters of eight wait long for their SMs (128 tokens, N = K = 2048: 23.5 us
-// against 9.0 with four)
+// against 8.8 with four)
 uint32_t f8_mid_parts(const p0_ctx *c, uint32_t M, uint32_t N, uint32_t KB) {
   const uint32_t TN = tokens_of(M);
   const uint64_t tiles = (uint64_t)((N + 127u) / 128u) * ((M + TN - 1u) / TN);
